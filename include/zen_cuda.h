@@ -632,6 +632,109 @@ int zen_cuda_dev_state_scan(const zen_cuda_linear_layer* l, int rule, const floa
 int zen_cuda_dev_decayed_write_scan(const zen_cuda_linear_layer* l, const float* d_proj, size_t ld, size_t tokens, const int* d_pos, void* d_workspace,
                                     size_t workspace_bytes, float* d_out, void* stream);
 
+/* ---- a key/value cache held in 4 bits: attention over it, and eviction from it ---------------------------------------------
+ * No counterpart in the reference, whose caches are fp32 (src/adapters/dense_transformer_runtime.cpp:4677-4684).  The form is that of Q4_0
+ * blocks: 32 consecutive values of a head share an f16 scale d and have codes 0 .. 15, value = d * (code - 8).  A slot (one token's
+ * key or value of one head) takes 18 bytes per 32 values where fp32 takes 128.  All memory is the caller's (device, 16-byte aligned):
+ *   codes   [kv_heads][slots / 8][head_dim / 32][8][16 bytes]: byte i of the 16 holds value i of the block (low half) and value i + 16
+ *   scales  [kv_heads][slots][head_dim / 32] f16
+ * head_dim: a multiple of 32 up to 256.  slots: a multiple of 32.  Slots may be filled in any order of positions: keys are stored
+ * rotated, so nothing but the slots' number is needed to attend to them. */
+typedef struct zen_cuda_q4_cache {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    uint16_t* k_scales;
+    uint16_t* v_scales;
+    uint32_t kv_heads, head_dim, slots;
+} zen_cuda_q4_cache;
+
+/* The attention of `tokens` new tokens (one: a decode step; more: a block to verify, or of a prompt), in a few launches:
+ *   - q and k are rotated by rows *position + t of the host-built tables [positions][pairs] (pairs (x[2i], x[2i+1]) when adjacent, else
+ *     (x[i], x[i+pairs]); every product and sum rounded on its own; pairs 0: no rotation); d_q, d_k and d_v are left as they are;
+ *   - k and v go into slots *filled + t: d = (the block's first value of largest magnitude) / -8 rounded to f16 (at most 65504 in
+ *     magnitude), code = the integer nearest to x / d + 8 (halves upwards) within 0 .. 15.  A block with a value that is not finite gets
+ *     d = NaN;
+ *   - token t attends to slots 0 .. *filled + t, its own among them as the cache holds it; query head h reads kv head
+ *     h / (heads / kv_heads); scale 0 means 1 / sqrt(head_dim);
+ *   - weight_out (or NULL) [kv_heads][slots]: what a slot received, summed over the group's heads and the tokens, plus weight_in for
+ *     slots below *filled; weight_in may be weight_out; slots behind the last token are left as they were;
+ *   - k_held, v_held (or NULL) [tokens][kv_heads * head_dim]: the new keys and values as the cache holds them.
+ * d_q [tokens][heads * head_dim] with rows q_ld apart, d_k and d_v [tokens][kv_heads * head_dim] with rows kv_ld apart (0: no gap);
+ * d_out [tokens][heads * head_dim].  position and filled are read on the device, so a captured call serves every step; the caller
+ * advances them.  Slots that do not fit the cache, or rows outside the tables, raise code 7 and nothing is written; a row whose scores
+ * are not finite raises code 8 and is NaN.  workspace: zen_cuda_q4_attention_workspace_bytes (16-byte aligned), nothing in it is kept between
+ * calls, and two calls in flight at a time need one each.  The bits of a row do not depend on earlier calls. */
+typedef struct zen_cuda_q4_attention {
+    zen_cuda_q4_cache cache;
+    uint32_t heads;
+    float scale;
+    const float* cos_t;
+    const float* sin_t;
+    uint32_t pairs, positions;
+    int adjacent;
+    const int32_t* position;
+    const int32_t* filled;
+    uint32_t q_ld, kv_ld;
+    const float* weight_in;
+    float* weight_out;
+    float* k_held;
+    float* v_held;
+    void* workspace;
+    size_t workspace_bytes;
+} zen_cuda_q4_attention;
+size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens); /* 0: not a valid call */
+int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, const float* d_k, const float* d_v, size_t tokens, float* d_out,
+                              void* stream);
+
+/* Drops slots that received little attention.  Of the slots 0 .. *filled - 1 of every kv head the first keep_first and the last keep_last
+ * stay, and of those between the ones with the largest weights (equal weights: the lowest slot; NaN counts as the least), `keep` in all;
+ * with *filled <= keep all of them.  What stays moves to slots 0 .. of `to` in its order, its weights to weight_to [kv_heads][to->slots].
+ * `to` is `from` itself (in place; weight_to is then weight), or shares no memory with it.  kept (or NULL) [kv_heads][keep]: the slot
+ * each came from.  Slots of `to` behind the kept ones are left as they were, and so is *filled: the caller sets it once every cache it counts for has
+ * been through.  1 <= keep <= to->slots, keep_first + keep_last <= keep.  *filled outside 0 .. from->slots raises code 7 and nothing is written. */
+size_t zen_cuda_q4_cache_evict_workspace_bytes(const zen_cuda_q4_cache* from); /* 0: not a valid cache */
+int zen_cuda_dev_q4_cache_evict(const zen_cuda_q4_cache* from, const float* weight, const int32_t* filled, const zen_cuda_q4_cache* to, float* weight_to,
+                                size_t keep, size_t keep_first, size_t keep_last, int32_t* kept, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- drafted tokens against the model's own distributions: the sampled form of a speculative block -------------------------
+ * The reference compares drafted tokens with the greedy picks of its verify block (src/adapters/dense_transformer_runtime.cpp:4874); with
+ * sampling, a drafted token x is accepted with probability min(1, p(x) / q(x)), and the first one that is not is replaced by a draw from
+ * max(p - q, 0), which leaves the tokens distributed as p.
+ *   logits    [drafts + 1] rows of vocab floats, logits_ld apart: row i is the model's answer after draft i - 1
+ *   p_i       the distribution zen_cuda_dev_sample draws from, of row i: finite logits only, the top_k highest (0: all; ties to the lowest ids),
+ *             exp((v - max) / temperature) normalised in double, cut to the shortest run of the most likely that reaches top_p (outside (0, 1):
+ *             no cut), without that call's limit on their number.  temperature 0: the greedy pick has all of it
+ *   q_i       what the draft was drawn from, as zen_cuda_dev_sample leaves it: q_ids, q_probs [drafts][ZEN_CUDA_SAMPLE_MAX_CANDIDATES], q_count
+ *             [drafts], ids distinct; all three NULL: the draft is certain (looked up, or a greedy pick)
+ *   uniforms  [drafts + 1] doubles in [0, 1): draft i is accepted when uniforms[i] * q_i(x) < p_i(x); the last draws the token behind the
+ *             accepted ones, the first id whose cumulative share of max(p - q, 0) (of p behind the last draft, or where nothing is left) reaches it
+ *   out       [drafts + 1]: the accepted drafts, the token that follows them (-1: its row has no finite logit), then -1
+ *   accepted  how many drafts were accepted;  probs (or NULL) [drafts]: p_i of every draft
+ * All pointers are device memory; drafts <= ZEN_CUDA_VERIFY_MAX_DRAFTS (0: one row is sampled), vocab <= ZEN_CUDA_VERIFY_MAX_VOCAB.  A draft outside the vocabulary raises code
+ * 6 and is not accepted.  The workspace is as the attention's above. */
+#define ZEN_CUDA_VERIFY_MAX_DRAFTS 64
+#define ZEN_CUDA_VERIFY_MAX_VOCAB 300000
+typedef struct zen_cuda_draft_check {
+    const float* logits;
+    size_t logits_ld;
+    uint32_t vocab, drafts;
+    const int64_t* tokens;
+    const int32_t* q_ids;
+    const double* q_probs;
+    const int32_t* q_count;
+    const double* uniforms;
+    float temperature;
+    uint32_t top_k;
+    float top_p;
+    int64_t* out;
+    int32_t* accepted;
+    double* probs;
+    void* workspace;
+    size_t workspace_bytes;
+} zen_cuda_draft_check;
+size_t zen_cuda_verify_drafts_workspace_bytes(const zen_cuda_draft_check* c); /* 0: not a valid call */
+int zen_cuda_dev_verify_drafts(const zen_cuda_draft_check* c, void* stream);
+
 /* The device-side error channel.  Synchronises `stream` (NULL: the backend's own), then reads and clears the error word
  * the kernels set.  Returns
  *    0      nothing to report;

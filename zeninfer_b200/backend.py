@@ -50,6 +50,8 @@ ABI_SYMBOLS = (
     "zen_cuda_dev_head_outputs_rows", "zen_cuda_dev_window_attention_rows", "zen_cuda_dev_window_attention_step", "zen_cuda_dev_state_step",
     "zen_cuda_dev_delta_inputs_rows", "zen_cuda_dev_gated_write_inputs_rows", "zen_cuda_dev_state_scan", "zen_cuda_dev_decayed_write_scan",
     "zen_cuda_state_scan_workspace_bytes",
+    "zen_cuda_q4_attention_workspace_bytes", "zen_cuda_dev_q4_attention", "zen_cuda_q4_cache_evict_workspace_bytes", "zen_cuda_dev_q4_cache_evict",
+    "zen_cuda_verify_drafts_workspace_bytes", "zen_cuda_dev_verify_drafts",
 )
 
 
@@ -121,6 +123,42 @@ class LinearLayer(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("heads", "kv_heads", "dim", "vdim", "taps")] + [("eps", C.c_float)] + [
         (n, C.c_void_p) for n in ("conv", "a_log", "dt_bias", "a2", "g2", "f_bias", "lower", "norm", "ring", "state", "decay")] + [
         ("inv_tau", C.c_float), ("rot_pairs", C.c_uint32), ("max_positions", C.c_uint32), ("rot_cos", C.c_void_p), ("rot_sin", C.c_void_p)]
+
+
+class Q4Cache(C.Structure):
+    """A key/value cache held in 4 bits: device memory of the caller (include/zen_cuda.h has the layout)."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "v_codes", "k_scales", "v_scales")] + [(n, C.c_uint32) for n in ("kv_heads", "head_dim", "slots")]
+
+    @staticmethod
+    def codes_shape(kv_heads: int, head_dim: int, slots: int) -> tuple[int, ...]:
+        return (kv_heads, slots // 8, head_dim // 32, 8, 16)
+
+    @staticmethod
+    def scales_shape(kv_heads: int, head_dim: int, slots: int) -> tuple[int, ...]:
+        return (kv_heads, slots, head_dim // 32)
+
+    @classmethod
+    def of(cls, k_codes, k_scales, v_codes, v_scales, *, kv_heads: int, head_dim: int, slots: int) -> "Q4Cache":
+        """The cache in these torch tensors: codes uint8, scales float16, contiguous, in the shapes above (or as many elements)."""
+        for t, size, what in ((k_codes, 1, "k_codes"), (v_codes, 1, "v_codes"), (k_scales, 2, "k_scales"), (v_scales, 2, "v_scales")):
+            per_slot = head_dim // 2 if size == 1 else head_dim // 32
+            if t.element_size() != size or not t.is_contiguous() or t.numel() != kv_heads * slots * per_slot:
+                raise ValueError(f"Q4Cache: {what} does not hold {kv_heads} heads of {slots} slots of {head_dim} values")
+        return cls(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), kv_heads, head_dim, slots)
+
+
+class Q4Attention(C.Structure):
+    _fields_ = [("cache", Q4Cache), ("heads", C.c_uint32), ("scale", C.c_float), ("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("pairs", C.c_uint32),
+                ("positions", C.c_uint32), ("adjacent", C.c_int), ("position", C.c_void_p), ("filled", C.c_void_p), ("q_ld", C.c_uint32), ("kv_ld", C.c_uint32)] + [
+        (n, C.c_void_p) for n in ("weight_in", "weight_out", "k_held", "v_held", "workspace")] + [("workspace_bytes", C.c_size_t)]
+
+
+class DraftCheck(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_ld", C.c_size_t), ("vocab", C.c_uint32), ("drafts", C.c_uint32)] + [
+        (n, C.c_void_p) for n in ("tokens", "q_ids", "q_probs", "q_count", "uniforms")] + [
+        ("temperature", C.c_float), ("top_k", C.c_uint32), ("top_p", C.c_float)] + [
+        (n, C.c_void_p) for n in ("out", "accepted", "probs", "workspace")] + [("workspace_bytes", C.c_size_t)]
 
 
 def load_library(path: str | None = None) -> C.CDLL:
@@ -232,6 +270,15 @@ def load_library(path: str | None = None) -> C.CDLL:
     lib.zen_cuda_dev_delta_inputs_rows.argtypes = [C.POINTER(LinearLayer), vp, sz, vp, sz, sz, vp, vp, vp, vp, vp, vp, vp]
     lib.zen_cuda_dev_gated_write_inputs_rows.argtypes = [C.POINTER(LinearLayer), vp, sz, sz, vp, vp, vp]
     lib.zen_cuda_dev_state_scan.argtypes = [C.POINTER(LinearLayer), i, vp, vp, vp, vp, sz, vp, sz, vp, sz, vp, vp]
+    lib.zen_cuda_q4_attention_workspace_bytes.argtypes = [C.POINTER(Q4Attention), sz]
+    lib.zen_cuda_q4_attention_workspace_bytes.restype = sz
+    lib.zen_cuda_dev_q4_attention.argtypes = [C.POINTER(Q4Attention), vp, vp, vp, sz, vp, vp]
+    lib.zen_cuda_q4_cache_evict_workspace_bytes.argtypes = [C.POINTER(Q4Cache)]
+    lib.zen_cuda_q4_cache_evict_workspace_bytes.restype = sz
+    lib.zen_cuda_dev_q4_cache_evict.argtypes = [C.POINTER(Q4Cache), vp, vp, C.POINTER(Q4Cache), vp, sz, sz, sz, vp, vp, sz, vp]
+    lib.zen_cuda_verify_drafts_workspace_bytes.argtypes = [C.POINTER(DraftCheck)]
+    lib.zen_cuda_verify_drafts_workspace_bytes.restype = sz
+    lib.zen_cuda_dev_verify_drafts.argtypes = [C.POINTER(DraftCheck), vp]
     lib.zen_cuda_dev_decayed_write_scan.argtypes = [C.POINTER(LinearLayer), vp, sz, sz, vp, vp, sz, vp, vp]
     lib.zen_cuda_state_scan_workspace_bytes.argtypes = [C.POINTER(LinearLayer), i, sz]
     lib.zen_cuda_state_scan_workspace_bytes.restype = sz
@@ -711,6 +758,32 @@ class Backend:
         """The decayed write over a block, straight from its projection rows."""
         if not self.lib.zen_cuda_dev_decayed_write_scan(C.byref(layer), d_proj, ld, tokens, d_pos, d_workspace, workspace_bytes, d_out, stream):
             self._fail("dev_decayed_write_scan")
+
+    # ---- the cache held in 4 bits, and drafted tokens ----
+    def q4_attention_workspace_bytes(self, a: Q4Attention, tokens: int) -> int:
+        return int(self.lib.zen_cuda_q4_attention_workspace_bytes(a, tokens))
+
+    def dev_q4_attention(self, a: Q4Attention, d_q: int, d_k: int, d_v: int, tokens: int, d_out: int, stream: int = 0) -> None:
+        """Rotation, append and attention of `tokens` new tokens over a cache held in 4 bits."""
+        if not self.lib.zen_cuda_dev_q4_attention(a, d_q, d_k, d_v, tokens, d_out, stream):
+            self._fail("dev_q4_attention")
+
+    def q4_cache_evict_workspace_bytes(self, cache: Q4Cache) -> int:
+        return int(self.lib.zen_cuda_q4_cache_evict_workspace_bytes(cache))
+
+    def dev_q4_cache_evict(self, source: Q4Cache, d_weight: int, d_filled: int, to: Q4Cache, d_weight_to: int, keep: int, keep_first: int, keep_last: int,
+                           workspace: int, workspace_bytes: int, stream: int = 0, *, d_kept: int | None = None) -> None:
+        """The `keep` slots per kv head that received most attention (and the first and last ones) move to the front of `to`."""
+        if not self.lib.zen_cuda_dev_q4_cache_evict(source, d_weight, d_filled, to, d_weight_to, keep, keep_first, keep_last, d_kept, workspace, workspace_bytes, stream):
+            self._fail("dev_q4_cache_evict")
+
+    def verify_drafts_workspace_bytes(self, check: DraftCheck) -> int:
+        return int(self.lib.zen_cuda_verify_drafts_workspace_bytes(check))
+
+    def dev_verify_drafts(self, check: DraftCheck, stream: int = 0) -> None:
+        """Accepts or replaces drafted tokens by the model's own distributions (check.uniforms: the random numbers)."""
+        if not self.lib.zen_cuda_dev_verify_drafts(check, stream):
+            self._fail("dev_verify_drafts")
 
     def dev_check(self, stream: int = 0) -> None:
         """Synchronises `stream` and raises if a kernel reported through the device-side error word (a bounded wait that

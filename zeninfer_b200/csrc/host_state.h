@@ -41,5 +41,6 @@ struct Entry {
 };
 
 bool set_dense_wait_budget(long long cycles);   // zen_cuda_dense.cu's copy of the bounded-wait budget
+bool set_q4_wait_budget(long long cycles);      // zen_cuda_q4.cu's
 
 }  // namespace zk_host

@@ -1,0 +1,303 @@
+// A key/value cache held in 4 bits: its layout, the quantisation of new keys and values, and the eviction of slots.
+//
+// 32 consecutive values of a head are a block, as in Q4_0: an f16 scale d and codes 0 .. 15, value = d * (code - 8).  The codes of eight
+// slots' equal blocks are 128 consecutive bytes ([slots / 8][blocks][8][16]): what a warp fetches as one 8 x 16-byte matrix has no bank
+// conflicts, and a run of slots is one piece of memory that a bulk copy takes.
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "zk_ptx.cuh"
+
+namespace zk {
+
+constexpr uint32_t kQ4Block = 32, kQ4MaxBlocks = 8;      // values of a block; blocks of a head (head_dim <= 256)
+
+struct Q4Cache {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    __half* k_scales;
+    __half* v_scales;
+    uint32_t kv_heads, blocks, slots;      // blocks = head_dim / 32
+};
+
+// Byte offset of a block's 16 code bytes, and index of its scale.
+__host__ __device__ __forceinline__ size_t q4_codes_at(uint32_t kv_head, uint32_t slot, uint32_t block, uint32_t blocks, uint32_t slots) {
+    return (((static_cast<size_t>(kv_head) * (slots >> 3) + (slot >> 3)) * blocks + block) * 8 + (slot & 7)) * 16;
+}
+__host__ __device__ __forceinline__ size_t q4_scale_at(uint32_t kv_head, uint32_t slot, uint32_t block, uint32_t blocks, uint32_t slots) {
+    return (static_cast<size_t>(kv_head) * slots + slot) * blocks + block;
+}
+
+// Whether `tokens` slots behind *filled are in the cache, and the rows of the tables exist.
+__device__ __forceinline__ bool q4_places_ok(int filled, int position, uint32_t tokens, uint32_t slots, uint32_t pairs, uint32_t positions) {
+    return filled >= 0 && static_cast<uint64_t>(filled) + tokens <= slots && (!pairs || (position >= 0 && static_cast<uint64_t>(position) + tokens <= positions));
+}
+
+struct Q4Rotation {
+    const float* cos_t;       // [positions][pairs]
+    const float* sin_t;
+    uint32_t pairs, positions;
+    uint32_t adjacent;
+};
+
+// Dimension `e` of a head vector, rotated by the tables' row: every product and sum rounded on its own, so that a key turns out the same in
+// every kernel that forms it.
+__device__ __forceinline__ float q4_rotated(const float* head, uint32_t e, const Q4Rotation& r, size_t row) {
+    if (e >= 2 * r.pairs) return __ldcg(head + e);
+    const uint32_t pair = r.adjacent ? e >> 1 : e < r.pairs ? e : e - r.pairs;
+    const bool low = r.adjacent ? !(e & 1u) : e < r.pairs;
+    const uint32_t other = r.adjacent ? e ^ 1u : low ? e + r.pairs : e - r.pairs;
+    const float mine = __ldcg(head + e), its = __ldcg(head + other);
+    const float c = __ldg(r.cos_t + row * r.pairs + pair), s = __ldg(r.sin_t + row * r.pairs + pair);
+    return low ? __fsub_rn(__fmul_rn(mine, c), __fmul_rn(its, s)) : __fadd_rn(__fmul_rn(its, s), __fmul_rn(mine, c));
+}
+
+// A warp quantises a block, a value a lane: the scale (of the first value of largest magnitude), the lane's code.  The code is the integer
+// nearest to x / d + 8, and the choice is exact: x / d >= c - 8.5 is x >= (c - 8.5) d for positive d, a product of five bits and eleven
+// that fp32 holds, so the estimate from the rounded quotient, off by one at most, is put right by two comparisons.
+struct Q4Quantised {
+    __half scale;
+    uint32_t code;
+};
+__device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
+    const uint32_t size = __float_as_uint(x) & 0x7fffffffu;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, size);
+    const float at = __shfl_sync(0xffffffffu, x, __ffs(__ballot_sync(0xffffffffu, size == top)) - 1);
+    Q4Quantised r;
+    if (top >= 0x7f800000u) {      // an infinity or a NaN among the values: the block reads as NaN
+        r.scale = __ushort_as_half(static_cast<unsigned short>(0x7e00u));
+        r.code = 8;
+        return r;
+    }
+    r.scale = __float2half_rn(fminf(fmaxf(at * -0.125f, -65504.0f), 65504.0f));
+    const float d = __half2float(r.scale);
+    if (d == 0.0f) {
+        r.code = 8;
+        return r;
+    }
+    const float guess = fminf(fmaxf(floorf(__fadd_rn(__fdiv_rn(x, d), 8.5f)), -1.0f), 16.0f);
+    auto reaches = [&](float c) { const float border = (c - 8.5f) * d; return d > 0.0f ? x >= border : x <= border; };
+    float c = guess;
+    if (!reaches(c)) c -= 1.0f;
+    else if (reaches(c + 1.0f)) c += 1.0f;
+    r.code = static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));
+    return r;
+}
+
+struct Q4Append {
+    Q4Cache cache;
+    Q4Rotation turn;
+    const float* k;            // rows kv_ld apart
+    const float* v;
+    const int* position;
+    const int* filled;
+    float* k_held;             // or null
+    float* v_held;
+    uint32_t tokens;
+    size_t kv_ld;
+    int* error_word;
+};
+
+// The new tokens' keys (rotated) and values into the slots behind *filled.  grid = (tokens, kv_heads), two warps per block of a head: one for
+// the key's, one for the value's.
+__global__ void __launch_bounds__(512) q4_append_kernel(const __grid_constant__ Q4Append p) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, blocks = p.cache.blocks, t = blockIdx.x, h = blockIdx.y;
+    const bool is_value = warp >= blocks;
+    const uint32_t block = is_value ? warp - blocks : warp;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
+    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {
+        if (threadIdx.x == 0 && t == 0 && h == 0) atomicExch(p.error_word, kErrBadPosition);
+        return;
+    }
+    const size_t head_at = t * p.kv_ld + static_cast<size_t>(h) * blocks * kQ4Block;
+    const uint32_t e = block * kQ4Block + lane;
+    const float x = is_value ? __ldcg(p.v + head_at + e) : q4_rotated(p.k + head_at, e, p.turn, static_cast<size_t>(position) + t);
+    const Q4Quantised q = q4_quantise(x, lane);
+    const uint32_t slot = static_cast<uint32_t>(filled) + t;
+    const uint32_t high = __shfl_down_sync(0xffffffffu, q.code, 16);
+    if (lane < 16) (is_value ? p.cache.v_codes : p.cache.k_codes)[q4_codes_at(h, slot, block, blocks, p.cache.slots) + lane] = static_cast<uint8_t>(q.code | high << 4);
+    if (lane == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, blocks, p.cache.slots)] = q.scale;
+    float* held = is_value ? p.v_held : p.k_held;
+    if (held) held[(static_cast<size_t>(t) * p.cache.kv_heads + h) * blocks * kQ4Block + e] = (static_cast<float>(q.code) - 8.0f) * __half2float(q.scale);
+}
+
+// ---- eviction ----------------------------------------------------------------------------------------------------------------
+//
+// A cluster of eight CTAs takes a kv head; each CTA a run of its slots, each warp a run of the CTA's.  The weight of the last slot that stays is found
+// by a radix select over order-preserving keys (four passes of eight bits, counts of the CTAs added through distributed shared memory), then
+// every warp counts what stays of its run, and a prefix over CTAs and warps gives each kept slot its place: the choice and the order are the
+// same in every run.  The move copies 16-byte pieces in rounds, all of a round read before any is written, so that it may be done in place:
+// a slot never moves up, so what a round overwrites lies in front of what later rounds read.
+// What bounds it: the moved bytes (read and written once) for large caches, a dozen cluster barriers for small ones.
+constexpr int kEvictThreads = 1024, kEvictCtas = 8, kEvictPieces = 4;
+
+struct Q4Evict {
+    Q4Cache from, to;
+    const float* weight;       // [kv_heads][from.slots]
+    float* weight_to;          // [kv_heads][to.slots]
+    const int* filled;
+    int* kept;                 // [kv_heads][keep], or null
+    int* list;                 // workspace [kv_heads][from.slots]: the slot at every rank
+    uint32_t keep, keep_first, keep_last;
+    int* error_word;
+};
+
+// Larger for larger weights; the zeros are equal, NaN is the least.
+__device__ __forceinline__ uint32_t evict_key(float w) {
+    if (w != w) return 0u;
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThreads) q4_evict_kernel(const __grid_constant__ Q4Evict p) {
+    namespace cg = cooperative_groups;
+    __shared__ uint32_t hist[256], total[256];
+    __shared__ uint32_t s_prefix, s_remaining;
+    __shared__ uint32_t warp_more[32], warp_ties[32];      // a warp's slots above the border, and at it
+    __shared__ uint32_t cta_more, cta_ties;                // read by the other CTAs
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), h = blockIdx.y;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
+    if (filled < 0 || static_cast<uint32_t>(filled) > p.from.slots) {      // the same for every CTA of the grid
+        if (tid == 0 && rank == 0 && h == 0) atomicExch(p.error_word, kErrBadPosition);
+        return;
+    }
+    const uint32_t n = filled, keep = min(n, p.keep);
+    const float* weight = p.weight + static_cast<size_t>(h) * p.from.slots;
+    int* list = p.list + static_cast<size_t>(h) * p.from.slots;
+    // slots [low, high) compete for `wanted` places; all others stay
+    const bool all = n <= p.keep;
+    const uint32_t low = all ? n : p.keep_first, high = all ? n : n - p.keep_last, wanted = all ? 0u : keep - p.keep_first - p.keep_last;
+    const uint32_t per_warp = ((n + kEvictCtas * 32 - 1) / (kEvictCtas * 32) + 31) & ~31u;
+    const uint32_t begin = min(n, (rank * 32 + warp) * per_warp), end = min(n, begin + per_warp);
+
+    // the wanted-th largest key among the competing slots, and how many that equal it stay
+    uint32_t border = 0xffffffffu, ties_wanted = 0;
+    if (wanted) {
+        if (tid == 0) { s_prefix = 0; s_remaining = wanted; }
+        uint32_t mask = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            if (tid < 256) hist[tid] = 0;
+            __syncthreads();
+            const uint32_t prefix = s_prefix;
+            for (uint32_t i = begin + lane; i < end; i += 32) {
+                const uint32_t key = evict_key(__ldcg(weight + i));
+                if (i >= low && i < high && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+            }
+            cluster.sync();
+            if (tid < 256) {
+                uint32_t sum = 0;
+                for (uint32_t r = 0; r < kEvictCtas; ++r) sum += cluster.map_shared_rank(hist, r)[tid];
+                total[tid] = sum;
+            }
+            cluster.sync();                                     // everybody has read everybody's counts
+            if (warp == 0) {
+                // lane l looks after bins 255 - 8 l .. 248 - 8 l, from the largest down
+                uint32_t mine = 0;
+                for (int j = 0; j < 8; ++j) mine += total[255 - 8 * lane - j];
+                uint32_t upto = mine;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (static_cast<int>(lane) >= o) upto += v;
+                }
+                const uint32_t remaining = s_remaining;
+                const uint32_t reached = __ballot_sync(0xffffffffu, upto >= remaining);
+                if (static_cast<int>(lane) == __ffs(reached) - 1) {
+                    uint32_t left = remaining - (upto - mine);
+                    int bin = 255 - 8 * static_cast<int>(lane);
+                    while (total[bin] < left) left -= total[bin--];
+                    s_prefix = prefix | static_cast<uint32_t>(bin) << shift;
+                    s_remaining = left;
+                }
+            }
+            __syncthreads();
+            mask |= 255u << shift;
+        }
+        border = s_prefix;
+        ties_wanted = s_remaining;
+    }
+    // what stays of every warp's run
+    uint32_t more = 0, ties = 0;
+    for (uint32_t i = begin + lane; i < end; i += 32) {
+        const bool competes = i >= low && i < high;
+        const uint32_t key = evict_key(__ldcg(weight + i));
+        more += !competes || (wanted && key > border);
+        ties += competes && wanted && key == border;
+    }
+    more = __reduce_add_sync(0xffffffffu, more);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) { warp_more[warp] = more; warp_ties[warp] = ties; }
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t m = 0, t = 0;
+        for (int w = 0; w < 32; ++w) { m += warp_more[w]; t += warp_ties[w]; }
+        cta_more = m;
+        cta_ties = t;
+    }
+    cluster.sync();
+    uint32_t before = 0, ties_before = 0;
+    for (uint32_t r = 0; r < rank; ++r) { before += *cluster.map_shared_rank(&cta_more, r); ties_before += *cluster.map_shared_rank(&cta_ties, r); }
+    for (uint32_t w = 0; w < warp; ++w) { before += warp_more[w]; ties_before += warp_ties[w]; }
+    for (uint32_t i0 = begin; i0 < end; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        const bool real = i < end, competes = i >= low && i < high;
+        const uint32_t key = real ? evict_key(__ldcg(weight + i)) : 0u;
+        const bool above = real && (!competes || (wanted && key > border)), tie = real && competes && wanted && key == border;
+        const uint32_t below = (1u << lane) - 1u, aboves = __ballot_sync(0xffffffffu, above), tied = __ballot_sync(0xffffffffu, tie);
+        const uint32_t tie_rank = ties_before + __popc(tied & below);
+        if (above || (tie && tie_rank < ties_wanted)) {
+            const uint32_t place = before + __popc(aboves & below) + min(tie_rank, ties_wanted);
+            list[place] = static_cast<int>(i);
+            if (p.kept) p.kept[static_cast<size_t>(h) * p.keep + place] = static_cast<int>(i);
+        }
+        before += __popc(aboves);
+        ties_before += __popc(tied);
+    }
+    cluster.sync();                                        // the list is whole, and nobody reads another CTA's counts any more
+
+    // the move: a kept slot is 2 * blocks pieces of 16 code bytes, and beside them its scales and its weight.  Eight neighbouring threads take
+    // one piece of eight neighbouring places, which are written as one line.
+    const bool in_place = p.to.k_codes == p.from.k_codes;
+    const uint32_t blocks = p.from.blocks, pieces = 2 * blocks, a_round = kEvictCtas * kEvictThreads * kEvictPieces / (8 * pieces) * 8;
+    for (uint32_t first = 0; first < keep; first += a_round) {
+        uint4 code[kEvictPieces];
+        __half scale[kEvictPieces];
+        float w[kEvictPieces];
+        uint32_t place[kEvictPieces], piece[kEvictPieces];
+        bool mine[kEvictPieces];
+#pragma unroll
+        for (int u = 0; u < kEvictPieces; ++u) {
+            const uint32_t i = (u * kEvictCtas + rank) * kEvictThreads + tid;
+            piece[u] = (i >> 3) % pieces;
+            place[u] = first + i / (8 * pieces) * 8 + (i & 7u);
+            mine[u] = i < a_round * pieces && place[u] < keep;
+            if (!mine[u]) continue;
+            const bool value = piece[u] >= blocks;
+            const uint32_t block = value ? piece[u] - blocks : piece[u], slot = static_cast<uint32_t>(__ldcg(list + place[u]));
+            code[u] = __ldcg(reinterpret_cast<const uint4*>((value ? p.from.v_codes : p.from.k_codes) + q4_codes_at(h, slot, block, blocks, p.from.slots)));
+            scale[u] = __ldcg((value ? p.from.v_scales : p.from.k_scales) + q4_scale_at(h, slot, block, blocks, p.from.slots));
+            if (piece[u] == 0) w[u] = __ldcg(weight + slot);
+        }
+        if (in_place) cluster.sync();
+#pragma unroll
+        for (int u = 0; u < kEvictPieces; ++u) {
+            if (!mine[u]) continue;
+            const bool value = piece[u] >= blocks;
+            const uint32_t block = value ? piece[u] - blocks : piece[u];
+            *reinterpret_cast<uint4*>((value ? p.to.v_codes : p.to.k_codes) + q4_codes_at(h, place[u], block, blocks, p.to.slots)) = code[u];
+            (value ? p.to.v_scales : p.to.k_scales)[q4_scale_at(h, place[u], block, blocks, p.to.slots)] = scale[u];
+            if (piece[u] == 0) p.weight_to[static_cast<size_t>(h) * p.to.slots + place[u]] = w[u];
+        }
+        if (in_place) cluster.sync();
+    }
+}
+
+}  // namespace zk

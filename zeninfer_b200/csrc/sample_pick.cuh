@@ -20,13 +20,12 @@
 #pragma once
 #include <cstdint>
 
+#include "sample_key.cuh"
 #include "zk_ptx.cuh"
 
 namespace zk {
 
 constexpr int kSampleThreads = 1024;
-constexpr uint32_t kSampleMaxCandidates = 1024;
-
 struct SampleParams {
     const float* logits;      // [n]
     uint32_t n;
@@ -40,13 +39,6 @@ struct SampleParams {
     int* kept_count;          // optional
     int* truncated;           // optional: 1 when the candidates' cumulative probability stayed below top_p
 };
-
-// Order-preserving key of a finite float (larger float, larger key); 0 for a non-finite one (never a candidate).
-__device__ __forceinline__ uint32_t sample_key(float v) {
-    const uint32_t b = __float_as_uint(v);
-    if ((b & 0x7f800000u) == 0x7f800000u) return 0u;
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
 
 __global__ void __launch_bounds__(kSampleThreads) sample_top_kernel(const SampleParams p) {
     __shared__ uint32_t hist[256];

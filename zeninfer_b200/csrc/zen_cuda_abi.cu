@@ -154,6 +154,7 @@ bool apply_wait_budget(State& s, unsigned ms) {
     const long long cycles = ms ? static_cast<long long>(ms) * std::max(1, s.clock_khz) : zk::kDefaultWaitBudgetCycles;
     ZC_CUDA(s, cudaMemcpyToSymbol(zk::g_wait_budget_cycles, &cycles, sizeof cycles));
     if (!zk_host::set_dense_wait_budget(cycles)) return set_error(s, "setting the dense kernels' wait budget failed");
+    if (!zk_host::set_q4_wait_budget(cycles)) return set_error(s, "setting the 4-bit cache kernels' wait budget failed");
     return true;
 }
 

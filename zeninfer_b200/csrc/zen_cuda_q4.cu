@@ -1,0 +1,195 @@
+// C-ABI of the 4-bit key/value cache and of the check of drafted tokens (include/zen_cuda.h): argument checks and launches.
+#include "../../include/zen_cuda.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <unordered_map>
+
+#include "host_state.h"
+#include "q4_attention.cuh"
+#include "q4_cache.cuh"
+#include "verify_drafts.cuh"
+
+namespace zk_host {
+bool set_q4_wait_budget(long long cycles) { return cudaMemcpyToSymbol(zk::g_wait_budget_cycles, &cycles, sizeof cycles) == cudaSuccess; }
+}  // namespace zk_host
+
+namespace {
+
+using zk_host::Entry;
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch(const Entry& e, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, unsigned cluster, Args... args) {
+    if (smem > 32 * 1024 || cluster > 8) {      // without an opt-in a block has 48 KB, what it declares statically among them
+        static std::unordered_map<const void*, size_t> allowed;      // what the kernels of this signature may use so far; under the Entry's lock
+        auto at = allowed.find(reinterpret_cast<const void*>(kernel));
+        if (at == allowed.end() || smem > at->second) {
+            cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (r == cudaSuccess && cluster > 8) r = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (r != cudaSuccess) return r;
+            allowed[reinterpret_cast<const void*>(kernel)] = smem;
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = e.stream;
+    cudaLaunchAttribute attr[2]{};
+    unsigned count = 0;
+    if (e.pdl) {
+        attr[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[count++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster) {
+        attr[count].id = cudaLaunchAttributeClusterDimension;
+        attr[count].val.clusterDim.x = cluster;
+        attr[count].val.clusterDim.y = attr[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = count;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+uint32_t u32(size_t v) { return static_cast<uint32_t>(v); }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
+
+bool cache_ok(const zen_cuda_q4_cache* c) {
+    return c && c->k_codes && c->v_codes && c->k_scales && c->v_scales && aligned16(c->k_codes) && aligned16(c->v_codes) && aligned16(c->k_scales) && aligned16(c->v_scales) &&
+           c->kv_heads && c->kv_heads <= 65535 && c->head_dim && c->head_dim % zk::kQ4Block == 0 && c->head_dim <= zk::kQ4Block * zk::kQ4MaxBlocks && c->slots &&
+           c->slots % 32 == 0 && c->slots <= 0x40000000u;
+}
+zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
+    return zk::Q4Cache{c.k_codes, c.v_codes, reinterpret_cast<__half*>(c.k_scales), reinterpret_cast<__half*>(c.v_scales), c.kv_heads, c.head_dim / zk::kQ4Block, c.slots};
+}
+
+// The workspace of a call, or 0 when its sizes are none.
+size_t attention_room(const zen_cuda_q4_attention* a, size_t tokens) {
+    if (!a || !cache_ok(&a->cache) || !a->heads || a->heads % a->cache.kv_heads || a->heads > 65535 || !tokens || tokens > a->cache.slots) return 0;
+    return up16(tokens * a->heads * 2 * sizeof(float));
+}
+
+template <typename Run>
+cudaError_t by_blocks(uint32_t blocks, Run run) {
+    switch (blocks) {
+    case 1: return run(std::integral_constant<int, 1>{});
+    case 2: return run(std::integral_constant<int, 2>{});
+    case 3: return run(std::integral_constant<int, 3>{});
+    case 4: return run(std::integral_constant<int, 4>{});
+    case 5: return run(std::integral_constant<int, 5>{});
+    case 6: return run(std::integral_constant<int, 6>{});
+    case 7: return run(std::integral_constant<int, 7>{});
+    default: return run(std::integral_constant<int, 8>{});
+    }
+}
+
+struct Span {
+    uintptr_t begin, end;
+};
+bool apart(const Span& a, const Span& b) { return a.end <= b.begin || b.end <= a.begin; }
+Span span_of(const void* p, size_t bytes) { return Span{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes}; }
+
+size_t verify_room(const zen_cuda_draft_check* c) {
+    if (!c || !c->vocab || c->vocab > ZEN_CUDA_VERIFY_MAX_VOCAB || c->drafts > ZEN_CUDA_VERIFY_MAX_DRAFTS) return 0;
+    return up16((size_t(c->drafts) + 1) * (sizeof(long long) + sizeof(int)));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens) { return attention_room(a, tokens); }
+
+int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, const float* d_k, const float* d_v, size_t tokens, float* d_out,
+                              void* stream) {
+    Entry e(stream);
+    const size_t room = attention_room(a, tokens);
+    if (!room) return e.fail("dev_q4_attention: bad arguments (head_dim a multiple of 32 up to 256, slots a multiple of 32, heads a multiple of kv_heads, 1 .. slots tokens)");
+    const size_t q_row = size_t(a->heads) * a->cache.head_dim, kv_row = size_t(a->cache.kv_heads) * a->cache.head_dim;
+    if (!d_q || !d_k || !d_v || !d_out || !a->filled || (a->q_ld && a->q_ld < q_row) || (a->kv_ld && a->kv_ld < kv_row) || !std::isfinite(a->scale))
+        return e.fail("dev_q4_attention: bad arguments (rows)");
+    if (a->pairs && (a->pairs > a->cache.head_dim / 2 || !a->cos_t || !a->sin_t || !a->position || !a->positions)) return e.fail("dev_q4_attention: bad arguments (rotation)");
+    if (!a->weight_in != !a->weight_out) return e.fail("dev_q4_attention: weight_in and weight_out go together");
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < room) return e.fail("dev_q4_attention: the workspace is missing, not 16-byte aligned or too small");
+    if (!e.ok) return 0;
+    const zk::Q4Rotation turn{a->cos_t, a->sin_t, a->pairs, a->positions, a->adjacent ? 1u : 0u};
+    const zk::Q4Cache cache = device_form(a->cache);
+    const zk::Q4Append append{cache, turn, d_k, d_v, a->position, a->filled, a->k_held, a->v_held, u32(tokens), a->kv_ld ? a->kv_ld : kv_row, e.d_error};
+    if (!e.leave(launch(e, zk::q4_append_kernel, dim3(u32(tokens), cache.kv_heads), dim3(64 * cache.blocks), 0, 0, append), "dev_q4_attention: append")) return 0;
+    const zk::Q4Attend p{cache, turn, d_q, a->position, a->filled, a->weight_in, a->weight_out, d_out, static_cast<float*>(a->workspace), u32(tokens), a->heads,
+                         a->q_ld ? a->q_ld : q_row, a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale, e.d_error};
+    const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) { return launch(e, zk::q4_attend_kernel<decltype(blocks)::value>, dim3(u32(tokens), a->heads), dim3(256), 0, 0, p); });
+    if (!e.leave(r, "dev_q4_attention") || !a->weight_out) return r == cudaSuccess;
+    return e.leave(by_blocks(cache.blocks, [&](auto blocks) { return launch(e, zk::q4_received_kernel<decltype(blocks)::value>, dim3(cache.slots / 8, cache.kv_heads), dim3(256), 0, 0, p); }),
+                   "dev_q4_attention: weights");
+}
+
+size_t zen_cuda_q4_cache_evict_workspace_bytes(const zen_cuda_q4_cache* from) {
+    return cache_ok(from) ? size_t(from->kv_heads) * from->slots * sizeof(int) : 0;
+}
+
+int zen_cuda_dev_q4_cache_evict(const zen_cuda_q4_cache* from, const float* weight, const int32_t* filled, const zen_cuda_q4_cache* to, float* weight_to, size_t keep,
+                                size_t keep_first, size_t keep_last, int32_t* kept, void* workspace, size_t workspace_bytes, void* stream) {
+    Entry e(stream);
+    if (!cache_ok(from) || !cache_ok(to) || from->kv_heads != to->kv_heads || from->head_dim != to->head_dim) return e.fail("dev_q4_cache_evict: bad arguments (caches)");
+    if (!weight || !weight_to || !filled || !keep || keep > to->slots || keep_first > keep || keep_last > keep - keep_first)
+        return e.fail("dev_q4_cache_evict: bad arguments (1 <= keep <= slots, keep_first + keep_last <= keep)");
+    if (!workspace || !aligned16(workspace) || workspace_bytes < zen_cuda_q4_cache_evict_workspace_bytes(from))
+        return e.fail("dev_q4_cache_evict: the workspace is missing, not 16-byte aligned or too small");
+    const bool in_place = from->k_codes == to->k_codes && from->v_codes == to->v_codes && from->k_scales == to->k_scales && from->v_scales == to->v_scales &&
+                          weight == weight_to && from->slots == to->slots;
+    if (!in_place) {      // nothing that is read may be something that is written
+        auto spans = [](const zen_cuda_q4_cache& c, const float* w, Span* s) {
+            const size_t cells = size_t(c.kv_heads) * c.slots;
+            s[0] = span_of(c.k_codes, cells * (c.head_dim / 2)); s[1] = span_of(c.v_codes, cells * (c.head_dim / 2));
+            s[2] = span_of(c.k_scales, cells * (c.head_dim / 16)); s[3] = span_of(c.v_scales, cells * (c.head_dim / 16));
+            s[4] = span_of(w, cells * sizeof(float));
+        };
+        Span read[5], written[5];
+        spans(*from, weight, read);
+        spans(*to, weight_to, written);
+        for (const Span& r : read)
+            for (const Span& w : written)
+                if (!apart(r, w)) return e.fail("dev_q4_cache_evict: the two caches are neither the same nor apart");
+    }
+    if (!e.ok) return 0;
+    const zk::Q4Evict p{device_form(*from), device_form(*to), weight, weight_to, filled, kept, static_cast<int*>(workspace), u32(keep), u32(keep_first), u32(keep_last), e.d_error};
+    return e.leave(launch(e, zk::q4_evict_kernel, dim3(zk::kEvictCtas, from->kv_heads), dim3(zk::kEvictThreads), 0, 0, p), "dev_q4_cache_evict");
+}
+
+size_t zen_cuda_verify_drafts_workspace_bytes(const zen_cuda_draft_check* c) { return verify_room(c); }
+
+int zen_cuda_dev_verify_drafts(const zen_cuda_draft_check* c, void* stream) {
+    Entry e(stream);
+    const size_t room = verify_room(c);
+    if (!room) return e.fail("dev_verify_drafts: bad arguments (1 .. ZEN_CUDA_VERIFY_MAX_VOCAB entries, at most ZEN_CUDA_VERIFY_MAX_DRAFTS drafts)");
+    if (!c->logits || c->logits_ld < c->vocab || (c->drafts && !c->tokens) || !c->uniforms || !c->out || !c->accepted || !c->q_ids != !c->q_probs || !c->q_ids != !c->q_count)
+        return e.fail("dev_verify_drafts: bad arguments");
+    if (!(c->temperature >= 0.0f) || !std::isfinite(c->temperature) || std::isnan(c->top_p)) return e.fail("dev_verify_drafts: the temperature is finite and not negative");
+    if (!c->workspace || !aligned16(c->workspace) || c->workspace_bytes < room) return e.fail("dev_verify_drafts: the workspace is missing, not 16-byte aligned or too small");
+    if (!e.ok) return 0;
+    const uint32_t rows = c->drafts + 1;
+    zk::VerifyParams p{};
+    p.logits = c->logits; p.logits_ld = c->logits_ld; p.vocab = c->vocab; p.drafts = c->drafts;
+    p.tokens = reinterpret_cast<const long long*>(c->tokens); p.q_ids = c->q_ids; p.q_probs = c->q_probs; p.q_count = c->q_count; p.uniforms = c->uniforms;
+    p.temperature = c->temperature; p.top_k = c->top_k; p.top_p = c->top_p;
+    p.out = reinterpret_cast<long long*>(c->out); p.accepted = c->accepted; p.probs = c->probs;
+    p.draws = static_cast<long long*>(c->workspace); p.fits = reinterpret_cast<int*>(p.draws + rows); p.error_word = e.d_error;
+    auto run = [&](auto ctas) {
+        constexpr int kCtas = decltype(ctas)::value;
+        p.per_cta = (c->vocab + kCtas - 1) / kCtas;
+        p.per_cta = (p.per_cta + 3) & ~3u;
+        return launch(e, zk::verify_rows_kernel<kCtas>, dim3(kCtas, rows), dim3(zk::kVerifyThreads), size_t(p.per_cta) * 12, kCtas, p);
+    };
+    // sixteen CTAs a row where a run of eight would not fit shared memory
+    const cudaError_t r = c->vocab > 8 * 18000 ? run(std::integral_constant<int, 16>{}) : run(std::integral_constant<int, 8>{});
+    if (!e.leave(r, "dev_verify_drafts")) return 0;
+    return e.leave(launch(e, zk::verify_answer_kernel, dim3(1), dim3(32), 0, 0, p), "dev_verify_drafts: answer");
+}
+
+}  // extern "C"
