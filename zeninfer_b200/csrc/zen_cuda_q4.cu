@@ -68,10 +68,44 @@ zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
     return zk::Q4Cache{c.k_codes, c.v_codes, reinterpret_cast<__half*>(c.k_scales), reinterpret_cast<__half*>(c.v_scales), c.kv_heads, c.head_dim / zk::kQ4Block, c.slots};
 }
 
-// The workspace of a call, or 0 when its sizes are none.
-size_t attention_room(const zen_cuda_q4_attention* a, size_t tokens) {
-    if (!a || !cache_ok(&a->cache) || !a->heads || a->heads % a->cache.kv_heads || a->heads > 65535 || !tokens || tokens > a->cache.slots) return 0;
-    return up16(tokens * a->heads * 2 * sizeof(float));
+constexpr size_t kWaveCtas = 2 * 148;      // two CTAs on every SM
+
+// How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
+struct AttentionPlan {
+    int columns{};
+    uint32_t rows{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{};
+    bool keep_scores{}, keep_queries{};
+    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
+};
+uint32_t query_quads(uint32_t blocks) { return (blocks * 10 + 2 + 3) / 4; }
+AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
+    AttentionPlan n;
+    if (!a || !cache_ok(&a->cache) || !a->heads || a->heads % a->cache.kv_heads || a->heads > 65535 || !tokens || tokens > a->cache.slots) return n;
+    const size_t kv_heads = a->cache.kv_heads, rows = tokens * (a->heads / kv_heads), blocks = a->cache.head_dim / zk::kQ4Block, tiles = a->cache.slots / zk::kQ4Tile;
+    n.columns = rows <= 4 ? zk::kQ4Digits : rows <= 8 || blocks > 4 ? zk::kQ4Rows8 : zk::kQ4Rows16;
+    const size_t per_warp = zk::q4_rows(n.columns), warps = zk::q4_warps(n.columns);
+    size_t row_warps = 1;
+    while (row_warps < warps && row_warps * per_warp < rows) row_warps *= 2;
+    const size_t cta_rows = row_warps * per_warp, row_ctas = (rows + cta_rows - 1) / cta_rows;
+    if (row_ctas > 65535) return n;
+    n.rows = u32(rows); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas); n.key_warps = u32(warps / row_warps);
+    // runs of slots side by side until every SM has its CTAs, no run shorter than a tile a warp
+    n.splits = u32(std::max<size_t>(1, std::min(kWaveCtas / (row_ctas * kv_heads), tiles / n.key_warps)));
+    n.keep_scores = rows <= 32;
+    n.keep_queries = !n.keep_scores;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
+    if (n.splits > 1) {
+        n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
+        n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
+    }
+    n.stats = take(kv_heads * rows * sizeof(float));
+    if (a->weight_out) {
+        if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
+        else n.queries = take(kv_heads * ((rows + 7) / 8) * query_quads(u32(blocks)) * 32 * sizeof(uint4));
+    }
+    n.bytes = at;
+    return n;
 }
 
 template <typename Run>
@@ -103,30 +137,56 @@ size_t verify_room(const zen_cuda_draft_check* c) {
 
 extern "C" {
 
-size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens) { return attention_room(a, tokens); }
+size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens) { return attention_plan(a, tokens).bytes; }
 
 int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, const float* d_k, const float* d_v, size_t tokens, float* d_out,
                               void* stream) {
     Entry e(stream);
-    const size_t room = attention_room(a, tokens);
-    if (!room) return e.fail("dev_q4_attention: bad arguments (head_dim a multiple of 32 up to 256, slots a multiple of 32, heads a multiple of kv_heads, 1 .. slots tokens)");
+    const AttentionPlan plan = attention_plan(a, tokens);
+    if (!plan.bytes) return e.fail("dev_q4_attention: bad arguments (head_dim a multiple of 32 up to 256, slots a multiple of 32, heads a multiple of kv_heads, 1 .. slots tokens)");
     const size_t q_row = size_t(a->heads) * a->cache.head_dim, kv_row = size_t(a->cache.kv_heads) * a->cache.head_dim;
     if (!d_q || !d_k || !d_v || !d_out || !a->filled || (a->q_ld && a->q_ld < q_row) || (a->kv_ld && a->kv_ld < kv_row) || !std::isfinite(a->scale))
         return e.fail("dev_q4_attention: bad arguments (rows)");
     if (a->pairs && (a->pairs > a->cache.head_dim / 2 || !a->cos_t || !a->sin_t || !a->position || !a->positions)) return e.fail("dev_q4_attention: bad arguments (rotation)");
     if (!a->weight_in != !a->weight_out) return e.fail("dev_q4_attention: weight_in and weight_out go together");
-    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < room) return e.fail("dev_q4_attention: the workspace is missing, not 16-byte aligned or too small");
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < plan.bytes) return e.fail("dev_q4_attention: the workspace is missing, not 16-byte aligned or too small");
     if (!e.ok) return 0;
     const zk::Q4Rotation turn{a->cos_t, a->sin_t, a->pairs, a->positions, a->adjacent ? 1u : 0u};
     const zk::Q4Cache cache = device_form(a->cache);
     const zk::Q4Append append{cache, turn, d_k, d_v, a->position, a->filled, a->k_held, a->v_held, u32(tokens), a->kv_ld ? a->kv_ld : kv_row, e.d_error};
     if (!e.leave(launch(e, zk::q4_append_kernel, dim3(u32(tokens), cache.kv_heads), dim3(64 * cache.blocks), 0, 0, append), "dev_q4_attention: append")) return 0;
-    const zk::Q4Attend p{cache, turn, d_q, a->position, a->filled, a->weight_in, a->weight_out, d_out, static_cast<float*>(a->workspace), u32(tokens), a->heads,
-                         a->q_ld ? a->q_ld : q_row, a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale, e.d_error};
-    const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) { return launch(e, zk::q4_attend_kernel<decltype(blocks)::value>, dim3(u32(tokens), a->heads), dim3(256), 0, 0, p); });
-    if (!e.leave(r, "dev_q4_attention") || !a->weight_out) return r == cudaSuccess;
-    return e.leave(by_blocks(cache.blocks, [&](auto blocks) { return launch(e, zk::q4_received_kernel<decltype(blocks)::value>, dim3(cache.slots / 8, cache.kv_heads), dim3(256), 0, 0, p); }),
-                   "dev_q4_attention: weights");
+    uint8_t* room = static_cast<uint8_t*>(a->workspace);
+    zk::Q4Attend p{};
+    p.cache = cache; p.turn = turn; p.q = d_q; p.position = a->position; p.filled = a->filled; p.weight_in = a->weight_in; p.weight_out = a->weight_out; p.out = d_out;
+    p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps;
+    p.q_ld = a->q_ld ? a->q_ld : q_row; p.scale = a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale; p.error_word = e.d_error;
+    if (plan.splits > 1) { p.part_out = reinterpret_cast<float*>(room + plan.part_out); p.part_stats = reinterpret_cast<float*>(room + plan.part_stats); }
+    if (a->weight_out) {
+        p.stats = reinterpret_cast<float*>(room + plan.stats);
+        if (plan.keep_scores) p.scores = reinterpret_cast<float*>(room + plan.scores);
+        else p.queries = reinterpret_cast<uint4*>(room + plan.queries);
+    }
+    const dim3 grid(plan.splits, plan.row_ctas, cache.kv_heads);
+    auto attend = [&](auto blocks, auto columns) {
+        constexpr int kBlocks = decltype(blocks)::value, kColumns = decltype(columns)::value;
+        return launch(e, zk::q4_attend_kernel<kBlocks, kColumns>, grid, dim3(zk::q4_warps(kColumns) * 32), zk::q4_attend_smem<kBlocks, kColumns>(plan.row_warps), 0, p);
+    };
+    const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) {
+        if (plan.columns == zk::kQ4Digits) return attend(blocks, std::integral_constant<int, zk::kQ4Digits>{});
+        if constexpr (decltype(blocks)::value <= 4) {
+            if (plan.columns == zk::kQ4Rows16) return attend(blocks, std::integral_constant<int, zk::kQ4Rows16>{});
+        }
+        return attend(blocks, std::integral_constant<int, zk::kQ4Rows8>{});
+    });
+    if (!e.leave(r, "dev_q4_attention")) return 0;
+    if (plan.splits > 1 && !e.leave(launch(e, zk::q4_join_kernel, dim3(plan.rows, cache.kv_heads), dim3(cache.blocks * 32), 0, 0, p, plan.cta_rows, plan.key_warps), "dev_q4_attention: join")) return 0;
+    if (!a->weight_out) return 1;
+    if (plan.keep_scores) return e.leave(launch(e, zk::q4_received_kernel, dim3((cache.slots + 255) / 256, cache.kv_heads), dim3(256), 0, 0, p), "dev_q4_attention: weights");
+    return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
+        constexpr int kBlocks = decltype(blocks)::value;
+        return launch(e, zk::q4_received_again_kernel<kBlocks>, dim3(zk::kReceivedCtas, (cache.slots + zk::kReceivedSlots - 1) / zk::kReceivedSlots, cache.kv_heads), dim3(zk::kReceivedWarps * 32),
+                      zk::kReceivedStages * zk::Q4Query<kBlocks, zk::kQ4Rows8>::kQuads * 512, 0, p);
+    }), "dev_q4_attention: weights");
 }
 
 size_t zen_cuda_q4_cache_evict_workspace_bytes(const zen_cuda_q4_cache* from) {
