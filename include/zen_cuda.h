@@ -713,7 +713,7 @@ int zen_cuda_dev_q4_cache_evict(const zen_cuda_q4_cache* from, const float* weig
  * All pointers are device memory; drafts <= ZEN_CUDA_VERIFY_MAX_DRAFTS (0: one row is sampled), vocab <= ZEN_CUDA_VERIFY_MAX_VOCAB.  A draft outside the vocabulary raises code
  * 6 and is not accepted.  The workspace is as the attention's above. */
 #define ZEN_CUDA_VERIFY_MAX_DRAFTS 64
-#define ZEN_CUDA_VERIFY_MAX_VOCAB 300000
+#define ZEN_CUDA_VERIFY_MAX_VOCAB 262144
 typedef struct zen_cuda_draft_check {
     const float* logits;
     size_t logits_ld;

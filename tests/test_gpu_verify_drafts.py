@@ -72,7 +72,7 @@ def draft_rows(rng, logits, drafts, kept, temperature):
     return q
 
 
-@pytest.mark.parametrize("drafts,vocab", [(0, 50), (1, 1), (1, 2), (1, 33), (2, 1000), (4, 8191), (8, 32000), (3, 128256), (33, 777), (64, 501), (2, 200003), (1, 300000)])
+@pytest.mark.parametrize("drafts,vocab", [(0, 50), (1, 1), (1, 2), (1, 33), (2, 1000), (4, 8191), (8, 32000), (3, 128256), (33, 777), (64, 501), (2, 200003), (1, 262144)])
 @pytest.mark.parametrize("filters", [(1.0, 0, 1.0), (0.0, 0, 1.0), (0.7, 40, 1.0), (1.3, 0, 0.9), (0.8, 50, 0.8), (1.0, 5000, 0.99), (1.0, 1, 0.5), (5.0, 0, 1e-6)], ids=str)
 @pytest.mark.parametrize("listed", [False, True])
 def test_against_the_plain_rule(be, drafts, vocab, filters, listed):

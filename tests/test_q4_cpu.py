@@ -77,7 +77,7 @@ def test_eviction_refusals(lib):
 def test_verify_refusals(lib):
     good = dict(logits=16, logits_ld=100, vocab=100, drafts=2, tokens=16, uniforms=16, temperature=1.0, top_k=0, top_p=1.0, out=16, accepted=16, workspace=16, workspace_bytes=1 << 20)
     assert lib.zen_cuda_verify_drafts_workspace_bytes(DraftCheck(**good)) > 0
-    for bad in (dict(vocab=0), dict(vocab=300001, logits_ld=300001), dict(drafts=65)):
+    for bad in (dict(vocab=0), dict(vocab=262145, logits_ld=262145), dict(drafts=65)):
         assert lib.zen_cuda_verify_drafts_workspace_bytes(DraftCheck(**{**good, **bad})) == 0
         assert "bad arguments" in refused(lib, lib.zen_cuda_dev_verify_drafts(DraftCheck(**{**good, **bad}), None))
     for bad in (dict(logits=0), dict(logits_ld=99), dict(tokens=0), dict(uniforms=0), dict(out=0), dict(accepted=0), dict(q_ids=16), dict(q_ids=16, q_probs=16), dict(q_count=16)):

@@ -556,18 +556,30 @@ __global__ void __launch_bounds__(256) q4_join_kernel(const __grid_constant__ Q4
     const uint32_t last_row = min(rows, (row / cta_rows + 1) * cta_rows) - 1;
     const uint32_t active = q4_runs(static_cast<uint32_t>(filled) + last_row / p.group + 1, p.splits, key_warps).active;
     const size_t first = static_cast<size_t>(h) * p.splits * rows + row;
-    float top = -INFINITY;
-    for (uint32_t s = 0; s < active; ++s) top = fmaxf(top, __ldcg(p.part_stats + 2 * (first + static_cast<size_t>(s) * rows)));
-    float sum = 0.0f, o = 0.0f;
-    for (uint32_t s = 0; s < active; ++s) {
-        const size_t part = first + static_cast<size_t>(s) * rows;
-        const float2 its = __ldcg(reinterpret_cast<const float2*>(p.part_stats) + part);
-        const float by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
-        sum += by * its.y;
-        if (threadIdx.x < dim) o += by * __ldcg(p.part_out + part * dim + threadIdx.x);
+    // every warp has all the runs' maxima and sums, a run a lane, and the runs' outputs are asked for eight at a time: two round trips
+    const uint32_t lane = threadIdx.x & 31u;
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t s = lane; s < active; s += 32) top = fmaxf(top, __ldcg(p.part_stats + 2 * (first + static_cast<size_t>(s) * rows)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float o = 0.0f;
+    for (uint32_t s0 = 0; s0 < active; s0 += 32) {
+        float by = 0.0f;
+        if (s0 + lane < active) {
+            const float2 its = __ldcg(reinterpret_cast<const float2*>(p.part_stats) + first + static_cast<size_t>(s0 + lane) * rows);
+            by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
+            sum += by * its.y;
+        }
+        const uint32_t count = min(32u, active - s0);
+        const float* from = p.part_out + (first + static_cast<size_t>(s0) * rows) * dim + threadIdx.x;
+        const size_t step = static_cast<size_t>(rows) * dim;
+#pragma unroll 8
+        for (uint32_t s = 0; s < count; ++s) o += __shfl_sync(0xffffffffu, by, s) * __ldcg(from + s * step);
     }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const uint32_t token = row / p.group, head = h * p.group + row % p.group;
-    if (threadIdx.x < dim) p.out[(static_cast<size_t>(token) * p.heads + head) * dim + threadIdx.x] = o / sum;
+    p.out[(static_cast<size_t>(token) * p.heads + head) * dim + threadIdx.x] = o / sum;
     if (threadIdx.x == 0) {
         if (!(sum > 0.0f) || !(sum < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
         if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = top + log2f(sum);

@@ -6,10 +6,15 @@
 //
 // A cluster takes a row and a CTA a run of the vocabulary, its logits and exponentials in shared memory.  Every row decides its own draft AND draws its
 // own replacement, as if all drafts before it had been accepted, so that nothing waits for a decision: the rows run side by side, and one warp
-// puts their answers together in a second launch.  The cuts are radix selects over order-preserving keys, four passes of eight bits: top_k over
-// counts, top_p over masses.  A mass is an integer, the exponential times 2^62 / sum, so that its sums do not depend on the order in which
-// threads add to a bin; sums of exponentials are added in a fixed order.
-// What bounds it: about thirty double-precision instructions an entry for exp, and a dozen cluster barriers.
+// puts their answers together in a second launch.
+//
+// The cuts (top_k over counts, top_p over masses) look for the entry, in descending order, at which a sum of weights is reached.  The range of values is divided into
+// 1024 equal bins, which spreads logits far better than the bits of their keys do (eight bits of a key put most of a row into five bins, and
+// its threads queued up there: 290 us for 9 rows of 128256); the bin of the border is divided again while it holds more than a list
+// takes, and the entries of the list are compared with each other, equal values by id.  A mass is an integer, the exponential's 2^-51ths of the
+// row's sum, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
+// added in a fixed order.
+// What bounds it: the double-precision instructions of exp, and a dozen cluster barriers.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -20,8 +25,17 @@
 
 namespace zk {
 
-constexpr int kVerifyThreads = 1024;
-constexpr double kVerifyUnit = 4611686018427387904.0;      // 2^62: the mass of a whole row
+constexpr int kVerifyThreads = 1024, kVerifyLimbs = 3, kVerifyLimbBits = 17, kVerifyMine = 256, kVerifyAll = 1024;
+constexpr uint32_t kVerifyBins = 1024, kVerifyRun = 16384;          // entries a CTA takes at most
+constexpr double kVerifyUnit = 2251799813685248.0;                  // 2^51: the mass of a whole row
+
+struct VerifyEntry {
+    unsigned long long weight;
+    float value;
+    uint32_t id;
+};
+// Dynamic shared memory: exponentials and logits of the CTA's run, the bins' limbs, the CTA's and the row's entries at the border.
+__host__ __device__ constexpr uint32_t verify_smem_bytes(uint32_t per_cta) { return per_cta * 12 + kVerifyLimbs * kVerifyBins * 4 + (kVerifyMine + kVerifyAll) * 16; }
 
 struct VerifyParams {
     const float* logits;       // rows logits_ld apart
@@ -45,11 +59,9 @@ struct VerifyParams {
 
 // What a CTA hands to the others.
 struct VerifyShare {
-    uint32_t hist[256];
-    unsigned long long mass[256];
     double sum;
     unsigned long long ties;
-    uint32_t top_key, count;
+    uint32_t top_key, low_key, count;
 };
 
 template <int kCtas>
@@ -57,19 +69,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) uint8_t verify_smem[];
     __shared__ VerifyShare share;
-    __shared__ unsigned long long total[256];
     __shared__ double warp_sum[32], s_q;
-    __shared__ uint32_t warp_count[32];
-    __shared__ uint32_t s_prefix;
-    __shared__ unsigned long long s_left;
-    __shared__ int s_winner;
+    __shared__ unsigned long long warp_total[32], s_left;
+    __shared__ uint32_t warp_count[32], s_bin, s_mine;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), row = blockIdx.y;
     double* e = reinterpret_cast<double*>(verify_smem);                      // [per_cta]
-    float* v = reinterpret_cast<float*>(e + p.per_cta);                      // [per_cta]
+    float* v = reinterpret_cast<float*>(e + p.per_cta);                      // [per_cta], per_cta a multiple of four
+    uint32_t* limbs = reinterpret_cast<uint32_t*>(v + p.per_cta);            // [kVerifyLimbs][kVerifyBins]
+    VerifyEntry* own_list = reinterpret_cast<VerifyEntry*>(limbs + kVerifyLimbs * kVerifyBins);
+    VerifyEntry* all_list = own_list + kVerifyMine;
     const uint32_t base = rank * p.per_cta, n = base < p.vocab ? min(p.per_cta, p.vocab - base) : 0u;
-    // a thread's run of consecutive entries, for sums in order of id
-    const uint32_t per_thread = (p.per_cta + kVerifyThreads - 1) / kVerifyThreads, begin = min(n, tid * per_thread), end = min(n, begin + per_thread);
+    // a thread's run of consecutive entries, for sums in order of id (an odd number of them: no two lanes of a warp on one bank)
+    const uint32_t per_thread = ((p.per_cta + kVerifyThreads - 1) / kVerifyThreads) | 1u, begin = min(n, tid * per_thread), end = min(n, begin + per_thread);
     pdl_launch_dependents();
     pdl_wait();
     const float* logits = p.logits + row * p.logits_ld + base;
@@ -126,67 +138,24 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         return;
     }
     const double highest = __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
-
-    // The first entries in descending order whose weight reaches `wanted`: their last key, and the weight of those that equal it which is
-    // still wanted.  weigh(i): an entry's weight, 0 for one that does not take part.
-    uint32_t border = 0;
-    auto select = [&](unsigned long long wanted, auto weigh) {
-        if (tid == 0) { s_prefix = 0; s_left = wanted; }
-        uint32_t mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) share.mass[tid] = 0;
-            __syncthreads();
-            const uint32_t prefix = s_prefix;
-            for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-                const uint32_t key = sample_key(v[i]);
-                const unsigned long long w = key && (key & mask) == prefix ? weigh(i) : 0ull;
-                if (w) atomicAdd(&share.mass[(key >> shift) & 255u], w);
-            }
-            cluster.sync();
-            if (tid < 256) {
-                unsigned long long sum = 0;
-                for (int r = 0; r < kCtas; ++r) sum += cluster.map_shared_rank(&share, r)->mass[tid];
-                total[tid] = sum;
-            }
-            cluster.sync();
-            if (warp == 0) {
-                unsigned long long mine = 0;
-                for (int j = 0; j < 8; ++j) mine += total[255 - 8 * lane - j];
-                unsigned long long upto = mine;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (static_cast<int>(lane) >= o) upto += x;
-                }
-                const unsigned long long left = s_left;
-                uint32_t reached = __ballot_sync(0xffffffffu, upto >= left);
-                // rounding may leave the whole a hair short of what is wanted: then the last bin that has any
-                const uint32_t any = __ballot_sync(0xffffffffu, mine != 0ull);
-                const int at = reached ? __ffs(reached) - 1 : 31 - __clz(any);
-                if (static_cast<int>(lane) == at) {
-                    unsigned long long rest = left - (upto - mine);
-                    int bin = 255 - 8 * static_cast<int>(lane), last = bin;
-                    for (int j = 0; j < 8; ++j, --bin) {
-                        if (!total[bin]) continue;
-                        last = bin;
-                        if (total[bin] >= rest) break;
-                        rest -= total[bin];
-                    }
-                    if (total[last] < rest || !reached) rest = total[last];
-                    s_prefix = prefix | static_cast<uint32_t>(last) << shift;
-                    s_left = rest;
-                }
-            }
-            __syncthreads();
-            mask |= 255u << shift;
-        }
-        border = s_prefix;
-        const unsigned long long left = s_left;
-        __syncthreads();
-        return left;
+    auto drop = [&](uint32_t i, bool with_exponentials) {
+        v[i] = NAN;
+        if (with_exponentials) e[i] = 0.0;
     };
-    // Entries that equal the border's key and come behind the first `ties` of them (in order of id) go: their value becomes NaN, the exponential 0;
-    // so do all below the border.
-    auto cut = [&](unsigned long long ties, bool with_exponentials) {
+    // the largest and the smallest key of the entries that take part, over the cluster
+    auto key_range = [&](uint32_t& high, uint32_t& low) {
+        high = __reduce_max_sync(0xffffffffu, high);
+        low = __reduce_min_sync(0xffffffffu, low);
+        if (tid == 0) { share.top_key = 0; share.low_key = 0xffffffffu; }
+        __syncthreads();
+        if (lane == 0) { atomicMax(&share.top_key, high); atomicMin(&share.low_key, low); }
+        cluster.sync();
+        for (int r = 0; r < kCtas; ++r) { high = max(high, cluster.map_shared_rank(&share, r)->top_key); low = min(low, cluster.map_shared_rank(&share, r)->low_key); }
+        cluster.sync();
+    };
+    auto value_of = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); };
+    // Of the entries that equal `border` all behind the first `ties` (in order of id) go, and so do all below it.
+    auto cut_ties = [&](uint32_t border, unsigned long long ties, bool with_exponentials) {
         uint32_t equal = 0;
         for (uint32_t i = begin; i < end; ++i) equal += sample_key(v[i]) == border;
         uint32_t upto = equal;
@@ -205,18 +174,143 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         cluster.sync();
         for (uint32_t i = begin; i < end; ++i) {
             const uint32_t key = sample_key(v[i]);
-            if (key < border || (key == border && seen++ >= ties)) {
-                v[i] = NAN;
-                if (with_exponentials) e[i] = 0.0;
-            }
+            if (key < border || (key == border && seen++ >= ties)) drop(i, with_exponentials);
         }
         __syncthreads();
+    };
+    // Leaves the shortest run of entries, in descending order (equal values: the lowest ids), whose weights reach `wanted` > 0, at least one.
+    // weigh(i): an entry's weight.  low: no entry that takes part is below it.
+    auto cut = [&](unsigned long long wanted, auto weigh, uint32_t low, double reach, bool with_exponentials) {
+        uint32_t high = top;
+        double v_low = fmax(static_cast<double>(value_of(low)), highest - reach);       // far below, nothing is worth bins of its own
+        for (;;) {
+            if (high == low) {         // equal values: so many of them as are wanted, each of the same weight
+                if (tid == 0) share.count = 0;
+                __syncthreads();
+                unsigned long long each = 0;
+                for (uint32_t i = tid; i < n; i += kVerifyThreads) if (sample_key(v[i]) == high) each = weigh(i);
+                if (each) atomicExch(&s_left, each);
+                if (each && !share.count) share.count = 1;
+                cluster.sync();
+                for (int r = 0; r < kCtas; ++r) if (cluster.map_shared_rank(&share, r)->count) each = *cluster.map_shared_rank(&s_left, r);
+                cluster.sync();
+                each = max(each, 1ull);
+                cut_ties(high, (wanted + each - 1) / each, with_exponentials);
+                return;
+            }
+            const double v_high = value_of(high), per = kVerifyBins / (v_high - v_low);
+            auto bin_of = [&](float x) { return static_cast<uint32_t>(fmin((v_high - static_cast<double>(x)) * per, kVerifyBins - 1.0)); };
+            for (uint32_t i = tid; i < kVerifyLimbs * kVerifyBins; i += kVerifyThreads) limbs[i] = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < n; i += kVerifyThreads) {
+                const uint32_t key = sample_key(v[i]);
+                if (!key || key > high || key < low) continue;
+                const unsigned long long w = weigh(i);
+                const uint32_t bin = bin_of(v[i]);
+#pragma unroll
+                for (int k = 0; k < kVerifyLimbs; ++k) {
+                    uint32_t limb = static_cast<uint32_t>(w >> (k * kVerifyLimbBits));
+                    if (k + 1 < kVerifyLimbs) limb &= (1u << kVerifyLimbBits) - 1u;          // an entry may be all of the row: 2^51
+                    if (limb) atomicAdd(limbs + k * kVerifyBins + bin, limb);
+                }
+            }
+            cluster.sync();
+            // thread j has bin j of the whole row
+            unsigned long long mine = 0;
+            for (int r = 0; r < kCtas; ++r) {
+                const uint32_t* its = cluster.map_shared_rank(limbs, r) + tid;
+#pragma unroll
+                for (int k = 0; k < kVerifyLimbs; ++k) mine += static_cast<unsigned long long>(its[k * kVerifyBins]) << (k * kVerifyLimbBits);
+            }
+            unsigned long long upto = mine;
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (static_cast<int>(lane) >= o) upto += x;
+            }
+            if (lane == 31) warp_total[warp] = upto;
+            if (tid == 0) { s_bin = 0xffffffffu; s_left = wanted; s_mine = 0; }
+            __syncthreads();
+            unsigned long long before = 0;
+            for (uint32_t w = 0; w < warp; ++w) before += warp_total[w];
+            upto += before;
+            if (upto >= wanted && upto - mine < wanted) { s_bin = tid; s_left = wanted - (upto - mine); }        // one thread at most
+            cluster.sync();                                                                                       // and everybody has read the limbs
+            if (s_bin == 0xffffffffu) {      // rounding left the whole short of what is wanted: everything stays
+                for (uint32_t i = tid; i < n; i += kVerifyThreads) if (sample_key(v[i]) < low) drop(i, with_exponentials);
+                cluster.sync();
+                return;
+            }
+            const uint32_t border = s_bin;
+            wanted = s_left;
+            // what lies below the border goes; the entries of its bin are listed, and counted on where there are too many
+            uint32_t bin_high = 0, bin_low = 0xffffffffu;
+            for (uint32_t i = tid; i < n; i += kVerifyThreads) {
+                const uint32_t key = sample_key(v[i]);
+                if (!key || key > high) continue;
+                const uint32_t bin = key < low ? kVerifyBins : bin_of(v[i]);
+                if (bin > border) drop(i, with_exponentials);
+                if (bin != border) continue;
+                bin_high = max(bin_high, key);
+                bin_low = min(bin_low, key);
+                const uint32_t at = atomicAdd(&s_mine, 1u);
+                if (at < kVerifyMine) own_list[at] = VerifyEntry{weigh(i), v[i], base + i};
+            }
+            __syncthreads();
+            if (tid == 0) share.count = s_mine;
+            cluster.sync();
+            uint32_t count = 0, before_mine = 0;
+            bool fits = true;
+            for (uint32_t r = 0; r < kCtas; ++r) {
+                const uint32_t its = cluster.map_shared_rank(&share, r)->count;
+                fits &= its <= kVerifyMine;
+                if (r < rank) before_mine += its;
+                count += its;
+            }
+            if (!fits || count > kVerifyAll) {
+                cluster.sync();
+                key_range(bin_high, bin_low);
+                high = bin_high;
+                low = bin_low;
+                v_low = value_of(low);
+                continue;
+            }
+            for (uint32_t r = 0, at = 0; r < kCtas; ++r) {
+                const uint32_t its = cluster.map_shared_rank(&share, r)->count;
+                if (tid < its) all_list[at + tid] = cluster.map_shared_rank(own_list, r)[tid];
+                at += its;
+            }
+            cluster.sync();
+            // a warp decides an entry of the CTA's: it stays when what comes before it does not reach what is wanted
+            for (uint32_t i = warp; i < s_mine; i += 32) {
+                const VerifyEntry me = all_list[before_mine + i];
+                unsigned long long sum = 0;
+                for (uint32_t j = lane; j < count; j += 32) {
+                    const VerifyEntry its = all_list[j];
+                    if (its.value > me.value || (its.value == me.value && its.id < me.id)) sum += its.weight;
+                }
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0 && sum >= wanted) drop(me.id - base, with_exponentials);
+            }
+            __syncthreads();
+            return;
+        }
     };
 
     const bool greedy = p.temperature == 0.0;
     const uint32_t top_k = greedy ? 1u : p.top_k;
     const double temperature = greedy ? 1.0 : p.temperature;
-    if (top_k && top_k < finite) cut(select(top_k, [](uint32_t) { return 1ull; }), false);
+    // the smallest key of a row is asked for once, by its first cut
+    uint32_t least = 0xffffffffu;
+    auto least_key = [&]() {
+        for (uint32_t i = tid; i < n; i += kVerifyThreads) {
+            const uint32_t key = sample_key(v[i]);
+            if (key) least = min(least, key);
+        }
+        uint32_t ignored = 0;
+        key_range(ignored, least);
+        return least;
+    };
+    if (top_k && top_k < finite) cut(top_k, [](uint32_t) { return 1ull; }, least_key(), 64.0 * temperature, false);
     double mine = 0.0;
     for (uint32_t i = begin; i < end; ++i) {
         const float x = v[i];
@@ -227,12 +321,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     double sum = cluster_sum(mine);
     if (!greedy && p.top_p > 0.0f && p.top_p < 1.0f) {
         const double unit = kVerifyUnit / sum;
-        auto weigh = [&](uint32_t i) { return static_cast<unsigned long long>(__double2ll_rn(e[i] * unit)); };
-        const unsigned long long wanted = max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit));
-        const unsigned long long rest = select(wanted, weigh);
-        const float at = __uint_as_float(border & 0x80000000u ? border & 0x7fffffffu : ~border);
-        const unsigned long long each = max(1ll, __double2ll_rn(exp((static_cast<double>(at) - highest) / temperature) * unit));
-        cut((rest + each - 1) / each, true);
+        least = 0xffffffffu;
+        cut(max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit)), [&](uint32_t i) { return static_cast<unsigned long long>(__double2ll_rn(e[i] * unit)); }, least_key(),
+            64.0 * temperature, true);
         mine = 0.0;
         for (uint32_t i = begin; i < end; ++i) mine += e[i];
         sum = cluster_sum(mine);
@@ -292,10 +383,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         if (static_cast<int>(lane) >= o) upto += x;
     }
     if (lane == 31) warp_sum[warp] = upto;
-    if (tid == 0) s_winner = 0x7fffffff;
     __syncthreads();
-    double before = upto - left;                    // replaced below by sums in a fixed order
-    before = __shfl_up_sync(0xffffffffu, upto, 1);
+    double before = __shfl_up_sync(0xffffffffu, upto, 1);
     if (lane == 0) before = 0.0;
     double warps = 0.0;
     for (uint32_t w = 0; w < warp; ++w) warps += warp_sum[w];

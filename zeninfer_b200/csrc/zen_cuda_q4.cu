@@ -244,10 +244,11 @@ int zen_cuda_dev_verify_drafts(const zen_cuda_draft_check* c, void* stream) {
         constexpr int kCtas = decltype(ctas)::value;
         p.per_cta = (c->vocab + kCtas - 1) / kCtas;
         p.per_cta = (p.per_cta + 3) & ~3u;
-        return launch(e, zk::verify_rows_kernel<kCtas>, dim3(kCtas, rows), dim3(zk::kVerifyThreads), size_t(p.per_cta) * 12, kCtas, p);
+        return launch(e, zk::verify_rows_kernel<kCtas>, dim3(kCtas, rows), dim3(zk::kVerifyThreads), zk::verify_smem_bytes(p.per_cta), kCtas, p);
     };
+    static_assert(ZEN_CUDA_VERIFY_MAX_VOCAB == 16 * zk::kVerifyRun, "what sixteen CTAs take");
     // sixteen CTAs a row where a run of eight would not fit shared memory
-    const cudaError_t r = c->vocab > 8 * 18000 ? run(std::integral_constant<int, 16>{}) : run(std::integral_constant<int, 8>{});
+    const cudaError_t r = c->vocab > 8 * zk::kVerifyRun ? run(std::integral_constant<int, 16>{}) : run(std::integral_constant<int, 8>{});
     if (!e.leave(r, "dev_verify_drafts")) return 0;
     return e.leave(launch(e, zk::verify_answer_kernel, dim3(1), dim3(32), 0, 0, p), "dev_verify_drafts: answer");
 }
