@@ -75,9 +75,8 @@ struct AttentionPlan {
     int columns{};
     uint32_t rows{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{};
     bool keep_scores{}, keep_queries{};
-    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
+    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
 };
-uint32_t query_quads(uint32_t blocks) { return (blocks * 10 + 2 + 3) / 4; }
 AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     AttentionPlan n;
     if (!a || !cache_ok(&a->cache) || !a->heads || a->heads % a->cache.kv_heads || a->heads > 65535 || !tokens || tokens > a->cache.slots) return n;
@@ -102,7 +101,10 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     n.stats = take(kv_heads * rows * sizeof(float));
     if (a->weight_out) {
         if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
-        else n.queries = take(kv_heads * ((rows + 7) / 8) * query_quads(u32(blocks)) * 32 * sizeof(uint4));
+        else {
+            n.queries = take(kv_heads * ((rows + 7) / 8) * blocks * 64 * sizeof(uint4));
+            n.factors = take(kv_heads * rows * sizeof(float));
+        }
     }
     n.bytes = at;
     return n;
@@ -164,7 +166,7 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     if (a->weight_out) {
         p.stats = reinterpret_cast<float*>(room + plan.stats);
         if (plan.keep_scores) p.scores = reinterpret_cast<float*>(room + plan.scores);
-        else p.queries = reinterpret_cast<uint4*>(room + plan.queries);
+        else { p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = reinterpret_cast<float*>(room + plan.factors); }
     }
     const dim3 grid(plan.splits, plan.row_ctas, cache.kv_heads);
     auto attend = [&](auto blocks, auto columns) {
@@ -179,13 +181,13 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
         return attend(blocks, std::integral_constant<int, zk::kQ4Rows8>{});
     });
     if (!e.leave(r, "dev_q4_attention")) return 0;
-    if (plan.splits > 1 && !e.leave(launch(e, zk::q4_join_kernel, dim3(plan.rows, cache.kv_heads), dim3(cache.blocks * 32), 0, 0, p, plan.cta_rows, plan.key_warps), "dev_q4_attention: join")) return 0;
+    if (plan.splits > 1 && !e.leave(launch(e, zk::q4_join_kernel, dim3(plan.rows, cache.kv_heads), dim3(zk::kQ4JoinSlices * cache.blocks * 32), 0, 0, p, plan.cta_rows, plan.key_warps), "dev_q4_attention: join")) return 0;
     if (!a->weight_out) return 1;
     if (plan.keep_scores) return e.leave(launch(e, zk::q4_received_kernel, dim3((cache.slots + 255) / 256, cache.kv_heads), dim3(256), 0, 0, p), "dev_q4_attention: weights");
     return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
         constexpr int kBlocks = decltype(blocks)::value;
         return launch(e, zk::q4_received_again_kernel<kBlocks>, dim3(zk::kReceivedCtas, (cache.slots + zk::kReceivedSlots - 1) / zk::kReceivedSlots, cache.kv_heads), dim3(zk::kReceivedWarps * 32),
-                      zk::kReceivedStages * zk::Q4Query<kBlocks, zk::kQ4Rows8>::kQuads * 512, 0, p);
+                      zk::kReceivedStages * kBlocks * 64 * sizeof(uint4), 0, p);
     }), "dev_q4_attention: weights");
 }
 
