@@ -49,11 +49,17 @@ struct Q4Attend {
     float* part_stats;         // workspace [kv_heads][splits][rows][2]: that maximum (of scores in units of log 2) and the sum of weights
     float* scores;             // workspace [kv_heads][rows][slots], or null: the scores are not kept
     float* stats;              // workspace [kv_heads][rows]: maximum + log2 of the sum, or null
-    uint4* queries;            // workspace [kv_heads][row tiles of eight][blocks][2][32 lanes]: the rows as the products take them, or null
-    float* factors;            // workspace [kv_heads][rows]: what makes scores of their products, or null
+    uint4* queries;            // workspace [kv_heads][row tiles of eight][blocks][2][32 lanes]: the rows as the products take them; kQ4Digits: [kv_heads][blocks][32]
+    float* factors;            // workspace [kv_heads][padded rows]: what makes scores of their products
+    float* starts;             // kQ4Digits: workspace [kv_heads][blocks][8]: -8 sum q of the columns, in the products' units
     uint32_t tokens, heads, group;      // group = heads / kv_heads; a kv head has tokens * group rows, row = token * group + head of the group
     uint32_t splits, row_warps;
-    size_t q_ld;
+    uint32_t padded;           // rows, rounded up to a whole number of what a warp takes
+    const float* k;            // rows kv_ld apart
+    const float* v;
+    float* k_held;             // or null
+    float* v_held;
+    size_t q_ld, kv_ld;
     float scale;
     int* error_word;
 };
@@ -112,6 +118,12 @@ __device__ __forceinline__ uint32_t signed_high(uint32_t x) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0x2c002c00u), "r"(0xd480d480u));   // (1024 + 16 c) / 16 - 72
     return r;
 }
+// a += b, two at a time
+__device__ __forceinline__ void add_pairs(float (&a)[4], const float (&b)[4]) {
+    asm("{ .reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;\n\t"
+        "mov.b64 x, {%2, %3}; mov.b64 y, {%6, %7}; add.rn.f32x2 x, x, y; mov.b64 {%2, %3}, x; }"
+        : "+f"(a[0]), "+f"(a[1]), "+f"(a[2]), "+f"(a[3]) : "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3]));
+}
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 // Four slots' scales of all blocks, kept as they are until they are used.
@@ -141,7 +153,23 @@ struct Q4Scales {
         }
     }
     __device__ __forceinline__ float of(int o, int block) const {
-        return __half2float(__ushort_as_half(static_cast<unsigned short>(block % 2 ? pair[o][block / 2] >> 16 : pair[o][block / 2] & 0xffffu)));
+        const __half2 two = *reinterpret_cast<const __half2*>(&pair[o][block / 2]);
+        return block % 2 ? __high2float(two) : __low2float(two);
+    }
+    // the largest magnitude among the scales of slot `at` alone, as f16 bits
+    static __device__ __forceinline__ uint32_t largest(const __half* s, uint32_t at) {
+        const __half* from = s + at * kBlocks;
+        if constexpr (kBlocks % 2 == 0) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int b = 0; b < kBlocks / 2; ++b) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(from)[b] & 0x7fff7fffu);
+            return max(top & 0xffffu, top >> 16);
+        } else {
+            uint32_t top = 0;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) top = max(top, __half_as_ushort(from[b]) & 0x7fffu);
+            return top;
+        }
     }
 };
 
@@ -156,10 +184,10 @@ __host__ __device__ constexpr uint32_t q4_attend_smem(uint32_t row_warps) {
 // A warp turns one row of queries into the products' second operand.  A lane's words of a block are its dimensions 4t, 4t+2 | 16+4t, 16+4t+2 (low and high nibbles of
 // bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kQ4Digits: columns 2r and 2r + 1 are row r's digits, those beside high
 // nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20); else
-// a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14).  Returns what makes scores
-// (in units of log 2) of the products; starts (kQ4Digits, [blocks][8 columns]): -8 sum q.
-template <int kBlocks, int kColumns>
-__device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to, uint32_t row, float scale, float* starts, uint32_t lane) {
+// a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14); the row's factor makes scores
+// (in units of log 2) of the products.
+template <int kBlocks, bool kDigits>
+__device__ __forceinline__ void q4_lay_row(const float (&x)[kBlocks], const Q4Attend& p, uint32_t h, uint32_t row, uint32_t lane) {
     float top = 0.0f;
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) top = fmaxf(top, fabsf(x[g]));
@@ -167,26 +195,68 @@ __device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to
     const int e = max(static_cast<int>(size >> 23) - 127, -114);
     const float up = power_of_two(13 - e);
     const uint32_t part = lane >> 4, t = (lane & 15u) >> 2, step = lane & 1u, half = (lane >> 1) & 1u, word = 2 * step + part;
-    const float unit = kColumns == kQ4Digits && part ? 0.0625f : 1.0f;
-    __half* const halves = reinterpret_cast<__half*>(to);
+    const float unit = kDigits && part ? 0.0625f : 1.0f;
+    __half* const halves = reinterpret_cast<__half*>(p.queries + static_cast<size_t>(h) * (kDigits ? kBlocks * 32 : p.padded * kBlocks * 8));
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
         const float y = x[g] * up, upper = upper_digit(y);
         const __half first = __float2half_rn(upper * unit), other = __float2half_rn((y - upper) * unit);
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
-            const uint32_t column = kColumns == kQ4Digits ? 2 * row + d : row & 7u;
-            const uint32_t at = kColumns == kQ4Digits ? g * 32 + column * 4 + t : (((row >> 3) * kBlocks + g) * 2 + d) * 32 + column * 4 + t;
+            const uint32_t column = kDigits ? 2 * row + d : row & 7u;
+            const size_t at = kDigits ? g * 32 + column * 4 + t : ((static_cast<size_t>(row >> 3) * kBlocks + g) * 2 + d) * 32 + column * 4 + t;
             halves[(at * 4 + word) * 2 + half] = d ? other : first;
-            if (kColumns == kQ4Digits) {
+            if (kDigits) {
                 float sum = __half2float(d ? other : first) * (part ? 16.0f : 1.0f);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) starts[g * 8 + column] = sum * -8.0f * 5.9604644775390625e-8f;      // 2^-24
+                if (lane == 0) p.starts[(h * kBlocks + g) * 8 + column] = sum * -8.0f * 5.9604644775390625e-8f;      // 2^-24
             }
         }
     }
-    return ldexpf(scale * 1.4426950408889634f, (kColumns == kQ4Digits ? 24 : 0) + e - 13);
+    if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = ldexpf(p.scale * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
+}
+
+// What the attention begins with: the new tokens' keys (rotated) and values go into the slots behind *filled, and their queries (rotated) are laid out
+// for the products.  grid = (tokens, kv_heads); a warp takes a block of the key or the value, or a row of queries.
+constexpr uint32_t kQ4PrepareWarps = 16;
+template <int kBlocks, bool kDigits>
+__global__ void __launch_bounds__(kQ4PrepareWarps * 32) q4_prepare_kernel(const __grid_constant__ Q4Attend p) {
+    constexpr uint32_t kDim = kBlocks * 32;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, t = blockIdx.x, h = blockIdx.y;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
+    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {
+        if (threadIdx.x == 0 && t == 0 && h == 0) atomicExch(p.error_word, kErrBadPosition);
+        return;
+    }
+    const size_t turned = static_cast<size_t>(position) + t;
+    const uint32_t rows = p.tokens * p.group, last = t + 1 == p.tokens ? p.padded - rows : 0u;       // the last token's CTA clears the rows that pad a tile
+    for (uint32_t item = warp; item < 2 * kBlocks + p.group + last; item += warps) {
+        if (item >= 2 * kBlocks) {
+            const uint32_t j = item - 2 * kBlocks;
+            float x[kBlocks] = {};
+            if (j < p.group) {
+                const float* from = p.q + t * p.q_ld + static_cast<size_t>(h * p.group + j) * kDim;
+#pragma unroll
+                for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, turned);
+            }
+            q4_lay_row<kBlocks, kDigits>(x, p, h, t * p.group + j, lane);
+            continue;
+        }
+        const bool is_value = item >= kBlocks;
+        const uint32_t block = is_value ? item - kBlocks : item, e = block * kQ4Block + lane, slot = static_cast<uint32_t>(filled) + t;
+        const size_t head_at = t * p.kv_ld + static_cast<size_t>(h) * kDim;
+        const float x = is_value ? __ldcg(p.v + head_at + e) : q4_rotated(p.k + head_at, e, p.turn, turned);
+        const Q4Quantised q = q4_quantise(x, lane);
+        const uint32_t high = __shfl_down_sync(0xffffffffu, q.code, 16);
+        if (lane < 16) (is_value ? p.cache.v_codes : p.cache.k_codes)[q4_codes_at(h, slot, block, kBlocks, p.cache.slots) + lane] = static_cast<uint8_t>(q.code | high << 4);
+        if (lane == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, kBlocks, p.cache.slots)] = q.scale;
+        float* held = is_value ? p.v_held : p.k_held;
+        if (held) held[(static_cast<size_t>(t) * p.cache.kv_heads + h) * kDim + e] = (static_cast<float>(q.code) - 8.0f) * __half2float(q.scale);
+    }
 }
 
 // grid = (splits, CTAs for the rows, kv_heads); the rows that see most slots come first.
@@ -196,16 +266,19 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     constexpr bool kDigits = kColumns == kQ4Digits;
     constexpr uint32_t kStage = q4_stage_bytes<kBlocks>(), kCodes = kQ4Tile * kBlocks * 16, kScales = kQ4Tile * kBlocks * 2;
     extern __shared__ __align__(128) uint8_t q4_smem[];
-    __shared__ uint64_t landed[kWarps][kStages];
-    __shared__ float row_max[kWarps][16], row_sum[kWarps][16], row_unit[kWarps], row_factor[kWarps * 16], starts[kDigits ? kBlocks * 8 : 1];
+    __shared__ uint64_t landed[kWarps][kStages], queries_landed;
+    __shared__ float row_max[kWarps][16], row_sum[kWarps][16], row_unit[kWarps];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, t = lane & 3u, h = blockIdx.z;
     const uint32_t key_warps = kWarps / p.row_warps, row_warp = warp % p.row_warps, key_warp = warp / p.row_warps;
     const uint32_t rows = p.tokens * p.group, cta_rows = p.row_warps * kRows;
     const uint32_t cta_first = (gridDim.y - 1 - blockIdx.y) * cta_rows, first = cta_first + row_warp * kRows;
     uint4* const queries = reinterpret_cast<uint4*>(q4_smem + kWarps * kStages * kStage);
-    if (lane == 0)
+    if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(&landed[warp][s], 1);
-    if (lane == 0) mbar_fence_init();
+        if (warp == 0) mbar_init(&queries_landed, 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
     const int filled_in = *reinterpret_cast<const volatile int*>(p.filled);
@@ -231,30 +304,13 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     };
     const uint32_t mine = begin + key_warp < end && first < rows ? (end - begin - key_warp + key_warps - 1) / key_warps : 0u;      // tiles of this warp
     if (lane == 0) {
-        asm volatile("fence.proxy.async;" ::: "memory");       // the append's stores come before the copies
+        asm volatile("fence.proxy.async;" ::: "memory");       // the stores of the launch before come ahead of the copies
+        if (warp == 0) {
+            const uint32_t bytes = kDigits ? kBlocks * 512 : min(cta_rows, p.padded - cta_first) * kBlocks * 128;
+            mbar_arrive_expect_tx(&queries_landed, bytes);
+            bulk_g2s(queries, p.queries + (kDigits ? static_cast<size_t>(h) * kBlocks * 32 : (static_cast<size_t>(h) * p.padded + cta_first) * kBlocks * 8), bytes, &queries_landed);
+        }
         for (uint32_t i = 0; i < min(mine, static_cast<uint32_t>(kStages)); ++i) fetch(begin + key_warp + i * key_warps, i);
-    }
-    // the CTA's rows, rotated and laid out; zeros where a tile has more
-    for (uint32_t r = warp; r < cta_rows; r += kWarps) {
-        float x[kBlocks] = {};
-        if (r < real_rows) {
-            const uint32_t row = cta_first + r, token = row / p.group, head = h * p.group + row % p.group;
-            const float* from = p.q + token * p.q_ld + static_cast<size_t>(head) * kDim;
-#pragma unroll
-            for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, static_cast<size_t>(position) + token);
-        }
-        const float factor = q4_lay_row<kBlocks, kColumns>(x, queries, r, p.scale, starts, lane);
-        if (lane == 0) {
-            row_factor[r] = factor;
-            if (p.factors && blockIdx.x == 0 && r < real_rows) p.factors[static_cast<size_t>(h) * rows + cta_first + r] = factor;
-        }
-    }
-    __syncthreads();
-    if constexpr (!kDigits) {
-        if (p.queries && blockIdx.x == 0) {
-            uint4* to = p.queries + (static_cast<size_t>(h) * ((rows + 7) / 8) + cta_first / 8) * kBlocks * 64;
-            for (uint32_t i = threadIdx.x; i < (real_rows + 7) / 8 * kBlocks * 64; i += kWarps * 32) to[i] = queries[i];
-        }
     }
     const uint4* const my_queries = queries + row_warp * kTiles * kBlocks * 64;
     // of the lane's rows: the last slot each sees, and what makes scores of its products
@@ -267,7 +323,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
             const uint32_t r = kDigits ? t : 8 * n + 2 * t + c;
             last_seen[n][c] = filled + min(first + r, rows - 1) / p.group;
             least = min(least, last_seen[n][c]);
-            factor[n][c] = row_factor[row_warp * kRows + r];
+            factor[n][c] = __ldcg(p.factors + static_cast<size_t>(h) * p.padded + min(first + r, p.padded - 1));
         }
     least = __reduce_min_sync(0xffffffffu, least);
     uint4 own_query[kDigits ? kBlocks : 1];
@@ -275,10 +331,16 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     if constexpr (kDigits) {
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g) {
-            own_query[g] = my_queries[g * 32 + lane];
-            start[g][0] = start[g][2] = starts[g * 8 + 2 * t];
-            start[g][1] = start[g][3] = starts[g * 8 + 2 * t + 1];
+            const float2 two = __ldcg(reinterpret_cast<const float2*>(p.starts + (h * kBlocks + g) * 8) + t);
+            start[g][0] = start[g][2] = two.x;
+            start[g][1] = start[g][3] = two.y;
         }
+    }
+    bool failed = !__all_sync(0xffffffffu, mbar_wait(&queries_landed, 0));
+    if (failed && lane == 0) atomicExch(p.error_word, kErrFullWaitTimeout);
+    if constexpr (kDigits) {
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) own_query[g] = my_queries[g * 32 + lane];
     }
 
     float acc[kTiles][2 * kBlocks][4];
@@ -344,12 +406,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
         }
         auto hidden = [&](int half, int n, int j) { return !kWhole && slot0 + 16 * half + 8 * (j / 2) + a > last_seen[n][j & 1]; };
         // the largest scale of a value that any row sees, as a power of two
-        uint32_t top = 0;
-        if (kWhole || slot0 + lane < seen) {
-#pragma unroll
-            for (int g = 0; g < kBlocks; ++g) top = max(top, static_cast<uint32_t>(__half_as_ushort(v_scales[lane * kBlocks + g])) & 0x7fffu);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, kWhole || slot0 + lane < seen ? Q4Scales<kBlocks>::largest(v_scales, lane) : 0u);
         const int new_unit = max(unit, min(static_cast<int>(top >> 10), 30) - 14);
         bool moved = new_unit != unit;
         float corr[kTiles][2], base[kTiles][2];
@@ -449,14 +506,11 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[n][2 * g + i][j] += sum[i][j];
+                for (int i = 0; i < 2; ++i) add_pairs(acc[n][2 * g + i], sum[i]);
             }
         }
     };
 
-    bool failed = false;
     for (uint32_t i = 0; i < mine; ++i) {
         const int stage = i % kStages;
         if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][stage], (i / kStages) & 1u))) {
@@ -536,48 +590,76 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     }
 }
 
-// The runs of a row put together: grid = (rows, kv_heads), four threads a dimension, each with every fourth run and all of its loads in flight.  Rows
-// are those of one CTA of the launch before (cta_rows of them), whose arithmetic gives the number of runs.
-constexpr uint32_t kQ4JoinSlices = 4;
-__global__ void __launch_bounds__(1024) q4_join_kernel(const __grid_constant__ Q4Attend p, uint32_t cta_rows, uint32_t key_warps) {
-    __shared__ float share[kQ4JoinSlices][256];
-    const uint32_t row = blockIdx.x, h = blockIdx.y, rows = p.tokens * p.group, dim = p.cache.blocks * 32, e = threadIdx.x % dim, slice = threadIdx.x / dim, lane = threadIdx.x & 31u;
+// The runs of a row put together: `parts` warps a row, each with every so-manieth run, all of their loads in flight at once (a step's time here is round trips);
+// the warps' shares meet in shared memory.  The rows of one CTA of the launch before (cta_rows of them) have their number of runs from its arithmetic.
+// grid = (rows / (16 / parts), kv_heads).
+constexpr uint32_t kQ4JoinWarps = 16, kQ4JoinRuns = 3;      // runs of a warp at a time
+__global__ void __launch_bounds__(kQ4JoinWarps * 32) q4_join_kernel(const __grid_constant__ Q4Attend p, uint32_t cta_rows, uint32_t key_warps, uint32_t parts) {
+    __shared__ float4 share[kQ4JoinWarps][64];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, part = warp % parts, h = blockIdx.y, rows = p.tokens * p.group, quads = p.cache.blocks * 8;
+    const uint32_t row = blockIdx.x * (kQ4JoinWarps / parts) + warp / parts;
     pdl_launch_dependents();
     pdl_wait();
     const int filled = *reinterpret_cast<const volatile int*>(p.filled);
     const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    const bool mine = row < rows;
     if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;
-    const uint32_t last_row = min(rows, (row / cta_rows + 1) * cta_rows) - 1;
-    const uint32_t active = q4_runs(static_cast<uint32_t>(filled) + last_row / p.group + 1, p.splits, key_warps).active;
-    const size_t first = static_cast<size_t>(h) * p.splits * rows + row, step = static_cast<size_t>(rows) * dim;
-    float top = -INFINITY, sum = 0.0f, o = 0.0f;
-    // every warp has all the runs' maxima and sums, a run a lane
-    for (uint32_t s = lane; s < active; s += 32) top = fmaxf(top, __ldcg(p.part_stats + 2 * (first + static_cast<size_t>(s) * rows)));
+    float top = -INFINITY, sum = 0.0f;
+    if (mine) {
+        const uint32_t last_row = min(rows, (row / cta_rows + 1) * cta_rows) - 1;
+        const uint32_t active = q4_runs(static_cast<uint32_t>(filled) + last_row / p.group + 1, p.splits, key_warps).active;
+        const size_t first = static_cast<size_t>(h) * p.splits * rows + row;
+        const float2* stats = reinterpret_cast<const float2*>(p.part_stats) + first;
+        const float4* from = reinterpret_cast<const float4*>(p.part_out) + first * quads;
+        float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        // a warp's first runs are asked for before anything is known of the maxima
+        auto ask = [&](float4 (&x)[kQ4JoinRuns][2], float (&its)[kQ4JoinRuns], uint32_t s0) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    for (uint32_t s0 = 0; s0 < active; s0 += 32) {
-        constexpr uint32_t kMine = 32 / kQ4JoinSlices;
-        float x[kMine], by = 0.0f;
-        const float* from = p.part_out + (first + static_cast<size_t>(s0 + slice) * rows) * dim + e;
+            for (uint32_t i = 0; i < kQ4JoinRuns; ++i) {
+                const uint32_t s = s0 + i * parts;
+                its[i] = s < active ? __ldcg(stats + static_cast<size_t>(s) * rows).x : -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) x[i] = s0 + slice + i * kQ4JoinSlices < active ? __ldcg(from + i * kQ4JoinSlices * step) : 0.0f;
-        if (s0 + lane < active) {
-            const float2 its = __ldcg(reinterpret_cast<const float2*>(p.part_stats) + first + static_cast<size_t>(s0 + lane) * rows);
-            by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
-            sum += by * its.y;
+                for (uint32_t q = 0; q < 2; ++q)
+                    x[i][q] = s < active && lane + 32 * q < quads ? __ldcg(from + static_cast<size_t>(s) * rows * quads + lane + 32 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        float4 x[kQ4JoinRuns][2];
+        float its[kQ4JoinRuns];
+        ask(x, its, part);
+        for (uint32_t s = lane; s < active; s += 32) {
+            const float2 all = __ldcg(stats + static_cast<size_t>(s) * rows);
+            const float next = fmaxf(top, all.x);
+            if (next != -INFINITY) sum = sum * exp2_fast(top - next) + exp2_fast(all.x - next) * all.y;
+            top = next;
+        }
+        const float own = top;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        sum = own == -INFINITY ? sum : sum * exp2_fast(own - top);      // a NaN stays, whatever the maxima are
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        for (uint32_t s0 = part; s0 < active; s0 += kQ4JoinRuns * parts) {
+            if (s0 != part) ask(x, its, s0);
+#pragma unroll
+            for (uint32_t i = 0; i < kQ4JoinRuns; ++i) {
+                const float w = its[i] == -INFINITY ? 0.0f : exp2_fast(its[i] - top);
+#pragma unroll
+                for (uint32_t q = 0; q < 2; ++q) { o[q].x += w * x[i][q].x; o[q].y += w * x[i][q].y; o[q].z += w * x[i][q].z; o[q].w += w * x[i][q].w; }
+            }
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) o += __shfl_sync(0xffffffffu, by, slice + i * kQ4JoinSlices) * x[i];
+        for (uint32_t q = 0; q < 2; ++q) share[warp][lane + 32 * q] = o[q];
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    share[slice][e] = o;
     __syncthreads();
-    if (slice) return;
-    for (uint32_t i = 1; i < kQ4JoinSlices; ++i) o += share[i][e];
+    if (part || !mine) return;
     const uint32_t token = row / p.group, head = h * p.group + row % p.group;
-    p.out[(static_cast<size_t>(token) * p.heads + head) * dim + e] = o / sum;
-    if (threadIdx.x == 0) {
+    for (uint32_t q = lane; q < quads; q += 32) {
+        float4 o = share[warp][q];
+        for (uint32_t i = 1; i < parts; ++i) { const float4 x = share[warp + i][q]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
+        float* to = p.out + ((static_cast<size_t>(token) * p.heads + head) * quads + q) * 4;
+        to[0] = o.x / sum; to[1] = o.y / sum; to[2] = o.z / sum; to[3] = o.w / sum;
+    }
+    if (lane == 0) {
         if (!(sum > 0.0f) || !(sum < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
         if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = top + log2f(sum);
     }
@@ -635,7 +717,7 @@ __global__ void __cluster_dims__(kReceivedCtas, 1, 1) __launch_bounds__(kReceive
     }
     // the row tiles that see the CTA's first slot, dealt out to the cluster's CTAs
     const uint32_t first_tile = cta_slot < filled ? 0u : (cta_slot - filled) * p.group / 8;
-    const uint4* from = p.queries + static_cast<size_t>(h) * row_tiles * kTile;
+    const uint4* from = p.queries + static_cast<size_t>(h) * (p.padded / 8) * kTile;
     auto fetch = [&](uint32_t tile, int stage) {
         for (uint32_t i = threadIdx.x; i < kTile; i += kReceivedWarps * 32) copy16_or_zero(smem_u32(tiles + stage * kTile + i), from + static_cast<size_t>(tile) * kTile + i, true);
     };
@@ -661,7 +743,7 @@ __global__ void __cluster_dims__(kReceivedCtas, 1, 1) __launch_bounds__(kReceive
             const uint32_t row = row0 + 2 * t + c;
             const size_t at = static_cast<size_t>(h) * rows + min(row, rows - 1);
             whole[c] = row < rows ? __ldcg(p.stats + at) : INFINITY;
-            factor[c] = __ldcg(p.factors + at);
+            factor[c] = __ldcg(p.factors + static_cast<size_t>(h) * p.padded + min(row, rows - 1));
             last_seen[c] = filled + min(row, rows - 1) / p.group;
         }
         float s[2][4] = {};

@@ -87,46 +87,6 @@ __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
     return r;
 }
 
-struct Q4Append {
-    Q4Cache cache;
-    Q4Rotation turn;
-    const float* k;            // rows kv_ld apart
-    const float* v;
-    const int* position;
-    const int* filled;
-    float* k_held;             // or null
-    float* v_held;
-    uint32_t tokens;
-    size_t kv_ld;
-    int* error_word;
-};
-
-// The new tokens' keys (rotated) and values into the slots behind *filled.  grid = (tokens, kv_heads), two warps per block of a head: one for
-// the key's, one for the value's.
-__global__ void __launch_bounds__(512) q4_append_kernel(const __grid_constant__ Q4Append p) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, blocks = p.cache.blocks, t = blockIdx.x, h = blockIdx.y;
-    const bool is_value = warp >= blocks;
-    const uint32_t block = is_value ? warp - blocks : warp;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
-    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
-    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {
-        if (threadIdx.x == 0 && t == 0 && h == 0) atomicExch(p.error_word, kErrBadPosition);
-        return;
-    }
-    const size_t head_at = t * p.kv_ld + static_cast<size_t>(h) * blocks * kQ4Block;
-    const uint32_t e = block * kQ4Block + lane;
-    const float x = is_value ? __ldcg(p.v + head_at + e) : q4_rotated(p.k + head_at, e, p.turn, static_cast<size_t>(position) + t);
-    const Q4Quantised q = q4_quantise(x, lane);
-    const uint32_t slot = static_cast<uint32_t>(filled) + t;
-    const uint32_t high = __shfl_down_sync(0xffffffffu, q.code, 16);
-    if (lane < 16) (is_value ? p.cache.v_codes : p.cache.k_codes)[q4_codes_at(h, slot, block, blocks, p.cache.slots) + lane] = static_cast<uint8_t>(q.code | high << 4);
-    if (lane == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, blocks, p.cache.slots)] = q.scale;
-    float* held = is_value ? p.v_held : p.k_held;
-    if (held) held[(static_cast<size_t>(t) * p.cache.kv_heads + h) * blocks * kQ4Block + e] = (static_cast<float>(q.code) - 8.0f) * __half2float(q.scale);
-}
-
 // ---- eviction ----------------------------------------------------------------------------------------------------------------
 //
 // A cluster of eight CTAs takes a kv head; each CTA a run of its slots, each warp a run of the CTA's.  The weight of the last slot that stays is found

@@ -73,9 +73,9 @@ constexpr size_t kWaveCtas = 2 * 148;      // two CTAs on every SM
 // How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
 struct AttentionPlan {
     int columns{};
-    uint32_t rows{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{};
-    bool keep_scores{}, keep_queries{};
-    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
+    uint32_t rows{}, padded{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{};
+    bool keep_scores{};
+    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, starts{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
 };
 AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     AttentionPlan n;
@@ -87,24 +87,23 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     while (row_warps < warps && row_warps * per_warp < rows) row_warps *= 2;
     const size_t cta_rows = row_warps * per_warp, row_ctas = (rows + cta_rows - 1) / cta_rows;
     if (row_ctas > 65535) return n;
-    n.rows = u32(rows); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas); n.key_warps = u32(warps / row_warps);
+    n.rows = u32(rows); n.padded = u32((rows + per_warp - 1) / per_warp * per_warp); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas); n.key_warps = u32(warps / row_warps);
     // runs of slots side by side until every SM has its CTAs, no run shorter than a tile a warp
     n.splits = u32(std::max<size_t>(1, std::min(kWaveCtas / (row_ctas * kv_heads), tiles / n.key_warps)));
     n.keep_scores = rows <= 32;
-    n.keep_queries = !n.keep_scores;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
     if (n.splits > 1) {
         n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
         n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
     }
-    n.stats = take(kv_heads * rows * sizeof(float));
+    const bool digits = n.columns == zk::kQ4Digits;
+    n.queries = take(kv_heads * (digits ? blocks * 32 : n.padded * blocks * 8) * sizeof(uint4));
+    n.factors = take(kv_heads * n.padded * sizeof(float));
+    if (digits) n.starts = take(kv_heads * blocks * 8 * sizeof(float));
     if (a->weight_out) {
+        n.stats = take(kv_heads * rows * sizeof(float));
         if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
-        else {
-            n.queries = take(kv_heads * ((rows + 7) / 8) * blocks * 64 * sizeof(uint4));
-            n.factors = take(kv_heads * rows * sizeof(float));
-        }
     }
     n.bytes = at;
     return n;
@@ -155,19 +154,28 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     if (!e.ok) return 0;
     const zk::Q4Rotation turn{a->cos_t, a->sin_t, a->pairs, a->positions, a->adjacent ? 1u : 0u};
     const zk::Q4Cache cache = device_form(a->cache);
-    const zk::Q4Append append{cache, turn, d_k, d_v, a->position, a->filled, a->k_held, a->v_held, u32(tokens), a->kv_ld ? a->kv_ld : kv_row, e.d_error};
-    if (!e.leave(launch(e, zk::q4_append_kernel, dim3(u32(tokens), cache.kv_heads), dim3(64 * cache.blocks), 0, 0, append), "dev_q4_attention: append")) return 0;
     uint8_t* room = static_cast<uint8_t*>(a->workspace);
+    auto part = [&](size_t at) { return reinterpret_cast<float*>(room + at); };
     zk::Q4Attend p{};
-    p.cache = cache; p.turn = turn; p.q = d_q; p.position = a->position; p.filled = a->filled; p.weight_in = a->weight_in; p.weight_out = a->weight_out; p.out = d_out;
-    p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps;
-    p.q_ld = a->q_ld ? a->q_ld : q_row; p.scale = a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale; p.error_word = e.d_error;
-    if (plan.splits > 1) { p.part_out = reinterpret_cast<float*>(room + plan.part_out); p.part_stats = reinterpret_cast<float*>(room + plan.part_stats); }
+    p.cache = cache; p.turn = turn; p.q = d_q; p.k = d_k; p.v = d_v; p.k_held = a->k_held; p.v_held = a->v_held;
+    p.position = a->position; p.filled = a->filled; p.weight_in = a->weight_in; p.weight_out = a->weight_out; p.out = d_out;
+    p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps; p.padded = plan.padded;
+    p.q_ld = a->q_ld ? a->q_ld : q_row; p.kv_ld = a->kv_ld ? a->kv_ld : kv_row; p.scale = a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale;
+    p.error_word = e.d_error;
+    if (plan.splits > 1) { p.part_out = part(plan.part_out); p.part_stats = part(plan.part_stats); }
+    p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors);
+    const bool digits = plan.columns == zk::kQ4Digits;
+    if (digits) p.starts = part(plan.starts);
     if (a->weight_out) {
-        p.stats = reinterpret_cast<float*>(room + plan.stats);
-        if (plan.keep_scores) p.scores = reinterpret_cast<float*>(room + plan.scores);
-        else { p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = reinterpret_cast<float*>(room + plan.factors); }
+        p.stats = part(plan.stats);
+        if (plan.keep_scores) p.scores = part(plan.scores);
     }
+    const dim3 prepare_grid(u32(tokens), cache.kv_heads), prepare_block(32 * std::min<uint32_t>(zk::kQ4PrepareWarps, 2 * cache.blocks + p.group));
+    const cudaError_t prepared = by_blocks(cache.blocks, [&](auto blocks) {
+        constexpr int kBlocks = decltype(blocks)::value;
+        return digits ? launch(e, zk::q4_prepare_kernel<kBlocks, true>, prepare_grid, prepare_block, 0, 0, p) : launch(e, zk::q4_prepare_kernel<kBlocks, false>, prepare_grid, prepare_block, 0, 0, p);
+    });
+    if (!e.leave(prepared, "dev_q4_attention: new slots")) return 0;
     const dim3 grid(plan.splits, plan.row_ctas, cache.kv_heads);
     auto attend = [&](auto blocks, auto columns) {
         constexpr int kBlocks = decltype(blocks)::value, kColumns = decltype(columns)::value;
@@ -181,7 +189,14 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
         return attend(blocks, std::integral_constant<int, zk::kQ4Rows8>{});
     });
     if (!e.leave(r, "dev_q4_attention")) return 0;
-    if (plan.splits > 1 && !e.leave(launch(e, zk::q4_join_kernel, dim3(plan.rows, cache.kv_heads), dim3(zk::kQ4JoinSlices * cache.blocks * 32), 0, 0, p, plan.cta_rows, plan.key_warps), "dev_q4_attention: join")) return 0;
+    if (plan.splits > 1) {
+        uint32_t parts = 1;
+        while (parts < zk::kQ4JoinWarps && parts < plan.splits) parts *= 2;
+        const uint32_t a_cta = zk::kQ4JoinWarps / parts;
+        if (!e.leave(launch(e, zk::q4_join_kernel, dim3((plan.rows + a_cta - 1) / a_cta, cache.kv_heads), dim3(zk::kQ4JoinWarps * 32), 0, 0, p, plan.cta_rows, plan.key_warps, parts),
+                     "dev_q4_attention: join"))
+            return 0;
+    }
     if (!a->weight_out) return 1;
     if (plan.keep_scores) return e.leave(launch(e, zk::q4_received_kernel, dim3((cache.slots + 255) / 256, cache.kv_heads), dim3(256), 0, 0, p), "dev_q4_attention: weights");
     return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
