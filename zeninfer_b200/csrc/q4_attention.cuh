@@ -8,7 +8,7 @@
 //   scores   A = codes [16 slots][16 dimensions], two ldmatrix'd words a lane and block
 //   output   A = codes^T [16 dimensions][16 slots], from the transposing ldmatrix
 // The scores come out slot by row and the weights go in row by slot: movmatrix turns 8 x 8 of them.  Weights are scaled by a power of two so
-// that the largest |d| seen so far, times a weight of 1, is just below 2^14: both digits stay in f16's normal range over 2^28.  The matrix
+// that the largest |d| seen so far, times the largest weight, is below 2^14: both digits stay in f16's normal range over 2^20 and more.  The matrix
 // instructions cut their sums off towards zero (measured: 1 + 1.5 * 2^-24, a thousand times, is 1), which a long chain would add up to a
 // bias, so a tile's output sums start at zero and join the running ones by a rounded addition; and codes enter with their offset taken off
 // wherever a sum would otherwise begin far from zero.
@@ -193,7 +193,7 @@ __device__ __forceinline__ void q4_lay_row(const float (&x)[kBlocks], const Q4At
     for (int g = 0; g < kBlocks; ++g) top = fmaxf(top, fabsf(x[g]));
     const uint32_t size = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
     const int e = max(static_cast<int>(size >> 23) - 127, -114);
-    const float up = power_of_two(13 - e);
+    const float up = p.scale < 0.0f ? -power_of_two(13 - e) : power_of_two(13 - e);
     const uint32_t part = lane >> 4, t = (lane & 15u) >> 2, step = lane & 1u, half = (lane >> 1) & 1u, word = 2 * step + part;
     const float unit = kDigits && part ? 0.0625f : 1.0f;
     __half* const halves = reinterpret_cast<__half*>(p.queries + static_cast<size_t>(h) * (kDigits ? kBlocks * 32 : p.padded * kBlocks * 8));
@@ -214,7 +214,7 @@ __device__ __forceinline__ void q4_lay_row(const float (&x)[kBlocks], const Q4At
             }
         }
     }
-    if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = ldexpf(p.scale * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
+    if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = ldexpf(fabsf(p.scale) * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
 }
 
 // What the attention begins with: the new tokens' keys (rotated) and values go into the slots behind *filled, and their queries (rotated) are laid out
@@ -354,7 +354,10 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[n][i][j] = 0.0f;
     }
-    int unit = -32;                       // the weights' power of two is 14 - unit
+    // Weights times 2^(kFull - unit) times their slot's d are below 2^14: d is below 2^unit and a weight at most 2^kSlack.
+    constexpr float kSlack = 8.0f;
+    constexpr int kFull = 6, kHeadroom = 14;            // f16's exponent field less 14: the power of two above a scale
+    int unit = -32;
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
     // A tile; kWhole: every row sees every slot of it.
@@ -407,28 +410,27 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
         auto hidden = [&](int half, int n, int j) { return !kWhole && slot0 + 16 * half + 8 * (j / 2) + a > last_seen[n][j & 1]; };
         // the largest scale of a value that any row sees, as a power of two
         const uint32_t top = __reduce_max_sync(0xffffffffu, kWhole || slot0 + lane < seen ? Q4Scales<kBlocks>::largest(v_scales, lane) : 0u);
-        const int new_unit = max(unit, min(static_cast<int>(top >> 10), 30) - 14);
+        const int new_unit = max(unit, min(static_cast<int>(top >> 10), 30) - kHeadroom);
         bool moved = new_unit != unit;
-        float corr[kTiles][2], base[kTiles][2];
+        float next[kTiles][2];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
+            if constexpr (!kWhole) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int j = 0; j < 4; j += kDigits ? 2 : 1) s[half][n][j] = hidden(half, n, j) ? -INFINITY : s[half][n][j] * factor[n][j & 1];
+                    for (int j = 0; j < 4; j += kDigits ? 2 : 1) s[half][n][j] = hidden(half, n, j) ? -INFINITY : s[half][n][j];
+            }
 #pragma unroll
             for (int c = 0; c < (kDigits ? 1 : 2); ++c) {
                 float x = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                const float next = fmaxf(m[n][c], x);
-                moved |= next != m[n][c];
-                base[n][c] = next == -INFINITY ? 0.0f : next;
-                corr[n][c] = exp2_fast(m[n][c] - base[n][c]);
-                m[n][c] = next;
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * factor[n][c];
+                next[n][c] = x > m[n][c] + kSlack ? x : m[n][c];      // a maximum that is little larger leaves the weights above one, and the sums as they are
+                moved |= next[n][c] != m[n][c];
             }
-            if (kDigits) { corr[n][1] = corr[n][0]; base[n][1] = base[n][0]; m[n][1] = m[n][0]; }
+            if (kDigits) next[n][1] = next[n][0];
         }
         if (p.scores) {
 #pragma unroll
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                     if (row >= rows) continue;
                     float* to = p.scores + (static_cast<size_t>(h) * rows + row) * p.cache.slots + slot0 + a;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) { to[16 * half] = s[half][n][c]; to[16 * half + 8] = s[half][n][2 + c]; }
+                    for (int half = 0; half < 2; ++half) { to[16 * half] = s[half][n][c] * factor[n][c]; to[16 * half + 8] = s[half][n][2 + c] * factor[n][c]; }
                 }
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -448,27 +450,30 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
             for (int n = 0; n < kTiles; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    l[n][c] *= corr[n][c];
-                    const float by = corr[n][c] * of_unit;
+                    const float corr = m[n][c] == -INFINITY ? 0.0f : exp2_fast(m[n][c] - next[n][c]);
+                    l[n][c] *= corr;
+                    m[n][c] = next[n][c];
 #pragma unroll
                     for (int j = 0; j < 2 * kBlocks; ++j) {
-                        acc[n][j][c] *= by;
-                        acc[n][j][2 + c] *= by;
+                        acc[n][j][c] *= corr * of_unit;
+                        acc[n][j][2 + c] *= corr * of_unit;
                     }
                 }
             unit = new_unit;
         }
-        const float up = power_of_two(14 - unit);
+        const float up = power_of_two(kFull - unit);
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int n = 0; n < kTiles; ++n)
+            for (int j = 0; j < 4; j += kDigits ? 2 : 1) {
+                const float by = factor[n][j & 1], from = m[n][j & 1] == -INFINITY ? 0.0f : m[n][j & 1];
 #pragma unroll
-                for (int j = 0; j < 4; j += kDigits ? 2 : 1) {
-                    const float w = exp2_fast(s[half][n][j] - base[n][j & 1]);
+                for (int half = 0; half < 2; ++half) {
+                    const float w = exp2_fast(fmaf(s[half][n][j], by, -from));
                     l[n][j & 1] += w;
                     s[half][n][j] = w * up;
                 }
+            }
         Q4Scales<kBlocks> d;
         d.load(v_scales, a);
 #pragma unroll
@@ -511,9 +516,10 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
         }
     };
 
+    int stage = 0;
+    uint32_t phase = 0;
     for (uint32_t i = 0; i < mine; ++i) {
-        const int stage = i % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][stage], (i / kStages) & 1u))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][stage], phase))) {
             // the copies that are under way land (or are given up) before the ring is used for anything else
             if (lane == 0) {
                 atomicExch(p.error_word, kErrFullWaitTimeout);
@@ -528,6 +534,10 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
         else work(ring + stage * kStage, slot0, std::false_type{});
         __syncwarp();                       // everybody is done with the stage
         if (lane == 0 && i + kStages < mine) fetch(tile + kStages * key_warps, stage);
+        if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+        }
     }
 
     // the warp's sums into its ring's memory, [row][dimension]
@@ -559,7 +569,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                 }
             }
     }
-    if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - 14);
+    if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - kFull);
     __syncthreads();
     // the key warps' shares of a row
     const bool alone = p.splits == 1;
