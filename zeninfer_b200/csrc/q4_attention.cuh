@@ -28,13 +28,13 @@ constexpr uint32_t kQ4Tile = 32;             // slots of a tile
 
 // How a warp's rows lie on the eight columns of a product.
 enum Q4Columns : int {
-    kQ4Digits = 0,       // four rows, a column a digit: half the products of the next for up to four rows (a step of a model with groups of four)
+    kQ4Digits = 0,       // four rows, a column a digit: half the products of the next for up to four rows (a step of a model with groups of four; q4_step.cuh)
     kQ4Rows8 = 1,        // eight rows, the digits one after the other
     kQ4Rows16 = 2        // sixteen rows: the unpacked codes serve two products
 };
 __host__ __device__ constexpr int q4_rows(int columns) { return columns == kQ4Digits ? 4 : columns == kQ4Rows8 ? 8 : 16; }
 __host__ __device__ constexpr int q4_warps(int columns) { return columns == kQ4Digits ? 8 : 4; }
-__host__ __device__ constexpr int q4_stages(int columns) { return columns == kQ4Digits ? 3 : 2; }      // tiles of a warp's ring
+constexpr int kQ4Stages = 2;                 // tiles of a warp's ring: three were no faster, and take an SM's shared memory
 
 struct Q4Attend {
     Q4Cache cache;
@@ -49,9 +49,8 @@ struct Q4Attend {
     float* part_stats;         // workspace [kv_heads][splits][rows][2]: that maximum (of scores in units of log 2) and the sum of weights
     float* scores;             // workspace [kv_heads][rows][slots], or null: the scores are not kept
     float* stats;              // workspace [kv_heads][rows]: maximum + log2 of the sum, or null
-    uint4* queries;            // workspace [kv_heads][row tiles of eight][blocks][2][32 lanes]: the rows as the products take them; kQ4Digits: [kv_heads][blocks][32]
+    uint4* queries;            // workspace [kv_heads][row tiles of eight][blocks][2][32 lanes]: the rows as the products take them
     float* factors;            // workspace [kv_heads][padded rows]: what makes scores of their products
-    float* starts;             // kQ4Digits: workspace [kv_heads][blocks][8]: -8 sum q of the columns, in the products' units
     uint32_t tokens, heads, group;      // group = heads / kv_heads; a kv head has tokens * group rows, row = token * group + head of the group
     uint32_t splits, row_warps;
     uint32_t padded;           // rows, rounded up to a whole number of what a warp takes
@@ -178,25 +177,25 @@ __host__ __device__ constexpr uint32_t q4_stage_bytes() { return kQ4Tile * kBloc
 // Dynamic shared memory of q4_attend_kernel: the warps' rings, then the rows of queries as the products take them.
 template <int kBlocks, int kColumns>
 __host__ __device__ constexpr uint32_t q4_attend_smem(uint32_t row_warps) {
-    return q4_warps(kColumns) * q4_stages(kColumns) * q4_stage_bytes<kBlocks>() + row_warps * (kColumns == kQ4Rows16 ? 4 : kColumns == kQ4Rows8 ? 2 : 1) * kBlocks * 512;
+    return q4_warps(kColumns) * kQ4Stages * q4_stage_bytes<kBlocks>() + row_warps * (kColumns == kQ4Rows16 ? 4 : 2) * kBlocks * 512;
 }
 
 // A warp turns one row of queries into the products' second operand.  A lane's words of a block are its dimensions 4t, 4t+2 | 16+4t, 16+4t+2 (low and high nibbles of
-// bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kQ4Digits: columns 2r and 2r + 1 are row r's digits, those beside high
-// nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20); else
-// a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14); the row's factor makes scores
+// bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kDigits: columns 2r and 2r + 1 are row r's digits, those beside high
+// nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20), and starts [blocks][8 columns] get -8 sum q; else
+// a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14).  Returns the row's factor, which makes scores
 // (in units of log 2) of the products.
 template <int kBlocks, bool kDigits>
-__device__ __forceinline__ void q4_lay_row(const float (&x)[kBlocks], const Q4Attend& p, uint32_t h, uint32_t row, uint32_t lane) {
+__device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to, uint32_t row, float scale, float* starts, uint32_t lane) {
     float top = 0.0f;
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) top = fmaxf(top, fabsf(x[g]));
     const uint32_t size = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
     const int e = max(static_cast<int>(size >> 23) - 127, -114);
-    const float up = p.scale < 0.0f ? -power_of_two(13 - e) : power_of_two(13 - e);
+    const float up = scale < 0.0f ? -power_of_two(13 - e) : power_of_two(13 - e);
     const uint32_t part = lane >> 4, t = (lane & 15u) >> 2, step = lane & 1u, half = (lane >> 1) & 1u, word = 2 * step + part;
     const float unit = kDigits && part ? 0.0625f : 1.0f;
-    __half* const halves = reinterpret_cast<__half*>(p.queries + static_cast<size_t>(h) * (kDigits ? kBlocks * 32 : p.padded * kBlocks * 8));
+    __half* const halves = reinterpret_cast<__half*>(to);
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
         const float y = x[g] * up, upper = upper_digit(y);
@@ -210,19 +209,40 @@ __device__ __forceinline__ void q4_lay_row(const float (&x)[kBlocks], const Q4At
                 float sum = __half2float(d ? other : first) * (part ? 16.0f : 1.0f);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) p.starts[(h * kBlocks + g) * 8 + column] = sum * -8.0f * 5.9604644775390625e-8f;      // 2^-24
+                if (lane == 0) starts[g * 8 + column] = sum * -8.0f * 5.9604644775390625e-8f;      // 2^-24
             }
         }
     }
-    if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = ldexpf(fabsf(p.scale) * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
+    return ldexpf(fabsf(scale) * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
 }
 
-// What the attention begins with: the new tokens' keys (rotated) and values go into the slots behind *filled, and their queries (rotated) are laid out
+// A lane's value of a block (0 .. kBlocks - 1 of the key, then of the value) of new token t, the key's rotated.
+template <int kBlocks>
+__device__ __forceinline__ float q4_new_value(const Q4Attend& p, uint32_t h, uint32_t t, uint32_t item, size_t turned, uint32_t lane) {
+    const size_t head_at = t * p.kv_ld + static_cast<size_t>(h) * kBlocks * 32;
+    return item >= kBlocks ? __ldcg(p.v + head_at + (item - kBlocks) * 32 + lane) : q4_rotated(p.k + head_at, item * 32 + lane, p.turn, turned);
+}
+// A warp quantises such a block into its slot.  Lanes 0 .. 15 return the block's bytes.
+template <int kBlocks>
+__device__ __forceinline__ uint8_t q4_append_block(const Q4Attend& p, float x, uint32_t h, uint32_t t, uint32_t item, uint32_t filled, uint32_t lane, __half& scale) {
+    const bool is_value = item >= kBlocks;
+    const uint32_t block = is_value ? item - kBlocks : item, slot = filled + t;
+    const Q4Quantised q = q4_quantise(x, lane);
+    const uint32_t high = __shfl_down_sync(0xffffffffu, q.code, 16);
+    const uint8_t byte = static_cast<uint8_t>(q.code | high << 4);
+    if (lane < 16) (is_value ? p.cache.v_codes : p.cache.k_codes)[q4_codes_at(h, slot, block, kBlocks, p.cache.slots) + lane] = byte;
+    if (lane == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, kBlocks, p.cache.slots)] = q.scale;
+    float* held = is_value ? p.v_held : p.k_held;
+    if (held) held[(static_cast<size_t>(t) * p.cache.kv_heads + h) * kBlocks * 32 + block * 32 + lane] = (static_cast<float>(q.code) - 8.0f) * __half2float(q.scale);
+    scale = q.scale;
+    return byte;
+}
+
+// What a block's attention begins with: the new tokens' keys (rotated) and values go into the slots behind *filled, and their queries (rotated) are laid out
 // for the products.  grid = (tokens, kv_heads); a warp takes a block of the key or the value, or a row of queries.
 constexpr uint32_t kQ4PrepareWarps = 16;
-template <int kBlocks, bool kDigits>
+template <int kBlocks>
 __global__ void __launch_bounds__(kQ4PrepareWarps * 32) q4_prepare_kernel(const __grid_constant__ Q4Attend p) {
-    constexpr uint32_t kDim = kBlocks * 32;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, t = blockIdx.x, h = blockIdx.y;
     pdl_launch_dependents();
     pdl_wait();
@@ -235,35 +255,27 @@ __global__ void __launch_bounds__(kQ4PrepareWarps * 32) q4_prepare_kernel(const 
     const size_t turned = static_cast<size_t>(position) + t;
     const uint32_t rows = p.tokens * p.group, last = t + 1 == p.tokens ? p.padded - rows : 0u;       // the last token's CTA clears the rows that pad a tile
     for (uint32_t item = warp; item < 2 * kBlocks + p.group + last; item += warps) {
-        if (item >= 2 * kBlocks) {
-            const uint32_t j = item - 2 * kBlocks;
-            float x[kBlocks] = {};
-            if (j < p.group) {
-                const float* from = p.q + t * p.q_ld + static_cast<size_t>(h * p.group + j) * kDim;
-#pragma unroll
-                for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, turned);
-            }
-            q4_lay_row<kBlocks, kDigits>(x, p, h, t * p.group + j, lane);
+        if (item < 2 * kBlocks) {
+            __half ignored;
+            q4_append_block<kBlocks>(p, q4_new_value<kBlocks>(p, h, t, item, turned, lane), h, t, item, static_cast<uint32_t>(filled), lane, ignored);
             continue;
         }
-        const bool is_value = item >= kBlocks;
-        const uint32_t block = is_value ? item - kBlocks : item, e = block * kQ4Block + lane, slot = static_cast<uint32_t>(filled) + t;
-        const size_t head_at = t * p.kv_ld + static_cast<size_t>(h) * kDim;
-        const float x = is_value ? __ldcg(p.v + head_at + e) : q4_rotated(p.k + head_at, e, p.turn, turned);
-        const Q4Quantised q = q4_quantise(x, lane);
-        const uint32_t high = __shfl_down_sync(0xffffffffu, q.code, 16);
-        if (lane < 16) (is_value ? p.cache.v_codes : p.cache.k_codes)[q4_codes_at(h, slot, block, kBlocks, p.cache.slots) + lane] = static_cast<uint8_t>(q.code | high << 4);
-        if (lane == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, kBlocks, p.cache.slots)] = q.scale;
-        float* held = is_value ? p.v_held : p.k_held;
-        if (held) held[(static_cast<size_t>(t) * p.cache.kv_heads + h) * kDim + e] = (static_cast<float>(q.code) - 8.0f) * __half2float(q.scale);
+        const uint32_t j = item - 2 * kBlocks, row = t * p.group + j;
+        float x[kBlocks] = {};
+        if (j < p.group) {
+            const float* from = p.q + t * p.q_ld + static_cast<size_t>(h * p.group + j) * kBlocks * 32;
+#pragma unroll
+            for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, turned);
+        }
+        const float factor = q4_lay_row<kBlocks, false>(x, p.queries + static_cast<size_t>(h) * p.padded * kBlocks * 8, row, p.scale, nullptr, lane);
+        if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = factor;
     }
 }
 
 // grid = (splits, CTAs for the rows, kv_heads); the rows that see most slots come first.
 template <int kBlocks, int kColumns>
-__global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kColumns == kQ4Digits ? 2 : 3) q4_attend_kernel(const __grid_constant__ Q4Attend p) {
-    constexpr int kWarps = q4_warps(kColumns), kStages = q4_stages(kColumns), kRows = q4_rows(kColumns), kDim = kBlocks * 32, kTiles = kColumns == kQ4Rows16 ? 2 : 1;
-    constexpr bool kDigits = kColumns == kQ4Digits;
+__global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : 3) q4_attend_kernel(const __grid_constant__ Q4Attend p) {
+    constexpr int kWarps = q4_warps(kColumns), kStages = kQ4Stages, kRows = q4_rows(kColumns), kDim = kBlocks * 32, kTiles = kColumns == kQ4Rows16 ? 2 : 1;
     constexpr uint32_t kStage = q4_stage_bytes<kBlocks>(), kCodes = kQ4Tile * kBlocks * 16, kScales = kQ4Tile * kBlocks * 2;
     extern __shared__ __align__(128) uint8_t q4_smem[];
     __shared__ uint64_t landed[kWarps][kStages], queries_landed;
@@ -306,9 +318,9 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     if (lane == 0) {
         asm volatile("fence.proxy.async;" ::: "memory");       // the stores of the launch before come ahead of the copies
         if (warp == 0) {
-            const uint32_t bytes = kDigits ? kBlocks * 512 : min(cta_rows, p.padded - cta_first) * kBlocks * 128;
+            const uint32_t bytes = min(cta_rows, p.padded - cta_first) * kBlocks * 128;
             mbar_arrive_expect_tx(&queries_landed, bytes);
-            bulk_g2s(queries, p.queries + (kDigits ? static_cast<size_t>(h) * kBlocks * 32 : (static_cast<size_t>(h) * p.padded + cta_first) * kBlocks * 8), bytes, &queries_landed);
+            bulk_g2s(queries, p.queries + (static_cast<size_t>(h) * p.padded + cta_first) * kBlocks * 8, bytes, &queries_landed);
         }
         for (uint32_t i = 0; i < min(mine, static_cast<uint32_t>(kStages)); ++i) fetch(begin + key_warp + i * key_warps, i);
     }
@@ -320,28 +332,14 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint32_t r = kDigits ? t : 8 * n + 2 * t + c;
+            const uint32_t r = 8 * n + 2 * t + c;
             last_seen[n][c] = filled + min(first + r, rows - 1) / p.group;
             least = min(least, last_seen[n][c]);
             factor[n][c] = __ldcg(p.factors + static_cast<size_t>(h) * p.padded + min(first + r, p.padded - 1));
         }
     least = __reduce_min_sync(0xffffffffu, least);
-    uint4 own_query[kDigits ? kBlocks : 1];
-    float start[kDigits ? kBlocks : 1][4];
-    if constexpr (kDigits) {
-#pragma unroll
-        for (int g = 0; g < kBlocks; ++g) {
-            const float2 two = __ldcg(reinterpret_cast<const float2*>(p.starts + (h * kBlocks + g) * 8) + t);
-            start[g][0] = start[g][2] = two.x;
-            start[g][1] = start[g][3] = two.y;
-        }
-    }
     bool failed = !__all_sync(0xffffffffu, mbar_wait(&queries_landed, 0));
     if (failed && lane == 0) atomicExch(p.error_word, kErrFullWaitTimeout);
-    if constexpr (kDigits) {
-#pragma unroll
-        for (int g = 0; g < kBlocks; ++g) own_query[g] = my_queries[g * 32 + lane];
-    }
 
     float acc[kTiles][2 * kBlocks][4];
     float m[kTiles][2], l[kTiles][2];
@@ -379,30 +377,20 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t u = w[2 * half], v = w[2 * half + 1], x = u >> 8, y = v >> 8;
                     const float da = d.of(2 * half, g), db = d.of(2 * half + 1, g);
-                    if constexpr (kDigits) {
-                        const uint32_t even[4] = {u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u};
-                        const uint32_t odd[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
-                        float c[4];
-                        mma_f16(c, even, own_query[g].x, own_query[g].y, start[g]);
-                        mma_f16(c, odd, own_query[g].z, own_query[g].w, c);
-                        s[half][0][0] = fmaf(da, c[0] + c[1], s[half][0][0]);
-                        s[half][0][2] = fmaf(db, c[2] + c[3], s[half][0][2]);
-                    } else {
-                        const uint32_t even[4] = {signed_low(u), signed_low(v), signed_high(u), signed_high(v)};
-                        const uint32_t odd[4] = {signed_low(x), signed_low(y), signed_high(x), signed_high(y)};
+                    const uint32_t even[4] = {signed_low(u), signed_low(v), signed_high(u), signed_high(v)};
+                    const uint32_t odd[4] = {signed_low(x), signed_low(y), signed_high(x), signed_high(y)};
 #pragma unroll
-                        for (int n = 0; n < kTiles; ++n) {
-                            const uint4 upper = my_queries[(n * kBlocks + g) * 64 + lane], lower = my_queries[(n * kBlocks + g) * 64 + 32 + lane];
-                            float c[4];
-                            mma_f16(c, even, lower.x, lower.y, zero);
-                            mma_f16(c, odd, lower.z, lower.w, c);
-                            mma_f16(c, even, upper.x, upper.y, c);
-                            mma_f16(c, odd, upper.z, upper.w, c);
-                            s[half][n][0] = fmaf(da, c[0], s[half][n][0]);
-                            s[half][n][1] = fmaf(da, c[1], s[half][n][1]);
-                            s[half][n][2] = fmaf(db, c[2], s[half][n][2]);
-                            s[half][n][3] = fmaf(db, c[3], s[half][n][3]);
-                        }
+                    for (int n = 0; n < kTiles; ++n) {
+                        const uint4 upper = my_queries[(n * kBlocks + g) * 64 + lane], lower = my_queries[(n * kBlocks + g) * 64 + 32 + lane];
+                        float c[4];
+                        mma_f16(c, even, lower.x, lower.y, zero);
+                        mma_f16(c, odd, lower.z, lower.w, c);
+                        mma_f16(c, even, upper.x, upper.y, c);
+                        mma_f16(c, odd, upper.z, upper.w, c);
+                        s[half][n][0] = fmaf(da, c[0], s[half][n][0]);
+                        s[half][n][1] = fmaf(da, c[1], s[half][n][1]);
+                        s[half][n][2] = fmaf(db, c[2], s[half][n][2]);
+                        s[half][n][3] = fmaf(db, c[3], s[half][n][3]);
                     }
                 }
             }
@@ -419,10 +407,10 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int j = 0; j < 4; j += kDigits ? 2 : 1) s[half][n][j] = hidden(half, n, j) ? -INFINITY : s[half][n][j];
+                    for (int j = 0; j < 4; ++j) s[half][n][j] = hidden(half, n, j) ? -INFINITY : s[half][n][j];
             }
 #pragma unroll
-            for (int c = 0; c < (kDigits ? 1 : 2); ++c) {
+            for (int c = 0; c < 2; ++c) {
                 float x = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
@@ -430,14 +418,13 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                 next[n][c] = x > m[n][c] + kSlack ? x : m[n][c];      // a maximum that is little larger leaves the weights above one, and the sums as they are
                 moved |= next[n][c] != m[n][c];
             }
-            if (kDigits) next[n][1] = next[n][0];
         }
         if (p.scores) {
 #pragma unroll
             for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-                for (int c = 0; c < (kDigits ? 1 : 2); ++c) {
-                    const uint32_t row = first + (kDigits ? t : 8 * n + 2 * t + c);
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t row = first + 8 * n + 2 * t + c;
                     if (row >= rows) continue;
                     float* to = p.scores + (static_cast<size_t>(h) * rows + row) * p.cache.slots + slot0 + a;
 #pragma unroll
@@ -465,7 +452,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; j += kDigits ? 2 : 1) {
+            for (int j = 0; j < 4; ++j) {
                 const float by = factor[n][j & 1], from = m[n][j & 1] == -INFINITY ? 0.0f : m[n][j & 1];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -494,21 +481,14 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
                 for (int half = 0; half < 2; ++half) {
                     // a slot that is not seen may hold anything
                     auto weight = [&](int j) { return hidden(half, n, j) ? 0.0f : s[half][n][j] * d.of(2 * half + j / 2, g); };
-                    if constexpr (kDigits) {
-                        const float wa = weight(0), wb = weight(2), ha = upper_digit(wa), hb = upper_digit(wb);
-                        const uint32_t b0 = transposed(pack_f16(ha, wa - ha)), b1 = transposed(pack_f16(hb, wb - hb));
-                        mma_f16(sum[0], even[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[0]) : zero);
-                        mma_f16(sum[1], odd[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[1]) : zero);
-                    } else {
-                        const float w0 = weight(0), w1 = weight(1), w2 = weight(2), w3 = weight(3);
-                        const float h0 = upper_digit(w0), h1 = upper_digit(w1), h2 = upper_digit(w2), h3 = upper_digit(w3);
-                        const uint32_t b0 = transposed(pack_f16(h0, h1)), b1 = transposed(pack_f16(h2, h3));
-                        const uint32_t c0 = transposed(pack_f16(w0 - h0, w1 - h1)), c1 = transposed(pack_f16(w2 - h2, w3 - h3));
-                        mma_f16(sum[0], even[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[0]) : zero);
-                        mma_f16(sum[1], odd[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[1]) : zero);
-                        mma_f16(sum[0], even[half], c0, c1, sum[0]);
-                        mma_f16(sum[1], odd[half], c0, c1, sum[1]);
-                    }
+                    const float w0 = weight(0), w1 = weight(1), w2 = weight(2), w3 = weight(3);
+                    const float h0 = upper_digit(w0), h1 = upper_digit(w1), h2 = upper_digit(w2), h3 = upper_digit(w3);
+                    const uint32_t b0 = transposed(pack_f16(h0, h1)), b1 = transposed(pack_f16(h2, h3));
+                    const uint32_t c0 = transposed(pack_f16(w0 - h0, w1 - h1)), c1 = transposed(pack_f16(w2 - h2, w3 - h3));
+                    mma_f16(sum[0], even[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[0]) : zero);
+                    mma_f16(sum[1], odd[half], b0, b1, half ? static_cast<const float (&)[4]>(sum[1]) : zero);
+                    mma_f16(sum[0], even[half], c0, c1, sum[0]);
+                    mma_f16(sum[1], odd[half], c0, c1, sum[1]);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) add_pairs(acc[n][2 * g + i], sum[i]);
@@ -545,11 +525,11 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-        for (int c = 0; c < (kDigits ? 1 : 2); ++c) {
+        for (int c = 0; c < 2; ++c) {
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
-            const uint32_t r = kDigits ? t : 8 * n + 2 * t + c;
+            const uint32_t r = 8 * n + 2 * t + c;
             if (lane < 4) { row_max[warp][r] = m[n][c]; row_sum[warp][r] = failed ? NAN : l[n][c]; }
         }
 #pragma unroll
@@ -558,15 +538,10 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
             for (int odd = 0; odd < 2; ++odd) {
                 const uint32_t e = g * 32 + 2 * (lane >> 2) + odd;
                 const float (&c)[4] = acc[n][2 * g + odd];
-                if (kDigits) {
-                    sums[t * kDim + e] = c[0] + c[1];
-                    sums[t * kDim + e + 16] = c[2] + c[3];
-                } else {
-                    sums[(8 * n + 2 * t) * kDim + e] = c[0];
-                    sums[(8 * n + 2 * t + 1) * kDim + e] = c[1];
-                    sums[(8 * n + 2 * t) * kDim + e + 16] = c[2];
-                    sums[(8 * n + 2 * t + 1) * kDim + e + 16] = c[3];
-                }
+                sums[(8 * n + 2 * t) * kDim + e] = c[0];
+                sums[(8 * n + 2 * t + 1) * kDim + e] = c[1];
+                sums[(8 * n + 2 * t) * kDim + e + 16] = c[2];
+                sums[(8 * n + 2 * t + 1) * kDim + e + 16] = c[3];
             }
     }
     if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - kFull);
@@ -591,6 +566,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
             if (e == 0) {
                 if (!(sum > 0.0f) || !(sum < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
                 if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = top + log2f(sum);
+                if (p.scores) reinterpret_cast<float2*>(p.part_stats)[static_cast<size_t>(h) * rows + row] = make_float2(top, sum);
             }
         } else {
             const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + row;
@@ -600,32 +576,76 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : kCo
     }
 }
 
-// The runs of a row put together: `parts` warps a row, each with every so-manieth run, all of their loads in flight at once (a step's time here is round trips);
-// the warps' shares meet in shared memory.  The rows of one CTA of the launch before (cta_rows of them) have their number of runs from its arithmetic.
-// grid = (rows / (16 / parts), kv_heads).
-constexpr uint32_t kQ4JoinWarps = 16, kQ4JoinRuns = 3;      // runs of a warp at a time
-__global__ void __launch_bounds__(kQ4JoinWarps * 32) q4_join_kernel(const __grid_constant__ Q4Attend p, uint32_t cta_rows, uint32_t key_warps, uint32_t parts) {
-    __shared__ float4 share[kQ4JoinWarps][64];
+// What the CTAs of a launch leave: the first `join_ctas` CTAs of a kv head put the runs of its rows together, the others add up what the slots received (512 each),
+// where scores were kept.  Neither waits for the other: a row's maximum and sum over its runs are formed where they are needed.
+//   rows     `parts` warps a row, each with every so-manieth run, all of their loads in flight at once (a step's time here is round trips)
+//   slots    a thread a slot
+// The rows of one CTA of the launch before (cta_rows of them) have their number of runs from its arithmetic.  grid = (join_ctas + CTAs for slots, kv_heads).
+constexpr uint32_t kQ4FinishWarps = 16, kQ4FinishRuns = 3, kQ4KeptRows = 32;      // runs of a warp at a time; rows whose scores are kept
+struct Q4Whole {
+    float top, sum;
+};
+// A row's maximum and sum over all of its runs, in every lane.
+__device__ __forceinline__ Q4Whole q4_whole(const float2* stats, uint32_t active, uint32_t rows, uint32_t lane) {
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t s = lane; s < active; s += 32) {
+        const float2 its = __ldcg(stats + static_cast<size_t>(s) * rows);
+        const float next = fmaxf(top, its.x);
+        // a run without a maximum has no sum, or that of scores that are not numbers
+        sum = (next == -INFINITY ? sum : sum * exp2_fast(top - next)) + (its.x == -INFINITY ? its.y : exp2_fast(its.x - next) * its.y);
+        top = next;
+    }
+    const float own = top;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    sum = own == -INFINITY ? sum : sum * exp2_fast(own - top);      // a NaN stays, whatever the maxima are
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return Q4Whole{top, sum};
+}
+
+__global__ void __launch_bounds__(kQ4FinishWarps * 32) q4_finish_kernel(const __grid_constant__ Q4Attend p, uint32_t cta_rows, uint32_t key_warps, uint32_t parts, uint32_t join_ctas) {
+    __shared__ float4 share[kQ4FinishWarps][64];
+    __shared__ float whole[kQ4KeptRows];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, part = warp % parts, h = blockIdx.y, rows = p.tokens * p.group, quads = p.cache.blocks * 8;
-    const uint32_t row = blockIdx.x * (kQ4JoinWarps / parts) + warp / parts;
     pdl_launch_dependents();
     pdl_wait();
-    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
+    const int filled_in = *reinterpret_cast<const volatile int*>(p.filled);
     const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;
+    const uint32_t filled = filled_in;
+    auto runs_of = [&](uint32_t row) { return q4_runs(filled + (min(rows, (row / cta_rows + 1) * cta_rows) - 1) / p.group + 1, p.splits, key_warps).active; };
+    auto stats_of = [&](uint32_t row) { return reinterpret_cast<const float2*>(p.part_stats) + static_cast<size_t>(h) * p.splits * rows + row; };
+    if (blockIdx.x >= join_ctas) {
+        const uint32_t slot = (blockIdx.x - join_ctas) * kQ4FinishWarps * 32 + threadIdx.x, seen = filled + p.tokens;
+        if (slot - threadIdx.x >= seen) return;
+        for (uint32_t row = warp; row < rows; row += kQ4FinishWarps) {
+            const Q4Whole w = q4_whole(stats_of(row), runs_of(row), rows, lane);
+            if (lane == 0) whole[row] = w.top + log2f(w.sum);
+        }
+        const size_t at = static_cast<size_t>(h) * p.cache.slots + slot;
+        const float before = slot < filled ? p.weight_in[at] : 0.0f;
+        __syncthreads();
+        if (slot >= seen) return;
+        float sum = 0.0f;
+#pragma unroll 4
+        for (uint32_t r = slot < filled ? 0u : (slot - filled) * p.group; r < rows; ++r)
+            sum += exp2_fast(__ldcg(p.scores + (static_cast<size_t>(h) * rows + r) * p.cache.slots + slot) - whole[r]);
+        p.weight_out[at] = sum + before;
+        return;
+    }
+    const uint32_t row = blockIdx.x * (kQ4FinishWarps / parts) + warp / parts;
     const bool mine = row < rows;
-    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;
-    float top = -INFINITY, sum = 0.0f;
+    Q4Whole w{};
     if (mine) {
-        const uint32_t last_row = min(rows, (row / cta_rows + 1) * cta_rows) - 1;
-        const uint32_t active = q4_runs(static_cast<uint32_t>(filled) + last_row / p.group + 1, p.splits, key_warps).active;
-        const size_t first = static_cast<size_t>(h) * p.splits * rows + row;
-        const float2* stats = reinterpret_cast<const float2*>(p.part_stats) + first;
-        const float4* from = reinterpret_cast<const float4*>(p.part_out) + first * quads;
+        const uint32_t active = runs_of(row);
+        const float2* stats = stats_of(row);
+        const float4* from = reinterpret_cast<const float4*>(p.part_out) + (static_cast<size_t>(h) * p.splits * rows + row) * quads;
         float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         // a warp's first runs are asked for before anything is known of the maxima
-        auto ask = [&](float4 (&x)[kQ4JoinRuns][2], float (&its)[kQ4JoinRuns], uint32_t s0) {
+        auto ask = [&](float4 (&x)[kQ4FinishRuns][2], float (&its)[kQ4FinishRuns], uint32_t s0) {
 #pragma unroll
-            for (uint32_t i = 0; i < kQ4JoinRuns; ++i) {
+            for (uint32_t i = 0; i < kQ4FinishRuns; ++i) {
                 const uint32_t s = s0 + i * parts;
                 its[i] = s < active ? __ldcg(stats + static_cast<size_t>(s) * rows).x : -INFINITY;
 #pragma unroll
@@ -633,28 +653,17 @@ __global__ void __launch_bounds__(kQ4JoinWarps * 32) q4_join_kernel(const __grid
                     x[i][q] = s < active && lane + 32 * q < quads ? __ldcg(from + static_cast<size_t>(s) * rows * quads + lane + 32 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         };
-        float4 x[kQ4JoinRuns][2];
-        float its[kQ4JoinRuns];
+        float4 x[kQ4FinishRuns][2];
+        float its[kQ4FinishRuns];
         ask(x, its, part);
-        for (uint32_t s = lane; s < active; s += 32) {
-            const float2 all = __ldcg(stats + static_cast<size_t>(s) * rows);
-            const float next = fmaxf(top, all.x);
-            if (next != -INFINITY) sum = sum * exp2_fast(top - next) + exp2_fast(all.x - next) * all.y;
-            top = next;
-        }
-        const float own = top;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        sum = own == -INFINITY ? sum : sum * exp2_fast(own - top);      // a NaN stays, whatever the maxima are
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        for (uint32_t s0 = part; s0 < active; s0 += kQ4JoinRuns * parts) {
+        w = q4_whole(stats, active, rows, lane);
+        for (uint32_t s0 = part; s0 < active; s0 += kQ4FinishRuns * parts) {
             if (s0 != part) ask(x, its, s0);
 #pragma unroll
-            for (uint32_t i = 0; i < kQ4JoinRuns; ++i) {
-                const float w = its[i] == -INFINITY ? 0.0f : exp2_fast(its[i] - top);
+            for (uint32_t i = 0; i < kQ4FinishRuns; ++i) {
+                const float by = its[i] == -INFINITY ? 0.0f : exp2_fast(its[i] - w.top);
 #pragma unroll
-                for (uint32_t q = 0; q < 2; ++q) { o[q].x += w * x[i][q].x; o[q].y += w * x[i][q].y; o[q].z += w * x[i][q].z; o[q].w += w * x[i][q].w; }
+                for (uint32_t q = 0; q < 2; ++q) { o[q].x += by * x[i][q].x; o[q].y += by * x[i][q].y; o[q].z += by * x[i][q].z; o[q].w += by * x[i][q].w; }
             }
         }
 #pragma unroll
@@ -667,29 +676,12 @@ __global__ void __launch_bounds__(kQ4JoinWarps * 32) q4_join_kernel(const __grid
         float4 o = share[warp][q];
         for (uint32_t i = 1; i < parts; ++i) { const float4 x = share[warp + i][q]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
         float* to = p.out + ((static_cast<size_t>(token) * p.heads + head) * quads + q) * 4;
-        to[0] = o.x / sum; to[1] = o.y / sum; to[2] = o.z / sum; to[3] = o.w / sum;
+        to[0] = o.x / w.sum; to[1] = o.y / w.sum; to[2] = o.z / w.sum; to[3] = o.w / w.sum;
     }
     if (lane == 0) {
-        if (!(sum > 0.0f) || !(sum < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
-        if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = top + log2f(sum);
+        if (!(w.sum > 0.0f) || !(w.sum < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
+        if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = w.top + log2f(w.sum);
     }
-}
-
-// What the slots received, from kept scores: a thread a slot.
-__global__ void __launch_bounds__(256) q4_received_kernel(const __grid_constant__ Q4Attend p) {
-    const uint32_t slot = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, rows = p.tokens * p.group;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
-    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
-    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions) || slot >= static_cast<uint32_t>(filled) + p.tokens) return;
-    float sum = 0.0f;
-    for (uint32_t r = slot < static_cast<uint32_t>(filled) ? 0u : (slot - filled) * p.group; r < rows; ++r) {
-        const size_t row = static_cast<size_t>(h) * rows + r;
-        sum += exp2_fast(__ldcg(p.scores + row * p.cache.slots + slot) - __ldcg(p.stats + row));
-    }
-    const size_t at = static_cast<size_t>(h) * p.cache.slots + slot;
-    p.weight_out[at] = sum + (slot < static_cast<uint32_t>(filled) ? p.weight_in[at] : 0.0f);
 }
 
 // What the slots received in a block of many rows: the scores are formed once more, now that the rows' sums are known.  A warp takes 32

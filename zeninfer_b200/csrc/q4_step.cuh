@@ -1,0 +1,331 @@
+// Attention of up to four rows a kv head over a cache held in 4 bits (a step of a model whose groups are of one to four query heads): one launch that
+// appends, attends and, for caches of moderate size, ends the call.
+//
+// The arithmetic is q4_attention.cuh's; a column of the products is a digit of a row, so that four rows fill the eight columns.  What is different is
+// what a step's time is made of: round trips to memory and launches.  So a CTA lays out the rows of queries itself while its first tiles are on
+// their way; the warp that has the tile of a new slot quantises it, writes it to the cache and into the tile when that has landed.
+//   kCluster    the CTAs of a kv head are a cluster (up to eight): their sums meet through distributed shared memory, the scores stay in shared memory, and what the
+//               slots received is added before the launch ends
+//   else        runs of slots on all SMs; q4_finish_kernel puts them together
+#pragma once
+#include <cooperative_groups.h>
+
+#include "q4_attention.cuh"
+
+namespace zk {
+
+constexpr uint32_t kQ4ClusterTiles = 4;      // tiles of a warp at most, in a cluster
+constexpr int kQ4StepWarps = 8;
+
+// Dynamic shared memory: the warps' rings, the queries, and (a cluster that adds up weights) the warps' scores [tile][row][slot].
+template <int kBlocks>
+__host__ __device__ constexpr uint32_t q4_step_smem(bool keep_scores) {
+    return kQ4StepWarps * kQ4Stages * q4_stage_bytes<kBlocks>() + kBlocks * 512 + (keep_scores ? kQ4StepWarps * kQ4ClusterTiles * 4 * kQ4Tile * 4 : 0);
+}
+
+// grid = (splits, 1, kv_heads); kCluster: a cluster of `splits`
+template <int kBlocks, bool kCluster>
+__global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_step_kernel(const __grid_constant__ Q4Attend p) {
+    namespace cg = cooperative_groups;
+    constexpr int kWarps = kQ4StepWarps, kDim = kBlocks * 32;
+    constexpr uint32_t kStage = q4_stage_bytes<kBlocks>(), kCodes = kQ4Tile * kBlocks * 16, kScales = kQ4Tile * kBlocks * 2, kPieces = 2 * kBlocks;
+    extern __shared__ __align__(128) uint8_t q4_smem[];
+    __shared__ uint64_t landed[kWarps][kQ4Stages];
+    __shared__ float row_max[kWarps][4], row_sum[kWarps][4], row_unit[kWarps], row_factor[4], starts[kBlocks * 8];
+    __shared__ __align__(16) uint4 fresh_codes[4][kPieces];       // the new slots this CTA has: blocks of the key, then of the value
+    __shared__ __half fresh_scales[4][kPieces];
+    __shared__ float cta_out[4][kDim], cta_max[4], cta_sum[4];    // read by the cluster
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, t = lane & 3u, h = blockIdx.z, rows = p.tokens * p.group;
+    uint4* const queries = reinterpret_cast<uint4*>(q4_smem + kWarps * kQ4Stages * kStage);
+    float* const kept = reinterpret_cast<float*>(queries + kBlocks * 32) + warp * kQ4ClusterTiles * 4 * kQ4Tile;
+    if (lane == 0) {
+        for (int s = 0; s < kQ4Stages; ++s) mbar_init(&landed[warp][s], 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled_in = *reinterpret_cast<const volatile int*>(p.filled);
+    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {       // all CTAs alike
+        if (threadIdx.x == 0 && blockIdx.x == 0 && h == 0) atomicExch(p.error_word, kErrBadPosition);
+        return;
+    }
+    const uint32_t filled = filled_in, seen = filled + p.tokens;
+    const Q4Runs runs = q4_runs(seen, p.splits, kWarps);
+    const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
+    if (!kCluster && begin >= end) return;                                                // nobody counts on this run
+    uint8_t* ring = q4_smem + warp * kQ4Stages * kStage;
+    const size_t head_slots = static_cast<size_t>(h) * p.cache.slots;
+    auto fetch = [&](uint32_t tile, int stage) {
+        const size_t slot = head_slots + static_cast<size_t>(tile) * kQ4Tile;
+        uint8_t* to = ring + stage * kStage;
+        mbar_arrive_expect_tx(&landed[warp][stage], kStage);
+        bulk_g2s(to, p.cache.k_codes + slot * (kBlocks * 16), kCodes, &landed[warp][stage]);
+        bulk_g2s(to + 2 * kCodes, p.cache.k_scales + slot * kBlocks, kScales, &landed[warp][stage]);
+        bulk_g2s(to + kCodes, p.cache.v_codes + slot * (kBlocks * 16), kCodes, &landed[warp][stage]);
+        bulk_g2s(to + 2 * kCodes + kScales, p.cache.v_scales + slot * kBlocks, kScales, &landed[warp][stage]);
+    };
+    const uint32_t mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0u;      // tiles of this warp
+    if (lane == 0) {
+        asm volatile("fence.proxy.async;" ::: "memory");       // the stores of earlier launches come ahead of the copies
+        for (uint32_t i = 0; i < min(mine, static_cast<uint32_t>(kQ4Stages)); ++i) fetch(begin + warp + i * kWarps, i);
+    }
+    // the rows, rotated and laid out; zeros where there are fewer than four
+    if (warp < 4) {
+        float x[kBlocks] = {};
+        if (warp < rows) {
+            const uint32_t token = warp / p.group, head = h * p.group + warp % p.group;
+            const float* from = p.q + token * p.q_ld + static_cast<size_t>(head) * kDim;
+#pragma unroll
+            for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, static_cast<size_t>(position) + token);
+        }
+        const float factor = q4_lay_row<kBlocks, true>(x, queries, warp, p.scale, starts, lane);
+        if (lane == 0) row_factor[warp] = factor;
+    }
+    // new slots in this CTA's tiles: each one's warp quantises it
+    for (uint32_t token = 0; token < p.tokens; ++token) {
+        const uint32_t tile = (filled + token) / kQ4Tile;
+        if (tile < begin || tile >= end || (tile - begin) % kWarps != warp) continue;
+        float x[kPieces];                  // all of them asked for before any is stored: one round trip
+#pragma unroll
+        for (uint32_t item = 0; item < kPieces; ++item) x[item] = q4_new_value<kBlocks>(p, h, token, item, static_cast<size_t>(position) + token, lane);
+#pragma unroll
+        for (uint32_t item = 0; item < kPieces; ++item) {
+            __half scale;
+            const uint8_t byte = q4_append_block<kBlocks>(p, x[item], h, token, item, filled, lane, scale);
+            if (lane < 16) reinterpret_cast<uint8_t*>(&fresh_codes[token][item])[lane] = byte;
+            if (lane == 0) fresh_scales[token][item] = scale;
+        }
+    }
+    __syncthreads();
+    const uint32_t last_seen = filled + min(t, rows - 1) / p.group, least = filled;      // of the lane's row, of all rows
+    const float factor = row_factor[t];
+    uint4 own_query[kBlocks];
+    float start[kBlocks][4];
+#pragma unroll
+    for (int g = 0; g < kBlocks; ++g) {
+        own_query[g] = queries[g * 32 + lane];
+        start[g][0] = start[g][2] = starts[g * 8 + 2 * t];
+        start[g][1] = start[g][3] = starts[g * 8 + 2 * t + 1];
+    }
+    float acc[2 * kBlocks][4] = {};
+    float m = -INFINITY, l = 0.0f;
+    // Weights times 2^(kFull - unit) times their slot's d are below 2^14: d is below 2^unit and a weight at most 2^kSlack.
+    constexpr float kSlack = 8.0f;
+    constexpr int kFull = 6, kHeadroom = 14;            // f16's exponent field less 14: the power of two above a scale
+    int unit = -32;
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    // A tile; kWhole: every row sees every slot of it.
+    auto work = [&](const uint8_t* stage, uint32_t slot0, uint32_t turn, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        const uint32_t a = lane >> 2;                     // the lane's slots are a, a + 8, a + 16, a + 24, its row is t
+        const __half* k_scales = reinterpret_cast<const __half*>(stage + 2 * kCodes);
+        const __half* v_scales = k_scales + kQ4Tile * kBlocks;
+        const uint32_t matrix = ((lane >> 3) * kBlocks * 8 + (lane & 7u)) * 16;
+        float s[4] = {};                                  // slot a + 8 i
+        {
+            Q4Scales<kBlocks> d;
+            d.load(k_scales, a);
+#pragma unroll
+            for (int g = 0; g < kBlocks; ++g) {
+                uint32_t w[4];
+                ldmatrix_x4(w, smem_u32(stage) + matrix + g * 128);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t u = w[2 * half], v = w[2 * half + 1], x = u >> 8, y = v >> 8;
+                    const uint32_t even[4] = {u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u};
+                    const uint32_t odd[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+                    float c[4];
+                    mma_f16(c, even, own_query[g].x, own_query[g].y, start[g]);
+                    mma_f16(c, odd, own_query[g].z, own_query[g].w, c);
+                    s[2 * half] = fmaf(d.of(2 * half, g), c[0] + c[1], s[2 * half]);
+                    s[2 * half + 1] = fmaf(d.of(2 * half + 1, g), c[2] + c[3], s[2 * half + 1]);
+                }
+            }
+        }
+        auto hidden = [&](int i) { return !kWhole && slot0 + 8 * i + a > last_seen; };
+        // the largest scale of a value that any row sees, as a power of two
+        const uint32_t top = __reduce_max_sync(0xffffffffu, kWhole || slot0 + lane < seen ? Q4Scales<kBlocks>::largest(v_scales, lane) : 0u);
+        const int new_unit = max(unit, min(static_cast<int>(top >> 10), 30) - kHeadroom);
+        if constexpr (!kWhole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = hidden(i) ? -INFINITY : s[i];
+        }
+        float x = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * factor;
+        const float next = x > m + kSlack ? x : m;        // a maximum that is little larger leaves the weights above one, and the sums as they are
+        if (kCluster ? p.weight_out != nullptr : p.scores != nullptr) {
+            if (kCluster || t < rows) {
+                float* to = kCluster ? kept + (turn * 4 + t) * kQ4Tile + a : p.scores + (static_cast<size_t>(h) * rows + t) * p.cache.slots + slot0 + a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[8 * i] = s[i] * factor;
+            }
+        }
+        if (__any_sync(0xffffffffu, next != m || new_unit != unit)) {
+            const float corr = m == -INFINITY ? 0.0f : exp2_fast(m - next);
+            l *= corr;
+            m = next;
+            const float by = unit == -32 ? 0.0f : corr * power_of_two(unit - new_unit);
+#pragma unroll
+            for (int j = 0; j < 2 * kBlocks; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][i] *= by;
+            unit = new_unit;
+        }
+        const float up = power_of_two(kFull - unit), from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = exp2_fast(fmaf(s[i], factor, -from));
+            l += w;
+            s[i] = w * up;
+        }
+        Q4Scales<kBlocks> d;
+        d.load(v_scales, a);
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) {
+            uint32_t w[4];
+            ldmatrix_x4_trans(w, smem_u32(stage) + kCodes + matrix + g * 128);
+            float sum[2][4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t u = w[2 * half], v = w[2 * half + 1], x = u >> 8, y = v >> 8;
+                // dimensions 2r and 16 + 2r, 2r + 1 and 17 + 2r of the block, r the lane's row of the operand
+                const uint32_t even[4] = {signed_low(u), signed_high(u), signed_low(v), signed_high(v)};
+                const uint32_t odd[4] = {signed_low(x), signed_high(x), signed_low(y), signed_high(y)};
+                // a slot that is not seen may hold anything
+                const float wa = hidden(2 * half) ? 0.0f : s[2 * half] * d.of(2 * half, g), wb = hidden(2 * half + 1) ? 0.0f : s[2 * half + 1] * d.of(2 * half + 1, g);
+                const float ha = upper_digit(wa), hb = upper_digit(wb);
+                const uint32_t b0 = transposed(pack_f16(ha, wa - ha)), b1 = transposed(pack_f16(hb, wb - hb));
+                mma_f16(sum[0], even, b0, b1, half ? static_cast<const float (&)[4]>(sum[0]) : zero);
+                mma_f16(sum[1], odd, b0, b1, half ? static_cast<const float (&)[4]>(sum[1]) : zero);
+            }
+            add_pairs(acc[2 * g], sum[0]);
+            add_pairs(acc[2 * g + 1], sum[1]);
+        }
+    };
+
+    bool failed = false;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (uint32_t i = 0; i < mine; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&landed[warp][stage], phase))) {
+            // the copies that are under way land (or are given up) before the ring is used for anything else
+            if (lane == 0) {
+                atomicExch(p.error_word, kErrFullWaitTimeout);
+                for (uint32_t j = i; j < min(mine, i + kQ4Stages); ++j) mbar_wait(&landed[warp][j % kQ4Stages], (j / kQ4Stages) & 1u);
+            }
+            __syncwarp();
+            failed = true;
+            break;
+        }
+        const uint32_t tile = begin + warp + i * kWarps, slot0 = tile * kQ4Tile;
+        uint8_t* const at = ring + stage * kStage;
+        if (slot0 + kQ4Tile > filled) {           // new slots into the tile, which came without them
+            for (uint32_t token = 0; token < p.tokens; ++token) {
+                const uint32_t slot = filled + token - slot0;                  // in the tile where it is below 32
+                if (slot >= kQ4Tile || lane >= kPieces) continue;
+                const uint32_t value = lane >= kBlocks, block = value ? lane - kBlocks : lane;
+                *reinterpret_cast<uint4*>(at + value * kCodes + (((slot >> 3) * kBlocks + block) * 8 + (slot & 7u)) * 16) = fresh_codes[token][lane];
+                reinterpret_cast<__half*>(at + 2 * kCodes + value * kScales)[slot * kBlocks + block] = fresh_scales[token][lane];
+            }
+            __syncwarp();
+        }
+        if (slot0 + kQ4Tile - 1 <= least) work(at, slot0, i, std::true_type{});
+        else work(at, slot0, i, std::false_type{});
+        __syncwarp();                       // everybody is done with the stage
+        if (lane == 0 && i + kQ4Stages < mine) fetch(tile + kQ4Stages * kWarps, stage);
+        if (++stage == kQ4Stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+
+    // the warp's sums into its ring's memory, [row][dimension]
+    float* sums = reinterpret_cast<float*>(ring);
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    if (lane < 4) { row_max[warp][t] = m; row_sum[warp][t] = failed ? NAN : l; }
+    if (mine) {
+#pragma unroll
+        for (int j = 0; j < 2 * kBlocks; ++j) {
+            const uint32_t e = (j / 2) * 32 + 2 * (lane >> 2) + (j & 1);
+            sums[t * kDim + e] = acc[j][0] + acc[j][1];
+            sums[t * kDim + e + 16] = acc[j][2] + acc[j][3];
+        }
+    }
+    if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - kFull);
+    __syncthreads();
+    // the warps' shares of a row
+    for (uint32_t i = threadIdx.x; i < rows * kDim; i += kWarps * 32) {
+        const uint32_t r = i / kDim, e = i % kDim;
+        float top = row_max[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, row_max[w][r]);
+        float sum = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float its = row_max[w][r], by = its == -INFINITY ? 0.0f : exp2_fast(its - top);
+            sum += by == 0.0f && its == -INFINITY ? row_sum[w][r] : by * row_sum[w][r];      // none, or what failed
+            if (its != -INFINITY) o += by * row_unit[w] * reinterpret_cast<const float*>(q4_smem + w * kQ4Stages * kStage)[r * kDim + e];
+        }
+        if (kCluster) {
+            cta_out[r][e] = o;
+            if (e == 0) { cta_max[r] = top; cta_sum[r] = sum; }
+        } else {
+            const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + r;
+            p.part_out[part * kDim + e] = o;
+            if (e == 0) { p.part_stats[2 * part] = top; p.part_stats[2 * part + 1] = sum; }
+        }
+    }
+    if constexpr (kCluster) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        // every CTA knows the rows' maxima and sums, and has a share of their dimensions
+        float top[4], sum[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            top[r] = -INFINITY;
+            sum[r] = 0.0f;
+            if (r >= static_cast<int>(rows)) continue;
+            for (uint32_t c = 0; c < p.splits; ++c) top[r] = fmaxf(top[r], cluster.map_shared_rank(cta_max, c)[r]);
+            for (uint32_t c = 0; c < p.splits; ++c) {
+                const float its = cluster.map_shared_rank(cta_max, c)[r], part = cluster.map_shared_rank(cta_sum, c)[r];
+                sum[r] += its == -INFINITY ? part : exp2_fast(its - top[r]) * part;
+            }
+        }
+        for (uint32_t i = blockIdx.x * (kWarps * 32) + threadIdx.x; i < rows * kDim; i += p.splits * kWarps * 32) {
+            const uint32_t r = i / kDim, e = i % kDim, token = r / p.group, head = h * p.group + r % p.group;
+            float o = 0.0f, all = 0.0f, high = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) if (k == static_cast<int>(r)) { all = sum[k]; high = top[k]; }
+            for (uint32_t c = 0; c < p.splits; ++c) {
+                const float its = cluster.map_shared_rank(cta_max, c)[r];
+                if (its != -INFINITY) o += exp2_fast(its - high) * cluster.map_shared_rank(&cta_out[0][0], c)[i];
+            }
+            p.out[(static_cast<size_t>(token) * p.heads + head) * kDim + e] = o / all;
+            if (e == 0 && (!(all > 0.0f) || !(all < INFINITY))) atomicExch(p.error_word, kErrNonFinite);
+        }
+        if (p.weight_out) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top[r] += log2f(sum[r]);
+            for (uint32_t i = 0; i < mine; ++i) {
+                const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
+                if (slot >= seen) continue;
+                const size_t at = head_slots + slot;
+                float x = slot < filled ? p.weight_in[at] : 0.0f, received = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < static_cast<int>(rows)) received += exp2_fast(kept[(i * 4 + r) * kQ4Tile + lane] - top[r]);      // a slot the row does not see: minus infinity
+                p.weight_out[at] = received + x;
+            }
+        }
+        cluster.sync();                     // nobody leaves while its shared memory is read
+    }
+}
+
+}  // namespace zk

@@ -11,6 +11,7 @@
 #include "host_state.h"
 #include "q4_attention.cuh"
 #include "q4_cache.cuh"
+#include "q4_step.cuh"
 #include "verify_drafts.cuh"
 
 namespace zk_host {
@@ -73,9 +74,9 @@ constexpr size_t kWaveCtas = 2 * 148;      // two CTAs on every SM
 // How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
 struct AttentionPlan {
     int columns{};
-    uint32_t rows{}, padded{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{};
+    uint32_t rows{}, padded{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{}, cluster{};
     bool keep_scores{};
-    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, starts{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
+    size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
 };
 AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     AttentionPlan n;
@@ -87,24 +88,28 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     while (row_warps < warps && row_warps * per_warp < rows) row_warps *= 2;
     const size_t cta_rows = row_warps * per_warp, row_ctas = (rows + cta_rows - 1) / cta_rows;
     if (row_ctas > 65535) return n;
-    n.rows = u32(rows); n.padded = u32((rows + per_warp - 1) / per_warp * per_warp); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas); n.key_warps = u32(warps / row_warps);
+    n.rows = u32(rows); n.padded = u32((rows + per_warp - 1) / per_warp * per_warp); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas);
+    n.key_warps = u32(warps / row_warps);
     // runs of slots side by side until every SM has its CTAs, no run shorter than a tile a warp
     n.splits = u32(std::max<size_t>(1, std::min(kWaveCtas / (row_ctas * kv_heads), tiles / n.key_warps)));
-    n.keep_scores = rows <= 32;
+    n.keep_scores = a->weight_out && rows <= zk::kQ4KeptRows;
+    if (n.columns == zk::kQ4Digits && tiles <= 8 * n.key_warps * zk::kQ4ClusterTiles) {
+        n.cluster = 1;
+        while (n.cluster < 8 && n.cluster * n.key_warps < tiles) n.cluster *= 2;
+        n.splits = n.cluster;
+        n.bytes = 16;                 // what the call needs stays in shared memory
+        return n;
+    }
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
-    if (n.splits > 1) {
-        n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
-        n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
+    if (n.splits > 1 || n.columns == zk::kQ4Digits) n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
+    if (n.splits > 1 || n.columns == zk::kQ4Digits || n.keep_scores) n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
+    if (n.columns != zk::kQ4Digits) {
+        n.queries = take(kv_heads * n.padded * blocks * 8 * sizeof(uint4));
+        n.factors = take(kv_heads * n.padded * sizeof(float));
     }
-    const bool digits = n.columns == zk::kQ4Digits;
-    n.queries = take(kv_heads * (digits ? blocks * 32 : n.padded * blocks * 8) * sizeof(uint4));
-    n.factors = take(kv_heads * n.padded * sizeof(float));
-    if (digits) n.starts = take(kv_heads * blocks * 8 * sizeof(float));
-    if (a->weight_out) {
-        n.stats = take(kv_heads * rows * sizeof(float));
-        if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
-    }
+    if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
+    else if (a->weight_out) n.stats = take(kv_heads * rows * sizeof(float));
     n.bytes = at;
     return n;
 }
@@ -156,49 +161,53 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     const zk::Q4Cache cache = device_form(a->cache);
     uint8_t* room = static_cast<uint8_t*>(a->workspace);
     auto part = [&](size_t at) { return reinterpret_cast<float*>(room + at); };
+    const bool digits = plan.columns == zk::kQ4Digits;
     zk::Q4Attend p{};
     p.cache = cache; p.turn = turn; p.q = d_q; p.k = d_k; p.v = d_v; p.k_held = a->k_held; p.v_held = a->v_held;
     p.position = a->position; p.filled = a->filled; p.weight_in = a->weight_in; p.weight_out = a->weight_out; p.out = d_out;
     p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps; p.padded = plan.padded;
     p.q_ld = a->q_ld ? a->q_ld : q_row; p.kv_ld = a->kv_ld ? a->kv_ld : kv_row; p.scale = a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale;
     p.error_word = e.d_error;
-    if (plan.splits > 1) { p.part_out = part(plan.part_out); p.part_stats = part(plan.part_stats); }
-    p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors);
-    const bool digits = plan.columns == zk::kQ4Digits;
-    if (digits) p.starts = part(plan.starts);
-    if (a->weight_out) {
-        p.stats = part(plan.stats);
-        if (plan.keep_scores) p.scores = part(plan.scores);
+    if (plan.cluster) {
+        return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
+            constexpr int kBlocks = decltype(blocks)::value;
+            return launch(e, zk::q4_step_kernel<kBlocks, true>, dim3(plan.cluster, 1, cache.kv_heads), dim3(zk::kQ4StepWarps * 32), zk::q4_step_smem<kBlocks>(a->weight_out), plan.cluster, p);
+        }), "dev_q4_attention");
     }
-    const dim3 prepare_grid(u32(tokens), cache.kv_heads), prepare_block(32 * std::min<uint32_t>(zk::kQ4PrepareWarps, 2 * cache.blocks + p.group));
-    const cudaError_t prepared = by_blocks(cache.blocks, [&](auto blocks) {
-        constexpr int kBlocks = decltype(blocks)::value;
-        return digits ? launch(e, zk::q4_prepare_kernel<kBlocks, true>, prepare_grid, prepare_block, 0, 0, p) : launch(e, zk::q4_prepare_kernel<kBlocks, false>, prepare_grid, prepare_block, 0, 0, p);
-    });
-    if (!e.leave(prepared, "dev_q4_attention: new slots")) return 0;
-    const dim3 grid(plan.splits, plan.row_ctas, cache.kv_heads);
+    p.part_out = part(plan.part_out); p.part_stats = part(plan.part_stats);
+    if (plan.keep_scores) p.scores = part(plan.scores);
+    else if (a->weight_out) p.stats = part(plan.stats);
+    if (!digits) {
+        p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors);
+        const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) {
+            return launch(e, zk::q4_prepare_kernel<decltype(blocks)::value>, dim3(u32(tokens), cache.kv_heads), dim3(32 * std::min<uint32_t>(zk::kQ4PrepareWarps, 2 * cache.blocks + p.group)), 0, 0, p);
+        });
+        if (!e.leave(r, "dev_q4_attention: new slots")) return 0;
+    }
     auto attend = [&](auto blocks, auto columns) {
         constexpr int kBlocks = decltype(blocks)::value, kColumns = decltype(columns)::value;
-        return launch(e, zk::q4_attend_kernel<kBlocks, kColumns>, grid, dim3(zk::q4_warps(kColumns) * 32), zk::q4_attend_smem<kBlocks, kColumns>(plan.row_warps), 0, p);
+        return launch(e, zk::q4_attend_kernel<kBlocks, kColumns>, dim3(plan.splits, plan.row_ctas, cache.kv_heads), dim3(zk::q4_warps(kColumns) * 32), zk::q4_attend_smem<kBlocks, kColumns>(plan.row_warps), 0, p);
     };
     const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) {
-        if (plan.columns == zk::kQ4Digits) return attend(blocks, std::integral_constant<int, zk::kQ4Digits>{});
-        if constexpr (decltype(blocks)::value <= 4) {
+        constexpr int kBlocks = decltype(blocks)::value;
+        if (digits) return launch(e, zk::q4_step_kernel<kBlocks, false>, dim3(plan.splits, 1, cache.kv_heads), dim3(zk::kQ4StepWarps * 32), zk::q4_step_smem<kBlocks>(false), 0, p);
+        if constexpr (kBlocks <= 4) {
             if (plan.columns == zk::kQ4Rows16) return attend(blocks, std::integral_constant<int, zk::kQ4Rows16>{});
         }
         return attend(blocks, std::integral_constant<int, zk::kQ4Rows8>{});
     });
     if (!e.leave(r, "dev_q4_attention")) return 0;
-    if (plan.splits > 1) {
+    const bool join = plan.splits > 1 || digits;
+    if (join || plan.keep_scores) {
         uint32_t parts = 1;
-        while (parts < zk::kQ4JoinWarps && parts < plan.splits) parts *= 2;
-        const uint32_t a_cta = zk::kQ4JoinWarps / parts;
-        if (!e.leave(launch(e, zk::q4_join_kernel, dim3((plan.rows + a_cta - 1) / a_cta, cache.kv_heads), dim3(zk::kQ4JoinWarps * 32), 0, 0, p, plan.cta_rows, plan.key_warps, parts),
-                     "dev_q4_attention: join"))
+        while (parts < zk::kQ4FinishWarps && parts < plan.splits) parts *= 2;
+        const uint32_t a_cta = zk::kQ4FinishWarps / parts, join_ctas = join ? (plan.rows + a_cta - 1) / a_cta : 0;
+        const uint32_t slot_ctas = plan.keep_scores ? (cache.slots + zk::kQ4FinishWarps * 32 - 1) / (zk::kQ4FinishWarps * 32) : 0;
+        if (!e.leave(launch(e, zk::q4_finish_kernel, dim3(join_ctas + slot_ctas, cache.kv_heads), dim3(zk::kQ4FinishWarps * 32), 0, 0, p, plan.cta_rows, plan.key_warps, parts, join_ctas),
+                     "dev_q4_attention: finish"))
             return 0;
     }
-    if (!a->weight_out) return 1;
-    if (plan.keep_scores) return e.leave(launch(e, zk::q4_received_kernel, dim3((cache.slots + 255) / 256, cache.kv_heads), dim3(256), 0, 0, p), "dev_q4_attention: weights");
+    if (!a->weight_out || plan.keep_scores) return 1;
     return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
         constexpr int kBlocks = decltype(blocks)::value;
         return launch(e, zk::q4_received_again_kernel<kBlocks>, dim3(zk::kReceivedCtas, (cache.slots + zk::kReceivedSlots - 1) / zk::kReceivedSlots, cache.kv_heads), dim3(zk::kReceivedWarps * 32),
