@@ -182,11 +182,11 @@ __host__ __device__ constexpr uint32_t q4_attend_smem(uint32_t row_warps) {
 
 // A warp turns one row of queries into the products' second operand.  A lane's words of a block are its dimensions 4t, 4t+2 | 16+4t, 16+4t+2 (low and high nibbles of
 // bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kDigits: columns 2r and 2r + 1 are row r's digits, those beside high
-// nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20), and starts [blocks][8 columns] get -8 sum q; else
+// nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20); else
 // a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14).  Returns the row's factor, which makes scores
 // (in units of log 2) of the products.
 template <int kBlocks, bool kDigits>
-__device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to, uint32_t row, float scale, float* starts, uint32_t lane) {
+__device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to, uint32_t row, float scale, uint32_t lane) {
     float top = 0.0f;
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) top = fmaxf(top, fabsf(x[g]));
@@ -205,15 +205,10 @@ __device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to
             const uint32_t column = kDigits ? 2 * row + d : row & 7u;
             const size_t at = kDigits ? g * 32 + column * 4 + t : ((static_cast<size_t>(row >> 3) * kBlocks + g) * 2 + d) * 32 + column * 4 + t;
             halves[(at * 4 + word) * 2 + half] = d ? other : first;
-            if (kDigits) {
-                float sum = __half2float(d ? other : first) * (part ? 16.0f : 1.0f);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) starts[g * 8 + column] = sum * -8.0f * 5.9604644775390625e-8f;      // 2^-24
-            }
         }
     }
-    return ldexpf(fabsf(scale) * 1.4426950408889634f, (kDigits ? 24 : 0) + e - 13);
+    const int units = (kDigits ? 24 : 0) + e - 13;                // in two steps, for it may be beyond what one power of two can be
+    return fabsf(scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2);
 }
 
 // A lane's value of a block (0 .. kBlocks - 1 of the key, then of the value) of new token t, the key's rotated.
@@ -267,7 +262,7 @@ __global__ void __launch_bounds__(kQ4PrepareWarps * 32) q4_prepare_kernel(const 
 #pragma unroll
             for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, turned);
         }
-        const float factor = q4_lay_row<kBlocks, false>(x, p.queries + static_cast<size_t>(h) * p.padded * kBlocks * 8, row, p.scale, nullptr, lane);
+        const float factor = q4_lay_row<kBlocks, false>(x, p.queries + static_cast<size_t>(h) * p.padded * kBlocks * 8, row, p.scale, lane);
         if (lane == 0) p.factors[static_cast<size_t>(h) * p.padded + row] = factor;
     }
 }

@@ -43,21 +43,27 @@ struct Q4Rotation {
     uint32_t adjacent;
 };
 
-// Dimension `e` of a head vector, rotated by the tables' row: every product and sum rounded on its own, so that a key turns out the same in
-// every kernel that forms it.
-__device__ __forceinline__ float q4_rotated(const float* head, uint32_t e, const Q4Rotation& r, size_t row) {
-    if (e >= 2 * r.pairs) return __ldcg(head + e);
+// Dimension `e` of a head vector, to be rotated by the tables' row: what is asked for without knowing the row, and the rest.  Every product and
+// sum is rounded on its own, so that a key turns out the same in every kernel that forms it.
+struct Q4Raw {
+    float mine, other;
+};
+__device__ __forceinline__ uint32_t q4_partner(uint32_t e, const Q4Rotation& r) { return r.adjacent ? e ^ 1u : e < r.pairs ? e + r.pairs : e - r.pairs; }
+__device__ __forceinline__ Q4Raw q4_raw(const float* head, uint32_t e, const Q4Rotation& r) {
+    return Q4Raw{__ldcg(head + e), e < 2 * r.pairs ? __ldcg(head + q4_partner(e, r)) : 0.0f};
+}
+__device__ __forceinline__ float q4_rotated(const Q4Raw& x, uint32_t e, const Q4Rotation& r, size_t row) {
+    if (e >= 2 * r.pairs) return x.mine;
     const uint32_t pair = r.adjacent ? e >> 1 : e < r.pairs ? e : e - r.pairs;
     const bool low = r.adjacent ? !(e & 1u) : e < r.pairs;
-    const uint32_t other = r.adjacent ? e ^ 1u : low ? e + r.pairs : e - r.pairs;
-    const float mine = __ldcg(head + e), its = __ldcg(head + other);
     const float c = __ldg(r.cos_t + row * r.pairs + pair), s = __ldg(r.sin_t + row * r.pairs + pair);
-    return low ? __fsub_rn(__fmul_rn(mine, c), __fmul_rn(its, s)) : __fadd_rn(__fmul_rn(its, s), __fmul_rn(mine, c));
+    return low ? __fsub_rn(__fmul_rn(x.mine, c), __fmul_rn(x.other, s)) : __fadd_rn(__fmul_rn(x.other, s), __fmul_rn(x.mine, c));
 }
+__device__ __forceinline__ float q4_rotated(const float* head, uint32_t e, const Q4Rotation& r, size_t row) { return q4_rotated(q4_raw(head, e, r), e, r, row); }
 
 // A warp quantises a block, a value a lane: the scale (of the first value of largest magnitude), the lane's code.  The code is the integer
 // nearest to x / d + 8, and the choice is exact: x / d >= c - 8.5 is x >= (c - 8.5) d for positive d, a product of five bits and eleven
-// that fp32 holds, so the estimate from the rounded quotient, off by one at most, is put right by two comparisons.
+// that fp32 holds, so the estimate by a rounded reciprocal, off by one at most, is put right by two comparisons.
 struct Q4Quantised {
     __half scale;
     uint32_t code;
@@ -78,7 +84,7 @@ __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
         r.code = 8;
         return r;
     }
-    const float guess = fminf(fmaxf(floorf(__fadd_rn(__fdiv_rn(x, d), 8.5f)), -1.0f), 16.0f);
+    const float guess = fminf(fmaxf(floorf(fmaf(x, __frcp_rn(d), 8.5f)), -1.0f), 16.0f);
     auto reaches = [&](float c) { const float border = (c - 8.5f) * d; return d > 0.0f ? x >= border : x <= border; };
     float c = guess;
     if (!reaches(c)) c -= 1.0f;

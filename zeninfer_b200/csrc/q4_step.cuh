@@ -31,10 +31,12 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     constexpr uint32_t kStage = q4_stage_bytes<kBlocks>(), kCodes = kQ4Tile * kBlocks * 16, kScales = kQ4Tile * kBlocks * 2, kPieces = 2 * kBlocks;
     extern __shared__ __align__(128) uint8_t q4_smem[];
     __shared__ uint64_t landed[kWarps][kQ4Stages];
-    __shared__ float row_max[kWarps][4], row_sum[kWarps][4], row_unit[kWarps], row_factor[4], starts[kBlocks * 8];
+    __shared__ float row_max[kWarps][4], row_sum[kWarps][4], row_unit[kWarps], row_factor[4];
     __shared__ __align__(16) uint4 fresh_codes[4][kPieces];       // the new slots this CTA has: blocks of the key, then of the value
     __shared__ __half fresh_scales[4][kPieces];
-    __shared__ float cta_out[4][kDim], cta_max[4], cta_sum[4];    // read by the cluster
+    __shared__ float cta_out[4 * kDim];                           // read by the cluster
+    __shared__ float2 cta_stats[4];
+    __shared__ float shares[4][8], whole[4];                      // what a CTA's sums of a row count; log2 of the row's sum of weights, its maximum added
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, t = lane & 3u, h = blockIdx.z, rows = p.tokens * p.group;
     uint4* const queries = reinterpret_cast<uint4*>(q4_smem + kWarps * kQ4Stages * kStage);
     float* const kept = reinterpret_cast<float*>(queries + kBlocks * 32) + warp * kQ4ClusterTiles * 4 * kQ4Tile;
@@ -45,6 +47,20 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     __syncwarp();
     pdl_launch_dependents();
     pdl_wait();
+    // what does not depend on the place is asked for beside it: the warp's row of queries, and its block of the first new slot
+    Q4Raw raw[kBlocks], raw_fresh;
+    const uint32_t own_item = kWarps - 1 - warp;
+    if (warp < rows) {
+        const float* from = p.q + (warp / p.group) * p.q_ld + static_cast<size_t>(h * p.group + warp % p.group) * kDim;
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) raw[g] = q4_raw(from, g * 32 + lane, p.turn);
+    }
+    const float* const new_k = p.k + static_cast<size_t>(h) * kDim;
+    const float* const new_v = p.v + static_cast<size_t>(h) * kDim;
+    auto fresh_raw = [&](uint32_t token, uint32_t item) {
+        return item >= kBlocks ? Q4Raw{__ldcg(new_v + token * p.kv_ld + (item - kBlocks) * 32 + lane), 0.0f} : q4_raw(new_k + token * p.kv_ld, item * 32 + lane, p.turn);
+    };
+    if (own_item < kPieces) raw_fresh = fresh_raw(0, own_item);
     const int filled_in = *reinterpret_cast<const volatile int*>(p.filled);
     const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
     if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {       // all CTAs alike
@@ -71,43 +87,41 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
         asm volatile("fence.proxy.async;" ::: "memory");       // the stores of earlier launches come ahead of the copies
         for (uint32_t i = 0; i < min(mine, static_cast<uint32_t>(kQ4Stages)); ++i) fetch(begin + warp + i * kWarps, i);
     }
-    // the rows, rotated and laid out; zeros where there are fewer than four
-    if (warp < 4) {
-        float x[kBlocks] = {};
-        if (warp < rows) {
-            const uint32_t token = warp / p.group, head = h * p.group + warp % p.group;
-            const float* from = p.q + token * p.q_ld + static_cast<size_t>(head) * kDim;
+    // the rows, rotated and laid out, by warps 0 .. 3; zeros where there are fewer.  Blocks of new slots that lie in this CTA's tiles are quantised by all warps, from the
+    // last one down.
+    float x[kBlocks] = {};
+    if (warp < rows) {
 #pragma unroll
-            for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(from, g * 32 + lane, p.turn, static_cast<size_t>(position) + token);
-        }
-        const float factor = q4_lay_row<kBlocks, true>(x, queries, warp, p.scale, starts, lane);
-        if (lane == 0) row_factor[warp] = factor;
+        for (int g = 0; g < kBlocks; ++g) x[g] = q4_rotated(raw[g], g * 32 + lane, p.turn, static_cast<size_t>(position) + warp / p.group);
     }
-    // new slots in this CTA's tiles: each one's warp quantises it
     for (uint32_t token = 0; token < p.tokens; ++token) {
         const uint32_t tile = (filled + token) / kQ4Tile;
-        if (tile < begin || tile >= end || (tile - begin) % kWarps != warp) continue;
-        float x[kPieces];                  // all of them asked for before any is stored: one round trip
-#pragma unroll
-        for (uint32_t item = 0; item < kPieces; ++item) x[item] = q4_new_value<kBlocks>(p, h, token, item, static_cast<size_t>(position) + token, lane);
-#pragma unroll
-        for (uint32_t item = 0; item < kPieces; ++item) {
+        if (tile < begin || tile >= end) continue;
+        for (uint32_t item = own_item; item < kPieces; item += kWarps) {
+            const Q4Raw its = token == 0 && item == own_item ? raw_fresh : fresh_raw(token, item);
+            const float value = item >= kBlocks ? its.mine : q4_rotated(its, item * 32 + lane, p.turn, static_cast<size_t>(position) + token);
             __half scale;
-            const uint8_t byte = q4_append_block<kBlocks>(p, x[item], h, token, item, filled, lane, scale);
+            const uint8_t byte = q4_append_block<kBlocks>(p, value, h, token, item, filled, lane, scale);
             if (lane < 16) reinterpret_cast<uint8_t*>(&fresh_codes[token][item])[lane] = byte;
             if (lane == 0) fresh_scales[token][item] = scale;
         }
     }
+    if (warp < 4) {
+        const float factor = q4_lay_row<kBlocks, true>(x, queries, warp, p.scale, lane);
+        if (lane == 0) row_factor[warp] = factor;
+    }
     __syncthreads();
     const uint32_t last_seen = filled + min(t, rows - 1) / p.group, least = filled;      // of the lane's row, of all rows
     const float factor = row_factor[t];
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     uint4 own_query[kBlocks];
-    float start[kBlocks][4];
+    float start[kBlocks][4];               // -8 sum q of the lane's two columns: a product with sixteen slots whose codes are all -8
+    const uint32_t eights[4] = {0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u};
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
         own_query[g] = queries[g * 32 + lane];
-        start[g][0] = start[g][2] = starts[g * 8 + 2 * t];
-        start[g][1] = start[g][3] = starts[g * 8 + 2 * t + 1];
+        mma_f16(start[g], eights, own_query[g].x, own_query[g].y, zero);
+        mma_f16(start[g], eights, own_query[g].z, own_query[g].w, start[g]);
     }
     float acc[2 * kBlocks][4] = {};
     float m = -INFINITY, l = 0.0f;
@@ -115,7 +129,6 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     constexpr float kSlack = 8.0f;
     constexpr int kFull = 6, kHeadroom = 14;            // f16's exponent field less 14: the power of two above a scale
     int unit = -32;
-    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
     // A tile; kWhole: every row sees every slot of it.
     auto work = [&](const uint8_t* stage, uint32_t slot0, uint32_t turn, auto whole) {
@@ -260,68 +273,82 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     }
     if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - kFull);
     __syncthreads();
-    // the warps' shares of a row
-    for (uint32_t i = threadIdx.x; i < rows * kDim; i += kWarps * 32) {
-        const uint32_t r = i / kDim, e = i % kDim;
-        float top = row_max[0][r];
+    // the warps' shares of the rows: lane w * 4 + r of every warp has what warp w's sums of row r count
+    {
+        const float its = row_max[lane >> 2][t];
+        float top = its;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float by = its == -INFINITY ? 0.0f : exp2_fast(its - top), by_unit = by * row_unit[lane >> 2];
+        float sum = its == -INFINITY ? row_sum[lane >> 2][t] : by * row_sum[lane >> 2][t];      // no maximum: none, or what is not a number
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        for (uint32_t i = threadIdx.x; i < rows * kDim; i += kWarps * 32) {
+            const uint32_t r = i / kDim;                       // the same for all of a warp
+            float o = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, row_max[w][r]);
-        float sum = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float its = row_max[w][r], by = its == -INFINITY ? 0.0f : exp2_fast(its - top);
-            sum += by == 0.0f && its == -INFINITY ? row_sum[w][r] : by * row_sum[w][r];      // none, or what failed
-            if (its != -INFINITY) o += by * row_unit[w] * reinterpret_cast<const float*>(q4_smem + w * kQ4Stages * kStage)[r * kDim + e];
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float count = __shfl_sync(0xffffffffu, by_unit, w * 4 + r);
+                if (count != 0.0f) o += count * reinterpret_cast<const float*>(q4_smem + w * kQ4Stages * kStage)[i];      // a warp without tiles has no sums
+            }
+            if (kCluster) cta_out[i] = o;
+            else p.part_out[((static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + r) * kDim + i % kDim] = o;
         }
-        if (kCluster) {
-            cta_out[r][e] = o;
-            if (e == 0) { cta_max[r] = top; cta_sum[r] = sum; }
-        } else {
-            const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + r;
-            p.part_out[part * kDim + e] = o;
-            if (e == 0) { p.part_stats[2 * part] = top; p.part_stats[2 * part + 1] = sum; }
+        if (warp == 0 && lane < rows) {
+            if (kCluster) cta_stats[lane] = make_float2(top, sum);
+            else reinterpret_cast<float2*>(p.part_stats)[(static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + lane] = make_float2(top, sum);
         }
     }
     if constexpr (kCluster) {
         cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        // every CTA knows the rows' maxima and sums, and has a share of their dimensions
-        float top[4], sum[4];
+        float before[kQ4ClusterTiles] = {};
+        if (p.weight_out) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            top[r] = -INFINITY;
-            sum[r] = 0.0f;
-            if (r >= static_cast<int>(rows)) continue;
-            for (uint32_t c = 0; c < p.splits; ++c) top[r] = fmaxf(top[r], cluster.map_shared_rank(cta_max, c)[r]);
-            for (uint32_t c = 0; c < p.splits; ++c) {
-                const float its = cluster.map_shared_rank(cta_max, c)[r], part = cluster.map_shared_rank(cta_sum, c)[r];
-                sum[r] += its == -INFINITY ? part : exp2_fast(its - top[r]) * part;
+            for (uint32_t i = 0; i < kQ4ClusterTiles; ++i) {
+                const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
+                if (i < mine && slot < filled) before[i] = __ldcg(p.weight_in + head_slots + slot);
             }
         }
-        for (uint32_t i = blockIdx.x * (kWarps * 32) + threadIdx.x; i < rows * kDim; i += p.splits * kWarps * 32) {
-            const uint32_t r = i / kDim, e = i % kDim, token = r / p.group, head = h * p.group + r % p.group;
-            float o = 0.0f, all = 0.0f, high = 0.0f;
+        cluster.sync();
+        // warp r has row r's maxima and sums, a CTA a lane
+        if (warp < rows) {
+            const float2 its = lane < p.splits ? *cluster.map_shared_rank(cta_stats + warp, lane) : make_float2(-INFINITY, 0.0f);
+            float top = its.x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) if (k == static_cast<int>(r)) { all = sum[k]; high = top[k]; }
-            for (uint32_t c = 0; c < p.splits; ++c) {
-                const float its = cluster.map_shared_rank(cta_max, c)[r];
-                if (its != -INFINITY) o += exp2_fast(its - high) * cluster.map_shared_rank(&cta_out[0][0], c)[i];
+            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
+            float sum = its.x == -INFINITY ? its.y : by * its.y;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane < 8) shares[warp][lane] = by / sum;
+            if (lane == 0) {
+                whole[warp] = top + log2f(sum);
+                if (blockIdx.x == 0 && (!(sum > 0.0f) || !(sum < INFINITY))) atomicExch(p.error_word, kErrNonFinite);
             }
-            p.out[(static_cast<size_t>(token) * p.heads + head) * kDim + e] = o / all;
-            if (e == 0 && (!(all > 0.0f) || !(all < INFINITY))) atomicExch(p.error_word, kErrNonFinite);
+        }
+        __syncthreads();
+        // each CTA has a share of the rows' dimensions
+        for (uint32_t i = blockIdx.x * (kWarps * 32) + threadIdx.x; i < rows * kDim; i += p.splits * kWarps * 32) {
+            const uint32_t r = i / kDim, token = r / p.group, head = h * p.group + r % p.group;
+            float o = 0.0f, part[8];
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) part[c] = c < p.splits ? *cluster.map_shared_rank(cta_out + i, c) : 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) if (c < p.splits) o += shares[r][c] * part[c];
+            p.out[(static_cast<size_t>(token) * p.heads + head) * kDim + i % kDim] = o;
         }
         if (p.weight_out) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) top[r] += log2f(sum[r]);
-            for (uint32_t i = 0; i < mine; ++i) {
+            for (uint32_t i = 0; i < kQ4ClusterTiles; ++i) {
                 const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
-                if (slot >= seen) continue;
-                const size_t at = head_slots + slot;
-                float x = slot < filled ? p.weight_in[at] : 0.0f, received = 0.0f;
+                if (i >= mine || slot >= seen) continue;
+                float received = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r < static_cast<int>(rows)) received += exp2_fast(kept[(i * 4 + r) * kQ4Tile + lane] - top[r]);      // a slot the row does not see: minus infinity
-                p.weight_out[at] = received + x;
+                for (uint32_t r = 0; r < 4; ++r)
+                    if (r < rows) received += exp2_fast(kept[(i * 4 + r) * kQ4Tile + lane] - whole[r]);      // a slot the row does not see: minus infinity
+                p.weight_out[head_slots + slot] = received + before[i];
             }
         }
         cluster.sync();                     // nobody leaves while its shared memory is read
