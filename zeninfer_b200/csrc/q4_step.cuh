@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     namespace cg = cooperative_groups;
     constexpr int kWarps = kQ4StepWarps, kDim = kBlocks * 32;
     constexpr uint32_t kStage = q4_stage_bytes<kBlocks>(), kCodes = kQ4Tile * kBlocks * 16, kScales = kQ4Tile * kBlocks * 2, kPieces = 2 * kBlocks;
+    constexpr uint32_t kPitch = kDim + 8;                         // of a row of a warp's sums: a quad's rows eight banks apart
     extern __shared__ __align__(128) uint8_t q4_smem[];
     __shared__ uint64_t landed[kWarps][kQ4Stages];
     __shared__ float row_max[kWarps][4], row_sum[kWarps][4], row_unit[kWarps], row_factor[4];
@@ -36,7 +37,6 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     __shared__ __half fresh_scales[4][kPieces];
     __shared__ float cta_out[4 * kDim];                           // read by the cluster
     __shared__ float2 cta_stats[4];
-    __shared__ float shares[4][8], whole[4];                      // what a CTA's sums of a row count; log2 of the row's sum of weights, its maximum added
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, t = lane & 3u, h = blockIdx.z, rows = p.tokens * p.group;
     uint4* const queries = reinterpret_cast<uint4*>(q4_smem + kWarps * kQ4Stages * kStage);
     float* const kept = reinterpret_cast<float*>(queries + kBlocks * 32) + warp * kQ4ClusterTiles * 4 * kQ4Tile;
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     pdl_wait();
     // what does not depend on the place is asked for beside it: the warp's row of queries, and its block of the first new slot
     Q4Raw raw[kBlocks], raw_fresh;
-    const uint32_t own_item = kWarps - 1 - warp;
+    const uint32_t own_item = warp >= 4 ? warp - 4 : kPieces;
     if (warp < rows) {
         const float* from = p.q + (warp / p.group) * p.q_ld + static_cast<size_t>(h * p.group + warp % p.group) * kDim;
 #pragma unroll
@@ -87,8 +87,7 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
         asm volatile("fence.proxy.async;" ::: "memory");       // the stores of earlier launches come ahead of the copies
         for (uint32_t i = 0; i < min(mine, static_cast<uint32_t>(kQ4Stages)); ++i) fetch(begin + warp + i * kWarps, i);
     }
-    // the rows, rotated and laid out, by warps 0 .. 3; zeros where there are fewer.  Blocks of new slots that lie in this CTA's tiles are quantised by all warps, from the
-    // last one down.
+    // the rows, rotated and laid out, by warps 0 .. 3; zeros where there are fewer.  Warps 4 .. 7 quantise the blocks of new slots that lie in this CTA's tiles.
     float x[kBlocks] = {};
     if (warp < rows) {
 #pragma unroll
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     for (uint32_t token = 0; token < p.tokens; ++token) {
         const uint32_t tile = (filled + token) / kQ4Tile;
         if (tile < begin || tile >= end) continue;
-        for (uint32_t item = own_item; item < kPieces; item += kWarps) {
+        for (uint32_t item = own_item; item < kPieces; item += 4) {
             const Q4Raw its = token == 0 && item == own_item ? raw_fresh : fresh_raw(token, item);
             const float value = item >= kBlocks ? its.mine : q4_rotated(its, item * 32 + lane, p.turn, static_cast<size_t>(position) + token);
             __half scale;
@@ -141,13 +140,14 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
         {
             Q4Scales<kBlocks> d;
             d.load(k_scales, a);
+            uint32_t w[kBlocks][4];
+#pragma unroll
+            for (int g = 0; g < kBlocks; ++g) ldmatrix_x4(w[g], smem_u32(stage) + matrix + g * 128);      // all at once: they are not moved past one another
 #pragma unroll
             for (int g = 0; g < kBlocks; ++g) {
-                uint32_t w[4];
-                ldmatrix_x4(w, smem_u32(stage) + matrix + g * 128);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint32_t u = w[2 * half], v = w[2 * half + 1], x = u >> 8, y = v >> 8;
+                    const uint32_t u = w[g][2 * half], v = w[g][2 * half + 1], x = u >> 8, y = v >> 8;
                     const uint32_t even[4] = {u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u};
                     const uint32_t odd[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
                     float c[4];
@@ -158,6 +158,9 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
                 }
             }
         }
+        uint32_t values[kBlocks][4];
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g) ldmatrix_x4_trans(values[g], smem_u32(stage) + kCodes + matrix + g * 128);
         auto hidden = [&](int i) { return !kWhole && slot0 + 8 * i + a > last_seen; };
         // the largest scale of a value that any row sees, as a power of two
         const uint32_t top = __reduce_max_sync(0xffffffffu, kWhole || slot0 + lane < seen ? Q4Scales<kBlocks>::largest(v_scales, lane) : 0u);
@@ -200,12 +203,10 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
         d.load(v_scales, a);
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g) {
-            uint32_t w[4];
-            ldmatrix_x4_trans(w, smem_u32(stage) + kCodes + matrix + g * 128);
             float sum[2][4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint32_t u = w[2 * half], v = w[2 * half + 1], x = u >> 8, y = v >> 8;
+                const uint32_t u = values[g][2 * half], v = values[g][2 * half + 1], x = u >> 8, y = v >> 8;
                 // dimensions 2r and 16 + 2r, 2r + 1 and 17 + 2r of the block, r the lane's row of the operand
                 const uint32_t even[4] = {signed_low(u), signed_high(u), signed_low(v), signed_high(v)};
                 const uint32_t odd[4] = {signed_low(x), signed_high(x), signed_low(y), signed_high(y)};
@@ -263,92 +264,88 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     l += __shfl_xor_sync(0xffffffffu, l, 8);
     l += __shfl_xor_sync(0xffffffffu, l, 16);
     if (lane < 4) { row_max[warp][t] = m; row_sum[warp][t] = failed ? NAN : l; }
-    if (mine) {
 #pragma unroll
-        for (int j = 0; j < 2 * kBlocks; ++j) {
-            const uint32_t e = (j / 2) * 32 + 2 * (lane >> 2) + (j & 1);
-            sums[t * kDim + e] = acc[j][0] + acc[j][1];
-            sums[t * kDim + e + 16] = acc[j][2] + acc[j][3];
-        }
+    for (int g = 0; g < kBlocks; ++g) {
+        const float (&c)[4] = acc[2 * g];
+        const float (&d)[4] = acc[2 * g + 1];
+        float2* to = reinterpret_cast<float2*>(sums + t * kPitch + g * 32) + (lane >> 2);
+        to[0] = make_float2(c[0] + c[1], d[0] + d[1]);
+        to[8] = make_float2(c[2] + c[3], d[2] + d[3]);
     }
     if (lane == 0) row_unit[warp] = unit == -32 ? 0.0f : power_of_two(unit - kFull);
     __syncthreads();
     // the warps' shares of the rows: lane w * 4 + r of every warp has what warp w's sums of row r count
+    auto over_groups_of_four = [](float x, auto op) {
+        x = op(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = op(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        return op(x, __shfl_xor_sync(0xffffffffu, x, 16));
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto added = [](float x, float y) { return x + y; };
+    float weight_before[kQ4ClusterTiles] = {};
+    if (kCluster && p.weight_out) {
+#pragma unroll
+        for (uint32_t i = 0; i < kQ4ClusterTiles; ++i) {
+            const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
+            if (i < mine && slot < filled) weight_before[i] = __ldcg(p.weight_in + head_slots + slot);
+        }
+    }
     {
-        const float its = row_max[lane >> 2][t];
-        float top = its;
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float its = row_max[lane >> 2][t], top = over_groups_of_four(its, larger);
         const float by = its == -INFINITY ? 0.0f : exp2_fast(its - top), by_unit = by * row_unit[lane >> 2];
-        float sum = its == -INFINITY ? row_sum[lane >> 2][t] : by * row_sum[lane >> 2][t];      // no maximum: none, or what is not a number
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const float sum = over_groups_of_four(its == -INFINITY ? row_sum[lane >> 2][t] : by * row_sum[lane >> 2][t], added);      // no maximum: none, or what is not a number
         for (uint32_t i = threadIdx.x; i < rows * kDim; i += kWarps * 32) {
             const uint32_t r = i / kDim;                       // the same for all of a warp
-            float o = 0.0f;
+            float o = 0.0f, part[kWarps];
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) {
-                const float count = __shfl_sync(0xffffffffu, by_unit, w * 4 + r);
-                if (count != 0.0f) o += count * reinterpret_cast<const float*>(q4_smem + w * kQ4Stages * kStage)[i];      // a warp without tiles has no sums
-            }
+            for (uint32_t w = 0; w < kWarps; ++w) part[w] = reinterpret_cast<const float*>(q4_smem + w * kQ4Stages * kStage)[r * kPitch + i % kDim];
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) o += __shfl_sync(0xffffffffu, by_unit, w * 4 + r) * part[w];
             if (kCluster) cta_out[i] = o;
             else p.part_out[((static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + r) * kDim + i % kDim] = o;
         }
-        if (warp == 0 && lane < rows) {
+        if (warp == 0 && lane < 4) {
             if (kCluster) cta_stats[lane] = make_float2(top, sum);
-            else reinterpret_cast<float2*>(p.part_stats)[(static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + lane] = make_float2(top, sum);
+            else if (lane < rows) reinterpret_cast<float2*>(p.part_stats)[(static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + lane] = make_float2(top, sum);
         }
     }
     if constexpr (kCluster) {
         cg::cluster_group cluster = cg::this_cluster();
-        float before[kQ4ClusterTiles] = {};
-        if (p.weight_out) {
-#pragma unroll
-            for (uint32_t i = 0; i < kQ4ClusterTiles; ++i) {
-                const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
-                if (i < mine && slot < filled) before[i] = __ldcg(p.weight_in + head_slots + slot);
-            }
-        }
         cluster.sync();
-        // warp r has row r's maxima and sums, a CTA a lane
-        if (warp < rows) {
-            const float2 its = lane < p.splits ? *cluster.map_shared_rank(cta_stats + warp, lane) : make_float2(-INFINITY, 0.0f);
-            float top = its.x;
+        // the CTAs' shares likewise: lane c * 4 + r of every warp has what CTA c's sums of row r count
+        const float2 its = (lane >> 2) < p.splits ? *cluster.map_shared_rank(cta_stats + t, lane >> 2) : make_float2(-INFINITY, 0.0f);
+        float part[8];
+        const uint32_t i = blockIdx.x * (kWarps * 32) + threadIdx.x;          // each CTA has a share of the rows' dimensions
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
-            float sum = its.x == -INFINITY ? its.y : by * its.y;
+        for (uint32_t c = 0; c < 8; ++c) part[c] = c < p.splits && i < rows * kDim ? *cluster.map_shared_rank(cta_out + i, c) : 0.0f;
+        const float top = over_groups_of_four(its.x, larger), by = its.x == -INFINITY ? 0.0f : exp2_fast(its.x - top);
+        const float sum = over_groups_of_four(its.x == -INFINITY ? its.y : by * its.y, added), share = by / sum;
+        if (blockIdx.x == 0 && warp == 0 && lane < rows && (!(sum > 0.0f) || !(sum < INFINITY))) atomicExch(p.error_word, kErrNonFinite);
+        auto put = [&](uint32_t at, const float (&of)[8]) {
+            const uint32_t r = min(at / kDim, 3u), token = r / p.group, head = h * p.group + r % p.group;
+            float o = 0.0f;
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane < 8) shares[warp][lane] = by / sum;
-            if (lane == 0) {
-                whole[warp] = top + log2f(sum);
-                if (blockIdx.x == 0 && (!(sum > 0.0f) || !(sum < INFINITY))) atomicExch(p.error_word, kErrNonFinite);
-            }
-        }
-        __syncthreads();
-        // each CTA has a share of the rows' dimensions
-        for (uint32_t i = blockIdx.x * (kWarps * 32) + threadIdx.x; i < rows * kDim; i += p.splits * kWarps * 32) {
-            const uint32_t r = i / kDim, token = r / p.group, head = h * p.group + r % p.group;
-            float o = 0.0f, part[8];
+            for (uint32_t c = 0; c < 8; ++c) o += __shfl_sync(0xffffffffu, share, c * 4 + r) * of[c];
+            if (at < rows * kDim) p.out[(static_cast<size_t>(token) * p.heads + head) * kDim + at % kDim] = o;
+        };
+        put(i, part);
+        for (uint32_t more = i + p.splits * kWarps * 32; more - threadIdx.x % 32 < rows * kDim; more += p.splits * kWarps * 32) {
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) part[c] = c < p.splits ? *cluster.map_shared_rank(cta_out + i, c) : 0.0f;
-#pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) if (c < p.splits) o += shares[r][c] * part[c];
-            p.out[(static_cast<size_t>(token) * p.heads + head) * kDim + i % kDim] = o;
+            for (uint32_t c = 0; c < 8; ++c) part[c] = c < p.splits && more < rows * kDim ? *cluster.map_shared_rank(cta_out + more, c) : 0.0f;
+            put(more, part);
         }
         if (p.weight_out) {
+            const float whole = top + log2f(sum);              // of row t
 #pragma unroll
-            for (uint32_t i = 0; i < kQ4ClusterTiles; ++i) {
-                const uint32_t slot = (begin + warp + i * kWarps) * kQ4Tile + lane;
-                if (i >= mine || slot >= seen) continue;
+            for (uint32_t j = 0; j < kQ4ClusterTiles; ++j) {
                 float received = 0.0f;
 #pragma unroll
-                for (uint32_t r = 0; r < 4; ++r)
-                    if (r < rows) received += exp2_fast(kept[(i * 4 + r) * kQ4Tile + lane] - whole[r]);      // a slot the row does not see: minus infinity
-                p.weight_out[head_slots + slot] = received + before[i];
+                for (uint32_t r = 0; r < 4; ++r) {
+                    const float of_row = __shfl_sync(0xffffffffu, whole, r);
+                    if (r < rows && j < mine) received += exp2_fast(kept[(j * 4 + r) * kQ4Tile + lane] - of_row);      // a slot the row does not see: minus infinity
+                }
+                const uint32_t slot = (begin + warp + j * kWarps) * kQ4Tile + lane;
+                if (j < mine && slot < seen) p.weight_out[head_slots + slot] = received + weight_before[j];
             }
         }
         cluster.sync();                     // nobody leaves while its shared memory is read
