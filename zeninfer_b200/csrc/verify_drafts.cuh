@@ -57,12 +57,18 @@ struct VerifyParams {
     int* error_word;
 };
 
-// What a CTA hands to the others.
+// What a CTA hands to the others, by the exchange it belongs to: a field is written for one of them only, so a reader needs no barrier behind it.
 struct VerifyShare {
-    double sum;
-    unsigned long long ties;
-    uint32_t top_key, low_key, count;
+    double reference, sum;             // the value its exponentials are relative to, and their sum
+    double kept, left;                 // the sum of what a cut left; of max(p - q, 0), both in the row's units
+    double left_again;
+    unsigned long long ties, each;
+    uint32_t top_key, low_key, finite;
+    uint32_t listed, bin_high, bin_low, any_each;
 };
+
+// The integer nearest to x, 0 <= x <= 2^51: what is left of 2^52 + x in its lower bits.
+__device__ __forceinline__ unsigned long long nearest(double x) { return static_cast<unsigned long long>(__double_as_longlong(x + 4503599627370496.0)) & 0xfffffffffffffull; }
 
 template <int kCtas>
 __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
@@ -71,12 +77,15 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     __shared__ VerifyShare share;
     __shared__ double warp_sum[32], s_q;
     __shared__ unsigned long long warp_total[32], s_left;
-    __shared__ uint32_t warp_count[32], s_bin, s_mine;
+    __shared__ uint32_t warp_high[32], warp_low[32], warp_count[32], s_bin, s_mine, s_high, s_low, s_count, s_before, s_fits;
+    __shared__ double s_sum, s_ahead, s_scale;
+    __shared__ int s_last;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), row = blockIdx.y;
     double* e = reinterpret_cast<double*>(verify_smem);                      // [per_cta]
     float* v = reinterpret_cast<float*>(e + p.per_cta);                      // [per_cta], per_cta a multiple of four
-    uint32_t* limbs = reinterpret_cast<uint32_t*>(v + p.per_cta);            // [kVerifyLimbs][kVerifyBins]
+    uint32_t* limbs = reinterpret_cast<uint32_t*>(v + p.per_cta);            // [kVerifyLimbs][kVerifyBins], then the bins' totals
+    unsigned long long* totals = reinterpret_cast<unsigned long long*>(limbs);
     VerifyEntry* own_list = reinterpret_cast<VerifyEntry*>(limbs + kVerifyLimbs * kVerifyBins);
     VerifyEntry* all_list = own_list + kVerifyMine;
     const uint32_t base = rank * p.per_cta, n = base < p.vocab ? min(p.per_cta, p.vocab - base) : 0u;
@@ -91,71 +100,65 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         if (rank == 0 && tid == 0) atomicExch(p.error_word, kErrBadToken);
         token = -1;
     }
-
-    // sums over the cluster, the same in every CTA: of a double a thread, in the order of threads and CTAs
-    auto cluster_sum = [&](double mine) {
+    const bool has_token = token >= 0 && token / p.per_cta == rank;
+    // What the CTAs hand over is read by warp 0, lane r from CTA r, and told to the others: a request of every warp for the same word costs as much as its own.
+    auto its = [&](uint32_t r) { return cluster.map_shared_rank(&share, r); };
+    const bool reads = warp == 0 && lane < kCtas;
+    auto value_of = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); };
+    // a CTA's sum, in every thread: of threads and warps in order
+    auto cta_sum = [&](double mine) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mine += __shfl_down_sync(0xffffffffu, mine, o);
+        __syncthreads();
         if (lane == 0) warp_sum[warp] = mine;
         __syncthreads();
-        if (tid == 0) {
-            double s = 0.0;
-            for (int w = 0; w < 32; ++w) s += warp_sum[w];
-            share.sum = s;
-        }
-        cluster.sync();
-        double s = 0.0;
-        for (int r = 0; r < kCtas; ++r) s += cluster.map_shared_rank(&share, r)->sum;
-        cluster.sync();
+        double s = warp_sum[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         return s;
     };
+    // the largest and the smallest key and the number of entries of a CTA, in every thread
+    auto cta_range = [&](uint32_t& high, uint32_t& low, uint32_t& count) {
+        high = __reduce_max_sync(0xffffffffu, high);
+        low = __reduce_min_sync(0xffffffffu, low);
+        count = __reduce_add_sync(0xffffffffu, count);
+        __syncthreads();
+        if (lane == 0) { warp_high[warp] = high; warp_low[warp] = low; warp_count[warp] = count; }
+        __syncthreads();
+        high = __reduce_max_sync(0xffffffffu, warp_high[lane]);
+        low = __reduce_min_sync(0xffffffffu, warp_low[lane]);
+        count = __reduce_add_sync(0xffffffffu, warp_count[lane]);
+    };
 
-    // the logits, the largest of the finite ones and how many there are
-    uint32_t top = 0, finite = 0;
-    for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-        const float x = __ldcg(logits + i) + 0.0f;      // the zeros are equal
+    // the logits, the largest and smallest of the finite ones and how many there are
+    uint32_t top = 0, low = 0xffffffffu, finite = 0;
+    auto take = [&](uint32_t i, float x) {
+        x += 0.0f;                                      // the zeros are equal
         const uint32_t key = sample_key(x);
         v[i] = x;
         top = max(top, key);
+        if (key) low = min(low, key);
         finite += key != 0u;
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    finite = __reduce_add_sync(0xffffffffu, finite);
-    if (tid == 0) { share.top_key = 0; share.count = 0; }
-    __syncthreads();
-    if (lane == 0) { atomicMax(&share.top_key, top); atomicAdd(&share.count, finite); }
-    cluster.sync();
-    top = 0;
-    finite = 0;
-    for (int r = 0; r < kCtas; ++r) { top = max(top, cluster.map_shared_rank(&share, r)->top_key); finite += cluster.map_shared_rank(&share, r)->count; }
-    cluster.sync();
-    if (!finite) {
-        if (rank == 0 && tid == 0) {
-            p.draws[row] = -1;
-            p.fits[row] = 0;
-            if (is_draft && p.probs) p.probs[row] = 0.0;
+    };
+    if (reinterpret_cast<uintptr_t>(logits) % 16 == 0) {
+#pragma unroll 4
+        for (uint32_t i = 4 * tid; i + 3 < n; i += 4 * kVerifyThreads) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(logits + i));
+            take(i, x.x); take(i + 1, x.y); take(i + 2, x.z); take(i + 3, x.w);
         }
-        return;
+        if (const uint32_t i = (n & ~3u) + tid; i < n) take(i, __ldcg(logits + i));
+    } else {
+#pragma unroll 4
+        for (uint32_t i = tid; i < n; i += kVerifyThreads) take(i, __ldcg(logits + i));
     }
-    const double highest = __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
-    auto drop = [&](uint32_t i, bool with_exponentials) {
-        v[i] = NAN;
-        if (with_exponentials) e[i] = 0.0;
-    };
-    // the largest and the smallest key of the entries that take part, over the cluster
-    auto key_range = [&](uint32_t& high, uint32_t& low) {
-        high = __reduce_max_sync(0xffffffffu, high);
-        low = __reduce_min_sync(0xffffffffu, low);
-        if (tid == 0) { share.top_key = 0; share.low_key = 0xffffffffu; }
-        __syncthreads();
-        if (lane == 0) { atomicMax(&share.top_key, high); atomicMin(&share.low_key, low); }
-        cluster.sync();
-        for (int r = 0; r < kCtas; ++r) { high = max(high, cluster.map_shared_rank(&share, r)->top_key); low = min(low, cluster.map_shared_rank(&share, r)->low_key); }
-        cluster.sync();
-    };
-    auto value_of = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); };
+    cta_range(top, low, finite);
+    const bool greedy = p.temperature == 0.0;
+    const uint32_t top_k = greedy ? 1u : p.top_k;
+    const double temperature = greedy ? 1.0 : p.temperature, per_unit = 1.0 / temperature;
+
+    auto drop = [&](uint32_t i) { v[i] = NAN; e[i] = 0.0; };
     // Of the entries that equal `border` all behind the first `ties` (in order of id) go, and so do all below it.
-    auto cut_ties = [&](uint32_t border, unsigned long long ties, bool with_exponentials) {
+    auto cut_ties = [&](uint32_t border, unsigned long long ties) {
         uint32_t equal = 0;
         for (uint32_t i = begin; i < end; ++i) equal += sample_key(v[i]) == border;
         uint32_t upto = equal;
@@ -170,43 +173,49 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         if (tid == kVerifyThreads - 1) share.ties = before + equal;
         cluster.sync();
         unsigned long long seen = before;
-        for (uint32_t r = 0; r < rank; ++r) seen += cluster.map_shared_rank(&share, r)->ties;
+        for (uint32_t r = 0; r < rank; ++r) seen += its(r)->ties;
         cluster.sync();
         for (uint32_t i = begin; i < end; ++i) {
             const uint32_t key = sample_key(v[i]);
-            if (key < border || (key == border && seen++ >= ties)) drop(i, with_exponentials);
+            if (key < border || (key == border && seen++ >= ties)) drop(i);
         }
         __syncthreads();
     };
     // Leaves the shortest run of entries, in descending order (equal values: the lowest ids), whose weights reach `wanted` > 0, at least one.
-    // weigh(i): an entry's weight.  low: no entry that takes part is below it.
-    auto cut = [&](unsigned long long wanted, auto weigh, uint32_t low, double reach, bool with_exponentials) {
-        uint32_t high = top;
-        double v_low = fmax(static_cast<double>(value_of(low)), highest - reach);       // far below, nothing is worth bins of its own
+    // weigh(i): an entry's weight.  high, low: keys that no entry which takes part is beyond.
+    auto cut = [&](unsigned long long wanted, auto weigh, uint32_t high, uint32_t low) {
+        double v_low = fmax(static_cast<double>(value_of(low)), static_cast<double>(value_of(high)) - 64.0 * temperature);      // far below, nothing is worth bins of its own
         for (;;) {
             if (high == low) {         // equal values: so many of them as are wanted, each of the same weight
-                if (tid == 0) share.count = 0;
-                __syncthreads();
                 unsigned long long each = 0;
+                if (tid == 0) share.any_each = 0;
+                __syncthreads();
                 for (uint32_t i = tid; i < n; i += kVerifyThreads) if (sample_key(v[i]) == high) each = weigh(i);
-                if (each) atomicExch(&s_left, each);
-                if (each && !share.count) share.count = 1;
+                if (each) { share.each = each; share.any_each = 1; }
                 cluster.sync();
-                for (int r = 0; r < kCtas; ++r) if (cluster.map_shared_rank(&share, r)->count) each = *cluster.map_shared_rank(&s_left, r);
+                for (int r = 0; r < kCtas; ++r) if (its(r)->any_each) each = its(r)->each;
                 cluster.sync();
                 each = max(each, 1ull);
-                cut_ties(high, (wanted + each - 1) / each, with_exponentials);
+                cut_ties(high, (wanted + each - 1) / each);
                 return;
             }
+            // 1024 bins from the top down; in 32 bits (of halves, which do not overflow) where the range allows it: either way a larger value has no larger bin
             const double v_high = value_of(high), per = kVerifyBins / (v_high - v_low);
-            auto bin_of = [&](float x) { return static_cast<uint32_t>(fmin((v_high - static_cast<double>(x)) * per, kVerifyBins - 1.0)); };
+            const float half_high = 0.5f * value_of(high), per_half = static_cast<float>(2.0 * per);
+            const bool narrow = !(per_half > 1e-30f && per_half < 1e30f);
+            auto bin_of = [&](float x) {
+                return narrow ? static_cast<uint32_t>(fmin((v_high - static_cast<double>(x)) * per, kVerifyBins - 1.0)) : static_cast<uint32_t>(fminf((half_high - 0.5f * x) * per_half, kVerifyBins - 1.0f));
+            };
             for (uint32_t i = tid; i < kVerifyLimbs * kVerifyBins; i += kVerifyThreads) limbs[i] = 0;
+            if (tid == 0) { s_bin = 0xffffffffu; s_mine = 0; }
             __syncthreads();
+#pragma unroll 4
             for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-                const uint32_t key = sample_key(v[i]);
+                const float x = v[i];
+                const uint32_t key = sample_key(x);
                 if (!key || key > high || key < low) continue;
                 const unsigned long long w = weigh(i);
-                const uint32_t bin = bin_of(v[i]);
+                const uint32_t bin = bin_of(x);
 #pragma unroll
                 for (int k = 0; k < kVerifyLimbs; ++k) {
                     uint32_t limb = static_cast<uint32_t>(w >> (k * kVerifyLimbBits));
@@ -214,210 +223,276 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
                     if (limb) atomicAdd(limbs + k * kVerifyBins + bin, limb);
                 }
             }
+            __syncthreads();
+            unsigned long long mine = 0;
+#pragma unroll
+            for (int k = 0; k < kVerifyLimbs; ++k) mine += static_cast<unsigned long long>(limbs[k * kVerifyBins + tid]) << (k * kVerifyLimbBits);
+            __syncthreads();
+            totals[tid] = mine;
             cluster.sync();
             // thread j has bin j of the whole row
-            unsigned long long mine = 0;
-            for (int r = 0; r < kCtas; ++r) {
-                const uint32_t* its = cluster.map_shared_rank(limbs, r) + tid;
+            mine = 0;
 #pragma unroll
-                for (int k = 0; k < kVerifyLimbs; ++k) mine += static_cast<unsigned long long>(its[k * kVerifyBins]) << (k * kVerifyLimbBits);
-            }
+            for (int r = 0; r < kCtas; ++r) mine += cluster.map_shared_rank(totals, r)[tid];
             unsigned long long upto = mine;
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
                 if (static_cast<int>(lane) >= o) upto += x;
             }
             if (lane == 31) warp_total[warp] = upto;
-            if (tid == 0) { s_bin = 0xffffffffu; s_left = wanted; s_mine = 0; }
             __syncthreads();
-            unsigned long long before = 0;
-            for (uint32_t w = 0; w < warp; ++w) before += warp_total[w];
+            unsigned long long before = lane < warp ? warp_total[lane] : 0ull;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
             upto += before;
             if (upto >= wanted && upto - mine < wanted) { s_bin = tid; s_left = wanted - (upto - mine); }        // one thread at most
-            cluster.sync();                                                                                       // and everybody has read the limbs
-            if (s_bin == 0xffffffffu) {      // rounding left the whole short of what is wanted: everything stays
-                for (uint32_t i = tid; i < n; i += kVerifyThreads) if (sample_key(v[i]) < low) drop(i, with_exponentials);
-                cluster.sync();
-                return;
-            }
-            const uint32_t border = s_bin;
-            wanted = s_left;
+            __syncthreads();
+            const uint32_t border = s_bin;                  // none: rounding left the whole short of what is wanted, and everything stays
+            if (border != 0xffffffffu) wanted = s_left;
             // what lies below the border goes; the entries of its bin are listed, and counted on where there are too many
-            uint32_t bin_high = 0, bin_low = 0xffffffffu;
+            uint32_t bin_high = 0, bin_low = 0xffffffffu, unused = 0;
+#pragma unroll 4
             for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-                const uint32_t key = sample_key(v[i]);
+                const float x = v[i];
+                const uint32_t key = sample_key(x);
                 if (!key || key > high) continue;
-                const uint32_t bin = key < low ? kVerifyBins : bin_of(v[i]);
-                if (bin > border) drop(i, with_exponentials);
-                if (bin != border) continue;
-                bin_high = max(bin_high, key);
-                bin_low = min(bin_low, key);
-                const uint32_t at = atomicAdd(&s_mine, 1u);
-                if (at < kVerifyMine) own_list[at] = VerifyEntry{weigh(i), v[i], base + i};
+                const uint32_t bin = key < low ? kVerifyBins : bin_of(x);
+                if (bin > border || key < low) drop(i);
+                else if (bin == border) {
+                    bin_high = max(bin_high, key);
+                    bin_low = min(bin_low, key);
+                    const uint32_t at = atomicAdd(&s_mine, 1u);
+                    if (at < kVerifyMine) own_list[at] = VerifyEntry{weigh(i), x, base + i};
+                }
+            }
+            cta_range(bin_high, bin_low, unused);
+            if (tid == 0) { share.listed = s_mine; share.bin_high = bin_high; share.bin_low = bin_low; }
+            cluster.sync();
+            if (border == 0xffffffffu) return;
+            if (warp == 0) {
+                const uint32_t listed = reads ? its(lane)->listed : 0u;
+                bin_high = __reduce_max_sync(0xffffffffu, reads ? its(lane)->bin_high : 0u);
+                bin_low = __reduce_min_sync(0xffffffffu, reads ? its(lane)->bin_low : 0xffffffffu);
+                const uint32_t all = __reduce_add_sync(0xffffffffu, listed), ahead = __reduce_add_sync(0xffffffffu, lane < rank ? listed : 0u);
+                const bool fit = __all_sync(0xffffffffu, listed <= kVerifyMine);
+                if (lane == 0) { s_count = all; s_before = ahead; s_fits = fit; s_high = bin_high; s_low = bin_low; }
             }
             __syncthreads();
-            if (tid == 0) share.count = s_mine;
-            cluster.sync();
-            uint32_t count = 0, before_mine = 0;
-            bool fits = true;
-            for (uint32_t r = 0; r < kCtas; ++r) {
-                const uint32_t its = cluster.map_shared_rank(&share, r)->count;
-                fits &= its <= kVerifyMine;
-                if (r < rank) before_mine += its;
-                count += its;
-            }
+            const uint32_t count = s_count, before_mine = s_before;
+            const bool fits = s_fits;
             if (!fits || count > kVerifyAll) {
-                cluster.sync();
-                key_range(bin_high, bin_low);
-                high = bin_high;
-                low = bin_low;
+                high = s_high;
+                low = s_low;
                 v_low = value_of(low);
                 continue;
             }
-            for (uint32_t r = 0, at = 0; r < kCtas; ++r) {
-                const uint32_t its = cluster.map_shared_rank(&share, r)->count;
-                if (tid < its) all_list[at + tid] = cluster.map_shared_rank(own_list, r)[tid];
-                at += its;
+            for (uint32_t r = warp; r < kCtas; r += 32) {      // a warp a CTA: its entries behind those of the CTAs before
+                uint32_t at = 0;
+                const uint32_t listed = lane < kCtas ? its(lane)->listed : 0u;
+                at = __reduce_add_sync(0xffffffffu, lane < r ? listed : 0u);
+                const uint32_t theirs = __shfl_sync(0xffffffffu, listed, r);
+                for (uint32_t i = lane; i < theirs; i += 32) all_list[at + i] = cluster.map_shared_rank(own_list, r)[i];
             }
-            cluster.sync();
+            __syncthreads();
             // a warp decides an entry of the CTA's: it stays when what comes before it does not reach what is wanted
             for (uint32_t i = warp; i < s_mine; i += 32) {
                 const VerifyEntry me = all_list[before_mine + i];
                 unsigned long long sum = 0;
                 for (uint32_t j = lane; j < count; j += 32) {
-                    const VerifyEntry its = all_list[j];
-                    if (its.value > me.value || (its.value == me.value && its.id < me.id)) sum += its.weight;
+                    const VerifyEntry other = all_list[j];
+                    if (other.value > me.value || (other.value == me.value && other.id < me.id)) sum += other.weight;
                 }
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0 && sum >= wanted) drop(me.id - base, with_exponentials);
+                if (lane == 0 && sum >= wanted) drop(me.id - base);
             }
             __syncthreads();
             return;
         }
     };
 
-    const bool greedy = p.temperature == 0.0;
-    const uint32_t top_k = greedy ? 1u : p.top_k;
-    const double temperature = greedy ? 1.0 : p.temperature;
-    // the smallest key of a row is asked for once, by its first cut
-    uint32_t least = 0xffffffffu;
-    auto least_key = [&]() {
-        for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-            const uint32_t key = sample_key(v[i]);
-            if (key) least = min(least, key);
+    double reference = value_of(top);              // what the CTA's exponentials are relative to; without an entry, anything
+    if (!top) reference = -INFINITY;
+    if (top_k && top_k < p.vocab) {
+        if (tid == 0) { share.top_key = top; share.low_key = low; share.finite = finite; }
+        cluster.sync();
+        if (warp == 0) {
+            const uint32_t high = __reduce_max_sync(0xffffffffu, reads ? its(lane)->top_key : 0u), lowest = __reduce_min_sync(0xffffffffu, reads ? its(lane)->low_key : 0xffffffffu);
+            const uint32_t all = __reduce_add_sync(0xffffffffu, reads ? its(lane)->finite : 0u);
+            if (lane == 0) { s_high = high; s_low = lowest; s_count = all; }
         }
-        uint32_t ignored = 0;
-        key_range(ignored, least);
-        return least;
-    };
-    if (top_k && top_k < finite) cut(top_k, [](uint32_t) { return 1ull; }, least_key(), 64.0 * temperature, false);
+        cluster.sync();                            // the fields are written again below
+        const uint32_t row_top = s_high, row_low = s_low, row_finite = s_count;
+        __syncthreads();
+        if (top_k < row_finite) cut(top_k, [](uint32_t) { return 1ull; }, row_top, row_low);
+    }
+    // exponentials relative to the CTA's own largest value: no one waits for the row's
     double mine = 0.0;
+#pragma unroll 4
     for (uint32_t i = begin; i < end; ++i) {
         const float x = v[i];
-        const double w = sample_key(x) ? exp((static_cast<double>(x) - highest) / temperature) : 0.0;
+        const double w = sample_key(x) ? exp((static_cast<double>(x) - reference) * per_unit) : 0.0;
         e[i] = w;
         mine += w;
     }
-    double sum = cluster_sum(mine);
-    if (!greedy && p.top_p > 0.0f && p.top_p < 1.0f) {
-        const double unit = kVerifyUnit / sum;
-        least = 0xffffffffu;
-        cut(max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit)), [&](uint32_t i) { return static_cast<unsigned long long>(__double2ll_rn(e[i] * unit)); }, least_key(),
-            64.0 * temperature, true);
-        mine = 0.0;
-        for (uint32_t i = begin; i < end; ++i) mine += e[i];
-        sum = cluster_sum(mine);
+    mine = cta_sum(mine);
+    if (tid == 0) { share.reference = reference; share.sum = mine; share.top_key = top; share.low_key = low; share.finite = finite; }
+    cluster.sync();
+    if (warp == 0) {
+        // what a CTA's exponentials count in the row
+        const double theirs = reads ? its(lane)->reference : -INFINITY;
+        double highest = theirs;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) highest = fmax(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+        const double factor = theirs == -INFINITY ? 0.0 : exp((theirs - highest) * per_unit);
+        double all = reads ? factor * its(lane)->sum : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        const uint32_t high = __reduce_max_sync(0xffffffffu, reads ? its(lane)->top_key : 0u), lowest = __reduce_min_sync(0xffffffffu, reads ? its(lane)->low_key : 0xffffffffu);
+        const uint32_t count = __reduce_add_sync(0xffffffffu, reads ? its(lane)->finite : 0u);
+        if (lane == rank) s_scale = factor;
+        if (lane == 0) { s_sum = all; s_high = high; s_low = lowest; s_count = count; }
     }
-    // e becomes p, then p - q
-    for (uint32_t i = begin; i < end; ++i) e[i] /= sum;
-    if (tid == 0) s_q = 0.0;
     __syncthreads();
-    const uint32_t entries = is_draft && p.q_ids ? static_cast<uint32_t>(min(max(__ldcg(p.q_count + row), 0), static_cast<int>(kSampleMaxCandidates))) : 0u;
-    const size_t list = static_cast<size_t>(row) * kSampleMaxCandidates;
-    if (is_draft && token >= 0 && token / p.per_cta == rank) {       // the CTA that has the draft decides
-        if (p.q_ids) {
-            for (uint32_t j = tid; j < entries; j += kVerifyThreads)
-                if (__ldcg(p.q_ids + list + j) == token) s_q = __ldcg(p.q_probs + list + j);
-            __syncthreads();
+    const double whole = s_sum, scale = s_scale;
+    const uint32_t row_top = s_high, row_low = s_low, row_finite = s_count;
+    if (!row_finite) {
+        if (rank == 0 && tid == 0) {
+            p.draws[row] = -1;
+            p.fits[row] = 0;
+            if (is_draft && p.probs) p.probs[row] = 0.0;
         }
-        if (tid == 0) {
-            const double mine_p = e[token - base], q = p.q_ids ? s_q : 1.0;
-            p.fits[row] = __ldcg(p.uniforms + row) * q < mine_p;
-            if (p.probs) p.probs[row] = mine_p;
+        cluster.sync();                            // nobody leaves while its shared memory is read
+        return;
+    }
+
+    double kept = whole;                           // the sum that makes probabilities of exponentials
+    if (!greedy && p.top_p > 0.0f && p.top_p < 1.0f) {
+        const double unit = kVerifyUnit * (scale / whole);
+        cut(max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit)), [&](uint32_t i) { return nearest(e[i] * unit); }, row_top, row_low);
+        mine = 0.0;
+#pragma unroll 4
+        for (uint32_t i = begin; i < end; ++i) mine += e[i];
+        mine = cta_sum(mine);
+        if (tid == 0) share.kept = mine * scale;
+        cluster.sync();
+        if (warp == 0) {
+            double all = reads ? its(lane)->kept : 0.0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            if (lane == 0) s_sum = all;
         }
         __syncthreads();
+        kept = s_sum;
+    }
+    // The CTA that has the draft decides, and e becomes p - q where a draft may be replaced, both in the CTA's units
+    const uint32_t entries = is_draft && p.q_ids ? static_cast<uint32_t>(min(max(__ldcg(p.q_count + row), 0), static_cast<int>(kSampleMaxCandidates))) : 0u;
+    const size_t list = static_cast<size_t>(row) * kSampleMaxCandidates;
+    const double of_one = kept / scale;            // a probability of 1
+    if (tid == 0) s_q = 0.0;
+    __syncthreads();
+    if (has_token) {
+        for (uint32_t j = tid; j < entries; j += kVerifyThreads)
+            if (__ldcg(p.q_ids + list + j) == token) s_q = __ldcg(p.q_probs + list + j);
+        __syncthreads();
+        if (tid == 0) {
+            const double mine_p = e[token - base] * scale / kept, q = p.q_ids ? s_q : 1.0;
+            p.fits[row] = __ldcg(p.uniforms + row) * q < mine_p;
+            if (p.probs) p.probs[row] = mine_p;
+            if (!p.q_ids) e[token - base] = fmax(e[token - base] - of_one, 0.0);
+        }
     } else if (is_draft && token < 0 && rank == 0 && tid == 0) {
         p.fits[row] = 0;
         if (p.probs) p.probs[row] = 0.0;
     }
-    // what is left, and whether anything is: a copy of p is not kept, a row with nothing left is formed anew
-    double left = 0.0;
-    if (is_draft) {
-        if (p.q_ids) {
-            for (uint32_t j = tid; j < entries; j += kVerifyThreads) {
-                const int id = __ldcg(p.q_ids + list + j);
-                if (id >= 0 && static_cast<uint32_t>(id) >= base && static_cast<uint32_t>(id) - base < n) e[id - base] = fmax(e[id - base] - __ldcg(p.q_probs + list + j), 0.0);
-            }
-        } else if (tid == 0 && token >= 0 && token / p.per_cta == rank) {
-            e[token - base] = fmax(e[token - base] - 1.0, 0.0);
+    __syncthreads();
+    for (uint32_t j = tid; j < entries; j += kVerifyThreads) {
+        const int id = __ldcg(p.q_ids + list + j);
+        if (id >= 0 && static_cast<uint32_t>(id) >= base && static_cast<uint32_t>(id) - base < n) e[id - base] = fmax(e[id - base] - __ldcg(p.q_probs + list + j) * of_one, 0.0);
+    }
+    __syncthreads();
+    // The draw: the first entry with a share whose cumulative sum, in order of id, reaches u of the whole.  A thread's sums begin at what lies before its run; the sums at
+    // the runs' ends are formed by the same additions wherever they are compared, so that one thread at most finds the goal in its run.
+    double mine_left, before, cta_left;
+    auto scan = [&]() {
+        mine_left = 0.0;
+#pragma unroll 4
+        for (uint32_t i = begin; i < end; ++i) mine_left += e[i];
+        double upto = mine_left;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (static_cast<int>(lane) >= o) upto += x;
         }
         __syncthreads();
-    }
-    for (uint32_t i = begin; i < end; ++i) left += e[i];
-    double whole = cluster_sum(left);
-    if (!(whole > 0.0)) {
-        left = 0.0;
+        if (lane == 31) warp_sum[warp] = upto;
+        __syncthreads();
+        double warps = 0.0, all = 0.0;
+        for (uint32_t w = 0; w < 32; ++w) {
+            if (w == warp) warps = all;
+            all += warp_sum[w];
+        }
+        const double lanes = __shfl_up_sync(0xffffffffu, upto, 1);
+        before = warps + (lane ? lanes : 0.0);
+        mine_left = warps + upto;                   // where the run ends
+        cta_left = all * scale;
+    };
+    scan();
+    if (tid == 0) share.left = cta_left;
+    cluster.sync();
+    // the CTAs' shares, added in order
+    auto shares = [&](bool again) {
+        if (warp == 0) {
+            const double theirs = reads ? (again ? its(lane)->left_again : its(lane)->left) : 0.0;
+            double sum = 0.0, mine_ahead = 0.0;
+#pragma unroll
+            for (int r = 0; r < kCtas; ++r) {
+                if (r == static_cast<int>(rank)) mine_ahead = sum;
+                sum += __shfl_sync(0xffffffffu, theirs, r);
+            }
+            const uint32_t any = __ballot_sync(0xffffffffu, theirs > 0.0);
+            if (lane == 0) { s_sum = sum; s_ahead = mine_ahead; s_last = 31 - __clz(any); }
+        }
+        __syncthreads();
+    };
+    shares(false);
+    double all = s_sum, ahead = s_ahead;
+    if (!(all > 0.0)) {                             // nothing is left: p itself, formed anew
+        __syncthreads();
         for (uint32_t i = begin; i < end; ++i) {
             const float x = v[i];
-            e[i] = sample_key(x) ? exp((static_cast<double>(x) - highest) / temperature) / sum : 0.0;
-            left += e[i];
+            e[i] = sample_key(x) ? exp((static_cast<double>(x) - reference) * per_unit) : 0.0;
         }
-        __syncthreads();
-        whole = cluster_sum(left);
+        scan();
+        if (tid == 0) share.left_again = cta_left;
+        cluster.sync();
+        shares(true);
+        all = s_sum;
+        ahead = s_ahead;
     }
-    // the draw: the first entry with a share whose cumulative sum, in order of id, reaches u of the whole; where rounding leaves the last
-    // sum short of it, the last such entry
-    double upto = left;
-    for (int o = 1; o < 32; o <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (static_cast<int>(lane) >= o) upto += x;
-    }
-    if (lane == 31) warp_sum[warp] = upto;
-    __syncthreads();
-    double before = __shfl_up_sync(0xffffffffu, upto, 1);
-    if (lane == 0) before = 0.0;
-    double warps = 0.0;
-    for (uint32_t w = 0; w < warp; ++w) warps += warp_sum[w];
-    if (tid == kVerifyThreads - 1) share.sum = warps + upto;
-    cluster.sync();
-    double ctas = 0.0, all = 0.0;
-    for (int r = 0; r < kCtas; ++r) {
-        const double s = cluster.map_shared_rank(&share, r)->sum;
-        if (r < static_cast<int>(rank)) ctas += s;
-        all += s;
-    }
-    const double goal = __ldcg(p.uniforms + p.drafts) * all;
-    double run = ctas + (warps + before);
-    int found = 0x7fffffff, last = -1;
-    for (uint32_t i = begin; i < end; ++i) {
-        if (e[i] <= 0.0) continue;
-        run += e[i];
-        last = static_cast<int>(base + i);
-        if (run >= goal) { found = last; break; }
-    }
-    found = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(found)));
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (tid == 0) { share.top_key = 0x7fffffffu; share.count = 0; }
-    __syncthreads();
-    if (lane == 0) { atomicMin(&share.top_key, static_cast<uint32_t>(found)); atomicMax(&share.count, static_cast<uint32_t>(last + 1)); }
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-        uint32_t first = 0x7fffffffu, end_of = 0;
-        for (int r = 0; r < kCtas; ++r) {
-            first = min(first, cluster.map_shared_rank(&share, r)->top_key);
-            end_of = max(end_of, cluster.map_shared_rank(&share, r)->count);
+    const int last_with_any = s_last;
+    // the product's rounding error decides where a sum equals it
+    const double u = __ldcg(p.uniforms + p.drafts), goal = u * all, goal_rest = fma(u, all, -goal);
+    auto at_goal = [&](double x) { return x > 0.0 && (x > goal || (x == goal && goal_rest <= 0.0)); };
+    auto reached = [&](double local) { return at_goal(ahead + local * scale); };
+    // the ends of runs by warps and lanes are monotone up to rounding; the first that has reached the goal is looked for, and the CTA's end is the others' beginning
+    uint32_t first = reached(mine_left) ? tid : 0xffffffffu, none = 0, counted = 0;
+    cta_range(none, first, counted);
+    const bool in_reach = !at_goal(ahead);                              // not before this CTA
+    if (in_reach && (first != 0xffffffffu || static_cast<int>(rank) == last_with_any)) {
+        if (first == 0xffffffffu) first = kVerifyThreads - 1;          // rounding left the last sum short: the last entry with a share
+        // from the thread's run on backwards until there is an entry with a share (its own run has one but for rounding)
+        if (tid == first) {
+            double run = before;
+            int found = -1;
+            for (uint32_t i = begin; i < end; ++i) {
+                if (!(e[i] * scale > 0.0)) continue;
+                run += e[i];
+                found = static_cast<int>(i);
+                if (reached(run)) break;
+            }
+            for (int i = static_cast<int>(begin) - 1; found < 0 && i >= 0; --i) if (e[i] * scale > 0.0) found = i;
+            for (uint32_t i = end; found < 0 && i < n; ++i) if (e[i] * scale > 0.0) found = static_cast<int>(i);
+            if (found >= 0) p.draws[row] = static_cast<long long>(base) + found;
         }
-        p.draws[row] = first != 0x7fffffffu ? static_cast<long long>(first) : static_cast<long long>(end_of) - 1;
     }
     cluster.sync();                                  // nobody leaves while its shared memory is read
 }
