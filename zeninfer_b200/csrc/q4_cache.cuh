@@ -95,13 +95,17 @@ __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
 
 // ---- eviction ----------------------------------------------------------------------------------------------------------------
 //
-// A cluster of eight CTAs takes a kv head; each CTA a run of its slots, each warp a run of the CTA's.  The weight of the last slot that stays is found
-// by a radix select over order-preserving keys (four passes of eight bits, counts of the CTAs added through distributed shared memory), then
-// every warp counts what stays of its run, and a prefix over CTAs and warps gives each kept slot its place: the choice and the order are the
-// same in every run.  The move copies 16-byte pieces in rounds, all of a round read before any is written, so that it may be done in place:
-// a slot never moves up, so what a round overwrites lies in front of what later rounds read.
-// What bounds it: the moved bytes (read and written once) for large caches, a dozen cluster barriers for small ones.
-constexpr int kEvictThreads = 1024, kEvictCtas = 8, kEvictPieces = 4;
+// A cluster of eight CTAs takes a kv head.  Up to kEvictSolo slots every CTA chooses for itself, for an exchange costs more than the work it saves; above, each
+// has a run of the slots, each warp a run of the CTA's.  The weight of the last slot that stays is found by a radix select over order-preserving keys, three
+// passes of 11, 11 and 10 bits.  In a cluster a CTA adds up an eighth of the bins of all CTAs (distributed shared memory gives some ten bytes a
+// clock: reading all bins of all CTAs took 7000 clocks a pass), and the one that has the border tells the others.  Then every warp counts what stays of its run, and a prefix over CTAs and
+// warps gives each kept slot its place: the choice and the order are the same in every run.
+//   into another cache   a CTA moves the places it knows: an eighth of them, or what stays of its own run
+//   in place             all move together in rounds, all of a round read before any of it is written: a slot never moves up, so what a round overwrites lies in front of what
+//                        later rounds read
+// What bounds it: the moved bytes (read and written once) for large caches, round trips and barriers for small ones.
+constexpr int kEvictThreads = 1024, kEvictCtas = 8, kEvictPieces = 4, kEvictHeld = 8;      // pieces of a thread in a round; weights of a thread in registers
+constexpr uint32_t kEvictBins = 2048, kEvictSolo = kEvictThreads * kEvictHeld, kEvictListed = 8192;      // places a CTA lists in shared memory
 
 struct Q4Evict {
     Q4Cache from, to;
@@ -123,13 +127,16 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
 
 __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThreads) q4_evict_kernel(const __grid_constant__ Q4Evict p) {
     namespace cg = cooperative_groups;
-    __shared__ uint32_t hist[256], total[256];
-    __shared__ uint32_t s_prefix, s_remaining;
+    constexpr uint32_t kChunk = kEvictBins / kEvictCtas;
+    extern __shared__ int own_list[];                      // [kEvictListed]: the slots at the places this CTA moves
+    __shared__ uint32_t hist[kEvictBins];
     __shared__ uint32_t warp_more[32], warp_ties[32];      // a warp's slots above the border, and at it
-    __shared__ uint32_t cta_more, cta_ties;                // read by the other CTAs
+    __shared__ uint32_t s_bin, s_left, s_before, s_ties_before, s_owner;
+    __shared__ uint32_t cta_chunk, cta_bin, cta_left, cta_more, cta_ties;      // read by the other CTAs
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), h = blockIdx.y;
     pdl_launch_dependents();
+    for (uint32_t i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
     pdl_wait();
     const int filled = *reinterpret_cast<const volatile int*>(p.filled);
     if (filled < 0 || static_cast<uint32_t>(filled) > p.from.slots) {      // the same for every CTA of the grid
@@ -140,100 +147,155 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
     const float* weight = p.weight + static_cast<size_t>(h) * p.from.slots;
     int* list = p.list + static_cast<size_t>(h) * p.from.slots;
     // slots [low, high) compete for `wanted` places; all others stay
-    const bool all = n <= p.keep;
+    const bool all = n <= p.keep, in_place = p.to.k_codes == p.from.k_codes, solo = n <= kEvictSolo;
     const uint32_t low = all ? n : p.keep_first, high = all ? n : n - p.keep_last, wanted = all ? 0u : keep - p.keep_first - p.keep_last;
-    const uint32_t per_warp = ((n + kEvictCtas * 32 - 1) / (kEvictCtas * 32) + 31) & ~31u;
-    const uint32_t begin = min(n, (rank * 32 + warp) * per_warp), end = min(n, begin + per_warp);
+    const uint32_t ctas = solo ? 1u : kEvictCtas, me = solo ? 0u : rank;
+    const uint32_t per_warp = ((n + ctas * 32 - 1) / (ctas * 32) + 31) & ~31u;
+    const uint32_t begin = min(n, (me * 32 + warp) * per_warp), end = min(n, begin + per_warp), turns = per_warp / 32;
+    float held[kEvictHeld];                 // slot begin + 32 j + lane
+#pragma unroll
+    for (uint32_t j = 0; j < kEvictHeld; ++j) held[j] = j < turns && begin + 32 * j + lane < end ? __ldcg(weight + begin + 32 * j + lane) : 0.0f;
+    // every slot of the warp's run: the first ones from registers
+    auto each = [&](auto run) {
+#pragma unroll
+        for (uint32_t j = 0; j < kEvictHeld; ++j) if (j < turns) run(begin + 32 * j + lane, held[j]);
+#pragma unroll 4
+        for (uint32_t j = kEvictHeld; j < turns; ++j) {
+            const uint32_t i = begin + 32 * j + lane;
+            run(i, i < end ? __ldcg(weight + i) : 0.0f);
+        }
+    };
+    // threads 0 .. warps * 32 - 1: the sum of `mine` up to and with this one
+    auto scanned = [&](uint32_t mine, uint32_t warps) {
+        uint32_t upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (static_cast<int>(lane) >= o) upto += v;
+        }
+        if (lane == 31 && warp < warps) warp_more[warp] = upto;
+        __syncthreads();
+        return upto + __reduce_add_sync(0xffffffffu, lane < min(warp, warps) ? warp_more[lane] : 0u);
+    };
 
     // the wanted-th largest key among the competing slots, and how many that equal it stay
     uint32_t border = 0xffffffffu, ties_wanted = 0;
     if (wanted) {
-        if (tid == 0) { s_prefix = 0; s_remaining = wanted; }
-        uint32_t mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+        uint32_t prefix = 0, remaining = wanted, mask = 0;
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t digits = pass == 2 ? 1023u : 2047u;
             __syncthreads();
-            const uint32_t prefix = s_prefix;
-            for (uint32_t i = begin + lane; i < end; i += 32) {
-                const uint32_t key = evict_key(__ldcg(weight + i));
-                if (i >= low && i < high && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-            }
-            cluster.sync();
-            if (tid < 256) {
-                uint32_t sum = 0;
-                for (uint32_t r = 0; r < kEvictCtas; ++r) sum += cluster.map_shared_rank(hist, r)[tid];
-                total[tid] = sum;
-            }
-            cluster.sync();                                     // everybody has read everybody's counts
-            if (warp == 0) {
-                // lane l looks after bins 255 - 8 l .. 248 - 8 l, from the largest down
+            each([&](uint32_t i, float w) {
+                const uint32_t key = evict_key(w);
+                if (i < end && i >= low && i < high && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digits], 1u);
+            });
+            if (solo) {
+                __syncthreads();
+                // thread t looks after bins 2047 - 2 t and 2046 - 2 t, from the largest down
+                const uint2 two = reinterpret_cast<const uint2*>(hist)[kEvictThreads - 1 - tid];
+                const uint32_t mine = two.x + two.y, upto = scanned(mine, 32);
+                if (upto >= remaining && upto - mine < remaining) {
+                    const uint32_t left = remaining - (upto - mine);
+                    s_bin = kEvictBins - 1 - 2 * tid - (two.y >= left ? 0u : 1u);
+                    s_left = two.y >= left ? left : left - two.y;
+                }
+            } else {
+                cluster.sync();
+                // CTA r looks after an eighth of all CTAs' bins, CTA 0 after the largest ones
                 uint32_t mine = 0;
-                for (int j = 0; j < 8; ++j) mine += total[255 - 8 * lane - j];
-                uint32_t upto = mine;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (static_cast<int>(lane) >= o) upto += v;
+                const uint32_t bin = kEvictBins - 1 - rank * kChunk - tid;
+                if (tid < kChunk) {
+#pragma unroll
+                    for (uint32_t r = 0; r < kEvictCtas; ++r) mine += cluster.map_shared_rank(hist, r)[bin];
                 }
-                const uint32_t remaining = s_remaining;
-                const uint32_t reached = __ballot_sync(0xffffffffu, upto >= remaining);
-                if (static_cast<int>(lane) == __ffs(reached) - 1) {
-                    uint32_t left = remaining - (upto - mine);
-                    int bin = 255 - 8 * static_cast<int>(lane);
-                    while (total[bin] < left) left -= total[bin--];
-                    s_prefix = prefix | static_cast<uint32_t>(bin) << shift;
-                    s_remaining = left;
+                const uint32_t upto = scanned(mine, kChunk / 32);
+                if (tid == kChunk - 1) cta_chunk = upto;
+                cluster.sync();
+                if (warp == 0) {
+                    const uint32_t theirs = lane < kEvictCtas ? *cluster.map_shared_rank(&cta_chunk, lane) : 0u;
+                    uint32_t sum = theirs;
+                    for (int o = 1; o < 8; o <<= 1) {
+                        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+                        if (static_cast<int>(lane) >= o) sum += v;
+                    }
+                    const bool owns = lane < kEvictCtas && sum >= remaining && sum - theirs < remaining;
+                    if (owns) { s_owner = lane; s_left = remaining - (sum - theirs); }
                 }
+                __syncthreads();
+                if (s_owner == rank && tid < kChunk && upto >= s_left && upto - mine < s_left) { cta_bin = bin; cta_left = s_left - (upto - mine); }
+                cluster.sync();
+                if (tid == 0) { s_bin = *cluster.map_shared_rank(&cta_bin, s_owner); s_left = *cluster.map_shared_rank(&cta_left, s_owner); }
             }
             __syncthreads();
-            mask |= 255u << shift;
+            prefix |= s_bin << shift;
+            remaining = s_left;
+            mask |= digits << shift;
+            if (pass < 2) for (uint32_t i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
         }
-        border = s_prefix;
-        ties_wanted = s_remaining;
+        border = prefix;
+        ties_wanted = remaining;
     }
     // what stays of every warp's run
     uint32_t more = 0, ties = 0;
-    for (uint32_t i = begin + lane; i < end; i += 32) {
-        const bool competes = i >= low && i < high;
-        const uint32_t key = evict_key(__ldcg(weight + i));
-        more += !competes || (wanted && key > border);
-        ties += competes && wanted && key == border;
-    }
+    each([&](uint32_t i, float w) {
+        const bool real = i < end, competes = i >= low && i < high;
+        const uint32_t key = evict_key(w);
+        more += real && (!competes || (wanted && key > border));
+        ties += real && competes && wanted && key == border;
+    });
     more = __reduce_add_sync(0xffffffffu, more);
     ties = __reduce_add_sync(0xffffffffu, ties);
-    if (lane == 0) { warp_more[warp] = more; warp_ties[warp] = ties; }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t m = 0, t = 0;
-        for (int w = 0; w < 32; ++w) { m += warp_more[w]; t += warp_ties[w]; }
-        cta_more = m;
-        cta_ties = t;
+    if (lane == 0) { warp_more[warp] = more; warp_ties[warp] = ties; }
+    if (tid == 0) s_before = s_ties_before = 0;
+    __syncthreads();
+    if (!solo) {
+        if (warp == 0) {
+            const uint32_t m = __reduce_add_sync(0xffffffffu, warp_more[lane]), t = __reduce_add_sync(0xffffffffu, warp_ties[lane]);
+            if (lane == 0) { cta_more = m; cta_ties = t; }
+        }
+        cluster.sync();
+        if (warp == 0) {
+            const uint32_t m = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(&cta_more, lane) : 0u);
+            const uint32_t t = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(&cta_ties, lane) : 0u);
+            if (lane == 0) { s_before = m; s_ties_before = t; }
+        }
+        cluster.sync();                                    // behind it no CTA reads another's shared memory
     }
-    cluster.sync();
-    uint32_t before = 0, ties_before = 0;
-    for (uint32_t r = 0; r < rank; ++r) { before += *cluster.map_shared_rank(&cta_more, r); ties_before += *cluster.map_shared_rank(&cta_ties, r); }
-    for (uint32_t w = 0; w < warp; ++w) { before += warp_more[w]; ties_before += warp_ties[w]; }
-    for (uint32_t i0 = begin; i0 < end; i0 += 32) {
-        const uint32_t i = i0 + lane;
+    // the places this CTA moves into another cache
+    const uint32_t share = ((keep + kEvictCtas - 1) / kEvictCtas + 7) & ~7u;
+    const uint32_t first_place = solo ? min(keep, rank * share) : s_before + min(s_ties_before, ties_wanted);
+    const uint32_t end_place = solo ? min(keep, first_place + share) : s_before + cta_more + min(s_ties_before + cta_ties, ties_wanted);
+    const bool listed = !in_place && end_place - first_place <= kEvictListed;
+    uint32_t before = s_before + __reduce_add_sync(0xffffffffu, lane < warp ? warp_more[lane] : 0u), ties_before = s_ties_before + __reduce_add_sync(0xffffffffu, lane < warp ? warp_ties[lane] : 0u);
+    each([&](uint32_t i, float w) {
         const bool real = i < end, competes = i >= low && i < high;
-        const uint32_t key = real ? evict_key(__ldcg(weight + i)) : 0u;
+        const uint32_t key = evict_key(w);
         const bool above = real && (!competes || (wanted && key > border)), tie = real && competes && wanted && key == border;
         const uint32_t below = (1u << lane) - 1u, aboves = __ballot_sync(0xffffffffu, above), tied = __ballot_sync(0xffffffffu, tie);
         const uint32_t tie_rank = ties_before + __popc(tied & below);
         if (above || (tie && tie_rank < ties_wanted)) {
             const uint32_t place = before + __popc(aboves & below) + min(tie_rank, ties_wanted);
-            list[place] = static_cast<int>(i);
-            if (p.kept) p.kept[static_cast<size_t>(h) * p.keep + place] = static_cast<int>(i);
+            const bool mine = place >= first_place && place < end_place;
+            if (listed) { if (mine) own_list[place - first_place] = static_cast<int>(i); }
+            else if (!solo || rank == 0) list[place] = static_cast<int>(i);
+            if (solo ? mine : true) {
+                if (p.kept) p.kept[static_cast<size_t>(h) * p.keep + place] = static_cast<int>(i);
+                if (!in_place) p.weight_to[static_cast<size_t>(h) * p.to.slots + place] = w;
+            }
         }
         before += __popc(aboves);
         ties_before += __popc(tied);
-    }
-    cluster.sync();                                        // the list is whole, and nobody reads another CTA's counts any more
+    });
+    if (!listed && (in_place || solo)) cluster.sync();     // the list is whole
+    else __syncthreads();                                  // the CTA's part of it
 
-    // the move: a kept slot is 2 * blocks pieces of 16 code bytes, and beside them its scales and its weight.  Eight neighbouring threads take
+    // the move: a kept slot is 2 * blocks pieces of 16 code bytes, and beside them its scales (and in place its weight).  Eight neighbouring threads take
     // one piece of eight neighbouring places, which are written as one line.
-    const bool in_place = p.to.k_codes == p.from.k_codes;
-    const uint32_t blocks = p.from.blocks, pieces = 2 * blocks, a_round = kEvictCtas * kEvictThreads * kEvictPieces / (8 * pieces) * 8;
-    for (uint32_t first = 0; first < keep; first += a_round) {
+    const uint32_t blocks = p.from.blocks, pieces = 2 * blocks, movers = in_place ? kEvictCtas : 1u, mover = in_place ? rank : 0u;
+    const uint32_t a_round = movers * kEvictThreads * kEvictPieces / (8 * pieces) * 8, from_place = in_place ? 0u : first_place & ~7u, to_place = in_place ? keep : end_place;
+    for (uint32_t first = from_place; first < to_place; first += a_round) {
         uint4 code[kEvictPieces];
         __half scale[kEvictPieces];
         float w[kEvictPieces];
@@ -241,16 +303,16 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
         bool mine[kEvictPieces];
 #pragma unroll
         for (int u = 0; u < kEvictPieces; ++u) {
-            const uint32_t i = (u * kEvictCtas + rank) * kEvictThreads + tid;
+            const uint32_t i = (u * movers + mover) * kEvictThreads + tid;
             piece[u] = (i >> 3) % pieces;
             place[u] = first + i / (8 * pieces) * 8 + (i & 7u);
-            mine[u] = i < a_round * pieces && place[u] < keep;
+            mine[u] = i < a_round * pieces && place[u] < to_place && (in_place || place[u] >= first_place);
             if (!mine[u]) continue;
             const bool value = piece[u] >= blocks;
-            const uint32_t block = value ? piece[u] - blocks : piece[u], slot = static_cast<uint32_t>(__ldcg(list + place[u]));
+            const uint32_t block = value ? piece[u] - blocks : piece[u], slot = static_cast<uint32_t>(listed ? own_list[place[u] - first_place] : __ldcg(list + place[u]));
             code[u] = __ldcg(reinterpret_cast<const uint4*>((value ? p.from.v_codes : p.from.k_codes) + q4_codes_at(h, slot, block, blocks, p.from.slots)));
             scale[u] = __ldcg((value ? p.from.v_scales : p.from.k_scales) + q4_scale_at(h, slot, block, blocks, p.from.slots));
-            if (piece[u] == 0) w[u] = __ldcg(weight + slot);
+            if (in_place && piece[u] == 0) w[u] = __ldcg(weight + slot);
         }
         if (in_place) cluster.sync();
 #pragma unroll
@@ -260,7 +322,7 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
             const uint32_t block = value ? piece[u] - blocks : piece[u];
             *reinterpret_cast<uint4*>((value ? p.to.v_codes : p.to.k_codes) + q4_codes_at(h, place[u], block, blocks, p.to.slots)) = code[u];
             (value ? p.to.v_scales : p.to.k_scales)[q4_scale_at(h, place[u], block, blocks, p.to.slots)] = scale[u];
-            if (piece[u] == 0) p.weight_to[static_cast<size_t>(h) * p.to.slots + place[u]] = w[u];
+            if (in_place && piece[u] == 0) p.weight_to[static_cast<size_t>(h) * p.to.slots + place[u]] = w[u];
         }
         if (in_place) cluster.sync();
     }

@@ -245,7 +245,7 @@ int zen_cuda_dev_q4_cache_evict(const zen_cuda_q4_cache* from, const float* weig
     }
     if (!e.ok) return 0;
     const zk::Q4Evict p{device_form(*from), device_form(*to), weight, weight_to, filled, kept, static_cast<int*>(workspace), u32(keep), u32(keep_first), u32(keep_last), e.d_error};
-    return e.leave(launch(e, zk::q4_evict_kernel, dim3(zk::kEvictCtas, from->kv_heads), dim3(zk::kEvictThreads), 0, 0, p), "dev_q4_cache_evict");
+    return e.leave(launch(e, zk::q4_evict_kernel, dim3(zk::kEvictCtas, from->kv_heads), dim3(zk::kEvictThreads), zk::kEvictListed * sizeof(int), 0, p), "dev_q4_cache_evict");
 }
 
 size_t zen_cuda_verify_drafts_workspace_bytes(const zen_cuda_draft_check* c) { return verify_room(c); }
