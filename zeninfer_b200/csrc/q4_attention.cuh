@@ -30,7 +30,8 @@ constexpr uint32_t kQ4Tile = 32;             // slots of a tile
 enum Q4Columns : int {
     kQ4Digits = 0,       // four rows, a column a digit: half the products of the next for up to four rows (a step of a model with groups of four; q4_step.cuh)
     kQ4Rows8 = 1,        // eight rows, the digits one after the other
-    kQ4Rows16 = 2        // sixteen rows: the unpacked codes serve two products
+    kQ4Rows16 = 2,       // sixteen rows: the unpacked codes serve two products
+    kQ4Prompt = 3        // none of these: the tensor cores proper (q4_prompt.cuh)
 };
 __host__ __device__ constexpr int q4_rows(int columns) { return columns == kQ4Digits ? 4 : columns == kQ4Rows8 ? 8 : 16; }
 __host__ __device__ constexpr int q4_warps(int columns) { return columns == kQ4Digits ? 8 : 4; }
@@ -53,6 +54,7 @@ struct Q4Attend {
     float* factors;            // workspace [kv_heads][padded rows]: what makes scores of their products
     uint32_t tokens, heads, group;      // group = heads / kv_heads; a kv head has tokens * group rows, row = token * group + head of the group
     uint32_t splits, row_warps;
+    uint32_t run_tile;         // slots of a tile that runs are counted in
     uint32_t padded;           // rows, rounded up to a whole number of what a warp takes
     const float* k;            // rows kv_ld apart
     const float* v;
@@ -67,9 +69,9 @@ struct Q4Attend {
 struct Q4Runs {
     uint32_t tiles, per, active;
 };
-__device__ __forceinline__ Q4Runs q4_runs(uint32_t slots_seen, uint32_t splits, uint32_t key_warps) {
+__device__ __forceinline__ Q4Runs q4_runs(uint32_t slots_seen, uint32_t splits, uint32_t key_warps, uint32_t tile) {
     Q4Runs r;
-    r.tiles = (slots_seen + kQ4Tile - 1) / kQ4Tile;
+    r.tiles = (slots_seen + tile - 1) / tile;
     r.per = max((r.tiles + splits - 1) / splits, key_warps);
     r.active = (r.tiles + r.per - 1) / r.per;
     return r;
@@ -233,6 +235,35 @@ __device__ __forceinline__ uint8_t q4_append_block(const Q4Attend& p, float x, u
     return byte;
 }
 
+// New keys (rotated) and values into the slots behind *filled, where nothing else is to be prepared: a warp takes several blocks, all asked for first.
+constexpr uint32_t kQ4AppendWarps = 8, kQ4AppendEach = 4;
+template <int kBlocks>
+__global__ void __launch_bounds__(kQ4AppendWarps * 32) q4_append_kernel(const __grid_constant__ Q4Attend p) {
+    const uint32_t lane = threadIdx.x & 31u, first = (blockIdx.x * kQ4AppendWarps + (threadIdx.x >> 5)) * kQ4AppendEach;
+    const uint32_t items = p.tokens * p.cache.kv_heads * 2 * kBlocks;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled = *reinterpret_cast<const volatile int*>(p.filled);
+    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(p.error_word, kErrBadPosition);
+        return;
+    }
+    float x[kQ4AppendEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kQ4AppendEach; ++i) {
+        const uint32_t item = min(first + i, items - 1), of_token = item / (2 * kBlocks), t = of_token / p.cache.kv_heads;
+        x[i] = q4_new_value<kBlocks>(p, of_token % p.cache.kv_heads, t, item % (2 * kBlocks), static_cast<size_t>(position) + t, lane);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kQ4AppendEach; ++i) {
+        const uint32_t item = first + i, of_token = item / (2 * kBlocks), t = of_token / p.cache.kv_heads;
+        if (item >= items) return;
+        __half ignored;
+        q4_append_block<kBlocks>(p, x[i], of_token % p.cache.kv_heads, t, item % (2 * kBlocks), static_cast<uint32_t>(filled), lane, ignored);
+    }
+}
+
 // What a block's attention begins with: the new tokens' keys (rotated) and values go into the slots behind *filled, and their queries (rotated) are laid out
 // for the products.  grid = (tokens, kv_heads); a warp takes a block of the key or the value, or a row of queries.
 constexpr uint32_t kQ4PrepareWarps = 16;
@@ -293,7 +324,7 @@ __global__ void __launch_bounds__(q4_warps(kColumns) * 32, kBlocks > 4 ? 1 : 3) 
     if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;      // the append has said so
     const uint32_t filled = filled_in, real_rows = min(cta_rows, rows - cta_first);
     const uint32_t seen = filled + (cta_first + real_rows - 1) / p.group + 1;           // slots of the CTA's last token
-    const Q4Runs runs = q4_runs(seen, p.splits, key_warps);
+    const Q4Runs runs = q4_runs(seen, p.splits, key_warps, kQ4Tile);
     const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
     if (begin >= end) return;                                                            // nobody counts on this run
 
@@ -609,7 +640,7 @@ __global__ void __launch_bounds__(kQ4FinishWarps * 32) q4_finish_kernel(const __
     const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
     if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;
     const uint32_t filled = filled_in;
-    auto runs_of = [&](uint32_t row) { return q4_runs(filled + (min(rows, (row / cta_rows + 1) * cta_rows) - 1) / p.group + 1, p.splits, key_warps).active; };
+    auto runs_of = [&](uint32_t row) { return q4_runs(filled + (min(rows, (row / cta_rows + 1) * cta_rows) - 1) / p.group + 1, p.splits, key_warps, p.run_tile).active; };
     auto stats_of = [&](uint32_t row) { return reinterpret_cast<const float2*>(p.part_stats) + static_cast<size_t>(h) * p.splits * rows + row; };
     if (blockIdx.x >= join_ctas) {
         const uint32_t slot = (blockIdx.x - join_ctas) * kQ4FinishWarps * 32 + threadIdx.x, seen = filled + p.tokens;

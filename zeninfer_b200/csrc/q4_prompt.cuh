@@ -1,0 +1,477 @@
+// Attention of a block of many rows over a cache held in 4 bits, heads of 64 or 128 values, on the tensor cores (tcgen05).
+//
+// The formulas and the bookkeeping are q4_attention.cuh's: queries and weights enter as two f16 numbers each, keys and values are exact.  What differs is where a
+// block's scale goes.  Here it goes into the operand: d (c - 8) is a number of fifteen bits, exactly the sum of two f16 numbers (the rounded product and
+// its remainder, a multiplication and a multiply-add of halves), so a product is three products of f16 numbers (the fourth is below 2^-22 of it), and nothing has to be
+// done per block and score.  A tile's scales are multiplied by the power of two that brings the largest below 2^9, so that both parts keep their bits
+// whatever the model's magnitudes are.  The dimensions of the scores' operands stand in the order in which the nibbles are unpacked.
+//
+// A CTA takes 128 rows (a row: a token times a query head of the kv head, any group) and walks its run of slots 64 at a time.  Sixteen warps:
+//   8 rows       a thread has half a row: 32 scores from TMEM, mask, running maximum (shared with the other half), exponentials, the weights' two parts back to
+//                TMEM, from where the tensor cores read them; then out = out * factor + O' of the tile before, in fp32 registers
+//   4 + 3        unpack keys and values (asked for from L2 a tile ahead) into the operands' 128-byte swizzle, two buffers each; values by eight slots, transposed
+//   1 issues     S = Q K^T into three accumulators (the corrections, and the leading products of each half of the head, for the tensor cores cut a sum at
+//                every 16 columns), O' = P V corrections first
+// The scores of tile j + 1 are formed while tile j is exponentiated.
+//
+// A scale that is not finite counts as zero in the operands and is remembered by its slot: the rows that see it are NaN (all of them for a key's, the
+// block's dimensions for a value's), and the others know nothing of it.
+#pragma once
+#include "attention_tc.cuh"
+#include "q4_attention.cuh"
+
+namespace zk {
+
+constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 16 * 32, kQpKeyWarp = 8, kQpValueWarp = 12, kQpIssueWarp = 15;      // first warps of the roles
+template <int kBlocks> constexpr uint32_t kQpQPlane = kQpRows * kBlocks * 64;      // bytes
+template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;
+template <int kBlocks> constexpr uint32_t kQpVPlane = kBlocks * 32 * kQpKeys * 2;
+template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 4 * kQpKPlane<kBlocks> + 4 * kQpVPlane<kBlocks>; }
+// TMEM columns: leading scores of the head's halves, corrections; the weights' parts; O'
+constexpr uint32_t kQpLead = 0, kQpCorrections = 128, kQpP = 192, kQpOut = 256, kQpColumns = 512;
+
+// Instruction descriptor, kind::f16: f16 x f16 -> fp32, both operands K-major, dense.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_rest(uint32_t a, uint32_t b, uint32_t product) {      // a * b - product
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(product ^ 0x80008000u));
+    return r;
+}
+// The power of two for a tile whose largest scale has these bits: times 2^shift it is below 2^9.
+__device__ __forceinline__ int q4_shift(uint32_t top) { return 23 - static_cast<int>(top >> 10); }
+__device__ __forceinline__ bool q4_finite(uint32_t half_bits) { return (half_bits & 0x7c00u) != 0x7c00u; }
+
+// The largest magnitude among the finite scales of `slots` slots from slot0 on that are seen, as f16 bits: every lane of a warp.  scales: the head's first.
+template <int kBlocks>
+__device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slot0, uint32_t slots, uint32_t seen, uint32_t lane) {
+    uint32_t top = 0;
+    for (uint32_t i = lane; i < slots * kBlocks / 8; i += 32) {            // eight scales at a time: 8 / kBlocks slots
+        const uint32_t slot = slot0 + i * 8 / kBlocks;
+        if (slot >= seen) break;
+        const uint4 eight = __ldcg(reinterpret_cast<const uint4*>(scales + static_cast<size_t>(slot0) * kBlocks) + i);
+        const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0x7fffu;
+            if (slot + j / kBlocks < seen && q4_finite(bits)) top = max(top, bits);
+        }
+    }
+    return __reduce_max_sync(0xffffffffu, top);
+}
+
+// Eight dimensions of a row of queries in the scores' order, 4j .. 4j+3 and 16+4j .. 16+4j+3 of a block, as they are unpacked from a word of codes.
+__device__ __forceinline__ void q4_split_queries(const float (&x)[8], float up, uint4& upper, uint4& lower) {
+    uint32_t u[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int at = (i & 1) * 4 + (i >> 1);            // {4j, 4j+2}, {16+4j, 16+4j+2}, {4j+1, 4j+3}, {17+4j, 19+4j}
+        const float a = x[at] * up, b = x[at + 2] * up, ua = upper_digit(a), ub = upper_digit(b);
+        u[i] = pack_f16(ua, ub);
+        l[i] = pack_f16(a - ua, b - ub);
+    }
+    upper = make_uint4(u[0], u[1], u[2], u[3]);
+    lower = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// A word of codes (eight dimensions) times a scale: the operand's sixteen bytes in both planes.
+__device__ __forceinline__ void q4_split_codes(uint32_t w, uint32_t d2, uint4& upper, uint4& lower) {
+    const uint32_t x = w >> 8, c[4] = {signed_low(w), signed_high(w), signed_low(x), signed_high(x)};
+    uint32_t u[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        u[i] = f16x2_mul(c[i], d2);
+        l[i] = f16x2_rest(c[i], d2, u[i]);
+    }
+    upper = make_uint4(u[0], u[1], u[2], u[3]);
+    lower = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// grid = (splits, tiles of 128 rows, kv_heads); the rows that see most slots come first.
+template <int kBlocks>
+__global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_constant__ Q4Attend p) {
+    constexpr uint32_t kDim = kBlocks * 32, kHalves = kBlocks / 2, kQPlane = kQpQPlane<kBlocks>, kKPlane = kQpKPlane<kBlocks>, kVPlane = kQpVPlane<kBlocks>;
+    extern __shared__ uint8_t qp_smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(qp_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* const q_smem = smem;                             // [plane][64 dimensions][128 rows][128 bytes]
+    uint8_t* const k_smem = q_smem + 2 * kQPlane;             // [buffer][plane][64 dimensions][64 slots][128 bytes]
+    uint8_t* const v_smem = k_smem + 4 * kKPlane;             // [buffer][plane][the head's dimensions][64 slots]
+    __shared__ float row_factor[kQpRows], top[2][2][kQpRows], sum[2][kQpRows];
+    __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_empty, p_full, o_full, o_empty;
+    __shared__ float k_unit[4], v_unit[4];                    // what a tile's operands are to be multiplied by: the rows read the last but one while the next is stored
+    __shared__ uint32_t tmem_slot, bad_key, bad_value[kBlocks];      // the first slots whose scales are not finite
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, h = blockIdx.z, rows = p.tokens * p.group;
+    const uint32_t first_row = (gridDim.y - 1 - blockIdx.y) * kQpRows, real_rows = min(kQpRows, rows - first_row);
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&k_full[b], kQpValueWarp - kQpKeyWarp); mbar_init(&v_full[b], kQpIssueWarp - kQpValueWarp);
+            mbar_init(&k_free[b], 1); mbar_init(&v_free[b], 1);
+        }
+        mbar_init(&s_full, 1); mbar_init(&s_empty, 8); mbar_init(&p_full, 8); mbar_init(&o_full, 1); mbar_init(&o_empty, 8);
+        mbar_fence_init();
+        bad_key = 0xffffffffu;
+        for (int b = 0; b < kBlocks; ++b) bad_value[b] = 0xffffffffu;
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    const int filled_in = *reinterpret_cast<const volatile int*>(p.filled);
+    const int position = p.turn.pairs ? *reinterpret_cast<const volatile int*>(p.position) : 0;
+    if (!q4_places_ok(filled_in, position, p.tokens, p.cache.slots, p.turn.pairs, p.turn.positions)) return;      // the append has said so
+    const uint32_t filled = filled_in, seen = filled + (first_row + real_rows - 1) / p.group + 1;                 // slots of the last token
+    const Q4Runs runs = q4_runs(seen, p.splits, 1, kQpKeys);
+    const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
+    if (begin >= end) return;                                                            // nobody counts on this run
+    if (warp == kQpIssueWarp) tmem_alloc(&tmem_slot, kQpColumns);
+
+    {      // Q: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
+        constexpr uint32_t kChunks = kDim / 8, kEach = kQpRows * kChunks / kQpThreads;
+        const uint32_t chunk = threadIdx.x % kChunks, dim = chunk / 4 * 32 + chunk % 4 * 4;
+        float x[kEach][8];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = threadIdx.x / kChunks + i * (kQpThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
+            const float* from = p.q + token * p.q_ld + static_cast<size_t>(h * p.group + row % p.group) * kDim;
+            const size_t turned = static_cast<size_t>(position) + token;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = q4_rotated(from, dim + (e & 3) + (e >> 2) * 16, p.turn, turned);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = threadIdx.x / kChunks + i * (kQpThreads / kChunks);
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (r >= real_rows) x[i][e] = 0.0f;
+                most = fmaxf(most, fabsf(x[i][e]));
+            }
+#pragma unroll
+            for (uint32_t o = kChunks / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -114);
+            uint4 upper, lower;
+            q4_split_queries(x[i], p.scale < 0.0f ? -power_of_two(13 - e) : power_of_two(13 - e), upper, lower);
+            const uint32_t at = (chunk / 8) * (kQPlane / kHalves) + r * 128 + (((chunk % 8) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4*>(q_smem + at) = upper;
+            *reinterpret_cast<uint4*>(q_smem + kQPlane + at) = lower;
+            if (chunk == 0) {
+                const int units = e - 13;
+                row_factor[r] = fabsf(p.scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2);
+            }
+            // the same for the launch that adds up what the slots received
+            if (p.queries && blockIdx.x == 0) {
+                uint8_t* to = reinterpret_cast<uint8_t*>(p.queries) + (static_cast<size_t>(h) * gridDim.y + first_row / kQpRows) * 2 * kQPlane + at;
+                *reinterpret_cast<uint4*>(to) = upper;
+                *reinterpret_cast<uint4*>(to + kQPlane) = lower;
+                if (chunk == 0) p.factors[static_cast<size_t>(h) * gridDim.y * kQpRows + first_row + r] = row_factor[r];
+            }
+        }
+        async_proxy_fence();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    auto gave_up = [&](int code) { if (lane == 0) atomicExch(p.error_word, code); };
+
+    // A wait that runs out ends its role's loop, and the others' follow.
+    if (warp < kQpKeyWarp) {                                  // rows
+        const uint32_t quad = warp & 3, half = warp >> 2, r = quad * 32 + lane, row = first_row + r, lane_base = (quad * 32) << 16;
+        const bool live = r < real_rows;
+        const uint32_t last_seen = live ? filled + row / p.group : 0xffffffffu;          // rows that are none: whatever comes, they write nothing
+        constexpr int kMine = kQpKeys / 2, kOut = kDim / 2;
+        const float factor = row_factor[r];
+        // the two warps of a row meet; true where one of them has given up
+        auto meet = [&](bool failed) {
+            uint32_t any;
+            asm volatile(
+                "{ .reg .pred p, q; setp.ne.u32 q, %3, 0; barrier.red.or.pred p, %1, %2, q; selp.u32 %0, 1, 0, p; }"
+                : "=r"(any) : "r"(quad + 1), "r"(64u), "r"(static_cast<uint32_t>(failed)) : "memory");
+            return any != 0;
+        };
+        constexpr float kFull = 16384.0f;                     // a weight of 1
+        float acc[kOut], m = -INFINITY, l = 0.0f, shrink = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) acc[i] = 0.0f;
+        auto take_output = [&](float by) {                    // acc = acc * shrink + O'
+#pragma unroll
+            for (int c = 0; c < kOut / 32; ++c) {
+                uint32_t v[2][16];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) tmem_ld_32x16(tmem + kQpOut + half * kOut + 32 * c + 16 * b + lane_base, v[b]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(v[i / 16][i % 16]), by, acc[32 * c + i] * shrink);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty);
+        };
+        bool ok = true;
+        uint32_t j = 0;
+        for (uint32_t tile = begin; tile < end; ++tile, ++j) {
+            ok = ok && warp_waited(&s_full, j & 1);
+            float s[kMine], most = -INFINITY, by = 0.0f;
+            if (ok) {
+                tc_fence_after_sync();
+#pragma unroll
+                for (int c = 0; c < kMine / 8; ++c) {
+                    uint32_t part[3][8];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) tmem_ld_32x8(tmem + (i < 2 ? kQpLead + i * kQpKeys : kQpCorrections) + half * kMine + 8 * c + lane_base, part[i]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[8 * c + i] = (__uint_as_float(part[0][i]) + __uint_as_float(part[1][i])) + __uint_as_float(part[2][i]);
+                }
+                by = factor * k_unit[j & 3];
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty);
+                const uint32_t first = tile * kQpKeys + half * kMine;
+                if (!__all_sync(0xffffffffu, first + kMine - 1 <= last_seen)) {
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i) if (first + i > last_seen) s[i] = -INFINITY;
+                }
+                float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) part[i & 3] = fmaxf(part[i & 3], s[i]);
+                most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * by;
+                top[j & 1][half][r] = most;
+                if (p.scores && live) {
+                    float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(h) * rows + row) * p.cache.slots + first);
+#pragma unroll
+                    for (int i = 0; i < kMine / 4; ++i) if (first + 4 * i < p.cache.slots) to[i] = make_float4(s[4 * i] * by, s[4 * i + 1] * by, s[4 * i + 2] * by, s[4 * i + 3] * by);
+                }
+            }
+            if (meet(!ok)) { ok = false; break; }
+            most = fmaxf(fmaxf(most, top[j & 1][half ^ 1][r]), m);
+            const float from = most == -INFINITY ? 0.0f : most, f = exp2_fast(m - from);          // exp2(-inf) = 0 on the first slots
+            m = most;
+            float part[4] = {};
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                s[i] = exp2_fast(fmaf(s[i], by, -from));
+                part[i & 3] += s[i];
+            }
+            l = l * f + ((part[0] + part[1]) + (part[2] + part[3]));
+            if (j > 0) ok = warp_waited(&o_full, (j - 1) & 1);                  // the tile before: its output is formed, and P's place free
+            if (ok) {
+                tc_fence_after_sync();
+#pragma unroll
+                for (int c = 0; c < kMine / 16; ++c) {
+                    uint32_t upper[8], lower[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float a = s[16 * c + 2 * i] * kFull, b = s[16 * c + 2 * i + 1] * kFull, ua = upper_digit(a), ub = upper_digit(b);
+                        upper[i] = pack_f16(ua, ub);
+                        lower[i] = pack_f16(a - ua, b - ub);
+                    }
+                    tmem_st_32x8(tmem + kQpP + 16 * half + 8 * c + lane_base, upper);
+                    tmem_st_32x8(tmem + kQpP + 32 + 16 * half + 8 * c + lane_base, lower);
+                }
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full);
+                if (j > 0) take_output(v_unit[(j - 1) & 3]);
+            }
+            shrink = f;
+        }
+        if (ok) ok = warp_waited(&o_full, (j - 1) & 1);
+        if (ok) { tc_fence_after_sync(); take_output(v_unit[(j - 1) & 3]); }
+        sum[half][r] = l;
+        if (meet(!ok)) {
+            gave_up(kErrTmemWaitTimeout);
+        } else if (live) {
+            l += sum[half ^ 1][r];
+            if (last_seen >= bad_key) l = NAN;
+            const bool alone = p.splits == 1;
+            const float inv = alone ? 1.0f / l : 1.0f;
+            const uint32_t token = row / p.group, head = h * p.group + row % p.group;
+            const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + row;
+            float* to = (alone ? p.out + (static_cast<size_t>(token) * p.heads + head) * kDim : p.part_out + part * kDim) + half * kOut;
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) {
+                const float o = last_seen >= bad_value[(half * kOut + i) / 32] ? NAN : acc[i] * inv;
+                to[i] = o;
+            }
+            if (half == 0) {
+                if (alone) {
+                    if (!(l > 0.0f) || !(l < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
+                    if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = m + log2f(l);
+                }
+                if (!alone || p.scores) reinterpret_cast<float2*>(p.part_stats)[part] = make_float2(m, l);
+            }
+        }
+    } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot
+        constexpr uint32_t kId = (kQpValueWarp - kQpKeyWarp) * 32, kEach = kQpKeys * kBlocks / kId;
+        const uint32_t id = threadIdx.x - kQpKeyWarp * 32;
+        const __half* const scales = p.cache.k_scales + static_cast<size_t>(h) * p.cache.slots * kBlocks;
+        uint4 codes[kEach];
+        uint32_t scale[kEach], largest = 0;
+        auto ask = [&](uint32_t tile) {
+            largest = q4_largest_scale<kBlocks>(scales, tile * kQpKeys, kQpKeys, seen, lane);
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t item = id + kId * i, slot = tile * kQpKeys + item % kQpKeys, block = item / kQpKeys;
+                const bool real = slot < seen;
+                codes[i] = real ? __ldcg(reinterpret_cast<const uint4*>(p.cache.k_codes + q4_codes_at(h, slot, block, kBlocks, p.cache.slots))) : make_uint4(0, 0, 0, 0);
+                scale[i] = real ? __half_as_ushort(__ldcg(scales + static_cast<size_t>(slot) * kBlocks + block)) : 0u;
+            }
+        };
+        ask(begin);
+        uint32_t j = 0;
+        for (uint32_t tile = begin; tile < end; ++tile, ++j) {
+            if (j > 1 && !warp_waited(&k_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
+            const int shift = q4_shift(largest);
+            uint8_t* const to = k_smem + (j & 1) * 2 * kKPlane;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t item = id + kId * i, r = item % kQpKeys, block = item / kQpKeys;
+                if (!q4_finite(scale[i])) {
+                    atomicMin(&bad_key, tile * kQpKeys + r);
+                    scale[i] = 0;
+                }
+                const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(scale[i]))) * power_of_two(shift);
+                const uint32_t d2 = pack_f16(d, d), w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+                for (uint32_t word = 0; word < 4; ++word) {
+                    uint4 upper, lower;
+                    q4_split_codes(w[word], d2, upper, lower);
+                    const uint32_t at = (block / 2) * (kKPlane / kHalves) + r * 128 + ((((block & 1) * 4 + word) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to + at) = upper;
+                    *reinterpret_cast<uint4*>(to + kKPlane + at) = lower;
+                }
+            }
+            if (id == 0) k_unit[j & 3] = power_of_two(-shift);
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[j & 1]);
+            if (tile + 1 < end) ask(tile + 1);
+        }
+    } else if (warp < kQpIssueWarp) {                         // values: a thread takes a word (eight dimensions) of eight slots
+        constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32, kItems = kQpKeys / 8 * kBlocks * 4, kEach = (kItems + kId - 1) / kId;
+        const uint32_t id = threadIdx.x - kQpValueWarp * 32;
+        const __half* const scales = p.cache.v_scales + static_cast<size_t>(h) * p.cache.slots * kBlocks;
+        uint32_t w[kEach][8], largest = 0;
+        auto ask = [&](uint32_t tile) {
+            largest = q4_largest_scale<kBlocks>(scales, tile * kQpKeys, kQpKeys, seen, lane);
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t item = id + kId * i, octet = item % 8, word = item / 8 % 4, block = item / 32;
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint32_t slot = tile * kQpKeys + octet * 8 + k;
+                    w[i][k] = item < kItems && slot < seen ? __ldcg(reinterpret_cast<const uint32_t*>(p.cache.v_codes + q4_codes_at(h, slot, block, kBlocks, p.cache.slots)) + word) : 0u;
+                }
+            }
+        };
+        ask(begin);
+        uint32_t j = 0;
+        for (uint32_t tile = begin; tile < end; ++tile, ++j) {
+            const int shift = q4_shift(largest);
+            const float up = power_of_two(shift);
+            uint32_t d2[kEach][4];
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t item = id + kId * i, octet = item % 8, block = item / 32;
+                float d[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint32_t slot = tile * kQpKeys + octet * 8 + k;
+                    uint32_t bits = item < kItems && slot < seen ? __half_as_ushort(__ldcg(scales + static_cast<size_t>(slot) * kBlocks + block)) : 0u;
+                    if (!q4_finite(bits)) {
+                        atomicMin(&bad_value[block], slot);
+                        bits = 0;
+                    }
+                    d[k] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) d2[i][k] = pack_f16(d[2 * k], d[2 * k + 1]);
+            }
+            if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
+            uint8_t* const to = v_smem + (j & 1) * 2 * kVPlane;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t item = id + kId * i, octet = item % 8, word = item / 8 % 4, block = item / 32;
+                if (item >= kItems) continue;
+#pragma unroll
+                for (uint32_t pair = 0; pair < 2; ++pair) {      // bytes 0 and 1, bytes 2 and 3 of the words
+                    uint32_t x[4];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) x[k] = __byte_perm(w[i][2 * k], w[i][2 * k + 1], pair ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (uint32_t nibble = 0; nibble < 4; ++nibble) {
+                        uint32_t upper[4], lower[4];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            const uint32_t y = nibble & 2 ? x[k] >> 8 : x[k], c = nibble & 1 ? signed_high(y) : signed_low(y);
+                            upper[k] = f16x2_mul(c, d2[i][k]);
+                            lower[k] = f16x2_rest(c, d2[i][k], upper[k]);
+                        }
+                        const uint32_t dim = block * 32 + (nibble & 1) * 16 + word * 4 + pair * 2 + (nibble >> 1);
+                        const uint32_t at = dim * 128 + ((octet ^ (dim & 7)) << 4);
+                        *reinterpret_cast<uint4*>(to + at) = make_uint4(upper[0], upper[1], upper[2], upper[3]);
+                        *reinterpret_cast<uint4*>(to + kVPlane + at) = make_uint4(lower[0], lower[1], lower[2], lower[3]);
+                    }
+                }
+            }
+            if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[j & 1]);
+            if (tile + 1 < end) ask(tile + 1);
+        }
+    } else if (lane == 0) {                                   // the tensor cores
+        constexpr uint32_t score_desc = umma_idesc_f16(kQpRows, kQpKeys), out_desc = umma_idesc_f16(kQpRows, kDim), kSteps = kDim / 16;
+        const uint64_t q_desc = umma_desc_k_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_sw128(smem_u32(k_smem)), v_desc = umma_desc_k_sw128(smem_u32(v_smem));
+        // a descriptor's start address counts 16-byte units; 16 columns of K are two of them
+        auto scores = [&](uint32_t b) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {                     // lower times upper, upper times lower, upper times upper
+                const uint32_t qp = c == 0 ? 1 : 0, kp = c == 1 ? 1 : 0;
+#pragma unroll
+                for (uint32_t k = 0; k < kSteps; ++k)
+                    tc_mma_f16(tmem + (c == 2 ? kQpLead + (k / (kSteps / 2)) * kQpKeys : kQpCorrections), q_desc + ((qp * kQPlane + (k / 4) * (kQPlane / kHalves)) >> 4) + 2 * (k % 4),
+                               k_desc + (((b * 2 + kp) * kKPlane + (k / 4) * (kKPlane / kHalves)) >> 4) + 2 * (k % 4), score_desc, c == 2 ? k % (kSteps / 2) > 0 : (c | k) > 0);
+            }
+            tc_commit(&k_free[b]);
+            tc_commit(&s_full);
+        };
+        bool ok = mbar_wait(&k_full[0], 0);
+        if (ok) { tc_fence_after_sync(); scores(0); }
+        const uint32_t count = end - begin;
+        for (uint32_t j = 0; ok && j < count; ++j) {
+            if (j + 1 < count) {
+                ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1) && mbar_wait(&s_empty, j & 1);
+                if (!ok) break;
+                tc_fence_after_sync();
+                scores((j + 1) & 1);
+            }
+            ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1) && mbar_wait(&p_full, j & 1) && (j == 0 || mbar_wait(&o_empty, (j - 1) & 1));
+            if (!ok) break;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                const uint32_t pp = c == 0 ? 1 : 0, vp = c == 1 ? 1 : 0;
+#pragma unroll
+                for (uint32_t k = 0; k < kQpKeys / 16; ++k)
+                    tc_mma_f16_ts(tmem + kQpOut, tmem + kQpP + 32 * pp + 8 * k, v_desc + (((j & 1) * 2 + vp) * kVPlane >> 4) + 2 * k, out_desc, (c | k) > 0);
+            }
+            tc_commit(&v_free[j & 1]);
+            tc_commit(&o_full);
+        }
+        if (!ok) atomicExch(p.error_word, kErrFullWaitTimeout);
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kQpIssueWarp) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, kQpColumns);
+    }
+}
+
+}  // namespace zk

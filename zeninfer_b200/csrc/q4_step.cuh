@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
         return;
     }
     const uint32_t filled = filled_in, seen = filled + p.tokens;
-    const Q4Runs runs = q4_runs(seen, p.splits, kWarps);
+    const Q4Runs runs = q4_runs(seen, p.splits, kWarps, kQ4Tile);
     const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
     if (!kCluster && begin >= end) return;                                                // nobody counts on this run
     uint8_t* ring = q4_smem + warp * kQ4Stages * kStage;

@@ -11,6 +11,7 @@
 #include "host_state.h"
 #include "q4_attention.cuh"
 #include "q4_cache.cuh"
+#include "q4_prompt.cuh"
 #include "q4_step.cuh"
 #include "verify_drafts.cuh"
 
@@ -69,12 +70,13 @@ zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
     return zk::Q4Cache{c.k_codes, c.v_codes, reinterpret_cast<__half*>(c.k_scales), reinterpret_cast<__half*>(c.v_scales), c.kv_heads, c.head_dim / zk::kQ4Block, c.slots};
 }
 
-constexpr size_t kWaveCtas = 2 * 148;      // two CTAs on every SM
+constexpr size_t kSms = 148, kWaveCtas = 2 * kSms;
+constexpr size_t kPromptRows = 8;          // above: q4_prompt.cuh, for the heads it takes
 
 // How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
 struct AttentionPlan {
     int columns{};
-    uint32_t rows{}, padded{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{}, cluster{};
+    uint32_t rows{}, padded{}, row_warps{}, cta_rows{}, row_ctas{}, splits{}, key_warps{}, cluster{}, run_tile{zk::kQ4Tile};
     bool keep_scores{};
     size_t part_out{}, part_stats{}, scores{}, stats{}, queries{}, factors{}, bytes{};      // offsets into the workspace, and its size; 0: not a call
 };
@@ -82,7 +84,23 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     AttentionPlan n;
     if (!a || !cache_ok(&a->cache) || !a->heads || a->heads % a->cache.kv_heads || a->heads > 65535 || !tokens || tokens > a->cache.slots) return n;
     const size_t kv_heads = a->cache.kv_heads, rows = tokens * (a->heads / kv_heads), blocks = a->cache.head_dim / zk::kQ4Block, tiles = a->cache.slots / zk::kQ4Tile;
+    if (tokens * a->heads > 0x1fffffffu / blocks) return n;      // what a launch counts in 32 bits
     n.columns = rows <= 4 ? zk::kQ4Digits : rows <= 8 || blocks > 4 ? zk::kQ4Rows8 : zk::kQ4Rows16;
+    if ((blocks == 2 || blocks == 4) && rows > kPromptRows && !(a->weight_out && rows > zk::kQ4KeptRows)) {
+        const size_t row_tiles = (rows + zk::kQpRows - 1) / zk::kQpRows, key_tiles = (a->cache.slots + zk::kQpKeys - 1) / zk::kQpKeys;
+        if (row_tiles > 65535) return n;
+        n.columns = zk::kQ4Prompt;
+        n.rows = u32(rows); n.cta_rows = zk::kQpRows; n.row_ctas = u32(row_tiles); n.padded = u32(row_tiles * zk::kQpRows); n.key_warps = 1; n.run_tile = zk::kQpKeys;
+        n.splits = u32(std::max<size_t>(1, std::min(kSms / (row_tiles * kv_heads), key_tiles)));
+        n.keep_scores = a->weight_out;
+        size_t at = 0;
+        auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
+        if (n.splits > 1) n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
+        if (n.splits > 1 || n.keep_scores) n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
+        if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
+        n.bytes = std::max<size_t>(at, 16);
+        return n;
+    }
     const size_t per_warp = zk::q4_rows(n.columns), warps = zk::q4_warps(n.columns);
     size_t row_warps = 1;
     while (row_warps < warps && row_warps * per_warp < rows) row_warps *= 2;
@@ -128,6 +146,9 @@ cudaError_t by_blocks(uint32_t blocks, Run run) {
     }
 }
 
+template <typename Run>
+cudaError_t by_prompt_blocks(uint32_t blocks, Run run) { return blocks == 2 ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{}); }
+
 struct Span {
     uintptr_t begin, end;
 };
@@ -165,7 +186,7 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     zk::Q4Attend p{};
     p.cache = cache; p.turn = turn; p.q = d_q; p.k = d_k; p.v = d_v; p.k_held = a->k_held; p.v_held = a->v_held;
     p.position = a->position; p.filled = a->filled; p.weight_in = a->weight_in; p.weight_out = a->weight_out; p.out = d_out;
-    p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps; p.padded = plan.padded;
+    p.tokens = u32(tokens); p.heads = a->heads; p.group = a->heads / cache.kv_heads; p.splits = plan.splits; p.row_warps = plan.row_warps; p.padded = plan.padded; p.run_tile = plan.run_tile;
     p.q_ld = a->q_ld ? a->q_ld : q_row; p.kv_ld = a->kv_ld ? a->kv_ld : kv_row; p.scale = a->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(a->cache.head_dim)) : a->scale;
     p.error_word = e.d_error;
     if (plan.cluster) {
@@ -177,7 +198,16 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     p.part_out = part(plan.part_out); p.part_stats = part(plan.part_stats);
     if (plan.keep_scores) p.scores = part(plan.scores);
     else if (a->weight_out) p.stats = part(plan.stats);
-    if (!digits) {
+    const bool prompt = plan.columns == zk::kQ4Prompt;
+    if (prompt) {
+        const size_t items = tokens * cache.kv_heads * 2 * cache.blocks, a_cta = zk::kQ4AppendWarps * zk::kQ4AppendEach;
+        const cudaError_t r = by_prompt_blocks(cache.blocks, [&](auto blocks) {
+            constexpr int kBlocks = decltype(blocks)::value;
+            const cudaError_t appended = launch(e, zk::q4_append_kernel<kBlocks>, dim3(u32((items + a_cta - 1) / a_cta)), dim3(zk::kQ4AppendWarps * 32), 0, 0, p);
+            return appended != cudaSuccess ? appended : launch(e, zk::q4_prompt_kernel<kBlocks>, dim3(plan.splits, plan.row_ctas, cache.kv_heads), dim3(zk::kQpThreads), zk::q4_prompt_smem<kBlocks>(), 0, p);
+        });
+        if (!e.leave(r, "dev_q4_attention")) return 0;
+    } else if (!digits) {
         p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors);
         const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) {
             return launch(e, zk::q4_prepare_kernel<decltype(blocks)::value>, dim3(u32(tokens), cache.kv_heads), dim3(32 * std::min<uint32_t>(zk::kQ4PrepareWarps, 2 * cache.blocks + p.group)), 0, 0, p);
@@ -188,7 +218,7 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
         constexpr int kBlocks = decltype(blocks)::value, kColumns = decltype(columns)::value;
         return launch(e, zk::q4_attend_kernel<kBlocks, kColumns>, dim3(plan.splits, plan.row_ctas, cache.kv_heads), dim3(zk::q4_warps(kColumns) * 32), zk::q4_attend_smem<kBlocks, kColumns>(plan.row_warps), 0, p);
     };
-    const cudaError_t r = by_blocks(cache.blocks, [&](auto blocks) {
+    const cudaError_t r = prompt ? cudaSuccess : by_blocks(cache.blocks, [&](auto blocks) {
         constexpr int kBlocks = decltype(blocks)::value;
         if (digits) return launch(e, zk::q4_step_kernel<kBlocks, false>, dim3(plan.splits, 1, cache.kv_heads), dim3(zk::kQ4StepWarps * 32), zk::q4_step_smem<kBlocks>(false), 0, p);
         if constexpr (kBlocks <= 4) {
