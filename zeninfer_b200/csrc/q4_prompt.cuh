@@ -9,7 +9,8 @@
 // A CTA takes 128 rows (a row: a token times a query head of the kv head, any group) and walks its run of slots 64 at a time.  Sixteen warps:
 //   8 rows       a thread has half a row: 32 scores from TMEM, mask, running maximum (shared with the other half), exponentials, the weights' two parts back to
 //                TMEM, from where the tensor cores read them; then out = out * factor + O' of the tile before, in fp32 registers
-//   4 + 3        unpack keys and values (asked for from L2 a tile ahead) into the operands' 128-byte swizzle, two buffers each; values by eight slots, transposed
+//   4 + 3        unpack keys and values (bulk copies bring the tiles into a ring, two ahead) into the operands' 128-byte swizzle, two buffers each; values by eight
+//                slots, transposed
 //   1 issues     S = Q K^T into three accumulators (the corrections, and the leading products of each half of the head, for the tensor cores cut a sum at
 //                every 16 columns), O' = P V corrections first
 // The scores of tile j + 1 are formed while tile j is exponentiated.
@@ -26,7 +27,9 @@ constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 16 * 32, kQpKeyWarp
 template <int kBlocks> constexpr uint32_t kQpQPlane = kQpRows * kBlocks * 64;      // bytes
 template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;
 template <int kBlocks> constexpr uint32_t kQpVPlane = kBlocks * 32 * kQpKeys * 2;
-template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 4 * kQpKPlane<kBlocks> + 4 * kQpVPlane<kBlocks>; }
+constexpr int kQpStages = 3;                 // tiles as they are in the cache, ahead of the warps that unpack them
+template <int kBlocks> constexpr uint32_t kQpRaw = kQpKeys * kBlocks * 36;
+template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 4 * kQpKPlane<kBlocks> + 4 * kQpVPlane<kBlocks> + kQpStages * kQpRaw<kBlocks>; }
 // TMEM columns: leading scores of the head's halves, corrections; the weights' parts; O'
 constexpr uint32_t kQpLead = 0, kQpCorrections = 128, kQpP = 192, kQpOut = 256, kQpColumns = 512;
 
@@ -47,22 +50,58 @@ __device__ __forceinline__ uint32_t f16x2_rest(uint32_t a, uint32_t b, uint32_t 
 __device__ __forceinline__ int q4_shift(uint32_t top) { return 23 - static_cast<int>(top >> 10); }
 __device__ __forceinline__ bool q4_finite(uint32_t half_bits) { return (half_bits & 0x7c00u) != 0x7c00u; }
 
-// The largest magnitude among the finite scales of `slots` slots from slot0 on that are seen, as f16 bits: every lane of a warp.  scales: the head's first.
+// The largest magnitude among the finite scales of the first `slots` of a tile's 64 slots, as f16 bits: every lane of a warp.
 template <int kBlocks>
-__device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slot0, uint32_t slots, uint32_t seen, uint32_t lane) {
+__device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slots, uint32_t lane) {
     uint32_t top = 0;
-    for (uint32_t i = lane; i < slots * kBlocks / 8; i += 32) {            // eight scales at a time: 8 / kBlocks slots
-        const uint32_t slot = slot0 + i * 8 / kBlocks;
-        if (slot >= seen) break;
-        const uint4 eight = __ldcg(reinterpret_cast<const uint4*>(scales + static_cast<size_t>(slot0) * kBlocks) + i);
+    if (lane < kQpKeys * kBlocks / 8) {                       // eight scales a lane: 8 / kBlocks slots
+        const uint4 eight = reinterpret_cast<const uint4*>(scales)[lane];
         const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0x7fffu;
-            if (slot + j / kBlocks < seen && q4_finite(bits)) top = max(top, bits);
+            if (lane * 8 / kBlocks + j / kBlocks < slots && q4_finite(bits)) top = max(top, bits);
         }
     }
     return __reduce_max_sync(0xffffffffu, top);
+}
+
+// Eight dimensions of a head vector, rotated: at .. at + 3 and at + 16 .. at + 19.  Four at a time where the whole head turns and everything is aligned, else one by one; the
+// operations are q4_rotated's.
+__device__ __forceinline__ bool q4_rotates_fours(const float* q, size_t q_ld, uint32_t dim, const Q4Rotation& r) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | (q_ld * 4) | (r.pairs ? reinterpret_cast<uintptr_t>(r.cos_t) | reinterpret_cast<uintptr_t>(r.sin_t) : 0);
+    return all % 16 == 0 && (!r.pairs || 2 * r.pairs == dim);
+}
+__device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row, bool fours) {
+    if (!fours) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = q4_rotated(head, at + (e & 3) + (e >> 2) * 16, r, row);
+        return;
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const uint32_t e = at + 16 * part;
+        const float4 mine = __ldcg(reinterpret_cast<const float4*>(head + e));
+        float* y = x + 4 * part;
+        if (!r.pairs) {
+            y[0] = mine.x; y[1] = mine.y; y[2] = mine.z; y[3] = mine.w;
+        } else if (r.adjacent) {
+            const float* const cos_t = r.cos_t + row * r.pairs + e / 2;
+            const float* const sin_t = r.sin_t + row * r.pairs + e / 2;
+            const float2 c = __ldg(reinterpret_cast<const float2*>(cos_t)), s = __ldg(reinterpret_cast<const float2*>(sin_t));
+            y[0] = __fsub_rn(__fmul_rn(mine.x, c.x), __fmul_rn(mine.y, s.x)); y[1] = __fadd_rn(__fmul_rn(mine.x, s.x), __fmul_rn(mine.y, c.x));
+            y[2] = __fsub_rn(__fmul_rn(mine.z, c.y), __fmul_rn(mine.w, s.y)); y[3] = __fadd_rn(__fmul_rn(mine.z, s.y), __fmul_rn(mine.w, c.y));
+        } else {
+            const bool low = e < r.pairs;
+            const uint32_t pair = low ? e : e - r.pairs;
+            const float4 its = __ldcg(reinterpret_cast<const float4*>(head + (low ? e + r.pairs : pair)));
+            const float* const cos_t = r.cos_t + row * r.pairs + pair;
+            const float* const sin_t = r.sin_t + row * r.pairs + pair;
+            const float4 c = __ldg(reinterpret_cast<const float4*>(cos_t)), s = __ldg(reinterpret_cast<const float4*>(sin_t));
+            auto turned = [&](float a, float b, float cc, float ss) { return low ? __fsub_rn(__fmul_rn(a, cc), __fmul_rn(b, ss)) : __fadd_rn(__fmul_rn(b, ss), __fmul_rn(a, cc)); };
+            y[0] = turned(mine.x, its.x, c.x, s.x); y[1] = turned(mine.y, its.y, c.y, s.y); y[2] = turned(mine.z, its.z, c.z, s.z); y[3] = turned(mine.w, its.w, c.w, s.w);
+        }
+    }
 }
 
 // Eight dimensions of a row of queries in the scores' order, 4j .. 4j+3 and 16+4j .. 16+4j+3 of a block, as they are unpacked from a word of codes.
@@ -100,13 +139,15 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     uint8_t* const q_smem = smem;                             // [plane][64 dimensions][128 rows][128 bytes]
     uint8_t* const k_smem = q_smem + 2 * kQPlane;             // [buffer][plane][64 dimensions][64 slots][128 bytes]
     uint8_t* const v_smem = k_smem + 4 * kKPlane;             // [buffer][plane][the head's dimensions][64 slots]
+    uint8_t* const raw_smem = v_smem + 4 * kVPlane;           // [stage]: codes of keys and of values, scales of keys and of values
     __shared__ float row_factor[kQpRows], top[2][2][kQpRows], sum[2][kQpRows];
-    __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_empty, p_full, o_full, o_empty;
+    __shared__ uint64_t raw_full[kQpStages], raw_free[kQpStages], k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_empty, p_full, o_full, o_empty;
     __shared__ float k_unit[4], v_unit[4];                    // what a tile's operands are to be multiplied by: the rows read the last but one while the next is stored
     __shared__ uint32_t tmem_slot, bad_key, bad_value[kBlocks];      // the first slots whose scales are not finite
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, h = blockIdx.z, rows = p.tokens * p.group;
     const uint32_t first_row = (gridDim.y - 1 - blockIdx.y) * kQpRows, real_rows = min(kQpRows, rows - first_row);
     if (threadIdx.x == 0) {
+        for (int b = 0; b < kQpStages; ++b) { mbar_init(&raw_full[b], 1); mbar_init(&raw_free[b], kQpIssueWarp - kQpKeyWarp); }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&k_full[b], kQpValueWarp - kQpKeyWarp); mbar_init(&v_full[b], kQpIssueWarp - kQpValueWarp);
             mbar_init(&k_free[b], 1); mbar_init(&v_free[b], 1);
@@ -126,18 +167,28 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
     if (begin >= end) return;                                                            // nobody counts on this run
     if (warp == kQpIssueWarp) tmem_alloc(&tmem_slot, kQpColumns);
-
+    constexpr uint32_t kCodes = kQpKeys * kBlocks * 16, kScales = kQpKeys * kBlocks * 2;
+    auto bring = [&](uint32_t tile, int stage) {              // the last tile may have half of its slots beyond the cache's end
+        const uint32_t slots = min(kQpKeys, p.cache.slots - tile * kQpKeys);
+        const size_t slot = static_cast<size_t>(h) * p.cache.slots + static_cast<size_t>(tile) * kQpKeys;
+        uint8_t* to = raw_smem + stage * kQpRaw<kBlocks>;
+        mbar_arrive_expect_tx(&raw_full[stage], slots * kBlocks * 36);
+        bulk_g2s(to, p.cache.k_codes + slot * (kBlocks * 16), slots * kBlocks * 16, &raw_full[stage]);
+        bulk_g2s(to + kCodes, p.cache.v_codes + slot * (kBlocks * 16), slots * kBlocks * 16, &raw_full[stage]);
+        bulk_g2s(to + 2 * kCodes, p.cache.k_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
+        bulk_g2s(to + 2 * kCodes + kScales, p.cache.v_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
+    };
     {      // Q: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
         constexpr uint32_t kChunks = kDim / 8, kEach = kQpRows * kChunks / kQpThreads;
         const uint32_t chunk = threadIdx.x % kChunks, dim = chunk / 4 * 32 + chunk % 4 * 4;
+        const bool fours = q4_rotates_fours(p.q, p.q_ld, kDim, p.turn);
         float x[kEach][8];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
             const uint32_t r = threadIdx.x / kChunks + i * (kQpThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
             const float* from = p.q + token * p.q_ld + static_cast<size_t>(h * p.group + row % p.group) * kDim;
             const size_t turned = static_cast<size_t>(position) + token;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = q4_rotated(from, dim + (e & 3) + (e >> 2) * 16, p.turn, turned);
+            q4_rotated_eight(x[i], from, dim, p.turn, turned, fours);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
@@ -305,37 +356,35 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 if (!alone || p.scores) reinterpret_cast<float2*>(p.part_stats)[part] = make_float2(m, l);
             }
         }
-    } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot
+    } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot; the first one keeps the ring filled
         constexpr uint32_t kId = (kQpValueWarp - kQpKeyWarp) * 32, kEach = kQpKeys * kBlocks / kId;
-        const uint32_t id = threadIdx.x - kQpKeyWarp * 32;
-        const __half* const scales = p.cache.k_scales + static_cast<size_t>(h) * p.cache.slots * kBlocks;
-        uint4 codes[kEach];
-        uint32_t scale[kEach], largest = 0;
-        auto ask = [&](uint32_t tile) {
-            largest = q4_largest_scale<kBlocks>(scales, tile * kQpKeys, kQpKeys, seen, lane);
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t item = id + kId * i, slot = tile * kQpKeys + item % kQpKeys, block = item / kQpKeys;
-                const bool real = slot < seen;
-                codes[i] = real ? __ldcg(reinterpret_cast<const uint4*>(p.cache.k_codes + q4_codes_at(h, slot, block, kBlocks, p.cache.slots))) : make_uint4(0, 0, 0, 0);
-                scale[i] = real ? __half_as_ushort(__ldcg(scales + static_cast<size_t>(slot) * kBlocks + block)) : 0u;
-            }
-        };
-        ask(begin);
-        uint32_t j = 0;
-        for (uint32_t tile = begin; tile < end; ++tile, ++j) {
+        const uint32_t id = threadIdx.x - kQpKeyWarp * 32, count = end - begin;
+        if (id == 0) {
+            asm volatile("fence.proxy.async;" ::: "memory");      // the stores of the launch before come ahead of the copies
+            for (uint32_t j = 0; j < min(count, kQpStages - 1u); ++j) bring(begin + j, j);
+        }
+        __syncwarp();
+        int stage = 0;
+        uint32_t phase = 0, j = 0, brought = min(count, kQpStages - 1u);
+        for (; j < count; ++j) {
+            const uint32_t tile = begin + j, slots = min(kQpKeys, seen - tile * kQpKeys);
+            if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
+            const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
+            const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes);
+            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane));
             if (j > 1 && !warp_waited(&k_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            const int shift = q4_shift(largest);
             uint8_t* const to = k_smem + (j & 1) * 2 * kKPlane;
 #pragma unroll
             for (uint32_t i = 0; i < kEach; ++i) {
                 const uint32_t item = id + kId * i, r = item % kQpKeys, block = item / kQpKeys;
-                if (!q4_finite(scale[i])) {
+                const uint4 codes = *reinterpret_cast<const uint4*>(raw + (((r >> 3) * kBlocks + block) * 8 + (r & 7u)) * 16);
+                uint32_t bits = r < slots ? __half_as_ushort(scales[r * kBlocks + block]) : 0u;
+                if (!q4_finite(bits)) {
                     atomicMin(&bad_key, tile * kQpKeys + r);
-                    scale[i] = 0;
+                    bits = 0;
                 }
-                const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(scale[i]))) * power_of_two(shift);
-                const uint32_t d2 = pack_f16(d, d), w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * power_of_two(shift);
+                const uint32_t d2 = pack_f16(d, d), w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
                 for (uint32_t word = 0; word < 4; ++word) {
                     uint4 upper, lower;
@@ -348,68 +397,70 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (id == 0) k_unit[j & 3] = power_of_two(-shift);
             async_proxy_fence();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[j & 1]);
-            if (tile + 1 < end) ask(tile + 1);
+            if (lane == 0) { mbar_arrive(&k_full[j & 1]); mbar_arrive(&raw_free[stage]); }
+            if (id == 0 && j + kQpStages - 1 < count) {           // the stage of the tile before, once the values' warps are done with it as well
+                const uint32_t to_stage = (j + kQpStages - 1) % kQpStages;
+                if (j == 0 || mbar_wait(&raw_free[to_stage], ((j - 1) / kQpStages) & 1u)) {
+                    bring(tile + kQpStages - 1, to_stage);
+                    ++brought;
+                } else {
+                    atomicExch(p.error_word, kErrEmptyWaitTimeout);       // the waits for the tile run out as well
+                }
+            }
+            __syncwarp();
+            if (++stage == kQpStages) { stage = 0; phase ^= 1u; }
         }
+        if (id == 0)                                              // given up: what is under way lands before the memory is another's
+            for (; j < brought; ++j) mbar_wait(&raw_full[j % kQpStages], (j / kQpStages) & 1u);
     } else if (warp < kQpIssueWarp) {                         // values: a thread takes a word (eight dimensions) of eight slots
         constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32, kItems = kQpKeys / 8 * kBlocks * 4, kEach = (kItems + kId - 1) / kId;
-        const uint32_t id = threadIdx.x - kQpValueWarp * 32;
-        const __half* const scales = p.cache.v_scales + static_cast<size_t>(h) * p.cache.slots * kBlocks;
-        uint32_t w[kEach][8], largest = 0;
-        auto ask = [&](uint32_t tile) {
-            largest = q4_largest_scale<kBlocks>(scales, tile * kQpKeys, kQpKeys, seen, lane);
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t item = id + kId * i, octet = item % 8, word = item / 8 % 4, block = item / 32;
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t slot = tile * kQpKeys + octet * 8 + k;
-                    w[i][k] = item < kItems && slot < seen ? __ldcg(reinterpret_cast<const uint32_t*>(p.cache.v_codes + q4_codes_at(h, slot, block, kBlocks, p.cache.slots)) + word) : 0u;
-                }
-            }
-        };
-        ask(begin);
-        uint32_t j = 0;
-        for (uint32_t tile = begin; tile < end; ++tile, ++j) {
-            const int shift = q4_shift(largest);
+        const uint32_t id = threadIdx.x - kQpValueWarp * 32, count = end - begin;
+        int stage = 0;
+        uint32_t phase = 0;
+        for (uint32_t j = 0; j < count; ++j) {
+            const uint32_t tile = begin + j, slots = min(kQpKeys, seen - tile * kQpKeys);
+            if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
+            const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
+            const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes + kScales);
+            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane));
             const float up = power_of_two(shift);
-            uint32_t d2[kEach][4];
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t item = id + kId * i, octet = item % 8, block = item / 32;
-                float d[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t slot = tile * kQpKeys + octet * 8 + k;
-                    uint32_t bits = item < kItems && slot < seen ? __half_as_ushort(__ldcg(scales + static_cast<size_t>(slot) * kBlocks + block)) : 0u;
-                    if (!q4_finite(bits)) {
-                        atomicMin(&bad_value[block], slot);
-                        bits = 0;
-                    }
-                    d[k] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) d2[i][k] = pack_f16(d[2 * k], d[2 * k + 1]);
-            }
             if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
             uint8_t* const to = v_smem + (j & 1) * 2 * kVPlane;
 #pragma unroll
             for (uint32_t i = 0; i < kEach; ++i) {
                 const uint32_t item = id + kId * i, octet = item % 8, word = item / 8 % 4, block = item / 32;
                 if (item >= kItems) continue;
+                uint32_t w[8], d2[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint32_t*>(raw + kCodes + ((octet * kBlocks + block) * 8 + k) * 16 + word * 4);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    float d[2];
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const uint32_t r = octet * 8 + 2 * k + e;
+                        uint32_t bits = r < slots ? __half_as_ushort(scales[r * kBlocks + block]) : 0u;
+                        if (!q4_finite(bits)) {
+                            atomicMin(&bad_value[block], tile * kQpKeys + r);
+                            bits = 0;
+                        }
+                        d[e] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
+                    }
+                    d2[k] = pack_f16(d[0], d[1]);
+                }
 #pragma unroll
                 for (uint32_t pair = 0; pair < 2; ++pair) {      // bytes 0 and 1, bytes 2 and 3 of the words
                     uint32_t x[4];
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) x[k] = __byte_perm(w[i][2 * k], w[i][2 * k + 1], pair ? 0x7632 : 0x5410);
+                    for (uint32_t k = 0; k < 4; ++k) x[k] = __byte_perm(w[2 * k], w[2 * k + 1], pair ? 0x7632 : 0x5410);
 #pragma unroll
                     for (uint32_t nibble = 0; nibble < 4; ++nibble) {
                         uint32_t upper[4], lower[4];
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
                             const uint32_t y = nibble & 2 ? x[k] >> 8 : x[k], c = nibble & 1 ? signed_high(y) : signed_low(y);
-                            upper[k] = f16x2_mul(c, d2[i][k]);
-                            lower[k] = f16x2_rest(c, d2[i][k], upper[k]);
+                            upper[k] = f16x2_mul(c, d2[k]);
+                            lower[k] = f16x2_rest(c, d2[k], upper[k]);
                         }
                         const uint32_t dim = block * 32 + (nibble & 1) * 16 + word * 4 + pair * 2 + (nibble >> 1);
                         const uint32_t at = dim * 128 + ((octet ^ (dim & 7)) << 4);
@@ -421,8 +472,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
             async_proxy_fence();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[j & 1]);
-            if (tile + 1 < end) ask(tile + 1);
+            if (lane == 0) { mbar_arrive(&v_full[j & 1]); mbar_arrive(&raw_free[stage]); }
+            if (++stage == kQpStages) { stage = 0; phase ^= 1u; }
         }
     } else if (lane == 0) {                                   // the tensor cores
         constexpr uint32_t score_desc = umma_idesc_f16(kQpRows, kQpKeys), out_desc = umma_idesc_f16(kQpRows, kDim), kSteps = kDim / 16;
