@@ -4,13 +4,13 @@
 // block's scale goes.  Here it goes into the operand: d (c - 8) is a number of fifteen bits, exactly the sum of two f16 numbers (the rounded product and
 // its remainder, a multiplication and a multiply-add of halves), so a product is three products of f16 numbers (the fourth is below 2^-22 of it), and nothing has to be
 // done per block and score.  A tile's scales are multiplied by the power of two that brings the largest below 2^9, so that both parts keep their bits
-// whatever the model's magnitudes are.  The dimensions of the scores' operands stand in the order in which the nibbles are unpacked.
+// whatever the model's magnitudes are.  The dimensions of the operands stand in the order in which the nibbles are unpacked.
 //
 // A CTA takes 128 rows (a row: a token times a query head of the kv head, any group) and walks its run of slots 64 at a time.  Sixteen warps:
 //   8 rows       a thread has half a row: 32 scores from TMEM, mask, running maximum (shared with the other half), exponentials, the weights' two parts back to
-//                TMEM, from where the tensor cores read them; then out = out * factor + O' of the tile before, in fp32 registers
-//   4 + 3        unpack keys and values (bulk copies bring the tiles into a ring, two ahead) into the operands' 128-byte swizzle, two buffers each; values by eight
-//                slots, transposed
+//                TMEM, from where the tensor cores read them (as they do the queries); then out = out * factor + O' of the tile before, in fp32 registers
+//   3 + 4        unpack keys and values (bulk copies bring the tiles into a ring, two ahead) into the operands' 128-byte swizzle, two buffers each, a slot's block a
+//                thread: to the tensor cores keys are a matrix with the summed index in its rows, values one with it in its columns, so neither is transposed
 //   1 issues     S = Q K^T into three accumulators (the corrections, and the leading products of each half of the head, for the tensor cores cut a sum at
 //                every 16 columns), O' = P V corrections first
 // The scores of tile j + 1 are formed while tile j is exponentiated.
@@ -23,18 +23,22 @@
 
 namespace zk {
 
-constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 16 * 32, kQpKeyWarp = 8, kQpValueWarp = 12, kQpIssueWarp = 15;      // first warps of the roles
+constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 16 * 32, kQpKeyWarp = 8, kQpValueWarp = 11, kQpIssueWarp = 15;      // first warps of the roles
 template <int kBlocks> constexpr uint32_t kQpQPlane = kQpRows * kBlocks * 64;      // bytes
-template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;
-template <int kBlocks> constexpr uint32_t kQpVPlane = kBlocks * 32 * kQpKeys * 2;
+template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;      // of keys, of values
 constexpr int kQpStages = 3;                 // tiles as they are in the cache, ahead of the warps that unpack them
 template <int kBlocks> constexpr uint32_t kQpRaw = kQpKeys * kBlocks * 36;
-template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 4 * kQpKPlane<kBlocks> + 4 * kQpVPlane<kBlocks> + kQpStages * kQpRaw<kBlocks>; }
-// TMEM columns: leading scores of the head's halves, corrections; the weights' parts; O'
-constexpr uint32_t kQpLead = 0, kQpCorrections = 128, kQpP = 192, kQpOut = 256, kQpColumns = 512;
+template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 8 * kQpKPlane<kBlocks> + kQpStages * kQpRaw<kBlocks>; }
+// TMEM columns: leading scores of the head's halves, corrections; the weights' parts; O'; the queries' parts
+constexpr uint32_t kQpLead = 0, kQpCorrections = 128, kQpP = 192, kQpOut = 256, kQpQ = 384, kQpColumns = 512;
 
-// Instruction descriptor, kind::f16: f16 x f16 -> fp32, both operands K-major, dense.
-__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+// Instruction descriptor, kind::f16: f16 x f16 -> fp32, dense, A K-major, B K-major or (across) MN-major.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n, bool across = false) { return (1u << 4) | (across ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+// Shared-memory descriptor of an MN-major operand with the 128-byte swizzle: rows of 64 columns (128 bytes), one for each index that is summed over, eight of them a group of
+// 1024 bytes; the next 64 columns begin `apart` bytes on.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t apart) {
+    return (umma_desc_k_sw128(smem_addr) & ~(static_cast<uint64_t>(0x3fff) << 16)) | (static_cast<uint64_t>(apart >> 4) << 16);
+}
 
 __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -50,18 +54,26 @@ __device__ __forceinline__ uint32_t f16x2_rest(uint32_t a, uint32_t b, uint32_t 
 __device__ __forceinline__ int q4_shift(uint32_t top) { return 23 - static_cast<int>(top >> 10); }
 __device__ __forceinline__ bool q4_finite(uint32_t half_bits) { return (half_bits & 0x7c00u) != 0x7c00u; }
 
-// The largest magnitude among the finite scales of the first `slots` of a tile's 64 slots, as f16 bits: every lane of a warp.
-template <int kBlocks>
-__device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slots, uint32_t lane) {
-    uint32_t top = 0;
+// The largest magnitude among the finite scales of the first `slots` of a tile's 64 slots, as f16 bits: every lane of a warp.  bad(slot, block) is called for the others.
+template <int kBlocks, typename Bad>
+__device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slots, uint32_t lane, Bad bad) {
+    uint32_t top = 0, w[4] = {};
+    bool odd = false;
     if (lane < kQpKeys * kBlocks / 8) {                       // eight scales a lane: 8 / kBlocks slots
         const uint4 eight = reinterpret_cast<const uint4*>(scales)[lane];
-        const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
+        w[0] = eight.x; w[1] = eight.y; w[2] = eight.z; w[3] = eight.w;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0x7fffu;
-            if (lane * 8 / kBlocks + j / kBlocks < slots && q4_finite(bits)) top = max(top, bits);
+            if (lane * 8 / kBlocks + j / kBlocks >= slots) continue;
+            if (q4_finite(bits)) top = max(top, bits);
+            else odd = true;
         }
+    }
+    if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+        for (uint32_t i = lane; i < slots * kBlocks; i += 32)
+            if (!q4_finite(__half_as_ushort(scales[i]))) bad(i / kBlocks, i % kBlocks);
     }
     return __reduce_max_sync(0xffffffffu, top);
 }
@@ -130,18 +142,44 @@ __device__ __forceinline__ void q4_split_codes(uint32_t w, uint32_t d2, uint4& u
     lower = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
+// A tile's codes (64 slots, as the cache holds them) times their scales, 2^shift as large, into both planes: rows of 64 dimensions a slot.  Scales that are not finite, and
+// those of slots that are not the rows' to see, count as zero.  kThreads threads, the id-th of them here.
+template <int kBlocks, uint32_t kThreads>
+__device__ __forceinline__ void q4_unpack_tile(const uint8_t* codes, const __half* scales, uint32_t slots, int shift, uint8_t* to, uint32_t id) {
+    constexpr uint32_t kItems = kQpKeys * kBlocks, kEach = (kItems + kThreads - 1) / kThreads, kPlane = kQpKPlane<kBlocks>, kHalves = kBlocks / 2;
+    const float up = power_of_two(shift);
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t item = id + kThreads * i, r = item % kQpKeys, block = item / kQpKeys;
+        if (kItems % kThreads && item >= kItems) break;       // a whole warp
+        const uint4 four = *reinterpret_cast<const uint4*>(codes + (((r >> 3) * kBlocks + block) * 8 + (r & 7u)) * 16);
+        uint32_t bits = __half_as_ushort(scales[r * kBlocks + block]);
+        if (!q4_finite(bits) || r >= slots) bits = 0;
+        const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
+        const uint32_t d2 = pack_f16(d, d), w[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (uint32_t word = 0; word < 4; ++word) {
+            uint4 upper, lower;
+            q4_split_codes(w[word], d2, upper, lower);
+            const uint32_t at = (block / 2) * (kPlane / kHalves) + r * 128 + ((((block & 1) * 4 + word) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4*>(to + at) = upper;
+            *reinterpret_cast<uint4*>(to + kPlane + at) = lower;
+        }
+    }
+}
+
 // grid = (splits, tiles of 128 rows, kv_heads); the rows that see most slots come first.
 template <int kBlocks>
 __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_constant__ Q4Attend p) {
-    constexpr uint32_t kDim = kBlocks * 32, kHalves = kBlocks / 2, kQPlane = kQpQPlane<kBlocks>, kKPlane = kQpKPlane<kBlocks>, kVPlane = kQpVPlane<kBlocks>;
+    constexpr uint32_t kDim = kBlocks * 32, kHalves = kBlocks / 2, kQPlane = kQpQPlane<kBlocks>, kKPlane = kQpKPlane<kBlocks>;
     extern __shared__ uint8_t qp_smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(qp_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const q_smem = smem;                             // [plane][64 dimensions][128 rows][128 bytes]
     uint8_t* const k_smem = q_smem + 2 * kQPlane;             // [buffer][plane][64 dimensions][64 slots][128 bytes]
-    uint8_t* const v_smem = k_smem + 4 * kKPlane;             // [buffer][plane][the head's dimensions][64 slots]
-    uint8_t* const raw_smem = v_smem + 4 * kVPlane;           // [stage]: codes of keys and of values, scales of keys and of values
+    uint8_t* const v_smem = k_smem + 4 * kKPlane;             // the same
+    uint8_t* const raw_smem = v_smem + 4 * kKPlane;           // [stage]: codes of keys and of values, scales of keys and of values
     __shared__ float row_factor[kQpRows], top[2][2][kQpRows], sum[2][kQpRows];
-    __shared__ uint64_t raw_full[kQpStages], raw_free[kQpStages], k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_empty, p_full, o_full, o_empty;
+    __shared__ uint64_t raw_full[kQpStages], raw_free[kQpStages], k_full[2], k_free[2], v_full[2], v_free[2], q_full, s_full, s_empty, p_full, o_full, o_empty;
     __shared__ float k_unit[4], v_unit[4];                    // what a tile's operands are to be multiplied by: the rows read the last but one while the next is stored
     __shared__ uint32_t tmem_slot, bad_key, bad_value[kBlocks];      // the first slots whose scales are not finite
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, h = blockIdx.z, rows = p.tokens * p.group;
@@ -152,7 +190,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             mbar_init(&k_full[b], kQpValueWarp - kQpKeyWarp); mbar_init(&v_full[b], kQpIssueWarp - kQpValueWarp);
             mbar_init(&k_free[b], 1); mbar_init(&v_free[b], 1);
         }
-        mbar_init(&s_full, 1); mbar_init(&s_empty, 8); mbar_init(&p_full, 8); mbar_init(&o_full, 1); mbar_init(&o_empty, 8);
+        mbar_init(&q_full, kQpKeyWarp); mbar_init(&s_full, 1); mbar_init(&s_empty, 8); mbar_init(&p_full, 8); mbar_init(&o_full, 1); mbar_init(&o_empty, 8);
         mbar_fence_init();
         bad_key = 0xffffffffu;
         for (int b = 0; b < kBlocks; ++b) bad_value[b] = 0xffffffffu;
@@ -225,6 +263,24 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_slot;
+    if (warp < kQpKeyWarp) {                                  // the queries into TMEM, a part of a row a thread: the products then read keys only from shared memory
+        const uint32_t r = (warp & 3u) * 32 + lane, plane = warp >> 2;
+#pragma unroll
+        for (uint32_t c = 0; c < kDim / 16; ++c) {
+            uint32_t both[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t chunk = 2 * c + i;
+                const uint4 its = *reinterpret_cast<const uint4*>(q_smem + plane * kQPlane + (chunk / 8) * (kQPlane / kHalves) + r * 128 + (((chunk % 8) ^ (r & 7)) << 4));
+                both[4 * i] = its.x; both[4 * i + 1] = its.y; both[4 * i + 2] = its.z; both[4 * i + 3] = its.w;
+            }
+            tmem_st_32x8(tmem + kQpQ + plane * (kDim / 2) + 8 * c + (((warp & 3u) * 32) << 16), both);
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+    }
     auto gave_up = [&](int code) { if (lane == 0) atomicExch(p.error_word, code); };
 
     // A wait that runs out ends its role's loop, and the others' follow.
@@ -343,10 +399,19 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             const uint32_t token = row / p.group, head = h * p.group + row % p.group;
             const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + row;
             float* to = (alone ? p.out + (static_cast<size_t>(token) * p.heads + head) * kDim : p.part_out + part * kDim) + half * kOut;
+            const bool fours = reinterpret_cast<uintptr_t>(to) % 16 == 0;
 #pragma unroll
-            for (int i = 0; i < kOut; ++i) {
-                const float o = last_seen >= bad_value[(half * kOut + i) / 32] ? NAN : acc[i] * inv;
-                to[i] = o;
+            for (int b = 0; b < kOut / 32; ++b) {
+                const bool bad = last_seen >= bad_value[half * (kOut / 32) + b];
+                const float by = bad ? NAN : inv;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {                 // four dimensions from 4i: where the nibbles are unpacked to
+                    const int at = 32 * b + i % 4 * 8 + i / 4 * 2;
+                    const float4 o = make_float4(acc[at] * by, acc[at + 4] * by, acc[at + 1] * by, acc[at + 5] * by);
+                    float* const here = to + 32 * b + 4 * i;
+                    if (fours) *reinterpret_cast<float4*>(here) = o;
+                    else { here[0] = o.x; here[1] = o.y; here[2] = o.z; here[3] = o.w; }
+                }
             }
             if (half == 0) {
                 if (alone) {
@@ -357,7 +422,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             }
         }
     } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot; the first one keeps the ring filled
-        constexpr uint32_t kId = (kQpValueWarp - kQpKeyWarp) * 32, kEach = kQpKeys * kBlocks / kId;
+        constexpr uint32_t kId = (kQpValueWarp - kQpKeyWarp) * 32;
         const uint32_t id = threadIdx.x - kQpKeyWarp * 32, count = end - begin;
         if (id == 0) {
             asm volatile("fence.proxy.async;" ::: "memory");      // the stores of the launch before come ahead of the copies
@@ -371,29 +436,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
             const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
             const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes);
-            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane));
+            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane, [&](uint32_t r, uint32_t) { atomicMin(&bad_key, tile * kQpKeys + r); }));
             if (j > 1 && !warp_waited(&k_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            uint8_t* const to = k_smem + (j & 1) * 2 * kKPlane;
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t item = id + kId * i, r = item % kQpKeys, block = item / kQpKeys;
-                const uint4 codes = *reinterpret_cast<const uint4*>(raw + (((r >> 3) * kBlocks + block) * 8 + (r & 7u)) * 16);
-                uint32_t bits = r < slots ? __half_as_ushort(scales[r * kBlocks + block]) : 0u;
-                if (!q4_finite(bits)) {
-                    atomicMin(&bad_key, tile * kQpKeys + r);
-                    bits = 0;
-                }
-                const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * power_of_two(shift);
-                const uint32_t d2 = pack_f16(d, d), w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-                for (uint32_t word = 0; word < 4; ++word) {
-                    uint4 upper, lower;
-                    q4_split_codes(w[word], d2, upper, lower);
-                    const uint32_t at = (block / 2) * (kKPlane / kHalves) + r * 128 + ((((block & 1) * 4 + word) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(to + at) = upper;
-                    *reinterpret_cast<uint4*>(to + kKPlane + at) = lower;
-                }
-            }
+            q4_unpack_tile<kBlocks, kId>(raw, scales, slots, shift, k_smem + (j & 1) * 2 * kKPlane, id);
             if (id == 0) k_unit[j & 3] = power_of_two(-shift);
             async_proxy_fence();
             __syncwarp();
@@ -412,8 +457,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         }
         if (id == 0)                                              // given up: what is under way lands before the memory is another's
             for (; j < brought; ++j) mbar_wait(&raw_full[j % kQpStages], (j / kQpStages) & 1u);
-    } else if (warp < kQpIssueWarp) {                         // values: a thread takes a word (eight dimensions) of eight slots
-        constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32, kItems = kQpKeys / 8 * kBlocks * 4, kEach = (kItems + kId - 1) / kId;
+    } else if (warp < kQpIssueWarp) {                         // values: the same
+        constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32;
         const uint32_t id = threadIdx.x - kQpValueWarp * 32, count = end - begin;
         int stage = 0;
         uint32_t phase = 0;
@@ -422,53 +467,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
             const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
             const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes + kScales);
-            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane));
-            const float up = power_of_two(shift);
+            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane, [&](uint32_t r, uint32_t block) { atomicMin(&bad_value[block], tile * kQpKeys + r); }));
             if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            uint8_t* const to = v_smem + (j & 1) * 2 * kVPlane;
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) {
-                const uint32_t item = id + kId * i, octet = item % 8, word = item / 8 % 4, block = item / 32;
-                if (item >= kItems) continue;
-                uint32_t w[8], d2[4];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint32_t*>(raw + kCodes + ((octet * kBlocks + block) * 8 + k) * 16 + word * 4);
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    float d[2];
-#pragma unroll
-                    for (uint32_t e = 0; e < 2; ++e) {
-                        const uint32_t r = octet * 8 + 2 * k + e;
-                        uint32_t bits = r < slots ? __half_as_ushort(scales[r * kBlocks + block]) : 0u;
-                        if (!q4_finite(bits)) {
-                            atomicMin(&bad_value[block], tile * kQpKeys + r);
-                            bits = 0;
-                        }
-                        d[e] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
-                    }
-                    d2[k] = pack_f16(d[0], d[1]);
-                }
-#pragma unroll
-                for (uint32_t pair = 0; pair < 2; ++pair) {      // bytes 0 and 1, bytes 2 and 3 of the words
-                    uint32_t x[4];
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) x[k] = __byte_perm(w[2 * k], w[2 * k + 1], pair ? 0x7632 : 0x5410);
-#pragma unroll
-                    for (uint32_t nibble = 0; nibble < 4; ++nibble) {
-                        uint32_t upper[4], lower[4];
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const uint32_t y = nibble & 2 ? x[k] >> 8 : x[k], c = nibble & 1 ? signed_high(y) : signed_low(y);
-                            upper[k] = f16x2_mul(c, d2[k]);
-                            lower[k] = f16x2_rest(c, d2[k], upper[k]);
-                        }
-                        const uint32_t dim = block * 32 + (nibble & 1) * 16 + word * 4 + pair * 2 + (nibble >> 1);
-                        const uint32_t at = dim * 128 + ((octet ^ (dim & 7)) << 4);
-                        *reinterpret_cast<uint4*>(to + at) = make_uint4(upper[0], upper[1], upper[2], upper[3]);
-                        *reinterpret_cast<uint4*>(to + kVPlane + at) = make_uint4(lower[0], lower[1], lower[2], lower[3]);
-                    }
-                }
-            }
+            q4_unpack_tile<kBlocks, kId>(raw + kCodes, scales, slots, shift, v_smem + (j & 1) * 2 * kKPlane, id);
             if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
             async_proxy_fence();
             __syncwarp();
@@ -476,22 +477,22 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (++stage == kQpStages) { stage = 0; phase ^= 1u; }
         }
     } else if (lane == 0) {                                   // the tensor cores
-        constexpr uint32_t score_desc = umma_idesc_f16(kQpRows, kQpKeys), out_desc = umma_idesc_f16(kQpRows, kDim), kSteps = kDim / 16;
-        const uint64_t q_desc = umma_desc_k_sw128(smem_u32(q_smem)), k_desc = umma_desc_k_sw128(smem_u32(k_smem)), v_desc = umma_desc_k_sw128(smem_u32(v_smem));
-        // a descriptor's start address counts 16-byte units; 16 columns of K are two of them
+        constexpr uint32_t score_desc = umma_idesc_f16(kQpRows, kQpKeys), out_desc = umma_idesc_f16(kQpRows, kDim, true), kSteps = kDim / 16;
+        const uint64_t k_desc = umma_desc_k_sw128(smem_u32(k_smem)), v_desc = umma_desc_mn_sw128(smem_u32(v_smem), kKPlane / kHalves);
+        // a descriptor's start address counts 16-byte units: 16 dimensions are two of them, 16 slots of values 128
         auto scores = [&](uint32_t b) {
 #pragma unroll
             for (int c = 0; c < 3; ++c) {                     // lower times upper, upper times lower, upper times upper
                 const uint32_t qp = c == 0 ? 1 : 0, kp = c == 1 ? 1 : 0;
 #pragma unroll
                 for (uint32_t k = 0; k < kSteps; ++k)
-                    tc_mma_f16(tmem + (c == 2 ? kQpLead + (k / (kSteps / 2)) * kQpKeys : kQpCorrections), q_desc + ((qp * kQPlane + (k / 4) * (kQPlane / kHalves)) >> 4) + 2 * (k % 4),
-                               k_desc + (((b * 2 + kp) * kKPlane + (k / 4) * (kKPlane / kHalves)) >> 4) + 2 * (k % 4), score_desc, c == 2 ? k % (kSteps / 2) > 0 : (c | k) > 0);
+                    tc_mma_f16_ts(tmem + (c == 2 ? kQpLead + (k / (kSteps / 2)) * kQpKeys : kQpCorrections), tmem + kQpQ + qp * (kDim / 2) + 8 * k,
+                                  k_desc + (((b * 2 + kp) * kKPlane + (k / 4) * (kKPlane / kHalves)) >> 4) + 2 * (k % 4), score_desc, c == 2 ? k % (kSteps / 2) > 0 : (c | k) > 0);
             }
             tc_commit(&k_free[b]);
             tc_commit(&s_full);
         };
-        bool ok = mbar_wait(&k_full[0], 0);
+        bool ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
         if (ok) { tc_fence_after_sync(); scores(0); }
         const uint32_t count = end - begin;
         for (uint32_t j = 0; ok && j < count; ++j) {
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 const uint32_t pp = c == 0 ? 1 : 0, vp = c == 1 ? 1 : 0;
 #pragma unroll
                 for (uint32_t k = 0; k < kQpKeys / 16; ++k)
-                    tc_mma_f16_ts(tmem + kQpOut, tmem + kQpP + 32 * pp + 8 * k, v_desc + (((j & 1) * 2 + vp) * kVPlane >> 4) + 2 * k, out_desc, (c | k) > 0);
+                    tc_mma_f16_ts(tmem + kQpOut, tmem + kQpP + 32 * pp + 8 * k, v_desc + (((j & 1) * 2 + vp) * kKPlane >> 4) + 128 * k, out_desc, (c | k) > 0);
             }
             tc_commit(&v_free[j & 1]);
             tc_commit(&o_full);
