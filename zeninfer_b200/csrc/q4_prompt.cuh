@@ -11,8 +11,8 @@
 //                TMEM, from where the tensor cores read them (as they do the queries); then out = out * factor + O' of the tile before, in fp32 registers
 //   3 + 4        unpack keys and values (bulk copies bring the tiles into a ring, two ahead) into the operands' 128-byte swizzle, two buffers each, a slot's block a
 //                thread: to the tensor cores keys are a matrix with the summed index in its rows, values one with it in its columns, so neither is transposed
-//   1 issues     S = Q K^T into three accumulators (the corrections, and the leading products of each half of the head, for the tensor cores cut a sum at
-//                every 16 columns), O' = P V corrections first
+//   1 issues     S = Q K^T into three accumulators in turn (a product waits for the sum that it adds to, and the tensor cores cut a sum at every 16 columns), O' = P V;
+//                corrections first
 // The scores of tile j + 1 are formed while tile j is exponentiated.
 //
 // A scale that is not finite counts as zero in the operands and is remembered by its slot: the rows that see it are NaN (all of them for a key's, the
@@ -29,8 +29,8 @@ template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;   
 constexpr int kQpStages = 3;                 // tiles as they are in the cache, ahead of the warps that unpack them
 template <int kBlocks> constexpr uint32_t kQpRaw = kQpKeys * kBlocks * 36;
 template <int kBlocks> constexpr uint32_t q4_prompt_smem() { return 1024 + 2 * kQpQPlane<kBlocks> + 8 * kQpKPlane<kBlocks> + kQpStages * kQpRaw<kBlocks>; }
-// TMEM columns: leading scores of the head's halves, corrections; the weights' parts; O'; the queries' parts
-constexpr uint32_t kQpLead = 0, kQpCorrections = 128, kQpP = 192, kQpOut = 256, kQpQ = 384, kQpColumns = 512;
+// TMEM columns: three shares of the scores; the weights' parts; O'; the queries' parts
+constexpr uint32_t kQpScores = 0, kQpShares = 3, kQpP = 192, kQpOut = 256, kQpQ = 384, kQpColumns = 512;
 
 // Instruction descriptor, kind::f16: f16 x f16 -> fp32, dense, A K-major, B K-major or (across) MN-major.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t m, uint32_t n, bool across = false) { return (1u << 4) | (across ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((m >> 4) << 24); }
@@ -54,18 +54,21 @@ __device__ __forceinline__ uint32_t f16x2_rest(uint32_t a, uint32_t b, uint32_t 
 __device__ __forceinline__ int q4_shift(uint32_t top) { return 23 - static_cast<int>(top >> 10); }
 __device__ __forceinline__ bool q4_finite(uint32_t half_bits) { return (half_bits & 0x7c00u) != 0x7c00u; }
 
-// The largest magnitude among the finite scales of the first `slots` of a tile's 64 slots, as f16 bits: every lane of a warp.  bad(slot, block) is called for the others.
-template <int kBlocks, typename Bad>
+// The largest magnitude among the finite scales of the first `slots` of kSlots slots, as f16 bits: every lane of a warp.  bad(slot, block) is called for the others.
+template <int kBlocks, uint32_t kSlots, typename Bad>
 __device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slots, uint32_t lane, Bad bad) {
-    uint32_t top = 0, w[4] = {};
+    uint32_t top = 0;
     bool odd = false;
-    if (lane < kQpKeys * kBlocks / 8) {                       // eight scales a lane: 8 / kBlocks slots
-        const uint4 eight = reinterpret_cast<const uint4*>(scales)[lane];
-        w[0] = eight.x; w[1] = eight.y; w[2] = eight.z; w[3] = eight.w;
+#pragma unroll
+    for (uint32_t at = 0; at < kSlots * kBlocks / 8; at += 32) {      // eight scales a lane: 8 / kBlocks slots
+        const uint32_t first = (at + lane) * 8 / kBlocks;
+        if (first >= min(slots, kSlots)) continue;
+        const uint4 eight = reinterpret_cast<const uint4*>(scales)[at + lane];
+        const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0x7fffu;
-            if (lane * 8 / kBlocks + j / kBlocks >= slots) continue;
+            if (first + j / kBlocks >= slots) continue;
             if (q4_finite(bits)) top = max(top, bits);
             else odd = true;
         }
@@ -142,19 +145,23 @@ __device__ __forceinline__ void q4_split_codes(uint32_t w, uint32_t d2, uint4& u
     lower = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// A tile's codes (64 slots, as the cache holds them) times their scales, 2^shift as large, into both planes: rows of 64 dimensions a slot.  Scales that are not finite, and
-// those of slots that are not the rows' to see, count as zero.  kThreads threads, the id-th of them here.
-template <int kBlocks, uint32_t kThreads>
+// The codes of kSlots slots, as the cache holds them, times their scales, 2^shift as large, into both planes: rows of 64 dimensions a slot.  Scales that are not finite
+// count as zero, and so do the slots from `slots` on, of which nothing is read.  kThreads threads, the id-th of them here.
+template <int kBlocks, uint32_t kSlots, uint32_t kThreads>
 __device__ __forceinline__ void q4_unpack_tile(const uint8_t* codes, const __half* scales, uint32_t slots, int shift, uint8_t* to, uint32_t id) {
-    constexpr uint32_t kItems = kQpKeys * kBlocks, kEach = (kItems + kThreads - 1) / kThreads, kPlane = kQpKPlane<kBlocks>, kHalves = kBlocks / 2;
+    constexpr uint32_t kItems = kSlots * kBlocks, kEach = (kItems + kThreads - 1) / kThreads, kPlane = kSlots * kBlocks * 64, kHalves = kBlocks / 2;
     const float up = power_of_two(shift);
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t item = id + kThreads * i, r = item % kQpKeys, block = item / kQpKeys;
+        const uint32_t item = id + kThreads * i, r = item % kSlots, block = item / kSlots;
         if (kItems % kThreads && item >= kItems) break;       // a whole warp
-        const uint4 four = *reinterpret_cast<const uint4*>(codes + (((r >> 3) * kBlocks + block) * 8 + (r & 7u)) * 16);
-        uint32_t bits = __half_as_ushort(scales[r * kBlocks + block]);
-        if (!q4_finite(bits) || r >= slots) bits = 0;
+        uint4 four = make_uint4(0, 0, 0, 0);
+        uint32_t bits = 0;
+        if (r < slots) {
+            four = *reinterpret_cast<const uint4*>(codes + (((r >> 3) * kBlocks + block) * 8 + (r & 7u)) * 16);
+            bits = __half_as_ushort(scales[r * kBlocks + block]);
+        }
+        if (!q4_finite(bits)) bits = 0;
         const float d = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
         const uint32_t d2 = pack_f16(d, d), w[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
@@ -327,7 +334,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 for (int c = 0; c < kMine / 8; ++c) {
                     uint32_t part[3][8];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) tmem_ld_32x8(tmem + (i < 2 ? kQpLead + i * kQpKeys : kQpCorrections) + half * kMine + 8 * c + lane_base, part[i]);
+                    for (int i = 0; i < 3; ++i) tmem_ld_32x8(tmem + kQpScores + i * kQpKeys + half * kMine + 8 * c + lane_base, part[i]);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[8 * c + i] = (__uint_as_float(part[0][i]) + __uint_as_float(part[1][i])) + __uint_as_float(part[2][i]);
@@ -436,9 +443,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
             const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
             const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes);
-            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane, [&](uint32_t r, uint32_t) { atomicMin(&bad_key, tile * kQpKeys + r); }));
+            const int shift = q4_shift(q4_largest_scale<kBlocks, kQpKeys>(scales, slots, lane, [&](uint32_t r, uint32_t) { atomicMin(&bad_key, tile * kQpKeys + r); }));
             if (j > 1 && !warp_waited(&k_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            q4_unpack_tile<kBlocks, kId>(raw, scales, slots, shift, k_smem + (j & 1) * 2 * kKPlane, id);
+            q4_unpack_tile<kBlocks, kQpKeys, kId>(raw, scales, slots, shift, k_smem + (j & 1) * 2 * kKPlane, id);
             if (id == 0) k_unit[j & 3] = power_of_two(-shift);
             async_proxy_fence();
             __syncwarp();
@@ -467,9 +474,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
             const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
             const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes + kScales);
-            const int shift = q4_shift(q4_largest_scale<kBlocks>(scales, slots, lane, [&](uint32_t r, uint32_t block) { atomicMin(&bad_value[block], tile * kQpKeys + r); }));
+            const int shift = q4_shift(q4_largest_scale<kBlocks, kQpKeys>(scales, slots, lane, [&](uint32_t r, uint32_t block) { atomicMin(&bad_value[block], tile * kQpKeys + r); }));
             if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            q4_unpack_tile<kBlocks, kId>(raw + kCodes, scales, slots, shift, v_smem + (j & 1) * 2 * kKPlane, id);
+            q4_unpack_tile<kBlocks, kQpKeys, kId>(raw + kCodes, scales, slots, shift, v_smem + (j & 1) * 2 * kKPlane, id);
             if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
             async_proxy_fence();
             __syncwarp();
@@ -486,8 +493,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 const uint32_t qp = c == 0 ? 1 : 0, kp = c == 1 ? 1 : 0;
 #pragma unroll
                 for (uint32_t k = 0; k < kSteps; ++k)
-                    tc_mma_f16_ts(tmem + (c == 2 ? kQpLead + (k / (kSteps / 2)) * kQpKeys : kQpCorrections), tmem + kQpQ + qp * (kDim / 2) + 8 * k,
-                                  k_desc + (((b * 2 + kp) * kKPlane + (k / 4) * (kKPlane / kHalves)) >> 4) + 2 * (k % 4), score_desc, c == 2 ? k % (kSteps / 2) > 0 : (c | k) > 0);
+                    tc_mma_f16_ts(tmem + kQpScores + k % kQpShares * kQpKeys, tmem + kQpQ + qp * (kDim / 2) + 8 * k,
+                                  k_desc + (((b * 2 + kp) * kKPlane + (k / 4) * (kKPlane / kHalves)) >> 4) + 2 * (k % 4), score_desc, c > 0 || k >= kQpShares);
             }
             tc_commit(&k_free[b]);
             tc_commit(&s_full);

@@ -12,6 +12,7 @@
 #include "q4_attention.cuh"
 #include "q4_cache.cuh"
 #include "q4_prompt.cuh"
+#include "q4_received.cuh"
 #include "q4_step.cuh"
 #include "verify_drafts.cuh"
 
@@ -71,6 +72,7 @@ zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
 }
 
 constexpr size_t kSms = 148, kWaveCtas = 2 * kSms;
+constexpr size_t kReceivedSingle = kSms;   // 128 slots a CTA of q4_received.cuh up to so many
 constexpr size_t kPromptRows = 8;          // above: q4_prompt.cuh, for the heads it takes
 
 // How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
@@ -86,18 +88,23 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     const size_t kv_heads = a->cache.kv_heads, rows = tokens * (a->heads / kv_heads), blocks = a->cache.head_dim / zk::kQ4Block, tiles = a->cache.slots / zk::kQ4Tile;
     if (tokens * a->heads > 0x1fffffffu / blocks) return n;      // what a launch counts in 32 bits
     n.columns = rows <= 4 ? zk::kQ4Digits : rows <= 8 || blocks > 4 ? zk::kQ4Rows8 : zk::kQ4Rows16;
-    if ((blocks == 2 || blocks == 4) && rows > kPromptRows && !(a->weight_out && rows > zk::kQ4KeptRows)) {
+    if ((blocks == 2 || blocks == 4) && rows > kPromptRows) {
         const size_t row_tiles = (rows + zk::kQpRows - 1) / zk::kQpRows, key_tiles = (a->cache.slots + zk::kQpKeys - 1) / zk::kQpKeys;
         if (row_tiles > 65535) return n;
         n.columns = zk::kQ4Prompt;
         n.rows = u32(rows); n.cta_rows = zk::kQpRows; n.row_ctas = u32(row_tiles); n.padded = u32(row_tiles * zk::kQpRows); n.key_warps = 1; n.run_tile = zk::kQpKeys;
         n.splits = u32(std::max<size_t>(1, std::min(kSms / (row_tiles * kv_heads), key_tiles)));
-        n.keep_scores = a->weight_out;
+        n.keep_scores = a->weight_out && rows <= zk::kQ4KeptRows;
         size_t at = 0;
         auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
         if (n.splits > 1) n.part_out = take(kv_heads * n.splits * rows * a->cache.head_dim * sizeof(float));
         if (n.splits > 1 || n.keep_scores) n.part_stats = take(kv_heads * n.splits * rows * 2 * sizeof(float));
         if (n.keep_scores) n.scores = take(kv_heads * rows * a->cache.slots * sizeof(float));
+        else if (a->weight_out) {
+            n.stats = take(kv_heads * rows * sizeof(float));
+            n.queries = take(kv_heads * row_tiles * 2 * zk::kQpRows * a->cache.head_dim * sizeof(uint16_t));
+            n.factors = take(kv_heads * n.padded * sizeof(float));
+        }
         n.bytes = std::max<size_t>(at, 16);
         return n;
     }
@@ -200,6 +207,7 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     else if (a->weight_out) p.stats = part(plan.stats);
     const bool prompt = plan.columns == zk::kQ4Prompt;
     if (prompt) {
+        if (p.stats) { p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors); }
         const size_t items = tokens * cache.kv_heads * 2 * cache.blocks, a_cta = zk::kQ4AppendWarps * zk::kQ4AppendEach;
         const cudaError_t r = by_prompt_blocks(cache.blocks, [&](auto blocks) {
             constexpr int kBlocks = decltype(blocks)::value;
@@ -238,6 +246,13 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
             return 0;
     }
     if (!a->weight_out || plan.keep_scores) return 1;
+    if (prompt) {
+        const uint32_t tiles = (cache.slots + zk::kQrSlots - 1) / zk::kQrSlots, sets = size_t(tiles) * cache.kv_heads > kReceivedSingle ? zk::kQrSets : 1;
+        return e.leave(by_prompt_blocks(cache.blocks, [&](auto blocks) {
+            constexpr int kBlocks = decltype(blocks)::value;
+            return launch(e, zk::q4_received_kernel<kBlocks>, dim3((tiles + sets - 1) / sets, cache.kv_heads), dim3(zk::kQrThreads), zk::q4_received_smem<kBlocks>(sets), 0, p, sets);
+        }), "dev_q4_attention: weights");
+    }
     return e.leave(by_blocks(cache.blocks, [&](auto blocks) {
         constexpr int kBlocks = decltype(blocks)::value;
         return launch(e, zk::q4_received_again_kernel<kBlocks>, dim3(zk::kReceivedCtas, (cache.slots + zk::kReceivedSlots - 1) / zk::kReceivedSlots, cache.kv_heads), dim3(zk::kReceivedWarps * 32),
