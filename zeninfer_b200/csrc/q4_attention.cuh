@@ -183,8 +183,7 @@ __host__ __device__ constexpr uint32_t q4_attend_smem(uint32_t row_warps) {
 }
 
 // A warp turns one row of queries into the products' second operand.  A lane's words of a block are its dimensions 4t, 4t+2 | 16+4t, 16+4t+2 (low and high nibbles of
-// bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kDigits: columns 2r and 2r + 1 are row r's digits, those beside high
-// nibbles a 16th as large, for the codes are then taken as they stand (the subnormals code * 2^-24 and code * 2^-20); else
+// bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kDigits: columns 2r and 2r + 1 are row r's digits; else
 // a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14).  Returns the row's factor, which makes scores
 // (in units of log 2) of the products.
 template <int kBlocks, bool kDigits>
@@ -196,12 +195,11 @@ __device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to
     const int e = max(static_cast<int>(size >> 23) - 127, -114);
     const float up = scale < 0.0f ? -power_of_two(13 - e) : power_of_two(13 - e);
     const uint32_t part = lane >> 4, t = (lane & 15u) >> 2, step = lane & 1u, half = (lane >> 1) & 1u, word = 2 * step + part;
-    const float unit = kDigits && part ? 0.0625f : 1.0f;
     __half* const halves = reinterpret_cast<__half*>(to);
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
         const float y = x[g] * up, upper = upper_digit(y);
-        const __half first = __float2half_rn(upper * unit), other = __float2half_rn((y - upper) * unit);
+        const __half first = __float2half_rn(upper), other = __float2half_rn(y - upper);
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
             const uint32_t column = kDigits ? 2 * row + d : row & 7u;
@@ -209,7 +207,7 @@ __device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to
             halves[(at * 4 + word) * 2 + half] = d ? other : first;
         }
     }
-    const int units = (kDigits ? 24 : 0) + e - 13;                // in two steps, for it may be beyond what one power of two can be
+    const int units = e - 13;                // in two steps, for it may be beyond what one power of two can be
     return fabsf(scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2);
 }
 

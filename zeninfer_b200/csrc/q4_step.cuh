@@ -114,14 +114,8 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
     const float factor = row_factor[t];
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     uint4 own_query[kBlocks];
-    float start[kBlocks][4];               // -8 sum q of the lane's two columns: a product with sixteen slots whose codes are all -8
-    const uint32_t eights[4] = {0x80088008u, 0x80088008u, 0x80808080u, 0x80808080u};
 #pragma unroll
-    for (int g = 0; g < kBlocks; ++g) {
-        own_query[g] = queries[g * 32 + lane];
-        mma_f16(start[g], eights, own_query[g].x, own_query[g].y, zero);
-        mma_f16(start[g], eights, own_query[g].z, own_query[g].w, start[g]);
-    }
+    for (int g = 0; g < kBlocks; ++g) own_query[g] = queries[g * 32 + lane];
     float acc[2 * kBlocks][4] = {};
     float m = -INFINITY, l = 0.0f;
     // Weights times 2^(kFull - unit) times their slot's d are below 2^14: d is below 2^unit and a weight at most 2^kSlack.
@@ -148,10 +142,11 @@ __global__ void __launch_bounds__(kQ4StepWarps * 32, kBlocks > 4 ? 1 : 2) q4_ste
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t u = w[g][2 * half], v = w[g][2 * half + 1], x = u >> 8, y = v >> 8;
-                    const uint32_t even[4] = {u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u};
-                    const uint32_t odd[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+                    // with their offset taken off: sums of codes as they stand are far from zero, and what the products cut off was a score's last 4 bits
+                    const uint32_t even[4] = {signed_low(u), signed_low(v), signed_high(u), signed_high(v)};
+                    const uint32_t odd[4] = {signed_low(x), signed_low(y), signed_high(x), signed_high(y)};
                     float c[4];
-                    mma_f16(c, even, own_query[g].x, own_query[g].y, start[g]);
+                    mma_f16(c, even, own_query[g].x, own_query[g].y, zero);
                     mma_f16(c, odd, own_query[g].z, own_query[g].w, c);
                     s[2 * half] = fmaf(d.of(2 * half, g), c[0] + c[1], s[2 * half]);
                     s[2 * half + 1] = fmaf(d.of(2 * half + 1, g), c[2] + c[3], s[2 * half + 1]);
