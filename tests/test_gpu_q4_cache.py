@@ -119,6 +119,7 @@ class Setup:
 SHAPES = [(1, 0, 4, 2, 64), (1, 1, 1, 1, 32), (1, 15, 4, 4, 128), (1, 16, 4, 1, 128), (1, 31, 8, 2, 96), (1, 63, 32, 8, 128), (1, 1000, 32, 8, 128), (1, 2047, 7, 1, 64), (1, 700, 28, 4, 128),
           (1, 333, 16, 2, 256), (1, 257, 5, 5, 160), (1, 129, 24, 2, 192), (1, 97, 3, 1, 224), (1, 9001, 4, 2, 128),
           (2, 0, 4, 2, 64), (2, 5, 8, 1, 128), (3, 30, 4, 4, 32), (5, 4003, 32, 8, 128), (7, 60, 12, 4, 96), (8, 31, 16, 4, 256), (9, 33, 7, 1, 64), (16, 100, 32, 8, 128), (17, 16, 6, 2, 64),
+          (40, 4001, 16, 8, 128), (35, 3333, 34, 34, 64), (130, 2500, 10, 10, 128),
           (33, 0, 4, 2, 64), (64, 64, 8, 2, 128), (77, 200, 16, 16, 64), (128, 0, 32, 8, 128), (129, 1, 12, 4, 96), (200, 55, 8, 1, 256), (512, 300, 8, 2, 128)]
 
 

@@ -140,3 +140,40 @@ def test_the_drawn_tokens_are_distributed_as_the_model_says():
     for t, uu in zip(drafts, u):
         seen[q4.verify(logits, [t], q, uu, 1.0, 0, 1.0)[0][0]] += 1
     assert np.abs(seen / n - p).max() < 5 * np.sqrt(0.25 / n)
+
+
+# ---- the decoder's side that needs no device ----
+def test_drafts_are_looked_up_at_the_last_place_that_reads_alike():
+    from zeninfer_b200.llama import LlamaDecoder
+    look = LlamaDecoder.look_up
+    assert look(LlamaDecoder, [1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
+    assert look(LlamaDecoder, [5, 2, 3, 7, 1, 2, 3, 8, 4, 2, 3], 3) == [8, 4, 2]      # two tokens alike, and the later place
+    assert look(LlamaDecoder, [4, 4], 5) == [4] and look(LlamaDecoder, [1, 2, 3], 4) == [] and look(LlamaDecoder, [1], 4) == []
+
+
+@pytest.mark.parametrize("argv", ["--kv-slots 64", "--kv-keep 8", "--kv q5", "--draft 65", "--draft -1"])
+def test_the_command_refuses(argv, capsys):
+    from zeninfer_b200.__main__ import main
+    with pytest.raises(SystemExit) as e:
+        main(["generate", "--model", "x", "--prompt-ids", "1"] + argv.split())
+    assert e.value.code == 2
+
+
+def test_options_of_other_models_are_refused(tmp_path):
+    import json
+    from zeninfer_b200 import registry
+    (tmp_path / "config.json").write_text(json.dumps({"architecture": "Kipirax"}))
+    with pytest.raises(ValueError, match="kv"):
+        registry.load_model(None, str(tmp_path), kv="q4")
+
+
+def test_the_plain_model_with_a_cache_reads_blocks_as_it_reads_tokens():
+    from q4_llama import PlainLlama
+    from zeninfer_b200.llama import LlamaConfig
+    cfg = LlamaConfig(embedding=64, layers=2, heads=2, kv_heads=1, head_dim=32, ffn=64, vocab=50, rope_base=10000.0, context=32)
+    a, b = PlainLlama(cfg, 1, 0.1, 32), PlainLlama(cfg, 1, 0.1, 32)
+    tokens = [3, 1, 4, 1, 5, 9, 2, 6]
+    whole = a.block(tokens, 0)
+    rows = [b.block([t], i)[0] for i, t in enumerate(tokens)]
+    assert np.abs(whole - rows).max() <= 1e-9 * np.abs(whole).max()
+    assert np.abs(b.block(tokens[5:], 5) - whole[5:]).max() <= 1e-9 * np.abs(whole).max()       # taken back and read again

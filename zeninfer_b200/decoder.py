@@ -12,7 +12,7 @@ from .backend import Backend
 
 
 class SequenceState:
-    """The device buffers that carry a sequence from step to step, fp32.  A buffer indexed by position (a KV cache) is simply
+    """The device buffers that carry a sequence from step to step, fp32 unless they are given a type.  A buffer indexed by position (a KV cache) is simply
     overwritten by the next sequence, because nothing reads past the positions written so far; a recurrent one is added with
     start_zero and cleared when a sequence begins."""
 
@@ -21,10 +21,10 @@ class SequenceState:
         self.buffers: dict[str, "torch.Tensor"] = {}
         self._zero: list["torch.Tensor"] = []
 
-    def add(self, name: str, shape: tuple[int, ...], start_zero: bool = False):
+    def add(self, name: str, shape: tuple[int, ...], start_zero: bool = False, dtype=None):
         if name in self.buffers:
             raise ValueError(f"state buffer {name!r} exists")
-        t = self.buffers[name] = self.torch.zeros(shape, dtype=self.torch.float32, device=self.dev)
+        t = self.buffers[name] = self.torch.zeros(shape, dtype=dtype or self.torch.float32, device=self.dev)
         if start_zero:
             self._zero.append(t)
         return t

@@ -32,7 +32,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import blocks
-from .backend import ACT_FP32, ACT_INT8, Backend
+from .backend import ACT_FP32, ACT_INT8, Backend, DraftCheck, Q4Attention, Q4Cache
 from .decoder import Decoder
 
 
@@ -109,7 +109,8 @@ class LlamaDecoder(Decoder):
 
     def __init__(self, backend: Backend, cfg: LlamaConfig, tensors, act_mode: int = ACT_INT8, max_positions: int | None = None, device=None,
                  fused: bool | str = "nrp", rank: int = 0, world: int = 1, group=None, gather: str = "peer", cut: str = "rows+cols",
-                 prompt_act_mode: int | None = None):
+                 prompt_act_mode: int | None = None, kv: str = "f32", kv_slots: int | None = None, kv_keep: int | None = None, kv_keep_first: int = 4,
+                 kv_keep_last: int | None = None):
         """fused: which of the layer's small operators are folded into the projection launches, as a string of letters:
         'n' RMSNorm into the q|k|v, gate|up and lm_head prologues, 's' SwiGLU into the down projection's prologue,
         'r' the residual adds into the o and down projections' stores, 'p' SwiGLU into the gate|up launch's store (the two
@@ -126,7 +127,11 @@ class LlamaDecoder(Decoder):
         The reference with ZEN_CPU_Q8_ACT=1 is such a mix: its prompt block goes through the fp32-activation GEMM
         (src/quant.cpp:1667-1680) and only single-token products quantise their input to int8 (:1088-1123); ACT_FP32 here
         with act_mode=ACT_INT8 reproduces it (prompt blocks go through the two-digit tensor-core product, leftover prompt
-        tokens one by one outside the step graphs)."""
+        tokens one by one outside the step graphs).
+        kv: "f32", or "q4": keys and values are held in 4 bits (zen_cuda_dev_q4_attention), 0.56 bytes a value instead of 4.
+        kv_slots (q4): how many tokens a layer holds, rounded up to a multiple of 32; with fewer than max_positions, the slots add up the
+        attention they receive, and when one more block does not fit, every kv head of every layer drops what received least, down to kv_keep
+        (default: three quarters), its first kv_keep_first and last kv_keep_last (default: a quarter of what is kept, at most 64) slots staying."""
         import torch
         self.cfg, self.act_mode = cfg, act_mode
         self.prompt_act_mode = prompt_act_mode if prompt_act_mode not in (None, act_mode) else None
@@ -179,8 +184,14 @@ class LlamaDecoder(Decoder):
         self.x, self.xn, self.tmp = torch.zeros(E, **f32), torch.zeros(E, **f32), torch.zeros(E, **f32)
         self.q, self.k, self.v, self.att = torch.zeros(QW // w, **f32), torch.zeros(KW // w, **f32), torch.zeros(KW // w, **f32), torch.zeros(QW, **f32)
         self.gate, self.up, self.hid = torch.zeros(F // w, **f32), torch.zeros(F // w, **f32), torch.zeros(F, **f32)
-        self.k_cache = self.sequence.add("k", (cfg.layers, self.max_positions, KW // w))
-        self.v_cache = self.sequence.add("v", (cfg.layers, self.max_positions, KW // w))
+        self.q4 = kv == "q4"
+        if kv not in ("f32", "q4"):
+            raise ValueError(f"kv = {kv!r}")
+        if not self.q4:
+            if kv_slots is not None or kv_keep is not None:
+                raise ValueError('kv_slots and kv_keep go with kv="q4"')
+            self.k_cache = self.sequence.add("k", (cfg.layers, self.max_positions, KW // w))
+            self.v_cache = self.sequence.add("v", (cfg.layers, self.max_positions, KW // w))
         mine = lambda t: t[self.rank * (t.numel() // w):(self.rank + 1) * (t.numel() // w)]     # the piece this rank's rows produce
         self.x_mine, self.att_mine, self.hid_mine, self.logits_mine = mine(self.x), mine(self.att), mine(self.hid), mine(self.logits)
         if self.gather_kind == "peer":
@@ -189,6 +200,86 @@ class LlamaDecoder(Decoder):
             self.peer = shard.PeerGather(backend, w, self.rank, (slot + 3) & ~3, group=group)     # collective: handles travel through the group
         cos, sin = rope_tables(cfg, self.max_positions)
         self.cos, self.sin = torch.from_numpy(cos).to(self.dev), torch.from_numpy(sin).to(self.dev)
+        if self.q4:
+            self._init_q4(kv_slots, kv_keep, kv_keep_first, kv_keep_last)
+
+    # ---- the cache in 4 bits ----
+    def _init_q4(self, slots: int | None, keep: int | None, keep_first: int, keep_last: int | None) -> None:
+        torch, be, cfg, w = self.torch, self.be, self.cfg, self.world
+        up = lambda n: (n + 31) // 32 * 32
+        self.slots = up(slots or self.max_positions)
+        if self.slots >= self.max_positions:
+            if keep is not None:
+                raise ValueError("kv_keep: the cache holds every position, nothing is dropped")
+            self.keep = None
+        else:
+            self.keep = keep if keep is not None else self.slots * 3 // 4
+            self.keep_first, self.keep_last = keep_first, min(64, self.keep // 4) if keep_last is None else keep_last
+            if self.keep_first < 0 or self.keep_last < 0 or self.keep_first + self.keep_last > self.keep or self.slots - self.keep < self.PREFILL_MIN or self.keep < 1:
+                raise ValueError(f"{self.slots} slots, keep {self.keep}, of these the first {self.keep_first} and the last {self.keep_last}: does not work out")
+            self.PREFILL_CHUNK = min(self.PREFILL_CHUNK, self.slots - self.keep)      # a block fits once the others are dropped
+        kv, d = cfg.kv_heads // w, cfg.head_dim
+        codes = lambda n: self.sequence.add(n, (cfg.layers,) + Q4Cache.codes_shape(kv, d, self.slots), dtype=torch.uint8)
+        scales = lambda n: self.sequence.add(n, (cfg.layers,) + Q4Cache.scales_shape(kv, d, self.slots), dtype=torch.float16)
+        kc, ks, vc, vs = codes("k_codes"), scales("k_scales"), codes("v_codes"), scales("v_scales")
+        self.weight = self.sequence.add("weight", (cfg.layers, kv, self.slots)) if self.keep is not None else None
+        self.filled = torch.zeros(1, dtype=torch.int32, device=self.dev)      # slots in use; self.pos goes on when some are dropped
+        self.held = self.place = self.floor = 0                               # the same, the position, and the slots the last drop left, on the host
+        self.q4_calls = []
+        for layer in range(cfg.layers):
+            a = Q4Attention(Q4Cache.of(kc[layer], ks[layer], vc[layer], vs[layer], kv_heads=kv, head_dim=d, slots=self.slots), cfg.heads // w, 0.0, self.cos.data_ptr(),
+                            self.sin.data_ptr(), d // 2, self.max_positions, 1, self.pos.data_ptr(), self.filled.data_ptr(), 0, 0)
+            if self.weight is not None:
+                a.weight_in = a.weight_out = self.weight[layer].data_ptr()
+            self.q4_calls.append(a)
+        a = self.q4_calls[0]
+        room = max(be.q4_attention_workspace_bytes(a, t) for t in range(1, min(self.PREFILL_CHUNK, self.slots) + 1))
+        room = max(room, be.q4_cache_evict_workspace_bytes(a.cache))
+        if not room:
+            raise ValueError(f'kv="q4": heads of {d} values')
+        self.q4_room = torch.zeros(room, dtype=torch.uint8, device=self.dev)      # the layers' launches follow one another
+        for a in self.q4_calls:
+            a.workspace, a.workspace_bytes = self.q4_room.data_ptr(), room
+
+    def _make_room(self, tokens: int) -> None:
+        """Before `tokens` more go in: drops slots where they would not fit."""
+        if not self.q4:
+            return
+        if self.held + tokens > self.slots:
+            if self.keep is None:
+                raise ValueError("the sequence does not fit the configured positions")
+            for layer, a in enumerate(self.q4_calls):
+                weight = self.weight[layer].data_ptr()
+                self.be.dev_q4_cache_evict(a.cache, weight, self.filled.data_ptr(), a.cache, weight, self.keep, self.keep_first, self.keep_last, a.workspace,
+                                           a.workspace_bytes, self.stream.cuda_stream)
+            self.held = self.floor = min(self.held, self.keep)
+            with self.torch.cuda.stream(self.stream):
+                self.filled.fill_(self.held)
+        self.held += tokens
+        self.place += tokens
+
+    def _rewind(self, position: int) -> None:
+        """The next token's position is `position`: the tokens behind it are taken back."""
+        if not self.q4 or position == self.place:
+            return
+        back = self.place - position
+        if back < 0 or self.held - back < self.floor:
+            raise ValueError(f"position {position}: the cache holds positions up to {self.place}, of which the last {self.held - self.floor} can be taken back")
+        self.held -= back
+        self.place = position
+        with self.torch.cuda.stream(self.stream):
+            self.filled.fill_(self.held)
+
+    def reset(self) -> None:
+        super().reset()
+        if self.q4:
+            with self.torch.cuda.stream(self.stream):
+                self.filled.zero_()
+            self.held = self.place = self.floor = 0
+
+    def step(self, want_token: bool) -> None:
+        self._make_room(1)
+        super().step(want_token)
 
     @classmethod
     def from_gguf(cls, backend: Backend, path: str, **kwargs) -> "LlamaDecoder":
@@ -236,9 +327,12 @@ class LlamaDecoder(Decoder):
             qkv = [self.h[p + "attn_q.weight"], self.h[p + "attn_k.weight"], self.h[p + "attn_v.weight"]]
             self._gemv(qkv, [P(self.q), P(self.k), P(self.v)], P(self.x) if fn else P(self.xn),
                        norm=P(self.norm[p + "attn_norm.weight"]) if fn else None, warm=self.h[p + "attn_output.weight"])
-            be.dev_attention_block(P(self.q), P(self.k), P(self.v), P(self.cos), P(self.sin), cfg.head_dim // 2, P(self.pos), P(self.k_cache[layer]),
-                                   P(self.v_cache[layer]), P(self.att_mine), cfg.heads // self.world, cfg.kv_heads // self.world, cfg.head_dim,
-                                   self.max_positions, 0.0, 0, st)
+            if self.q4:
+                be.dev_q4_attention(self.q4_calls[layer], P(self.q), P(self.k), P(self.v), 1, P(self.att_mine), st)
+            else:
+                be.dev_attention_block(P(self.q), P(self.k), P(self.v), P(self.cos), P(self.sin), cfg.head_dim // 2, P(self.pos), P(self.k_cache[layer]),
+                                       P(self.v_cache[layer]), P(self.att_mine), cfg.heads // self.world, cfg.kv_heads // self.world, cfg.head_dim,
+                                       self.max_positions, 0.0, 0, st)
             # attention output projection and its residual add (x += o(att))
             if self.col_cut:      # this rank's heads times their columns of o: a partial product of every output, summed over the ranks into x
                 self._gemv([self.h[p + "attn_output.weight"]], [P(self.tmp)], P(self.att_mine), warm=self.h[p + "ffn_gate.weight"])
@@ -272,6 +366,8 @@ class LlamaDecoder(Decoder):
             elif not fr:
                 be.dev_rms_norm(P(self.x), P(self.tmp), None, None, E, 1, eps, st)
         be.dev_advance_position(P(self.pos), 1, st)
+        if self.q4:
+            be.dev_advance_position(P(self.filled), 1, st)
 
     def _enqueue_head(self) -> None:
         fn = "n" in self.fuse
@@ -317,6 +413,7 @@ class LlamaDecoder(Decoder):
         if not self.can_prefill_blocks():
             raise ValueError("the block prefill needs one GPU, or the column cut with an NCCL group; this decoder takes its prompt token by token")
         be, cfg, st, w = self.be, self.cfg, self.stream.cuda_stream, self.world
+        self._make_room(count)
         b = self._prefill_buffers()
         P = lambda t: t.data_ptr()
         T, E, eps = count, cfg.embedding, cfg.rms_eps
@@ -332,10 +429,13 @@ class LlamaDecoder(Decoder):
         for layer in range(cfg.layers):
             p = f"blk.{layer}."
             gemm([self.h[p + "attn_q.weight"], self.h[p + "attn_k.weight"], self.h[p + "attn_v.weight"]], [b["q"], b["k"], b["v"]], b["xn"])
-            be.dev_rope_kv_append_rows(P(b["q"]), P(b["k"]), P(b["v"]), T, P(self.cos), P(self.sin), P(self.pos), cfg.heads // w, cfg.kv_heads // w, cfg.head_dim,
-                                       cfg.head_dim // 2, True, P(self.k_cache[layer]), P(self.v_cache[layer]), self.max_positions, st)
-            be.dev_attention_prefill(P(b["q"]), P(self.k_cache[layer]), P(self.v_cache[layer]), P(self.pos), P(b["att"]), T, cfg.heads // w, cfg.kv_heads // w,
-                                     cfg.head_dim, self.max_positions, 0.0, 0, st)
+            if self.q4:
+                be.dev_q4_attention(self.q4_calls[layer], P(b["q"]), P(b["k"]), P(b["v"]), T, P(b["att"]), st)
+            else:
+                be.dev_rope_kv_append_rows(P(b["q"]), P(b["k"]), P(b["v"]), T, P(self.cos), P(self.sin), P(self.pos), cfg.heads // w, cfg.kv_heads // w, cfg.head_dim,
+                                           cfg.head_dim // 2, True, P(self.k_cache[layer]), P(self.v_cache[layer]), self.max_positions, st)
+                be.dev_attention_prefill(P(b["q"]), P(self.k_cache[layer]), P(self.v_cache[layer]), P(self.pos), P(b["att"]), T, cfg.heads // w, cfg.kv_heads // w,
+                                         cfg.head_dim, self.max_positions, 0.0, 0, st)
             gemm([self.h[p + "attn_output.weight"]], [b["tmp"]], b["att"])
             reduce_partials()
             be.dev_rms_norm(P(b["x"]), P(b["tmp"]), P(self.norm[p + "ffn_norm.weight"]), P(b["xn"]), E, T, eps, st)          # x += o; xn = norm(x)
@@ -346,6 +446,8 @@ class LlamaDecoder(Decoder):
             nxt = self.norm[f"blk.{layer + 1}.attn_norm.weight"] if layer + 1 < cfg.layers else self.norm["output_norm.weight"]
             be.dev_rms_norm(P(b["x"]), P(b["tmp"]), P(nxt), P(b["xn"]), E, T, eps, st)                                       # x += down; xn = next norm
         be.dev_advance_position(P(self.pos), T, st)
+        if self.q4:
+            be.dev_advance_position(P(self.filled), T, st)
         with self.torch.cuda.stream(self.stream):
             self.x.copy_(b["x"][T - 1])
             self.xn.copy_(b["xn"][T - 1])
@@ -357,7 +459,8 @@ class LlamaDecoder(Decoder):
         Speculative verification is this call with tail_count = len(proposals) (:4874): row i is the target model's
         distribution after proposal i.  Afterwards the position is start_pos + len(tokens); a caller that rejects proposals
         passes the position after the last accepted token as the next start_pos (the cache rows past it are overwritten,
-        as in the reference, whose caches are indexed by the position it is given).
+        as in the reference, whose caches are indexed by the position it is given; with a cache in 4 bits that drops slots, back to
+        where it last did).
         The layers run through prefill() (tcgen05 GEMMs, causal block attention); the lm_head takes the tail rows through
         the decode kernel (up to eight, in the decode activation mode) or the GEMM (more, in the block's mode).  One GPU only."""
         if self.world != 1:
@@ -371,6 +474,7 @@ class LlamaDecoder(Decoder):
             start_pos = int(self.pos.item())
         if start_pos + T > self.max_positions:
             raise ValueError("forward_block: the block does not fit the configured positions")
+        self._rewind(start_pos)
         with torch.cuda.stream(self.stream):
             self.pos.fill_(start_pos)
             d_ids = torch.tensor(tokens, dtype=torch.int64).pin_memory().to(self.dev, non_blocking=True)
@@ -390,10 +494,83 @@ class LlamaDecoder(Decoder):
             self.token.copy_(self.block_picks[tail_count - 1:tail_count])
         return self.block_logits[:tail_count]
 
+    # ---- generation by drafted blocks ----
+    LOOKUP = 3              # tokens of the context's end that a draft is looked up by, at most
+
+    def look_up(self, context: list[int], drafts: int) -> list[int]:
+        """What followed the last place where the context's last tokens (as many as LOOKUP, else fewer) stood before, up to `drafts` tokens."""
+        for n in range(min(self.LOOKUP, len(context) - 1), 0, -1):
+            tail = context[-n:]
+            for at in range(len(context) - n - 1, -1, -1):
+                if context[at:at + n] == tail:
+                    return context[at + n:at + n + drafts]
+        return []
+
+    def generate_drafted(self, prompt: list[int], max_new: int, drafts: int = 4, propose=None, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
+                         seed: int = 0) -> list[int]:
+        """generate() with several tokens per pass of the model: `propose(context, drafts)` (default: look_up) drafts up to `drafts` tokens, forward_block
+        answers all of them, and zen_cuda_dev_verify_drafts keeps those that the model would have drawn, with one token more.  The tokens are distributed as
+        generate()'s are, greedy ones are its own up to the rounding of the block's products against the step's; what a seed draws differs, for a
+        block takes several random numbers at once.  A pass for which nothing is drafted is a step.  One GPU only."""
+        if self.world != 1:
+            raise ValueError("generate_drafted: one GPU only")
+        if not prompt or len(prompt) + max_new > self.max_positions:
+            raise ValueError("prompt + max_new exceeds the configured positions")
+        if not 1 <= drafts <= min(64, self.PREFILL_CHUNK - 1):
+            raise ValueError("drafts: 1 .. 64, and less than a block")
+        torch, be, st = self.torch, self.be, self.stream.cuda_stream
+        propose = propose or self.look_up
+        rng = np.random.default_rng(seed)
+        self.reset()
+        i64 = dict(dtype=torch.int64, device=self.dev)
+        out, accepted = torch.zeros(drafts + 2, **i64), torch.zeros(1, dtype=torch.int32, device=self.dev)
+        uniforms = torch.zeros(drafts + 1, dtype=torch.float64, device=self.dev)
+        check = DraftCheck(None, self.vocab, self.vocab, drafts, None, None, None, None, uniforms.data_ptr(), max(temperature, 0.0), top_k, top_p, out.data_ptr(), accepted.data_ptr())
+        room = torch.zeros(be.verify_drafts_workspace_bytes(check), dtype=torch.uint8, device=self.dev)
+        check.workspace, check.workspace_bytes = room.data_ptr(), room.numel()
+        got: list[int] = []
+
+        def draw(logits, proposed: list[int]) -> list[int]:
+            with torch.cuda.stream(self.stream):
+                d_tokens = torch.tensor(proposed or [0], dtype=torch.int64).pin_memory().to(self.dev, non_blocking=True)
+                uniforms[:len(proposed) + 1].copy_(torch.from_numpy(rng.random(len(proposed) + 1)).pin_memory(), non_blocking=True)
+                check.logits, check.drafts, check.tokens = logits.data_ptr(), len(proposed), d_tokens.data_ptr()
+                be.dev_verify_drafts(check, st)
+                out[drafts + 1:].copy_(accepted)                  # one read: the tokens and how many were accepted
+                answer = out.tolist()
+            if answer[answer[-1]] < 0:
+                be.dev_check(st)
+                raise ValueError("generate_drafted: a row of logits has no finite value")
+            return answer[:answer[-1] + 1]
+
+        with torch.cuda.stream(self.stream):
+            self.feed_prompt(prompt)
+        position = len(prompt)
+        if max_new > 0:
+            got += draw(self.logits, [])
+        while len(got) < max_new:
+            proposed = list(propose(prompt + got, min(drafts, max_new - len(got) - 1))) if max_new - len(got) > 1 else []
+            if len(proposed) > min(drafts, max_new - len(got) - 1) or any(not 0 <= t < self.vocab for t in proposed):
+                raise ValueError("generate_drafted: more tokens than asked for, or a token outside the vocabulary")
+            if proposed:
+                new = draw(self.forward_block([got[-1]] + proposed, position, len(proposed) + 1), proposed)
+            else:
+                self._rewind(position)
+                with torch.cuda.stream(self.stream):
+                    self.pos.fill_(position)
+                    self.token.fill_(got[-1])
+                self.step(want_token=True)
+                new = draw(self.logits, [])
+            got += new
+            position += len(new)
+        be.dev_check(st)
+        return got
+
     def _prompt_token(self, last: bool) -> None:
         if self.prompt_act_mode is None:
             self.step(want_token=last)
             return
+        self._make_room(1)
         decode_mode, self.act_mode = self.act_mode, self.prompt_act_mode
         try:
             self._enqueue_layers()            # eager: the captured graphs hold the decode mode

@@ -20,13 +20,13 @@ class UnsupportedDtype(ValueError):
     """No decoder of this architecture computes in the precision asked for."""
 
 
-def _llama(backend: Backend, path: str, dtype: str, max_positions: int | None) -> Decoder:
+def _llama(backend: Backend, path: str, dtype: str, max_positions: int | None, **options) -> Decoder:
     # Q8_0 weights: "bfloat16" is the serving default (int8 activation codes); "float32" the two-digit activations, whose products
     # are fp32-equivalent but not fp32 arithmetic, so it is not offered under that name
     from .llama import LlamaDecoder
     if dtype == "float32":
         raise UnsupportedDtype("the Q8_0 llama decoder has no 32-bit arithmetic; act_mode=ACT_FP32 is its closest mode")
-    return LlamaDecoder.from_gguf(backend, path, act_mode=ACT_INT8, prompt_act_mode=ACT_FP32, max_positions=max_positions)
+    return LlamaDecoder.from_gguf(backend, path, act_mode=ACT_INT8, prompt_act_mode=ACT_FP32, max_positions=max_positions, **options)
 
 
 def _kipirax(backend: Backend, path: str, dtype: str, max_positions: int | None) -> Decoder:
@@ -58,10 +58,13 @@ def architecture_of(path: str) -> str:
     return name
 
 
-def load_model(backend: Backend, path: str, dtype: str = "bfloat16", max_positions: int | None = None) -> Decoder:
-    """The model at `path`, resident and with its step graphs captured."""
+def load_model(backend: Backend, path: str, dtype: str = "bfloat16", max_positions: int | None = None, **options) -> Decoder:
+    """The model at `path`, resident and with its step graphs captured.  options: LlamaDecoder's kv, kv_slots and kv_keep."""
     if dtype not in ("bfloat16", "float32"):
         raise UnsupportedDtype(f"dtype {dtype!r}")
-    dec = MODELS[architecture_of(path)](backend, path, dtype, max_positions)
+    name = architecture_of(path)
+    if options and name != "llama":
+        raise ValueError(f"{name}: {', '.join(options)} is for llama models")
+    dec = MODELS[name](backend, path, dtype, max_positions, **options)
     dec.capture()
     return dec
