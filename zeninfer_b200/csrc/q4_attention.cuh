@@ -233,12 +233,15 @@ __device__ __forceinline__ uint8_t q4_append_block(const Q4Attend& p, float x, u
     return byte;
 }
 
-// New keys (rotated) and values into the slots behind *filled, where nothing else is to be prepared: a warp takes several blocks, all asked for first.
-constexpr uint32_t kQ4AppendWarps = 8, kQ4AppendEach = 4;
+// New keys (rotated) and values into the slots behind *filled, where nothing else is to be prepared: four lanes a block, a lane has eight values, which are a word of its
+// codes.  512 tokens of 8 kv heads of 128 values: APPEND_US (a lane a value, which rotates every pair twice and quantises through the warp: 14).
+constexpr uint32_t kQ4AppendThreads = 256;
 template <int kBlocks>
-__global__ void __launch_bounds__(kQ4AppendWarps * 32) q4_append_kernel(const __grid_constant__ Q4Attend p) {
-    const uint32_t lane = threadIdx.x & 31u, first = (blockIdx.x * kQ4AppendWarps + (threadIdx.x >> 5)) * kQ4AppendEach;
-    const uint32_t items = p.tokens * p.cache.kv_heads * 2 * kBlocks;
+__global__ void __launch_bounds__(kQ4AppendThreads) q4_append_kernel(const __grid_constant__ Q4Attend p) {
+    const uint32_t items = p.tokens * p.cache.kv_heads * 2 * kBlocks, item = blockIdx.x * (kQ4AppendThreads / 4) + threadIdx.x / 4, mine = min(item, items - 1), j = threadIdx.x & 3u;
+    const uint32_t piece = mine % (2 * kBlocks), h = mine / (2 * kBlocks) % p.cache.kv_heads, t = mine / (2 * kBlocks) / p.cache.kv_heads;
+    const bool is_value = piece >= kBlocks;
+    const uint32_t block = is_value ? piece - kBlocks : piece;
     pdl_launch_dependents();
     pdl_wait();
     const int filled = *reinterpret_cast<const volatile int*>(p.filled);
@@ -247,18 +250,38 @@ __global__ void __launch_bounds__(kQ4AppendWarps * 32) q4_append_kernel(const __
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(p.error_word, kErrBadPosition);
         return;
     }
-    float x[kQ4AppendEach];
+    Q4Rotation turn = p.turn;
+    if (is_value) turn.pairs = 0;
+    const float* const from = is_value ? p.v : p.k;
+    float x[8];
+    q4_rotated_eight(x, from + t * p.kv_ld + static_cast<size_t>(h) * kBlocks * 32, block * 32 + 4 * j, turn, static_cast<size_t>(position) + t, q4_rotates_fours(from, p.kv_ld, kBlocks * 32, turn));
+    uint32_t top = 0, first = 0xffffffffu;                    // the largest magnitude; its first place, above the sign there
 #pragma unroll
-    for (uint32_t i = 0; i < kQ4AppendEach; ++i) {
-        const uint32_t item = min(first + i, items - 1), of_token = item / (2 * kBlocks), t = of_token / p.cache.kv_heads;
-        x[i] = q4_new_value<kBlocks>(p, of_token % p.cache.kv_heads, t, item % (2 * kBlocks), static_cast<size_t>(position) + t, lane);
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if ((__float_as_uint(x[e]) & 0x7fffffffu) == top) first = min(first, (4 * j + (e & 3) + (e >> 2) * 16) * 2 + (__float_as_uint(x[e]) >> 31));
+    first = min(first, __shfl_xor_sync(0xffffffffu, first, 1));
+    first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
+    if (item >= items) return;
+    const __half scale = q4_scale_of(__uint_as_float(top | (first & 1u) << 31));
+    const float d = __half2float(scale), inverse = __frcp_rn(d);
+    uint32_t word = 0, code[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        code[e] = q4_code_of(x[e], d, inverse);
+        word |= code[e] << (8 * (e & 3) + 4 * (e >> 2));
     }
+    const uint32_t slot = static_cast<uint32_t>(filled) + t;
+    reinterpret_cast<uint32_t*>((is_value ? p.cache.v_codes : p.cache.k_codes) + q4_codes_at(h, slot, block, kBlocks, p.cache.slots))[j] = word;
+    if (j == 0) (is_value ? p.cache.v_scales : p.cache.k_scales)[q4_scale_at(h, slot, block, kBlocks, p.cache.slots)] = scale;
+    float* held = is_value ? p.v_held : p.k_held;
+    if (held) {
+        held += (static_cast<size_t>(t) * p.cache.kv_heads + h) * kBlocks * 32 + block * 32 + 4 * j;
 #pragma unroll
-    for (uint32_t i = 0; i < kQ4AppendEach; ++i) {
-        const uint32_t item = first + i, of_token = item / (2 * kBlocks), t = of_token / p.cache.kv_heads;
-        if (item >= items) return;
-        __half ignored;
-        q4_append_block<kBlocks>(p, x[i], of_token % p.cache.kv_heads, t, item % (2 * kBlocks), static_cast<uint32_t>(filled), lane, ignored);
+        for (int e = 0; e < 8; ++e) held[(e & 3) + (e >> 2) * 16] = (static_cast<float>(code[e]) - 8.0f) * d;
     }
 }
 

@@ -61,9 +61,63 @@ __device__ __forceinline__ float q4_rotated(const Q4Raw& x, uint32_t e, const Q4
 }
 __device__ __forceinline__ float q4_rotated(const float* head, uint32_t e, const Q4Rotation& r, size_t row) { return q4_rotated(q4_raw(head, e, r), e, r, row); }
 
-// A warp quantises a block, a value a lane: the scale (of the first value of largest magnitude), the lane's code.  The code is the integer
-// nearest to x / d + 8, and the choice is exact: x / d >= c - 8.5 is x >= (c - 8.5) d for positive d, a product of five bits and eleven
+// Eight dimensions of a head vector, rotated: at .. at + 3 and at + 16 .. at + 19.  Four at a time where the whole head turns and everything is aligned, else one by one; the
+// operations are q4_rotated's.
+__device__ __forceinline__ bool q4_rotates_fours(const float* q, size_t q_ld, uint32_t dim, const Q4Rotation& r) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | (q_ld * 4) | (r.pairs ? reinterpret_cast<uintptr_t>(r.cos_t) | reinterpret_cast<uintptr_t>(r.sin_t) : 0);
+    return all % 16 == 0 && (!r.pairs || 2 * r.pairs == dim);
+}
+__device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row, bool fours) {
+    if (!fours) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = q4_rotated(head, at + (e & 3) + (e >> 2) * 16, r, row);
+        return;
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const uint32_t e = at + 16 * part;
+        const float4 mine = __ldcg(reinterpret_cast<const float4*>(head + e));
+        float* y = x + 4 * part;
+        if (!r.pairs) {
+            y[0] = mine.x; y[1] = mine.y; y[2] = mine.z; y[3] = mine.w;
+        } else if (r.adjacent) {
+            const float* const cos_t = r.cos_t + row * r.pairs + e / 2;
+            const float* const sin_t = r.sin_t + row * r.pairs + e / 2;
+            const float2 c = __ldg(reinterpret_cast<const float2*>(cos_t)), s = __ldg(reinterpret_cast<const float2*>(sin_t));
+            y[0] = __fsub_rn(__fmul_rn(mine.x, c.x), __fmul_rn(mine.y, s.x)); y[1] = __fadd_rn(__fmul_rn(mine.x, s.x), __fmul_rn(mine.y, c.x));
+            y[2] = __fsub_rn(__fmul_rn(mine.z, c.y), __fmul_rn(mine.w, s.y)); y[3] = __fadd_rn(__fmul_rn(mine.z, s.y), __fmul_rn(mine.w, c.y));
+        } else {
+            const bool low = e < r.pairs;
+            const uint32_t pair = low ? e : e - r.pairs;
+            const float4 its = __ldcg(reinterpret_cast<const float4*>(head + (low ? e + r.pairs : pair)));
+            const float* const cos_t = r.cos_t + row * r.pairs + pair;
+            const float* const sin_t = r.sin_t + row * r.pairs + pair;
+            const float4 c = __ldg(reinterpret_cast<const float4*>(cos_t)), s = __ldg(reinterpret_cast<const float4*>(sin_t));
+            auto turned = [&](float a, float b, float cc, float ss) { return low ? __fsub_rn(__fmul_rn(a, cc), __fmul_rn(b, ss)) : __fadd_rn(__fmul_rn(b, ss), __fmul_rn(a, cc)); };
+            y[0] = turned(mine.x, its.x, c.x, s.x); y[1] = turned(mine.y, its.y, c.y, s.y); y[2] = turned(mine.z, its.z, c.z, s.z); y[3] = turned(mine.w, its.w, c.w, s.w);
+        }
+    }
+}
+
+// The quantisation of a block: the scale is that of the first value of largest magnitude, `at`, and the code the integer
+// nearest to x / d + 8.  The choice is exact: x / d >= c - 8.5 is x >= (c - 8.5) d for positive d, a product of five bits and eleven
 // that fp32 holds, so the estimate by a rounded reciprocal, off by one at most, is put right by two comparisons.
+__device__ __forceinline__ __half q4_scale_of(float at) {
+    if ((__float_as_uint(at) & 0x7fffffffu) >= 0x7f800000u) return __ushort_as_half(static_cast<unsigned short>(0x7e00u));      // an infinity or a NaN among the values: the block reads as NaN
+    return __float2half_rn(fminf(fmaxf(at * -0.125f, -65504.0f), 65504.0f));
+}
+// d: the scale as fp32, inverse: __frcp_rn(d)
+__device__ __forceinline__ uint32_t q4_code_of(float x, float d, float inverse) {
+    if (!(fabsf(d) > 0.0f)) return 8;      // zero, or NaN
+    const float guess = fminf(fmaxf(floorf(fmaf(x, inverse, 8.5f)), -1.0f), 16.0f);
+    auto reaches = [&](float c) { const float border = (c - 8.5f) * d; return d > 0.0f ? x >= border : x <= border; };
+    float c = guess;
+    if (!reaches(c)) c -= 1.0f;
+    else if (reaches(c + 1.0f)) c += 1.0f;
+    return static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));
+}
+
+// A warp quantises a block, a value a lane: the scale, and the lane's code.
 struct Q4Quantised {
     __half scale;
     uint32_t code;
@@ -71,25 +125,10 @@ struct Q4Quantised {
 __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
     const uint32_t size = __float_as_uint(x) & 0x7fffffffu;
     const uint32_t top = __reduce_max_sync(0xffffffffu, size);
-    const float at = __shfl_sync(0xffffffffu, x, __ffs(__ballot_sync(0xffffffffu, size == top)) - 1);
     Q4Quantised r;
-    if (top >= 0x7f800000u) {      // an infinity or a NaN among the values: the block reads as NaN
-        r.scale = __ushort_as_half(static_cast<unsigned short>(0x7e00u));
-        r.code = 8;
-        return r;
-    }
-    r.scale = __float2half_rn(fminf(fmaxf(at * -0.125f, -65504.0f), 65504.0f));
+    r.scale = q4_scale_of(__shfl_sync(0xffffffffu, x, __ffs(__ballot_sync(0xffffffffu, size == top)) - 1));
     const float d = __half2float(r.scale);
-    if (d == 0.0f) {
-        r.code = 8;
-        return r;
-    }
-    const float guess = fminf(fmaxf(floorf(fmaf(x, __frcp_rn(d), 8.5f)), -1.0f), 16.0f);
-    auto reaches = [&](float c) { const float border = (c - 8.5f) * d; return d > 0.0f ? x >= border : x <= border; };
-    float c = guess;
-    if (!reaches(c)) c -= 1.0f;
-    else if (reaches(c + 1.0f)) c += 1.0f;
-    r.code = static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));
+    r.code = q4_code_of(x, d, __frcp_rn(d));
     return r;
 }
 

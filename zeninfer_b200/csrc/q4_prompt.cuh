@@ -81,44 +81,6 @@ __device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint3
     return __reduce_max_sync(0xffffffffu, top);
 }
 
-// Eight dimensions of a head vector, rotated: at .. at + 3 and at + 16 .. at + 19.  Four at a time where the whole head turns and everything is aligned, else one by one; the
-// operations are q4_rotated's.
-__device__ __forceinline__ bool q4_rotates_fours(const float* q, size_t q_ld, uint32_t dim, const Q4Rotation& r) {
-    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | (q_ld * 4) | (r.pairs ? reinterpret_cast<uintptr_t>(r.cos_t) | reinterpret_cast<uintptr_t>(r.sin_t) : 0);
-    return all % 16 == 0 && (!r.pairs || 2 * r.pairs == dim);
-}
-__device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row, bool fours) {
-    if (!fours) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = q4_rotated(head, at + (e & 3) + (e >> 2) * 16, r, row);
-        return;
-    }
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-        const uint32_t e = at + 16 * part;
-        const float4 mine = __ldcg(reinterpret_cast<const float4*>(head + e));
-        float* y = x + 4 * part;
-        if (!r.pairs) {
-            y[0] = mine.x; y[1] = mine.y; y[2] = mine.z; y[3] = mine.w;
-        } else if (r.adjacent) {
-            const float* const cos_t = r.cos_t + row * r.pairs + e / 2;
-            const float* const sin_t = r.sin_t + row * r.pairs + e / 2;
-            const float2 c = __ldg(reinterpret_cast<const float2*>(cos_t)), s = __ldg(reinterpret_cast<const float2*>(sin_t));
-            y[0] = __fsub_rn(__fmul_rn(mine.x, c.x), __fmul_rn(mine.y, s.x)); y[1] = __fadd_rn(__fmul_rn(mine.x, s.x), __fmul_rn(mine.y, c.x));
-            y[2] = __fsub_rn(__fmul_rn(mine.z, c.y), __fmul_rn(mine.w, s.y)); y[3] = __fadd_rn(__fmul_rn(mine.z, s.y), __fmul_rn(mine.w, c.y));
-        } else {
-            const bool low = e < r.pairs;
-            const uint32_t pair = low ? e : e - r.pairs;
-            const float4 its = __ldcg(reinterpret_cast<const float4*>(head + (low ? e + r.pairs : pair)));
-            const float* const cos_t = r.cos_t + row * r.pairs + pair;
-            const float* const sin_t = r.sin_t + row * r.pairs + pair;
-            const float4 c = __ldg(reinterpret_cast<const float4*>(cos_t)), s = __ldg(reinterpret_cast<const float4*>(sin_t));
-            auto turned = [&](float a, float b, float cc, float ss) { return low ? __fsub_rn(__fmul_rn(a, cc), __fmul_rn(b, ss)) : __fadd_rn(__fmul_rn(b, ss), __fmul_rn(a, cc)); };
-            y[0] = turned(mine.x, its.x, c.x, s.x); y[1] = turned(mine.y, its.y, c.y, s.y); y[2] = turned(mine.z, its.z, c.z, s.z); y[3] = turned(mine.w, its.w, c.w, s.w);
-        }
-    }
-}
-
 // Eight dimensions of a row of queries in the scores' order, 4j .. 4j+3 and 16+4j .. 16+4j+3 of a block, as they are unpacked from a word of codes.
 __device__ __forceinline__ void q4_split_queries(const float (&x)[8], float up, uint4& upper, uint4& lower) {
     uint32_t u[4], l[4];

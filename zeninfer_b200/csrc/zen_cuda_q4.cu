@@ -208,10 +208,10 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     const bool prompt = plan.columns == zk::kQ4Prompt;
     if (prompt) {
         if (p.stats) { p.queries = reinterpret_cast<uint4*>(room + plan.queries); p.factors = part(plan.factors); }
-        const size_t items = tokens * cache.kv_heads * 2 * cache.blocks, a_cta = zk::kQ4AppendWarps * zk::kQ4AppendEach;
+        const size_t items = tokens * cache.kv_heads * 2 * cache.blocks, a_cta = zk::kQ4AppendThreads / 4;
         const cudaError_t r = by_prompt_blocks(cache.blocks, [&](auto blocks) {
             constexpr int kBlocks = decltype(blocks)::value;
-            const cudaError_t appended = launch(e, zk::q4_append_kernel<kBlocks>, dim3(u32((items + a_cta - 1) / a_cta)), dim3(zk::kQ4AppendWarps * 32), 0, 0, p);
+            const cudaError_t appended = launch(e, zk::q4_append_kernel<kBlocks>, dim3(u32((items + a_cta - 1) / a_cta)), dim3(zk::kQ4AppendThreads), 0, 0, p);
             return appended != cudaSuccess ? appended : launch(e, zk::q4_prompt_kernel<kBlocks>, dim3(plan.splits, plan.row_ctas, cache.kv_heads), dim3(zk::kQpThreads), zk::q4_prompt_smem<kBlocks>(), 0, p);
         });
         if (!e.leave(r, "dev_q4_attention")) return 0;
