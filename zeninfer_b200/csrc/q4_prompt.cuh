@@ -6,8 +6,8 @@
 // done per block and score.  A tile's scales are multiplied by the power of two that brings the largest below 2^9, so that both parts keep their bits
 // whatever the model's magnitudes are.  The dimensions of the operands stand in the order in which the nibbles are unpacked.
 //
-// A CTA takes 128 rows (a row: a token times a query head of the kv head, any group) and walks its run of slots 64 at a time.  Sixteen warps:
-//   8 rows       a thread has half a row: 32 scores from TMEM, mask, running maximum (shared with the other half), exponentials, the weights' two parts back to
+// A CTA takes 128 rows (a row: a token times a query head of the kv head, any group) and walks its run of slots 64 at a time.  24 warps:
+//   16 rows      a thread has a quarter of a row: 16 scores from TMEM, mask, running maximum (of the quarters), exponentials, the weights' two parts back to
 //                TMEM, from where the tensor cores read them (as they do the queries); then out = out * factor + O' of the tile before, in fp32 registers
 //   3 + 4        unpack keys and values (bulk copies bring the tiles into a ring, two ahead) into the operands' 128-byte swizzle, two buffers each, a slot's block a
 //                thread: to the tensor cores keys are a matrix with the summed index in its rows, values one with it in its columns, so neither is transposed
@@ -23,7 +23,7 @@
 
 namespace zk {
 
-constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 16 * 32, kQpKeyWarp = 8, kQpValueWarp = 11, kQpIssueWarp = 15;      // first warps of the roles
+constexpr uint32_t kQpRows = 128, kQpKeys = 64, kQpThreads = 24 * 32, kQpKeyWarp = 16, kQpValueWarp = 19, kQpIssueWarp = 23;      // first warps of the roles
 template <int kBlocks> constexpr uint32_t kQpQPlane = kQpRows * kBlocks * 64;      // bytes
 template <int kBlocks> constexpr uint32_t kQpKPlane = kQpKeys * kBlocks * 64;      // of keys, of values
 constexpr int kQpStages = 3;                 // tiles as they are in the cache, ahead of the warps that unpack them
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     uint8_t* const k_smem = q_smem + 2 * kQPlane;             // [buffer][plane][64 dimensions][64 slots][128 bytes]
     uint8_t* const v_smem = k_smem + 4 * kKPlane;             // the same
     uint8_t* const raw_smem = v_smem + 4 * kKPlane;           // [stage]: codes of keys and of values, scales of keys and of values
-    __shared__ float row_factor[kQpRows], top[2][2][kQpRows], sum[2][kQpRows];
+    __shared__ float row_factor[kQpRows], top[2][4][kQpRows], sum[4][kQpRows];
     __shared__ uint64_t raw_full[kQpStages], raw_free[kQpStages], k_full[2], k_free[2], v_full[2], v_free[2], q_full, s_full, s_empty, p_full, o_full, o_empty;
     __shared__ float k_unit[4], v_unit[4];                    // what a tile's operands are to be multiplied by: the rows read the last but one while the next is stored
     __shared__ uint32_t tmem_slot, bad_key, bad_value[kBlocks];      // the first slots whose scales are not finite
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             mbar_init(&k_full[b], kQpValueWarp - kQpKeyWarp); mbar_init(&v_full[b], kQpIssueWarp - kQpValueWarp);
             mbar_init(&k_free[b], 1); mbar_init(&v_free[b], 1);
         }
-        mbar_init(&q_full, kQpKeyWarp); mbar_init(&s_full, 1); mbar_init(&s_empty, 8); mbar_init(&p_full, 8); mbar_init(&o_full, 1); mbar_init(&o_empty, 8);
+        mbar_init(&q_full, kQpKeyWarp); mbar_init(&s_full, 1); mbar_init(&s_empty, kQpKeyWarp); mbar_init(&p_full, kQpKeyWarp); mbar_init(&o_full, 1); mbar_init(&o_empty, kQpKeyWarp);
         mbar_fence_init();
         bad_key = 0xffffffffu;
         for (int b = 0; b < kBlocks; ++b) bad_value[b] = 0xffffffffu;
@@ -185,21 +185,21 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         bulk_g2s(to + 2 * kCodes, p.cache.k_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
         bulk_g2s(to + 2 * kCodes + kScales, p.cache.v_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
     };
-    {      // Q: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
-        constexpr uint32_t kChunks = kDim / 8, kEach = kQpRows * kChunks / kQpThreads;
+    if (warp < kQpKeyWarp) {      // Q: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
+        constexpr uint32_t kChunks = kDim / 8, kRowThreads = kQpKeyWarp * 32, kEach = kQpRows * kChunks / kRowThreads;
         const uint32_t chunk = threadIdx.x % kChunks, dim = chunk / 4 * 32 + chunk % 4 * 4;
         const bool fours = q4_rotates_fours(p.q, p.q_ld, kDim, p.turn);
         float x[kEach][8];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t r = threadIdx.x / kChunks + i * (kQpThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
+            const uint32_t r = threadIdx.x / kChunks + i * (kRowThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
             const float* from = p.q + token * p.q_ld + static_cast<size_t>(h * p.group + row % p.group) * kDim;
             const size_t turned = static_cast<size_t>(position) + token;
             q4_rotated_eight(x[i], from, dim, p.turn, turned, fours);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t r = threadIdx.x / kChunks + i * (kQpThreads / kChunks);
+            const uint32_t r = threadIdx.x / kChunks + i * (kRowThreads / kChunks);
             float most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -232,10 +232,10 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    if (warp < kQpKeyWarp) {                                  // the queries into TMEM, a part of a row a thread: the products then read keys only from shared memory
-        const uint32_t r = (warp & 3u) * 32 + lane, plane = warp >> 2;
+    if (warp < kQpKeyWarp) {                                  // the queries into TMEM, half a row's part a thread: the products then read keys only from shared memory
+        const uint32_t r = (warp & 3u) * 32 + lane, plane = warp >> 3, c0 = (warp >> 2 & 1u) * (kDim / 32);
 #pragma unroll
-        for (uint32_t c = 0; c < kDim / 16; ++c) {
+        for (uint32_t c = c0; c < c0 + kDim / 32; ++c) {
             uint32_t both[8];
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
@@ -254,17 +254,17 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
 
     // A wait that runs out ends its role's loop, and the others' follow.
     if (warp < kQpKeyWarp) {                                  // rows
-        const uint32_t quad = warp & 3, half = warp >> 2, r = quad * 32 + lane, row = first_row + r, lane_base = (quad * 32) << 16;
+        const uint32_t quad = warp & 3, quarter = warp >> 2, r = quad * 32 + lane, row = first_row + r, lane_base = (quad * 32) << 16;
         const bool live = r < real_rows;
         const uint32_t last_seen = live ? filled + row / p.group : 0xffffffffu;          // rows that are none: whatever comes, they write nothing
-        constexpr int kMine = kQpKeys / 2, kOut = kDim / 2;
+        constexpr int kMine = kQpKeys / 4, kOut = kDim / 4;
         const float factor = row_factor[r];
-        // the two warps of a row meet; true where one of them has given up
+        // the four warps of a row meet; true where one of them has given up
         auto meet = [&](bool failed) {
             uint32_t any;
             asm volatile(
                 "{ .reg .pred p, q; setp.ne.u32 q, %3, 0; barrier.red.or.pred p, %1, %2, q; selp.u32 %0, 1, 0, p; }"
-                : "=r"(any) : "r"(quad + 1), "r"(64u), "r"(static_cast<uint32_t>(failed)) : "memory");
+                : "=r"(any) : "r"(quad + 1), "r"(128u), "r"(static_cast<uint32_t>(failed)) : "memory");
             return any != 0;
         };
         constexpr float kFull = 16384.0f;                     // a weight of 1
@@ -272,15 +272,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
 #pragma unroll
         for (int i = 0; i < kOut; ++i) acc[i] = 0.0f;
         auto take_output = [&](float by) {                    // acc = acc * shrink + O'
+            uint32_t v[kOut / 16][16];
 #pragma unroll
-            for (int c = 0; c < kOut / 32; ++c) {
-                uint32_t v[2][16];
+            for (int b = 0; b < kOut / 16; ++b) tmem_ld_32x16(tmem + kQpOut + quarter * kOut + 16 * b + lane_base, v[b]);
+            tmem_ld_wait();
 #pragma unroll
-                for (int b = 0; b < 2; ++b) tmem_ld_32x16(tmem + kQpOut + half * kOut + 32 * c + 16 * b + lane_base, v[b]);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(__uint_as_float(v[i / 16][i % 16]), by, acc[32 * c + i] * shrink);
-            }
+            for (int i = 0; i < kOut; ++i) acc[i] = fmaf(__uint_as_float(v[i / 16][i % 16]), by, acc[i] * shrink);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_empty);
@@ -296,7 +293,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 for (int c = 0; c < kMine / 8; ++c) {
                     uint32_t part[3][8];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) tmem_ld_32x8(tmem + kQpScores + i * kQpKeys + half * kMine + 8 * c + lane_base, part[i]);
+                    for (int i = 0; i < 3; ++i) tmem_ld_32x8(tmem + kQpScores + i * kQpKeys + quarter * kMine + 8 * c + lane_base, part[i]);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[8 * c + i] = (__uint_as_float(part[0][i]) + __uint_as_float(part[1][i])) + __uint_as_float(part[2][i]);
@@ -305,7 +302,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_empty);
-                const uint32_t first = tile * kQpKeys + half * kMine;
+                const uint32_t first = tile * kQpKeys + quarter * kMine;
                 if (!__all_sync(0xffffffffu, first + kMine - 1 <= last_seen)) {
 #pragma unroll
                     for (int i = 0; i < kMine; ++i) if (first + i > last_seen) s[i] = -INFINITY;
@@ -314,7 +311,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) part[i & 3] = fmaxf(part[i & 3], s[i]);
                 most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * by;
-                top[j & 1][half][r] = most;
+                top[j & 1][quarter][r] = most;
                 if (p.scores && live) {
                     float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(h) * rows + row) * p.cache.slots + first);
 #pragma unroll
@@ -322,7 +319,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 }
             }
             if (meet(!ok)) { ok = false; break; }
-            most = fmaxf(fmaxf(most, top[j & 1][half ^ 1][r]), m);
+            most = fmaxf(fmaxf(fmaxf(top[j & 1][0][r], top[j & 1][1][r]), fmaxf(top[j & 1][2][r], top[j & 1][3][r])), m);
             const float from = most == -INFINITY ? 0.0f : most, f = exp2_fast(m - from);          // exp2(-inf) = 0 on the first slots
             m = most;
             float part[4] = {};
@@ -335,18 +332,15 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             if (j > 0) ok = warp_waited(&o_full, (j - 1) & 1);                  // the tile before: its output is formed, and P's place free
             if (ok) {
                 tc_fence_after_sync();
+                uint32_t upper[8], lower[8];
 #pragma unroll
-                for (int c = 0; c < kMine / 16; ++c) {
-                    uint32_t upper[8], lower[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float a = s[16 * c + 2 * i] * kFull, b = s[16 * c + 2 * i + 1] * kFull, ua = upper_digit(a), ub = upper_digit(b);
-                        upper[i] = pack_f16(ua, ub);
-                        lower[i] = pack_f16(a - ua, b - ub);
-                    }
-                    tmem_st_32x8(tmem + kQpP + 16 * half + 8 * c + lane_base, upper);
-                    tmem_st_32x8(tmem + kQpP + 32 + 16 * half + 8 * c + lane_base, lower);
+                for (int i = 0; i < 8; ++i) {
+                    const float a = s[2 * i] * kFull, b = s[2 * i + 1] * kFull, ua = upper_digit(a), ub = upper_digit(b);
+                    upper[i] = pack_f16(ua, ub);
+                    lower[i] = pack_f16(a - ua, b - ub);
                 }
+                tmem_st_32x8(tmem + kQpP + 8 * quarter + lane_base, upper);
+                tmem_st_32x8(tmem + kQpP + 32 + 8 * quarter + lane_base, lower);
                 tmem_st_wait();
                 tc_fence_before_sync();
                 __syncwarp();
@@ -357,32 +351,32 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         }
         if (ok) ok = warp_waited(&o_full, (j - 1) & 1);
         if (ok) { tc_fence_after_sync(); take_output(v_unit[(j - 1) & 3]); }
-        sum[half][r] = l;
+        sum[quarter][r] = l;
         if (meet(!ok)) {
             gave_up(kErrTmemWaitTimeout);
         } else if (live) {
-            l += sum[half ^ 1][r];
+            l = (sum[0][r] + sum[1][r]) + (sum[2][r] + sum[3][r]);
             if (last_seen >= bad_key) l = NAN;
             const bool alone = p.splits == 1;
             const float inv = alone ? 1.0f / l : 1.0f;
             const uint32_t token = row / p.group, head = h * p.group + row % p.group;
             const size_t part = (static_cast<size_t>(h) * p.splits + blockIdx.x) * rows + row;
-            float* to = (alone ? p.out + (static_cast<size_t>(token) * p.heads + head) * kDim : p.part_out + part * kDim) + half * kOut;
+            float* const to = alone ? p.out + (static_cast<size_t>(token) * p.heads + head) * kDim : p.part_out + part * kDim;
             const bool fours = reinterpret_cast<uintptr_t>(to) % 16 == 0;
 #pragma unroll
-            for (int b = 0; b < kOut / 32; ++b) {
-                const bool bad = last_seen >= bad_value[half * (kOut / 32) + b];
-                const float by = bad ? NAN : inv;
+            for (int w = 0; w < kOut / 8; ++w) {              // a word's eight dimensions, where the nibbles are unpacked to: 4w .. 4w + 3 and 16 more
+                const uint32_t word = quarter * (kOut / 8) + w, block = word / 4;
+                const float by = last_seen >= bad_value[block] ? NAN : inv;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {                 // four dimensions from 4i: where the nibbles are unpacked to
-                    const int at = 32 * b + i % 4 * 8 + i / 4 * 2;
+                for (int high = 0; high < 2; ++high) {
+                    const int at = 8 * w + 2 * high;
                     const float4 o = make_float4(acc[at] * by, acc[at + 4] * by, acc[at + 1] * by, acc[at + 5] * by);
-                    float* const here = to + 32 * b + 4 * i;
+                    float* const here = to + block * 32 + high * 16 + word % 4 * 4;
                     if (fours) *reinterpret_cast<float4*>(here) = o;
                     else { here[0] = o.x; here[1] = o.y; here[2] = o.z; here[3] = o.w; }
                 }
             }
-            if (half == 0) {
+            if (quarter == 0) {
                 if (alone) {
                     if (!(l > 0.0f) || !(l < INFINITY)) atomicExch(p.error_word, kErrNonFinite);
                     if (p.stats) p.stats[static_cast<size_t>(h) * rows + row] = m + log2f(l);

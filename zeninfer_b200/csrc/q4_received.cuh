@@ -6,14 +6,15 @@
 //
 // A CTA keeps 128 or 256 slots unpacked in shared memory and walks the tiles of 128 rows; a stage of its ring is 64 dimensions of a tile's two parts.  With 256 slots a
 // tile that comes out of L2 serves two matrices, which alternate between the accumulators' two buffers: 16 warps exponentiate one while the other is formed.  Each 64
-// dimensions have an accumulator of their own, corrections first.  Bounded by the tensor cores: a product of 128 x 128 x 16 takes 70 cycles with both operands in shared
+// dimensions have an accumulator of their own, corrections first.  Two warps issue the products, a unit each in turn: what one spends on waits and commits the other fills, for
+// the tensor cores take an instruction only when they are done with the one before.  Bounded by the tensor cores: a product of 128 x 128 x 16 takes 70 cycles with both operands in shared
 // memory (64 at their full rate).
 #pragma once
 #include "q4_prompt.cuh"
 
 namespace zk {
 
-constexpr uint32_t kQrSlots = 128, kQrStages = 3, kQrSumWarps = 16, kQrIssueWarp = 16, kQrCopyWarp = 17, kQrThreads = 18 * 32, kQrSets = 2;
+constexpr uint32_t kQrSlots = 128, kQrStages = 3, kQrSumWarps = 16, kQrIssueWarp = 16, kQrCopyWarp = 18, kQrThreads = 19 * 32, kQrSets = 2;
 template <int kBlocks> constexpr uint32_t kQrPlane = kQrSlots * kBlocks * 64;
 constexpr uint32_t kQrChunk = kQpRows * 128;                  // bytes: a part of 64 dimensions of a tile of rows
 template <int kBlocks> constexpr uint32_t q4_received_smem(uint32_t sets) { return 1024 + sets * 2 * kQrPlane<kBlocks> + kQrStages * 2 * kQrChunk; }
@@ -26,13 +27,13 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(qr_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* const k_smem = smem;                             // [set][plane][64 dimensions][128 slots][128 bytes]
     uint8_t* const q_smem = k_smem + sets * 2 * kPlane;       // [stage][plane][128 rows][128 bytes]
-    __shared__ float2 of_row[kQpRows];                        // what makes scores of a row's products; its e
+    __shared__ __align__(16) float2 of_row[kQpRows];                        // what makes scores of a row's products; its e
     __shared__ uint64_t q_full[kQrStages], q_free[kQrStages], s_full[2], s_free[2];
     __shared__ uint32_t tmem_slot;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, h = blockIdx.y, rows = p.tokens * p.group, row_tiles = (rows + kQpRows - 1) / kQpRows;
     const uint32_t cta_slot = blockIdx.x * sets * kQrSlots;
     if (threadIdx.x == 0) {
-        for (uint32_t b = 0; b < kQrStages; ++b) { mbar_init(&q_full[b], 1); mbar_init(&q_free[b], 1); }
+        for (uint32_t b = 0; b < kQrStages; ++b) { mbar_init(&q_full[b], 1); mbar_init(&q_free[b], sets); }
         for (uint32_t b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1); mbar_init(&s_free[b], kQrSumWarps); }
         mbar_fence_init();
     }
@@ -108,12 +109,15 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
                         if (lane == 0) mbar_arrive(&s_free[b]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float s = __uint_as_float(share[0][i]);
-                        if (kHalves > 1) s += __uint_as_float(share[kHalves - 1][i]);
-                        const float2 its = of_row[part * 32 + 16 * c + i];
-                        const float w = exp2_fast(fmaf(s, its.x, -its.y));
-                        if (all || column0 + 16 * c + i >= sees) added[i & 3] += w;
+                    for (int i = 0; i < 16; i += 2) {
+                        const float4 two = reinterpret_cast<const float4*>(of_row)[(part * 32 + 16 * c + i) / 2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float s = __uint_as_float(share[0][i + e]);
+                            if (kHalves > 1) s += __uint_as_float(share[kHalves - 1][i + e]);
+                            const float w = exp2_fast(e ? fmaf(s, two.z, -two.w) : fmaf(s, two.x, -two.y));
+                            if (all || column0 + 16 * c + i + e >= sees) added[(i + e) & 3] += w;
+                        }
                     }
                 }
                 const float both = (added[0] + added[1]) + (added[2] + added[3]);
@@ -134,18 +138,18 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
             const size_t at = static_cast<size_t>(h) * p.cache.slots + slot;
             p.weight_out[at] = share[threadIdx.x] + (slot < filled ? p.weight_in[at] : 0.0f);
         }
-    } else if (warp == kQrIssueWarp) {
+    } else if (warp < kQrCopyWarp) {
         if (lane == 0) {
+            const uint32_t b = warp - kQrIssueWarp;           // the accumulators' buffer: units b, b + 2, ..
             constexpr uint32_t desc = umma_idesc_f16(kQrSlots, kQpRows);
             const uint64_t k_desc = umma_desc_k_sw128(smem_u32(k_smem)), q_desc = umma_desc_k_sw128(smem_u32(q_smem));
             bool ok = true;
-            uint32_t stage0 = 0, phase0 = 0;                  // of a tile's first 64 dimensions
-            for (uint32_t u = 0; ok && u < units; ++u) {
-                const uint32_t set = u % sets, b = u & 1u;
+            for (uint32_t u = b; ok && u < units; u += 2) {
+                const uint32_t set = u % sets;
                 ok = u < 2 || mbar_wait(&s_free[b], ((u >> 1) - 1) & 1u);
-                uint32_t stage = stage0, phase = phase0;
                 for (uint32_t c = 0; ok && c < kHalves; ++c) {
-                    if (set == 0) ok = mbar_wait(&q_full[stage], phase);
+                    const uint32_t chunk = u / sets * kHalves + c, stage = chunk % kQrStages;
+                    ok = mbar_wait(&q_full[stage], (chunk / kQrStages) & 1u);
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint64_t k_at = k_desc + ((set * 2 * kPlane + c * (kPlane / kHalves)) >> 4), q_at = q_desc + (stage * 2 * kQrChunk >> 4);
@@ -156,12 +160,10 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
                         for (uint32_t k = 0; k < 4; ++k)
                             tc_mma_f16(tmem + b * kScores + c * kQpRows, k_at + (kp * kPlane >> 4) + 2 * k, q_at + (qp * kQrChunk >> 4) + 2 * k, desc, (i | k) > 0);
                     }
-                    if (set + 1 == sets) tc_commit(&q_free[stage]);
-                    if (++stage == kQrStages) { stage = 0; phase ^= 1u; }
+                    tc_commit(&q_free[stage]);
                 }
                 if (!ok) break;
                 tc_commit(&s_full[b]);
-                if (set + 1 == sets) { stage0 = stage; phase0 = phase; }
             }
             if (!ok) atomicExch(p.error_word, kErrFullWaitTimeout);
         }
