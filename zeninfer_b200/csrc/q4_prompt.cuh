@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t f16x2_rest(uint32_t a, uint32_t b, uint32_t product) {      // a * b - product
     uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(product ^ 0x80008000u));
+    asm("{ .reg .b32 n; neg.f16x2 n, %3; fma.rn.f16x2 %0, %1, %2, n; }" : "=r"(r) : "r"(a), "r"(b), "r"(product));
     return r;
 }
 // The power of two for a tile whose largest scale has these bits: times 2^shift it is below 2^9.
@@ -57,26 +57,29 @@ __device__ __forceinline__ bool q4_finite(uint32_t half_bits) { return (half_bit
 // The largest magnitude among the finite scales of the first `slots` of kSlots slots, as f16 bits: every lane of a warp.  bad(slot, block) is called for the others.
 template <int kBlocks, uint32_t kSlots, typename Bad>
 __device__ __forceinline__ uint32_t q4_largest_scale(const __half* scales, uint32_t slots, uint32_t lane, Bad bad) {
-    uint32_t top = 0;
-    bool odd = false;
+    uint32_t both = 0;                                        // two maxima side by side
 #pragma unroll
     for (uint32_t at = 0; at < kSlots * kBlocks / 8; at += 32) {      // eight scales a lane: 8 / kBlocks slots
         const uint32_t first = (at + lane) * 8 / kBlocks;
         if (first >= min(slots, kSlots)) continue;
         const uint4 eight = reinterpret_cast<const uint4*>(scales)[at + lane];
-        const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
+        uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
+        if (slots < kSlots) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0x7fffu;
-            if (first + j / kBlocks >= slots) continue;
-            if (q4_finite(bits)) top = max(top, bits);
-            else odd = true;
+            for (int j = 0; j < 8; ++j)
+                if (first + j / kBlocks >= slots) w[j / 2] &= j % 2 ? 0x0000ffffu : 0xffff0000u;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) both = __vmaxu2(both, w[j] & 0x7fff7fffu);
     }
-    if (__any_sync(0xffffffffu, odd)) {
+    uint32_t top = __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
+    if (q4_finite(top)) return top;
+    top = 0;
 #pragma unroll 1
-        for (uint32_t i = lane; i < slots * kBlocks; i += 32)
-            if (!q4_finite(__half_as_ushort(scales[i]))) bad(i / kBlocks, i % kBlocks);
+    for (uint32_t i = lane; i < min(slots, kSlots) * kBlocks; i += 32) {
+        const uint32_t bits = __half_as_ushort(scales[i]) & 0x7fffu;
+        if (q4_finite(bits)) top = max(top, bits);
+        else bad(i / kBlocks, i % kBlocks);
     }
     return __reduce_max_sync(0xffffffffu, top);
 }
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 : "=r"(any) : "r"(quad + 1), "r"(128u), "r"(static_cast<uint32_t>(failed)) : "memory");
             return any != 0;
         };
-        constexpr float kFull = 16384.0f;                     // a weight of 1
+        constexpr float kFull = 14.0f;                        // a weight of 1 is 2^14: its parts are f16's normal numbers over 2^20 and more
         float acc[kOut], m = -INFINITY, l = 0.0f, shrink = 0.0f;
 #pragma unroll
         for (int i = 0; i < kOut; ++i) acc[i] = 0.0f;
@@ -320,12 +323,13 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             }
             if (meet(!ok)) { ok = false; break; }
             most = fmaxf(fmaxf(fmaxf(top[j & 1][0][r], top[j & 1][1][r]), fmaxf(top[j & 1][2][r], top[j & 1][3][r])), m);
-            const float from = most == -INFINITY ? 0.0f : most, f = exp2_fast(m - from);          // exp2(-inf) = 0 on the first slots
+            most = ceilf(most);                               // a whole number: neither taking it off nor 2 to it is rounded
+            const float from = most == -INFINITY ? kFull : kFull - most, f = exp2_fast(m - (kFull - from));          // exp2(-inf) = 0 on the first slots
             m = most;
             float part[4] = {};
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
-                s[i] = exp2_fast(fmaf(s[i], by, -from));
+                s[i] = exp2_fast(fmaf(s[i], by, from));
                 part[i & 3] += s[i];
             }
             l = l * f + ((part[0] + part[1]) + (part[2] + part[3]));
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 uint32_t upper[8], lower[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float a = s[2 * i] * kFull, b = s[2 * i + 1] * kFull, ua = upper_digit(a), ub = upper_digit(b);
+                    const float a = s[2 * i], b = s[2 * i + 1], ua = upper_digit(a), ub = upper_digit(b);
                     upper[i] = pack_f16(ua, ub);
                     lower[i] = pack_f16(a - ua, b - ub);
                 }
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         if (meet(!ok)) {
             gave_up(kErrTmemWaitTimeout);
         } else if (live) {
-            l = (sum[0][r] + sum[1][r]) + (sum[2][r] + sum[3][r]);
+            l = ((sum[0][r] + sum[1][r]) + (sum[2][r] + sum[3][r])) * (1.0f / 16384.0f);
             if (last_seen >= bad_key) l = NAN;
             const bool alone = p.splits == 1;
             const float inv = alone ? 1.0f / l : 1.0f;
@@ -384,17 +388,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 if (!alone || p.scores) reinterpret_cast<float2*>(p.part_stats)[part] = make_float2(m, l);
             }
         }
-    } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot; the first one keeps the ring filled
+    } else if (warp < kQpValueWarp) {                         // keys: a thread takes blocks of a slot
         constexpr uint32_t kId = (kQpValueWarp - kQpKeyWarp) * 32;
         const uint32_t id = threadIdx.x - kQpKeyWarp * 32, count = end - begin;
-        if (id == 0) {
-            asm volatile("fence.proxy.async;" ::: "memory");      // the stores of the launch before come ahead of the copies
-            for (uint32_t j = 0; j < min(count, kQpStages - 1u); ++j) bring(begin + j, j);
-        }
-        __syncwarp();
         int stage = 0;
-        uint32_t phase = 0, j = 0, brought = min(count, kQpStages - 1u);
-        for (; j < count; ++j) {
+        uint32_t phase = 0;
+        for (uint32_t j = 0; j < count; ++j) {
             const uint32_t tile = begin + j, slots = min(kQpKeys, seen - tile * kQpKeys);
             if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
             const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
@@ -406,6 +405,30 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             async_proxy_fence();
             __syncwarp();
             if (lane == 0) { mbar_arrive(&k_full[j & 1]); mbar_arrive(&raw_free[stage]); }
+            if (++stage == kQpStages) { stage = 0; phase ^= 1u; }
+        }
+    } else if (warp < kQpIssueWarp) {                         // values: the same; the first thread keeps the ring filled, ahead of what the warp has to wait for
+        constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32;
+        const uint32_t id = threadIdx.x - kQpValueWarp * 32, count = end - begin;
+        if (id == 0) {
+            asm volatile("fence.proxy.async;" ::: "memory");      // the stores of the launch before come ahead of the copies
+            for (uint32_t j = 0; j < min(count, kQpStages - 1u); ++j) bring(begin + j, j);
+        }
+        __syncwarp();
+        int stage = 0;
+        uint32_t phase = 0, j = 0, brought = min(count, kQpStages - 1u);
+        for (; j < count; ++j) {
+            const uint32_t tile = begin + j, slots = min(kQpKeys, seen - tile * kQpKeys);
+            if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
+            const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
+            const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes + kScales);
+            const int shift = q4_shift(q4_largest_scale<kBlocks, kQpKeys>(scales, slots, lane, [&](uint32_t r, uint32_t block) { atomicMin(&bad_value[block], tile * kQpKeys + r); }));
+            if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
+            q4_unpack_tile<kBlocks, kQpKeys, kId>(raw + kCodes, scales, slots, shift, v_smem + (j & 1) * 2 * kKPlane, id);
+            if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&v_full[j & 1]); mbar_arrive(&raw_free[stage]); }
             if (id == 0 && j + kQpStages - 1 < count) {           // the stage of the tile before, once the values' warps are done with it as well
                 const uint32_t to_stage = (j + kQpStages - 1) % kQpStages;
                 if (j == 0 || mbar_wait(&raw_free[to_stage], ((j - 1) / kQpStages) & 1u)) {
@@ -420,25 +443,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         }
         if (id == 0)                                              // given up: what is under way lands before the memory is another's
             for (; j < brought; ++j) mbar_wait(&raw_full[j % kQpStages], (j / kQpStages) & 1u);
-    } else if (warp < kQpIssueWarp) {                         // values: the same
-        constexpr uint32_t kId = (kQpIssueWarp - kQpValueWarp) * 32;
-        const uint32_t id = threadIdx.x - kQpValueWarp * 32, count = end - begin;
-        int stage = 0;
-        uint32_t phase = 0;
-        for (uint32_t j = 0; j < count; ++j) {
-            const uint32_t tile = begin + j, slots = min(kQpKeys, seen - tile * kQpKeys);
-            if (!warp_waited(&raw_full[stage], phase)) { gave_up(kErrFullWaitTimeout); break; }
-            const uint8_t* const raw = raw_smem + stage * kQpRaw<kBlocks>;
-            const __half* const scales = reinterpret_cast<const __half*>(raw + 2 * kCodes + kScales);
-            const int shift = q4_shift(q4_largest_scale<kBlocks, kQpKeys>(scales, slots, lane, [&](uint32_t r, uint32_t block) { atomicMin(&bad_value[block], tile * kQpKeys + r); }));
-            if (j > 1 && !warp_waited(&v_free[j & 1], ((j >> 1) - 1) & 1)) { gave_up(kErrEmptyWaitTimeout); break; }
-            q4_unpack_tile<kBlocks, kQpKeys, kId>(raw + kCodes, scales, slots, shift, v_smem + (j & 1) * 2 * kKPlane, id);
-            if (id == 0) v_unit[j & 3] = power_of_two(-shift) * (1.0f / 16384.0f);      // a weight of 1 is 2^14
-            async_proxy_fence();
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(&v_full[j & 1]); mbar_arrive(&raw_free[stage]); }
-            if (++stage == kQpStages) { stage = 0; phase ^= 1u; }
-        }
     } else if (lane == 0) {                                   // the tensor cores
         constexpr uint32_t score_desc = umma_idesc_f16(kQpRows, kQpKeys), out_desc = umma_idesc_f16(kQpRows, kDim, true), kSteps = kDim / 16;
         const uint64_t k_desc = umma_desc_k_sw128(smem_u32(k_smem)), v_desc = umma_desc_mn_sw128(smem_u32(v_smem), kKPlane / kHalves);
