@@ -139,20 +139,20 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
             p.weight_out[at] = share[threadIdx.x] + (slot < filled ? p.weight_in[at] : 0.0f);
         }
     } else if (warp < kQrCopyWarp) {
-        if (lane == 0) {
-            const uint32_t b = warp - kQrIssueWarp;           // the accumulators' buffer: units b, b + 2, ..
-            constexpr uint32_t desc = umma_idesc_f16(kQrSlots, kQpRows);
-            const uint64_t k_desc = umma_desc_k_sw128(smem_u32(k_smem)), q_desc = umma_desc_k_sw128(smem_u32(q_smem));
-            bool ok = true;
-            for (uint32_t u = b; ok && u < units; u += 2) {
-                const uint32_t set = u % sets;
-                ok = u < 2 || mbar_wait(&s_free[b], ((u >> 1) - 1) & 1u);
-                for (uint32_t c = 0; ok && c < kHalves; ++c) {
-                    const uint32_t chunk = u / sets * kHalves + c, stage = chunk % kQrStages;
-                    ok = mbar_wait(&q_full[stage], (chunk / kQrStages) & 1u);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    const uint64_t k_at = k_desc + ((set * 2 * kPlane + c * (kPlane / kHalves)) >> 4), q_at = q_desc + (stage * 2 * kQrChunk >> 4);
+        constexpr uint32_t desc = umma_idesc_f16(kQrSlots, kQpRows);
+        const uint32_t b = warp - kQrIssueWarp;               // the accumulators' buffer: units b, b + 2, ..
+        const uint64_t k_desc = umma_desc_k_sw128(smem_u32(k_smem)), q_desc = umma_desc_k_sw128(smem_u32(q_smem));
+        bool ok = true;
+        for (uint32_t u = b; ok && u < units; u += 2) {
+            const uint32_t set = u % sets;
+            ok = u < 2 || warp_waited(&s_free[b], ((u >> 1) - 1) & 1u);
+            for (uint32_t c = 0; ok && c < kHalves; ++c) {
+                const uint32_t chunk = u / sets * kHalves + c, stage = chunk % kQrStages;
+                ok = warp_waited(&q_full[stage], (chunk / kQrStages) & 1u);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint64_t k_at = k_desc + ((set * 2 * kPlane + c * (kPlane / kHalves)) >> 4), q_at = q_desc + (stage * 2 * kQrChunk >> 4);
+                if (elected()) {
 #pragma unroll
                     for (uint32_t i = 0; i < 3; ++i) {        // lower times upper, upper times lower, upper times upper
                         const uint32_t kp = i == 0 ? 1 : 0, qp = i == 1 ? 1 : 0;
@@ -161,12 +161,12 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
                             tc_mma_f16(tmem + b * kScores + c * kQpRows, k_at + (kp * kPlane >> 4) + 2 * k, q_at + (qp * kQrChunk >> 4) + 2 * k, desc, (i | k) > 0);
                     }
                     tc_commit(&q_free[stage]);
+                    if (c + 1 == kHalves) tc_commit(&s_full[b]);
                 }
-                if (!ok) break;
-                tc_commit(&s_full[b]);
+                __syncwarp();
             }
-            if (!ok) atomicExch(p.error_word, kErrFullWaitTimeout);
         }
+        if (!ok) gave_up(kErrFullWaitTimeout);
     } else if (lane == 0) {                                   // copies, a stage each 64 dimensions of a tile
         const uint32_t count = (row_tiles - first_tile) * kHalves;
         const uint8_t* const from = reinterpret_cast<const uint8_t*>(p.queries) + (static_cast<size_t>(h) * row_tiles + first_tile) * 2 * kQpQPlane<kBlocks>;
