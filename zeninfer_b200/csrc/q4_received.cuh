@@ -76,17 +76,23 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
         const uint32_t quad = warp & 3u, part = warp >> 2;
         float sum[kQrSets] = {};
         const float unit = power_of_two(-shift);
+        // what a tile's row has, asked for a tile ahead; rows that are none: weights of zero
+        auto ask = [&](uint32_t tile) {
+            float2 its = make_float2(0.0f, INFINITY);
+            if (tile < row_tiles && threadIdx.x < kQpRows && tile * kQpRows + threadIdx.x < rows) {
+                its.x = __ldcg(p.factors + (static_cast<size_t>(h) * row_tiles + tile) * kQpRows + threadIdx.x);
+                its.y = __ldcg(p.stats + static_cast<size_t>(h) * rows + tile * kQpRows + threadIdx.x);
+            }
+            return its;
+        };
+        float2 next = ask(first_tile);
         bool ok = true;
         for (uint32_t u = 0; u < units; ++u) {
             const uint32_t tile = first_tile + u / sets, set = u % sets, b = u & 1u, row0 = tile * kQpRows;
             if (set == 0) {
-                float2 its = make_float2(0.0f, INFINITY);     // rows that are none: weights of zero
-                if (threadIdx.x < kQpRows && row0 + threadIdx.x < rows) {
-                    its.x = __ldcg(p.factors + (static_cast<size_t>(h) * row_tiles + tile) * kQpRows + threadIdx.x) * unit;
-                    its.y = __ldcg(p.stats + static_cast<size_t>(h) * rows + row0 + threadIdx.x);
-                }
                 if (meet(!ok)) { ok = false; break; }         // the tile before is done with the place
-                if (threadIdx.x < kQpRows) of_row[threadIdx.x] = its;
+                if (threadIdx.x < kQpRows) of_row[threadIdx.x] = make_float2(next.x * unit, next.y);
+                next = ask(tile + 1);
                 meet(false);
             }
             ok = ok && warp_waited(&s_full[b], (u >> 1) & 1u);
@@ -95,31 +101,38 @@ __global__ void __launch_bounds__(kQrThreads, 1) q4_received_kernel(const __grid
                 const uint32_t slot = cta_slot + set * kQrSlots + quad * 32 + lane, from = tmem + b * kScores + part * 32 + ((quad * 32) << 16);
                 // the columns from here on see the slot
                 const uint32_t sees = slot < filled ? 0u : (slot - filled) * p.group, column0 = row0 + part * 32;
-                const bool all = __all_sync(0xffffffffu, sees <= column0);
                 float added[4] = {};
+                uint32_t share[2][kHalves][16];
+                auto load = [&](int c) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t share[kHalves][16];
-#pragma unroll
-                    for (uint32_t i = 0; i < kHalves; ++i) tmem_ld_32x16(from + i * kQpRows + 16 * c, share[i]);
-                    tmem_ld_wait();
-                    if (c == 1) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&s_free[b]);
-                    }
+                    for (uint32_t i = 0; i < kHalves; ++i) tmem_ld_32x16(from + i * kQpRows + 16 * c, share[c][i]);
+                };
+                auto add = [&](int c, auto all) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float4 two = reinterpret_cast<const float4*>(of_row)[(part * 32 + 16 * c + i) / 2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float s = __uint_as_float(share[0][i + e]);
-                            if (kHalves > 1) s += __uint_as_float(share[kHalves - 1][i + e]);
+                            float s = __uint_as_float(share[c][0][i + e]);
+                            if (kHalves > 1) s += __uint_as_float(share[c][kHalves - 1][i + e]);
                             const float w = exp2_fast(e ? fmaf(s, two.z, -two.w) : fmaf(s, two.x, -two.y));
-                            if (all || column0 + 16 * c + i + e >= sees) added[(i + e) & 3] += w;
+                            if (decltype(all)::value || column0 + 16 * c + i + e >= sees) added[(i + e) & 3] += w;
                         }
                     }
-                }
+                };
+                auto work = [&](auto all) {
+                    load(0);
+                    tmem_ld_wait();
+                    load(1);
+                    add(0, all);
+                    tmem_ld_wait();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[b]);
+                    add(1, all);
+                };
+                if (__all_sync(0xffffffffu, sees <= column0)) work(std::true_type{});
+                else work(std::false_type{});
                 const float both = (added[0] + added[1]) + (added[2] + added[3]);
                 if (set == 0) sum[0] += both;
                 else sum[1] += both;
