@@ -184,6 +184,10 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     const uint32_t begin = blockIdx.x * runs.per, end = min(runs.tiles, begin + runs.per);
     if (begin >= end) return;                                                            // nobody counts on this run
     if (warp == kQpIssueWarp) tmem_alloc(&tmem_slot, kQpColumns);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot;
     constexpr uint32_t kCodes = kQpKeys * kBlocks * 16, kScales = kQpKeys * kBlocks * 2;
     auto bring = [&](uint32_t tile, int stage) {              // the last tile may have half of its slots beyond the cache's end
         const uint32_t slots = min(kQpKeys, p.cache.slots - tile * kQpKeys);
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         bulk_g2s(to + 2 * kCodes, p.cache.k_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
         bulk_g2s(to + 2 * kCodes + kScales, p.cache.v_scales + slot * kBlocks, slots * kBlocks * 2, &raw_full[stage]);
     };
-    if (warp < kQpKeyWarp) {      // Q: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
+    if (warp < kQpKeyWarp) {      // Q, while the other warps begin with the tiles: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
         constexpr uint32_t kChunks = kDim / 8, kRowThreads = kQpKeyWarp * 32, kEach = kQpRows * kChunks / kRowThreads;
         const uint32_t chunk = threadIdx.x % kChunks, dim = chunk / 4 * 32 + chunk % 4 * 4;
         const bool fours = q4_rotates_fours(p.q, p.q_ld, kDim, p.turn);
@@ -236,24 +240,19 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
                 if (chunk == 0) p.factors[static_cast<size_t>(h) * gridDim.y * kQpRows + first_row + r] = row_factor[r];
             }
         }
-        async_proxy_fence();
-    }
-    tc_fence_before_sync();
-    __syncthreads();
-    tc_fence_after_sync();
-    const uint32_t tmem = tmem_slot;
-    if (warp < kQpKeyWarp) {                                  // the queries into TMEM, half a row's part a thread: the products then read keys only from shared memory
+        // and into TMEM, half a row's part a thread: the products then read keys only from shared memory
+        asm volatile("barrier.sync 9, %0;" ::"n"(kQpKeyWarp * 32) : "memory");
         const uint32_t r = (warp & 3u) * 32 + lane, plane = warp >> 3, c0 = (warp >> 2 & 1u) * (kDim / 32);
 #pragma unroll
-        for (uint32_t c = c0; c < c0 + kDim / 32; ++c) {
+        for (uint32_t c = 0; c < kDim / 32; ++c) {
             uint32_t both[8];
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
-                const uint32_t chunk = 2 * c + i;
+                const uint32_t chunk = 2 * (c0 + c) + i;
                 const uint4 its = *reinterpret_cast<const uint4*>(q_smem + plane * kQPlane + (chunk / 8) * (kQPlane / kHalves) + r * 128 + (((chunk % 8) ^ (r & 7)) << 4));
                 both[4 * i] = its.x; both[4 * i + 1] = its.y; both[4 * i + 2] = its.z; both[4 * i + 3] = its.w;
             }
-            tmem_st_32x8(tmem + kQpQ + plane * (kDim / 2) + 8 * c + (((warp & 3u) * 32) << 16), both);
+            tmem_st_32x8(tmem + kQpQ + plane * (kDim / 2) + 8 * (c0 + c) + (((warp & 3u) * 32) << 16), both);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     // A wait that runs out ends its role's loop, and the others' follow.
     if (warp < kQpKeyWarp) {                                  // rows
         const uint32_t quad = warp & 3, quarter = warp >> 2, r = quad * 32 + lane, row = first_row + r, lane_base = (quad * 32) << 16;
-        const bool live = r < real_rows;
+        const bool live = r < real_rows, any_live = quad * 32 < real_rows;      // warps without rows arrive where the others do, and leave TMEM as it is
         const uint32_t last_seen = live ? filled + row / p.group : 0xffffffffu;          // rows that are none: whatever comes, they write nothing
         constexpr int kMine = kQpKeys / 4, kOut = kDim / 4;
         const float factor = row_factor[r];
@@ -297,6 +296,16 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
         for (uint32_t tile = begin; tile < end; ++tile, ++j) {
             ok = ok && warp_waited(&s_full, j & 1);
             float s[kMine], most = -INFINITY, by = 0.0f;
+            if (!any_live) {
+                if (ok && j > 0) ok = warp_waited(&o_full, (j - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_arrive(&s_empty);
+                    mbar_arrive(&p_full);
+                    if (j > 0) mbar_arrive(&o_empty);
+                }
+                continue;
+            }
             if (ok) {
                 tc_fence_after_sync();
 #pragma unroll
@@ -361,7 +370,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             shrink = f;
         }
         if (ok) ok = warp_waited(&o_full, (j - 1) & 1);
-        if (ok) { tc_fence_after_sync(); take_output(v_unit[(j - 1) & 3]); }
+        if (ok && any_live) { tc_fence_after_sync(); take_output(v_unit[(j - 1) & 3]); }
         sum[quarter][r] = l;
         if (meet(!ok)) {
             gave_up(kErrTmemWaitTimeout);

@@ -237,8 +237,8 @@ int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, 
     if (!e.leave(r, "dev_q4_attention")) return 0;
     const bool join = plan.splits > 1 || digits;
     if (join || plan.keep_scores) {
-        uint32_t parts = 1;
-        while (parts < zk::kQ4FinishWarps && parts < plan.splits) parts *= 2;
+        uint32_t parts = 1;      // warps of a row, while all of them are on the SMs at once: 5328 rows of three runs take 10 us with one, 21 with four
+        while (parts < zk::kQ4FinishWarps && parts < plan.splits && size_t(plan.rows) * cache.kv_heads * parts * 2 <= kSms * 64) parts *= 2;
         const uint32_t a_cta = zk::kQ4FinishWarps / parts, join_ctas = join ? (plan.rows + a_cta - 1) / a_cta : 0;
         const uint32_t slot_ctas = plan.keep_scores ? (cache.slots + zk::kQ4FinishWarps * 32 - 1) / (zk::kQ4FinishWarps * 32) : 0;
         if (!e.leave(launch(e, zk::q4_finish_kernel, dim3(join_ctas + slot_ctas, cache.kv_heads), dim3(zk::kQ4FinishWarps * 32), 0, 0, p, plan.cta_rows, plan.key_warps, parts, join_ctas),
