@@ -73,7 +73,10 @@ zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
 
 constexpr size_t kSms = 148, kWaveCtas = 2 * kSms;
 constexpr size_t kReceivedSingle = kSms;   // 128 slots a CTA of q4_received.cuh up to so many
-constexpr size_t kPromptRows = 8;          // above: q4_prompt.cuh, for the heads it takes
+constexpr size_t kOneRun = 8, kOneRunRows = 1024;      // tiles of a cache that q4_prompt.cuh does not split for more than so many rows of all kv heads
+// Above so many rows of a kv head: q4_prompt.cuh, whose time hardly depends on them.  Heads of 128, 12 rows: 39 us by q4_attention.cuh and 50 by q4_prompt.cuh at 20000 slots, 20 rows:
+// 56 and 50 (31 and 26 at 4003); heads of 64, 17 rows: 56 and 68, 24 rows: 23.4 and 23.2.
+constexpr size_t prompt_rows(size_t blocks) { return blocks == 2 ? 24 : 16; }
 
 // How a call is cut up, from its sizes alone: how many slots are filled is known on the device only.
 struct AttentionPlan {
@@ -88,12 +91,14 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     const size_t kv_heads = a->cache.kv_heads, rows = tokens * (a->heads / kv_heads), blocks = a->cache.head_dim / zk::kQ4Block, tiles = a->cache.slots / zk::kQ4Tile;
     if (tokens * a->heads > 0x1fffffffu / blocks) return n;      // what a launch counts in 32 bits
     n.columns = rows <= 4 ? zk::kQ4Digits : rows <= 8 || blocks > 4 ? zk::kQ4Rows8 : zk::kQ4Rows16;
-    if ((blocks == 2 || blocks == 4) && rows > kPromptRows) {
+    if ((blocks == 2 || blocks == 4) && rows > prompt_rows(blocks)) {
         const size_t row_tiles = (rows + zk::kQpRows - 1) / zk::kQpRows, key_tiles = (a->cache.slots + zk::kQpKeys - 1) / zk::kQpKeys;
         if (row_tiles > 65535) return n;
         n.columns = zk::kQ4Prompt;
         n.rows = u32(rows); n.cta_rows = zk::kQpRows; n.row_ctas = u32(row_tiles); n.padded = u32(row_tiles * zk::kQpRows); n.key_warps = 1; n.run_tile = zk::kQpKeys;
-        n.splits = u32(std::max<size_t>(1, std::min(kSms / (row_tiles * kv_heads), key_tiles)));
+        // runs side by side until every SM has its CTA; a few tiles of many rows are one run, for joining many rows costs more than that saves (333 tokens of 16 heads, 7 tiles:
+        // 34.4 us in one run, 37.5 in three; but 3 tokens of 32 heads, 8 tiles: 25.2 us in one, 18.0 in eight)
+        n.splits = key_tiles <= kOneRun && rows * kv_heads > kOneRunRows ? 1u : u32(std::max<size_t>(1, std::min(kSms / (row_tiles * kv_heads), key_tiles)));
         n.keep_scores = a->weight_out && rows <= zk::kQ4KeptRows;
         size_t at = 0;
         auto take = [&](size_t bytes) { const size_t mine = at; at += up16(bytes); return mine; };
