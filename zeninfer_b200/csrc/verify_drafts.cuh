@@ -70,6 +70,21 @@ struct VerifyShare {
 // The integer nearest to x, 0 <= x <= 2^51: what is left of 2^52 + x in its lower bits.
 __device__ __forceinline__ unsigned long long nearest(double x) { return static_cast<unsigned long long>(__double_as_longlong(x + 4503599627370496.0)) & 0xfffffffffffffull; }
 
+// e^y for y <= 0, given 2^(j / 64) for j = 0 .. 63: y = n ln 2 / 64 + r with |r| < 0.0055, whose series up to r^5 / 120 leaves out less than 2^-54.  About half of the double-precision
+// instructions of exp.
+constexpr uint32_t kVerifyPowers = 64;
+__device__ __forceinline__ double verify_exp(double y, const double* powers) {
+    if (y < -700.0) return exp(y);
+    constexpr double kRound = 6755399441055744.0;             // 1.5 * 2^52: a sum with it has the nearest whole number in its lower bits
+    constexpr double kUpper = 0x1.62e42ffp-7, kRest = -0x1.718432a1b0e26p-41;                // ln 2 / 64 = kUpper + kRest; n * kUpper is exact
+    const double shifted = fma(y, 92.33248261689366, kRound), n = shifted - kRound;          // 64 / ln 2
+    const int whole = __double2loint(shifted);
+    const double r = fma(-n, kRest, fma(-n, kUpper, y));
+    const double s = fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0);
+    const double of = powers[whole & 63], e = fma(of, r * s, of);
+    return __hiloint2double(__double2hiint(e) + ((whole >> 6) << 20), __double2loint(e));
+}
+
 template <int kCtas>
 __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
     namespace cg = cooperative_groups;
@@ -78,7 +93,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     __shared__ double warp_sum[32], s_q;
     __shared__ unsigned long long warp_total[32], s_left;
     __shared__ uint32_t warp_high[32], warp_low[32], warp_count[32], s_bin, s_mine, s_high, s_low, s_count, s_before, s_fits;
-    __shared__ double s_sum, s_ahead, s_scale;
+    __shared__ double s_sum, s_ahead, s_scale, powers[kVerifyPowers];
+    __shared__ unsigned long long groups[32];          // totals of 32 bins each
     __shared__ int s_last;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), row = blockIdx.y;
@@ -92,6 +108,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     // a thread's run of consecutive entries, for sums in order of id (an odd number of them: no two lanes of a warp on one bank)
     const uint32_t per_thread = ((p.per_cta + kVerifyThreads - 1) / kVerifyThreads) | 1u, begin = min(n, tid * per_thread), end = min(n, begin + per_thread);
     pdl_launch_dependents();
+    if (tid < kVerifyPowers) powers[tid] = exp2(tid / 64.0);
     pdl_wait();
     const float* logits = p.logits + row * p.logits_ld + base;
     const bool is_draft = row < p.drafts;
@@ -209,19 +226,28 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
             for (uint32_t i = tid; i < kVerifyLimbs * kVerifyBins; i += kVerifyThreads) limbs[i] = 0;
             if (tid == 0) { s_bin = 0xffffffffu; s_mine = 0; }
             __syncthreads();
-#pragma unroll 4
-            for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-                const float x = v[i];
-                const uint32_t key = sample_key(x);
-                if (!key || key > high || key < low) continue;
-                const unsigned long long w = weigh(i);
-                const uint32_t bin = bin_of(x);
+            uint32_t bins[kVerifyRun / kVerifyThreads / 2];   // of the thread's entries, two a word; kVerifyBins: it goes whatever the border is, kNone: it stays, or is gone
+            constexpr uint32_t kNone = 0xffff;
 #pragma unroll
-                for (int k = 0; k < kVerifyLimbs; ++k) {
-                    uint32_t limb = static_cast<uint32_t>(w >> (k * kVerifyLimbBits));
-                    if (k + 1 < kVerifyLimbs) limb &= (1u << kVerifyLimbBits) - 1u;          // an entry may be all of the row: 2^51
-                    if (limb) atomicAdd(limbs + k * kVerifyBins + bin, limb);
+            for (uint32_t j = 0; j < kVerifyRun / kVerifyThreads; ++j) {
+                const uint32_t i = tid + j * kVerifyThreads;
+                uint32_t bin = kNone;
+                if (i < n) {
+                    const float x = v[i];
+                    const uint32_t key = sample_key(x);
+                    if (key && key < low) bin = kVerifyBins;
+                    else if (key && key <= high) {
+                        const unsigned long long w = weigh(i);
+                        bin = bin_of(x);
+#pragma unroll
+                        for (int k = 0; k < kVerifyLimbs; ++k) {
+                            uint32_t limb = static_cast<uint32_t>(w >> (k * kVerifyLimbBits));
+                            if (k + 1 < kVerifyLimbs) limb &= (1u << kVerifyLimbBits) - 1u;          // an entry may be all of the row: 2^51
+                            if (limb) atomicAdd(limbs + k * kVerifyBins + bin, limb);
+                        }
+                    }
                 }
+                bins[j / 2] = j % 2 ? bins[j / 2] | bin << 16 : bin;
             }
             __syncthreads();
             unsigned long long mine = 0;
@@ -229,40 +255,52 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
             for (int k = 0; k < kVerifyLimbs; ++k) mine += static_cast<unsigned long long>(limbs[k * kVerifyBins + tid]) << (k * kVerifyLimbBits);
             __syncthreads();
             totals[tid] = mine;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+            if (lane == 0) groups[warp] = mine;
             cluster.sync();
-            // thread j has bin j of the whole row
-            mine = 0;
+            // the border among the row's groups of 32 bins, and then among the bins of one: distributed shared memory gives some ten bytes a clock, so few are read
+            if (warp == 0) {
+                auto reached = [&](unsigned long long sum, unsigned long long from, unsigned long long& left) {      // the lane at which sums reach `from`, or 32; what is left there
+                    unsigned long long upto = sum;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (static_cast<int>(lane) >= o) upto += x;
+                    }
+                    const int at = __ffs(__ballot_sync(0xffffffffu, upto >= from)) - 1;
+                    left = from - __shfl_sync(0xffffffffu, upto - sum, at & 31);
+                    return at < 0 ? 32 : at;
+                };
+                unsigned long long sum = 0, left = 0;
 #pragma unroll
-            for (int r = 0; r < kCtas; ++r) mine += cluster.map_shared_rank(totals, r)[tid];
-            unsigned long long upto = mine;
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (static_cast<int>(lane) >= o) upto += x;
+                for (int r = 0; r < kCtas; ++r) sum += cluster.map_shared_rank(groups, r)[lane];
+                const int group = reached(sum, wanted, left);
+                if (group < 32) {
+                    sum = 0;
+#pragma unroll
+                    for (int r = 0; r < kCtas; ++r) sum += cluster.map_shared_rank(totals, r)[32 * group + lane];
+                    const int at = reached(sum, left, left);
+                    if (lane == 0) { s_bin = 32 * group + at; s_left = left; }
+                }
             }
-            if (lane == 31) warp_total[warp] = upto;
-            __syncthreads();
-            unsigned long long before = lane < warp ? warp_total[lane] : 0ull;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-            upto += before;
-            if (upto >= wanted && upto - mine < wanted) { s_bin = tid; s_left = wanted - (upto - mine); }        // one thread at most
             __syncthreads();
             const uint32_t border = s_bin;                  // none: rounding left the whole short of what is wanted, and everything stays
             if (border != 0xffffffffu) wanted = s_left;
             // what lies below the border goes; the entries of its bin are listed, and counted on where there are too many
             uint32_t bin_high = 0, bin_low = 0xffffffffu, unused = 0;
-#pragma unroll 4
-            for (uint32_t i = tid; i < n; i += kVerifyThreads) {
-                const float x = v[i];
-                const uint32_t key = sample_key(x);
-                if (!key || key > high) continue;
-                const uint32_t bin = key < low ? kVerifyBins : bin_of(x);
-                if (bin > border || key < low) drop(i);
-                else if (bin == border) {
+#pragma unroll
+            for (uint32_t j = 0; j < kVerifyRun / kVerifyThreads; ++j) {
+                const uint32_t i = tid + j * kVerifyThreads, bin = j % 2 ? bins[j / 2] >> 16 : bins[j / 2] & 0xffffu;
+                if (bin == kNone) continue;
+                if (bin == border) {
+                    const float x = v[i];
+                    const uint32_t key = sample_key(x);
                     bin_high = max(bin_high, key);
                     bin_low = min(bin_low, key);
                     const uint32_t at = atomicAdd(&s_mine, 1u);
                     if (at < kVerifyMine) own_list[at] = VerifyEntry{weigh(i), x, base + i};
+                } else if (bin > border || bin == kVerifyBins) {
+                    drop(i);
                 }
             }
             cta_range(bin_high, bin_low, unused);
@@ -330,7 +368,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
 #pragma unroll 4
     for (uint32_t i = begin; i < end; ++i) {
         const float x = v[i];
-        const double w = sample_key(x) ? exp((static_cast<double>(x) - reference) * per_unit) : 0.0;
+        const double w = sample_key(x) ? verify_exp((static_cast<double>(x) - reference) * per_unit, powers) : 0.0;
         e[i] = w;
         mine += w;
     }
