@@ -142,7 +142,8 @@ __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
 //   into another cache   a CTA moves the places it knows: an eighth of them, or what stays of its own run
 //   in place             all move together in rounds, all of a round read before any of it is written: a slot never moves up, so what a round overwrites lies in front of what
 //                        later rounds read
-// What bounds it: the moved bytes (read and written once) for large caches, round trips and barriers for small ones.
+// What bounds it: three passes of select with four cluster barriers each, and the moved bytes (pieces of 16 bytes out of lines of 128) for large caches; round trips and barriers
+// for small ones.  8 kv heads of 128: 76 of 1100 dropped in 8.2 us, 57309 of 65501 in 29 us (the bytes alone: 3.3).
 constexpr int kEvictThreads = 1024, kEvictCtas = 8, kEvictPieces = 4, kEvictHeld = 8;      // pieces of a thread in a round; weights of a thread in registers
 constexpr uint32_t kEvictBins = 2048, kEvictSolo = kEvictThreads * kEvictHeld, kEvictListed = 8192;      // places a CTA lists in shared memory
 

@@ -7,8 +7,9 @@
 // A CTA keeps 128 or 256 slots unpacked in shared memory and walks the tiles of 128 rows; a stage of its ring is 64 dimensions of a tile's two parts.  With 256 slots a
 // tile that comes out of L2 serves two matrices, which alternate between the accumulators' two buffers: 16 warps exponentiate one while the other is formed.  Each 64
 // dimensions have an accumulator of their own, corrections first.  Two warps issue the products, a unit each in turn: what one spends on waits and commits the other fills, for
-// the tensor cores take an instruction only when they are done with the one before.  Bounded by the tensor cores: a product of 128 x 128 x 16 takes 70 cycles with both operands in shared
-// memory (64 at their full rate).
+// the tensor cores take an instruction only when they are done with the one before.  Bounded by the shared memory: a product of 128 x 128 x 16 reads 8 KB there (64 cycles, what it takes
+// on the tensor cores), and the copies and the rows' factors need the rest of some 95 cycles.  512 tokens at 8192 slots of 8 kv heads of 128: 105 us, 0.6 of the rate three products could
+// have; 131 with 128 slots a CTA, 381 with mma.sync.
 #pragma once
 #include "q4_prompt.cuh"
 

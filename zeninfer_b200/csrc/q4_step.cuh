@@ -7,6 +7,8 @@
 //   kCluster    the CTAs of a kv head are a cluster (up to eight): their sums meet through distributed shared memory, the scores stay in shared memory, and what the
 //               slots received is added before the launch ends
 //   else        runs of slots on all SMs; q4_finish_kernel puts them together
+// What bounds it: round trips and cluster barriers up to some thousand slots (5.7 us at 20 slots of 2 kv heads of 64, 8.6 at 1000 of 8 of 128 with weights, of which a launch is 3); the
+// instructions of a tile beyond (29.5 us at 65501 slots, 2.6 TB/s of codes and scales; the bytes alone would be 11.6).
 #pragma once
 #include <cooperative_groups.h>
 

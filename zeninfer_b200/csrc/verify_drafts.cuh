@@ -14,7 +14,8 @@
 // takes, and the entries of the list are compared with each other, equal values by id.  A mass is an integer, the exponential's 2^-51ths of the
 // row's sum, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
 // added in a fixed order.
-// What bounds it: the double-precision instructions of exp, and a dozen cluster barriers.
+// What bounds it: passes over the CTA's 16 entries a thread (load, exponentials, histogram, cut, two sums: 2 to 7 thousand cycles each) and a dozen cluster barriers of some 1500.
+// 9 rows of 128256, top-p: 31 us, 5 rows, top-k 40 and top-p: 34 us, 3 rows of 32000, no cut: 10.9 us; clusters of 16 CTAs take 63, 47 and 10.4, for eight of them fit the GPU at a time.
 #pragma once
 #include <cooperative_groups.h>
 

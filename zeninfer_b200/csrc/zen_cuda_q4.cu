@@ -72,7 +72,8 @@ zk::Q4Cache device_form(const zen_cuda_q4_cache& c) {
 }
 
 constexpr size_t kSms = 148, kWaveCtas = 2 * kSms;
-constexpr size_t kReceivedSingle = kSms;   // 128 slots a CTA of q4_received.cuh up to so many
+// 128 slots a CTA of q4_received.cuh up to one CTA an SM, 256 above: a tile of rows out of L2 then serves both (8192 slots of 8 kv heads: 111 us, 131 with 128).
+constexpr size_t kReceivedSingle = kSms;
 constexpr size_t kOneRun = 8, kOneRunRows = 1024;      // tiles of a cache that q4_prompt.cuh does not split for more than so many rows of all kv heads
 // Above so many rows of a kv head: q4_prompt.cuh, whose time hardly depends on them.  Heads of 128, 12 rows: 39 us by q4_attention.cuh and 50 by q4_prompt.cuh at 20000 slots, 20 rows:
 // 56 and 50 (31 and 26 at 4003); heads of 64, 17 rows: 56 and 68, 24 rows: 23.4 and 23.2.
