@@ -136,14 +136,14 @@ __device__ __forceinline__ Q4Quantised q4_quantise(float x, uint32_t lane) {
 //
 // A cluster of eight CTAs takes a kv head.  Up to kEvictSolo slots every CTA chooses for itself, for an exchange costs more than the work it saves; above, each
 // has a run of the slots, each warp a run of the CTA's.  The weight of the last slot that stays is found by a radix select over order-preserving keys, three
-// passes of 11, 11 and 10 bits.  In a cluster a CTA adds up an eighth of the bins of all CTAs (distributed shared memory gives some ten bytes a
-// clock: reading all bins of all CTAs took 7000 clocks a pass), and the one that has the border tells the others.  Then every warp counts what stays of its run, and a prefix over CTAs and
+// passes of 11, 11 and 10 bits.  In a cluster every CTA reads the others' sums of 32 bins, and then the bins of the one sum that has the border (distributed shared memory gives some ten
+// bytes a clock: reading all bins of all CTAs took 7000 clocks a pass); bins and sums have two places in turn, so that a pass is one barrier of the cluster.  Then every warp counts what stays of its run, and a prefix over CTAs and
 // warps gives each kept slot its place: the choice and the order are the same in every run.
 //   into another cache   a CTA moves the places it knows: an eighth of them, or what stays of its own run
 //   in place             all move together in rounds, all of a round read before any of it is written: a slot never moves up, so what a round overwrites lies in front of what
 //                        later rounds read
-// What bounds it: three passes of select with four cluster barriers each, and the moved bytes (pieces of 16 bytes out of lines of 128) for large caches; round trips and barriers
-// for small ones.  8 kv heads of 128: 76 of 1100 dropped in 8.2 us, 57309 of 65501 in 29 us (the bytes alone: 3.3).
+// What bounds it: the chain of three select passes, counting and listing, and the moved bytes (pieces of 16 bytes out of lines of 128) for large caches; round trips and barriers
+// for small ones.  8 kv heads of 128: 76 of 1100 dropped in 8.2 us, 57309 of 65501 in 27 us (the bytes alone: 3.3).
 constexpr int kEvictThreads = 1024, kEvictCtas = 8, kEvictPieces = 4, kEvictHeld = 8;      // pieces of a thread in a round; weights of a thread in registers
 constexpr uint32_t kEvictBins = 2048, kEvictSolo = kEvictThreads * kEvictHeld, kEvictListed = 8192;      // places a CTA lists in shared memory
 
@@ -167,16 +167,16 @@ __device__ __forceinline__ uint32_t evict_key(float w) {
 
 __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThreads) q4_evict_kernel(const __grid_constant__ Q4Evict p) {
     namespace cg = cooperative_groups;
-    constexpr uint32_t kChunk = kEvictBins / kEvictCtas;
     extern __shared__ int own_list[];                      // [kEvictListed]: the slots at the places this CTA moves
-    __shared__ uint32_t hist[kEvictBins];
+    __shared__ uint32_t hists[2][kEvictBins];
+    __shared__ __align__(8) uint32_t groups[2][kEvictBins / 32];
     __shared__ uint32_t warp_more[32], warp_ties[32];      // a warp's slots above the border, and at it
-    __shared__ uint32_t s_bin, s_left, s_before, s_ties_before, s_owner;
-    __shared__ uint32_t cta_chunk, cta_bin, cta_left, cta_more, cta_ties;      // read by the other CTAs
+    __shared__ uint32_t s_bin, s_left, s_before, s_ties_before;
+    __shared__ uint32_t cta_more, cta_ties;                // read by the other CTAs
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), h = blockIdx.y;
     pdl_launch_dependents();
-    for (uint32_t i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
+    for (uint32_t i = tid; i < 2 * kEvictBins; i += kEvictThreads) hists[0][i] = 0;
     pdl_wait();
     const int filled = *reinterpret_cast<const volatile int*>(p.filled);
     if (filled < 0 || static_cast<uint32_t>(filled) > p.from.slots) {      // the same for every CTA of the grid
@@ -205,16 +205,12 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
             run(i, i < end ? __ldcg(weight + i) : 0.0f);
         }
     };
-    // threads 0 .. warps * 32 - 1: the sum of `mine` up to and with this one
-    auto scanned = [&](uint32_t mine, uint32_t warps) {
-        uint32_t upto = mine;
+    auto lanes_upto = [&](uint32_t mine) {                 // the sum of a warp's `mine` up to and with this lane's
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (static_cast<int>(lane) >= o) upto += v;
+            const uint32_t v = __shfl_up_sync(0xffffffffu, mine, o);
+            if (static_cast<int>(lane) >= o) mine += v;
         }
-        if (lane == 31 && warp < warps) warp_more[warp] = upto;
-        __syncthreads();
-        return upto + __reduce_add_sync(0xffffffffu, lane < min(warp, warps) ? warp_more[lane] : 0u);
+        return mine;
     };
 
     // the wanted-th largest key among the competing slots, and how many that equal it stay
@@ -225,6 +221,7 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t digits = pass == 2 ? 1023u : 2047u;
+            uint32_t* const hist = hists[pass & 1];
             __syncthreads();
             each([&](uint32_t i, float w) {
                 const uint32_t key = evict_key(w);
@@ -234,44 +231,45 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
                 __syncthreads();
                 // thread t looks after bins 2047 - 2 t and 2046 - 2 t, from the largest down
                 const uint2 two = reinterpret_cast<const uint2*>(hist)[kEvictThreads - 1 - tid];
-                const uint32_t mine = two.x + two.y, upto = scanned(mine, 32);
+                const uint32_t mine = two.x + two.y;
+                uint32_t upto = lanes_upto(mine);
+                if (lane == 31) warp_more[warp] = upto;
+                __syncthreads();
+                upto += __reduce_add_sync(0xffffffffu, lane < warp ? warp_more[lane] : 0u);
                 if (upto >= remaining && upto - mine < remaining) {
                     const uint32_t left = remaining - (upto - mine);
                     s_bin = kEvictBins - 1 - 2 * tid - (two.y >= left ? 0u : 1u);
                     s_left = two.y >= left ? left : left - two.y;
                 }
             } else {
-                cluster.sync();
-                // CTA r looks after an eighth of all CTAs' bins, CTA 0 after the largest ones
-                uint32_t mine = 0;
-                const uint32_t bin = kEvictBins - 1 - rank * kChunk - tid;
-                if (tid < kChunk) {
-#pragma unroll
-                    for (uint32_t r = 0; r < kEvictCtas; ++r) mine += cluster.map_shared_rank(hist, r)[bin];
-                }
-                const uint32_t upto = scanned(mine, kChunk / 32);
-                if (tid == kChunk - 1) cta_chunk = upto;
-                cluster.sync();
-                if (warp == 0) {
-                    const uint32_t theirs = lane < kEvictCtas ? *cluster.map_shared_rank(&cta_chunk, lane) : 0u;
-                    uint32_t sum = theirs;
-                    for (int o = 1; o < 8; o <<= 1) {
-                        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-                        if (static_cast<int>(lane) >= o) sum += v;
-                    }
-                    const bool owns = lane < kEvictCtas && sum >= remaining && sum - theirs < remaining;
-                    if (owns) { s_owner = lane; s_left = remaining - (sum - theirs); }
-                }
                 __syncthreads();
-                if (s_owner == rank && tid < kChunk && upto >= s_left && upto - mine < s_left) { cta_bin = bin; cta_left = s_left - (upto - mine); }
+                const uint32_t first = __reduce_add_sync(0xffffffffu, hist[64 * warp + lane]), second = __reduce_add_sync(0xffffffffu, hist[64 * warp + 32 + lane]);
+                if (lane == 0) { groups[pass & 1][2 * warp] = first; groups[pass & 1][2 * warp + 1] = second; }
                 cluster.sync();
-                if (tid == 0) { s_bin = *cluster.map_shared_rank(&cta_bin, s_owner); s_left = *cluster.map_shared_rank(&cta_left, s_owner); }
+                if (warp == 0) {      // from the largest down: a lane has two groups, then a bin of the one with the border
+                    uint32_t x = 0, y = 0;
+#pragma unroll
+                    for (uint32_t r = 0; r < kEvictCtas; ++r) {
+                        const uint2 two = reinterpret_cast<const uint2*>(cluster.map_shared_rank(groups[pass & 1], r))[31 - lane];
+                        x += two.x;
+                        y += two.y;
+                    }
+                    uint32_t upto = lanes_upto(x + y), before = upto - x - y;
+                    const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= remaining)) - 1;      // there is one: as many compete as are wanted
+                    const uint32_t upper = before + y >= remaining;                // the lane's larger group has it
+                    const uint32_t group = __shfl_sync(0xffffffffu, 2 * (31 - lane) + upper, owner), left = remaining - __shfl_sync(0xffffffffu, upper ? before : before + y, owner);
+                    uint32_t mine = 0;
+#pragma unroll
+                    for (uint32_t r = 0; r < kEvictCtas; ++r) mine += cluster.map_shared_rank(hist, r)[32 * group + 31 - lane];
+                    upto = lanes_upto(mine);
+                    if (upto >= left && upto - mine < left) { s_bin = 32 * group + 31 - lane; s_left = left - (upto - mine); }
+                }
             }
             __syncthreads();
             prefix |= s_bin << shift;
             remaining = s_left;
             mask |= digits << shift;
-            if (pass < 2) for (uint32_t i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
+            if (pass == 1) for (uint32_t i = tid; i < kEvictBins; i += kEvictThreads) hists[0][i] = 0;      // which nobody reads behind this pass's barrier
         }
         border = prefix;
         ties_wanted = remaining;

@@ -26,7 +26,7 @@ using zk_host::Entry;
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch(const Entry& e, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, unsigned cluster, Args... args) {
-    if (smem > 32 * 1024 || cluster > 8) {      // without an opt-in a block has 48 KB, what it declares statically among them
+    if (smem > 24 * 1024 || cluster > 8) {      // without an opt-in a block has 48 KB, what it declares statically among them
         static std::unordered_map<const void*, size_t> allowed;      // what the kernels of this signature may use so far; under the Entry's lock
         auto at = allowed.find(reinterpret_cast<const void*>(kernel));
         if (at == allowed.end() || smem > at->second) {
