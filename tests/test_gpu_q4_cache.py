@@ -204,6 +204,51 @@ def test_two_calls_at_once(be):
     b.check()
 
 
+def test_two_blocks_at_once(be):
+    import torch
+    a, b = Setup(be, 100, 1900, 16, 8, 128, weights=True, seed=3), Setup(be, 150, 900, 16, 16, 64, weights=True, seed=4)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):
+        a.enqueue(sa.cuda_stream)
+        b.enqueue(sb.cuda_stream)
+    be.dev_check(sa.cuda_stream)
+    be.dev_check(sb.cuda_stream)
+    a.check()
+    b.check()
+
+
+@pytest.mark.parametrize("shape", [(1, 9, 4, 2, 64), (1, 1500, 32, 8, 128), (1, 9000, 16, 8, 64), (3, 700, 32, 8, 128), (6, 600, 12, 4, 96), (30, 900, 8, 2, 128), (64, 2100, 16, 16, 64)], ids=str)
+def test_the_error_is_that_of_32_bits(be, shape):
+    """The error of all outputs together.  Scores are about 1 and pass some twelve sums, each off by 2^-24 of them; so are weights, and twice as many roundings follow: 2^-24 * 24 is
+    below 2^-19.  Codes that entered the sums with their offset on were at 2^-18."""
+    s = Setup(be, *shape, weights=True, seed=11 + sum(shape)).run()
+    got, (out, received) = s.check(), s.expected()
+    assert np.linalg.norm(got - out) <= 2.0 ** -19 * np.linalg.norm(out)
+    w = s.t["weight_out"].cpu().numpy()[:, :received.shape[1]]
+    assert np.linalg.norm(w - received) <= 2.0 ** -19 * np.linalg.norm(received)
+
+
+@pytest.mark.parametrize("tokens,dim", [(1, 64), (5, 128), (40, 128), (40, 64)])
+def test_rows_that_begin_anywhere(be, tokens, dim):
+    """Inputs and outputs four bytes behind an aligned place: the same bits."""
+    import torch
+    s = Setup(be, tokens, 70, 8, 2, dim).run()
+    first = s.check().copy()
+    moved = {n: torch.cat([torch.zeros(1, device="cuda"), s.t[n].flatten()])[1:] for n in ("q", "k", "v", "out", "k_held", "v_held", "cos", "sin")}
+    for n, x in moved.items():
+        assert x.data_ptr() % 16 == 4
+        if n not in ("q", "k", "v", "out"):
+            setattr(s.a, {"cos": "cos_t", "sin": "sin_t"}.get(n, n), x.data_ptr())
+    moved["out"].fill_(5.0)
+    moved["k_held"].fill_(5.0)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    be.dev_q4_attention(s.a, moved["q"].data_ptr(), moved["k"].data_ptr(), moved["v"].data_ptr(), tokens, moved["out"].data_ptr(), st.cuda_stream)
+    be.dev_check(st.cuda_stream)
+    assert np.array_equal(moved["out"].cpu().numpy().reshape(first.shape), first)
+    assert torch.equal(moved["k_held"], s.t["k_held"].flatten()) and torch.equal(moved["v_held"], s.t["v_held"].flatten())
+
+
 @pytest.mark.parametrize("tokens,filled,position", [(1, 64, 5), (3, 62, 5), (1, -1, 5), (2, 10, 9), (1, 10, -1), (40, 30, 0), (1, 2 ** 31 - 1, 0)])
 def test_places_outside_the_cache_or_the_tables_write_nothing(be, tokens, filled, position):
     import torch
