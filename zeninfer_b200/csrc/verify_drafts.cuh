@@ -15,7 +15,7 @@
 // row's sum, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
 // added in a fixed order.
 // What bounds it: passes over the CTA's 16 entries a thread (load, exponentials, histogram, cut, two sums: 2 to 7 thousand cycles each) and a dozen cluster barriers of some 1500.
-// 9 rows of 128256, top-p: 31 us, 5 rows, top-k 40 and top-p: 34 us, 3 rows of 32000, no cut: 10.9 us; clusters of 16 CTAs take 63, 47 and 10.4, for eight of them fit the GPU at a time.
+// 9 rows of 128256, top-p: 31.0 us, 5 rows, top-k 40 and top-p: 31.6 us, 3 rows of 32000, no cut: 10.7 us; clusters of 16 CTAs take 63, 47 and 10.4, for eight of them fit the GPU at a time.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     extern __shared__ __align__(16) uint8_t verify_smem[];
     __shared__ VerifyShare share;
     __shared__ double warp_sum[32], s_q;
-    __shared__ unsigned long long warp_total[32], s_left;
+    __shared__ unsigned long long s_left;
     __shared__ uint32_t warp_high[32], warp_low[32], warp_count[32], s_bin, s_mine, s_high, s_low, s_count, s_before, s_fits;
     __shared__ double s_sum, s_ahead, s_scale, powers[kVerifyPowers];
     __shared__ unsigned long long groups[32];          // totals of 32 bins each
@@ -105,9 +105,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     unsigned long long* totals = reinterpret_cast<unsigned long long*>(limbs);
     VerifyEntry* own_list = reinterpret_cast<VerifyEntry*>(limbs + kVerifyLimbs * kVerifyBins);
     VerifyEntry* all_list = own_list + kVerifyMine;
-    const uint32_t base = rank * p.per_cta, n = base < p.vocab ? min(p.per_cta, p.vocab - base) : 0u;
+    const uint32_t base = rank * p.per_cta;
+    const uint32_t whole_run = base < p.vocab ? min(p.per_cta, p.vocab - base) : 0u;
+    uint32_t n = whole_run;                            // entries left in it
     // a thread's run of consecutive entries, for sums in order of id (an odd number of them: no two lanes of a warp on one bank)
-    const uint32_t per_thread = ((p.per_cta + kVerifyThreads - 1) / kVerifyThreads) | 1u, begin = min(n, tid * per_thread), end = min(n, begin + per_thread);
+    const uint32_t per_thread = ((p.per_cta + kVerifyThreads - 1) / kVerifyThreads) | 1u;
+    uint32_t begin = min(n, tid * per_thread), end = min(n, begin + per_thread);
     pdl_launch_dependents();
     if (tid < kVerifyPowers) powers[tid] = exp2(tid / 64.0);
     pdl_wait();
@@ -175,6 +178,44 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     const double temperature = greedy ? 1.0 : p.temperature, per_unit = 1.0 / temperature;
 
     auto drop = [&](uint32_t i) { v[i] = NAN; e[i] = 0.0; };
+    // Once few entries are left they close ranks, an entry a thread; their places in the run are kept behind the values.  The order, by which equal values are told apart, stays.
+    uint32_t* const places = reinterpret_cast<uint32_t*>(v + p.per_cta) - kVerifyAll;
+    bool few = false;
+    auto close_ranks = [&]() {
+        if (p.per_cta < 2 * kVerifyAll) return;
+        uint32_t left = 0;
+        for (uint32_t i = begin; i < end; ++i) left += sample_key(v[i]) != 0u;
+        uint32_t at = left;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, at, o);
+            if (static_cast<int>(lane) >= o) at += x;
+        }
+        __syncthreads();
+        if (lane == 31) warp_count[warp] = at;
+        __syncthreads();
+        at += __reduce_add_sync(0xffffffffu, lane < warp ? warp_count[lane] : 0u) - left;
+        const uint32_t all = __reduce_add_sync(0xffffffffu, warp_count[lane]);
+        if (all > kVerifyAll) return;
+        for (uint32_t i = begin; i < end; ++i) if (sample_key(v[i])) all_list[at++] = VerifyEntry{0, v[i], i};
+        __syncthreads();
+        n = all;
+        if (tid < n) { v[tid] = all_list[tid].value; places[tid] = all_list[tid].id; }
+        begin = min(n, tid);
+        end = min(n, tid + 1);
+        few = true;
+        __syncthreads();
+    };
+    // where the run's entry `local` is now, or -1
+    auto place_of = [&](uint32_t local) {
+        if (!few) return static_cast<int>(local);
+        uint32_t low_end = 0, high_end = n;
+        while (low_end < high_end) {
+            const uint32_t mid = (low_end + high_end) / 2;
+            if (places[mid] < local) low_end = mid + 1;
+            else high_end = mid;
+        }
+        return low_end < n && places[low_end] == local ? static_cast<int>(low_end) : -1;
+    };
     // Of the entries that equal `border` all behind the first `ties` (in order of id) go, and so do all below it.
     auto cut_ties = [&](uint32_t border, unsigned long long ties) {
         uint32_t equal = 0;
@@ -362,7 +403,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         cluster.sync();                            // the fields are written again below
         const uint32_t row_top = s_high, row_low = s_low, row_finite = s_count;
         __syncthreads();
-        if (top_k < row_finite) cut(top_k, [](uint32_t) { return 1ull; }, row_top, row_low);
+        if (top_k < row_finite) {
+            cut(top_k, [](uint32_t) { return 1ull; }, row_top, row_low);
+            close_ranks();
+        }
     }
     // exponentials relative to the CTA's own largest value: no one waits for the row's
     double mine = 0.0;
@@ -434,10 +478,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
             if (__ldcg(p.q_ids + list + j) == token) s_q = __ldcg(p.q_probs + list + j);
         __syncthreads();
         if (tid == 0) {
-            const double mine_p = e[token - base] * scale / kept, q = p.q_ids ? s_q : 1.0;
+            const int at = place_of(static_cast<uint32_t>(token) - base);
+            const double mine_p = at < 0 ? 0.0 : e[at] * scale / kept, q = p.q_ids ? s_q : 1.0;
             p.fits[row] = __ldcg(p.uniforms + row) * q < mine_p;
             if (p.probs) p.probs[row] = mine_p;
-            if (!p.q_ids) e[token - base] = fmax(e[token - base] - of_one, 0.0);
+            if (!p.q_ids && at >= 0) e[at] = fmax(e[at] - of_one, 0.0);
         }
     } else if (is_draft && token < 0 && rank == 0 && tid == 0) {
         p.fits[row] = 0;
@@ -446,7 +491,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     __syncthreads();
     for (uint32_t j = tid; j < entries; j += kVerifyThreads) {
         const int id = __ldcg(p.q_ids + list + j);
-        if (id >= 0 && static_cast<uint32_t>(id) >= base && static_cast<uint32_t>(id) - base < n) e[id - base] = fmax(e[id - base] - __ldcg(p.q_probs + list + j) * of_one, 0.0);
+        if (id < 0 || static_cast<uint32_t>(id) < base || static_cast<uint32_t>(id) - base >= whole_run) continue;
+        if (const int at = place_of(static_cast<uint32_t>(id) - base); at >= 0) e[at] = fmax(e[at] - __ldcg(p.q_probs + list + j) * of_one, 0.0);
     }
     __syncthreads();
     // The draw: the first entry with a share whose cumulative sum, in order of id, reaches u of the whole.  A thread's sums begin at what lies before its run; the sums at
@@ -498,7 +544,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         __syncthreads();
         for (uint32_t i = begin; i < end; ++i) {
             const float x = v[i];
-            e[i] = sample_key(x) ? exp((static_cast<double>(x) - reference) * per_unit) : 0.0;
+            e[i] = sample_key(x) ? verify_exp((static_cast<double>(x) - reference) * per_unit, powers) : 0.0;
         }
         scan();
         if (tid == 0) share.left_again = cta_left;
@@ -530,7 +576,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
             }
             for (int i = static_cast<int>(begin) - 1; found < 0 && i >= 0; --i) if (e[i] * scale > 0.0) found = i;
             for (uint32_t i = end; found < 0 && i < n; ++i) if (e[i] * scale > 0.0) found = static_cast<int>(i);
-            if (found >= 0) p.draws[row] = static_cast<long long>(base) + found;
+            if (found >= 0) p.draws[row] = static_cast<long long>(base) + (few ? static_cast<int>(places[found]) : found);
         }
     }
     cluster.sync();                                  // nobody leaves while its shared memory is read
