@@ -67,20 +67,17 @@ __device__ __forceinline__ bool q4_rotates_fours(const float* q, size_t q_ld, ui
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | (q_ld * 4) | (r.pairs ? reinterpret_cast<uintptr_t>(r.cos_t) | reinterpret_cast<uintptr_t>(r.sin_t) : 0);
     return all % 16 == 0 && (!r.pairs || 2 * r.pairs == dim);
 }
-__device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row, bool fours) {
-    if (!fours) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = q4_rotated(head, at + (e & 3) + (e >> 2) * 16, r, row);
-        return;
-    }
+// kTurn: 0 not at all, 1 adjacent pairs, 2 pairs a half apart; for those that go four at a time.
+template <int kTurn>
+__device__ __forceinline__ void q4_rotated_fours(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row) {
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         const uint32_t e = at + 16 * part;
         const float4 mine = __ldcg(reinterpret_cast<const float4*>(head + e));
         float* y = x + 4 * part;
-        if (!r.pairs) {
+        if constexpr (kTurn == 0) {
             y[0] = mine.x; y[1] = mine.y; y[2] = mine.z; y[3] = mine.w;
-        } else if (r.adjacent) {
+        } else if constexpr (kTurn == 1) {
             const float* const cos_t = r.cos_t + row * r.pairs + e / 2;
             const float* const sin_t = r.sin_t + row * r.pairs + e / 2;
             const float2 c = __ldg(reinterpret_cast<const float2*>(cos_t)), s = __ldg(reinterpret_cast<const float2*>(sin_t));
@@ -96,6 +93,18 @@ __device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* hea
             auto turned = [&](float a, float b, float cc, float ss) { return low ? __fsub_rn(__fmul_rn(a, cc), __fmul_rn(b, ss)) : __fadd_rn(__fmul_rn(b, ss), __fmul_rn(a, cc)); };
             y[0] = turned(mine.x, its.x, c.x, s.x); y[1] = turned(mine.y, its.y, c.y, s.y); y[2] = turned(mine.z, its.z, c.z, s.z); y[3] = turned(mine.w, its.w, c.w, s.w);
         }
+    }
+}
+__device__ __forceinline__ void q4_rotated_eight(float (&x)[8], const float* head, uint32_t at, const Q4Rotation& r, size_t row, bool fours) {
+    if (!fours) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = q4_rotated(head, at + (e & 3) + (e >> 2) * 16, r, row);
+    } else if (!r.pairs) {
+        q4_rotated_fours<0>(x, head, at, r, row);
+    } else if (r.adjacent) {
+        q4_rotated_fours<1>(x, head, at, r, row);
+    } else {
+        q4_rotated_fours<2>(x, head, at, r, row);
     }
 }
 

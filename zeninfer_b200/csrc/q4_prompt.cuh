@@ -207,15 +207,22 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
     if (warp < kQpKeyWarp) {      // Q, while the other warps begin with the tiles: a thread takes eight dimensions of several rows, neighbouring threads a row's, all asked for first
         constexpr uint32_t kChunks = kDim / 8, kRowThreads = kQpKeyWarp * 32, kEach = kQpRows * kChunks / kRowThreads;
         const uint32_t chunk = threadIdx.x % kChunks, dim = chunk / 4 * 32 + chunk % 4 * 4;
-        const bool fours = q4_rotates_fours(p.q, p.q_ld, kDim, p.turn);
         float x[kEach][8];
+        auto ask = [&](auto turn) {                           // which way they turn is decided once, so that no row's loads wait for another's
+            constexpr int kTurn = decltype(turn)::value;
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t r = threadIdx.x / kChunks + i * (kRowThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
-            const float* from = p.q + token * p.q_ld + static_cast<size_t>(h * p.group + row % p.group) * kDim;
-            const size_t turned = static_cast<size_t>(position) + token;
-            q4_rotated_eight(x[i], from, dim, p.turn, turned, fours);
-        }
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint32_t r = threadIdx.x / kChunks + i * (kRowThreads / kChunks), row = first_row + min(r, real_rows - 1), token = row / p.group;
+                const float* from = p.q + token * p.q_ld + static_cast<size_t>(h * p.group + row % p.group) * kDim;
+                const size_t turned = static_cast<size_t>(position) + token;
+                if constexpr (kTurn < 3) q4_rotated_fours<kTurn>(x[i], from, dim, p.turn, turned);
+                else q4_rotated_eight(x[i], from, dim, p.turn, turned, false);
+            }
+        };
+        if (!q4_rotates_fours(p.q, p.q_ld, kDim, p.turn)) ask(std::integral_constant<int, 3>{});
+        else if (!p.turn.pairs) ask(std::integral_constant<int, 0>{});
+        else if (p.turn.adjacent) ask(std::integral_constant<int, 1>{});
+        else ask(std::integral_constant<int, 2>{});
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
             const uint32_t r = threadIdx.x / kChunks + i * (kRowThreads / kChunks);
