@@ -16,8 +16,8 @@
 // The scores of tile j + 1 are formed while tile j is exponentiated.
 //
 // What bounds it: the chain of a row's warps (scores out of TMEM, maximum of the quarters, exponentials, split, weights into TMEM, output sum), some 4000 cycles a tile, beside which
-// the matrix instructions take 2000 and unpacking, shared by all rows of the CTA, 3000.  512 tokens (2048 rows of 8 kv heads of 128): 34 us into an empty cache with the append,
-// 342 us into 7680 slots with the append and the weights received.  Measured on the way there, the last case: values unpacked transposed 1000 us of attention alone, as the
+// the matrix instructions take 2000 and unpacking, shared by all rows of the CTA, 3000.  512 tokens (2048 rows of 8 kv heads of 128): 33 us into an empty cache with the append,
+// 346 us into 7680 slots with the append and the weights received.  Measured on the way there, the last case: values unpacked transposed 1000 us of attention alone, as the
 // transposed operand 420, four threads a row instead of two 350, elect.sync 230.
 //
 // A scale that is not finite counts as zero in the operands and is remembered by its slot: the rows that see it are NaN (all of them for a key's, the
