@@ -429,3 +429,25 @@ def test_a_sequence_with_evictions(be):
         assert np.linalg.norm(got - out) <= 8e-6 * np.linalg.norm(out)
         assert np.abs(s.t["weight_in"].cpu().numpy()[:, :filled + 1] - received).max() <= 1e-5 * received.max()
         filled += 1
+
+
+@pytest.mark.parametrize("shape", [(1, 70, 8, 2, 64), (1, 9001, 4, 2, 128), (6, 70, 8, 2, 128), (9, 31, 8, 2, 96), (40, 70, 8, 2, 64), (40, 0, 8, 2, 128), (40, 4001, 16, 8, 128), (64, 40, 8, 2, 96)], ids=str)
+@pytest.mark.parametrize("keys", [0.0, 2.0 ** -14, 1.0])
+def test_rows_of_zeros_and_scales_that_leave_nothing_of_a_score(be, shape, keys):
+    """A row whose scores are zero, or too small to be told from it, is the mean of what it sees, whatever the keys' sizes are: its products' factor may be less than the smallest
+    normal number, and what is masked must stay masked after it."""
+    import torch
+    tokens, filled, heads, kv_heads, dim = shape
+    for zeros, scale, weights in ((slice(None), 0.0, True), (slice(0, None, 3), 0.0, True), (slice(0, None, 2), 1e-3, False), (slice(0, 0), 1e-9, True), (slice(0, 0), -1e-38, False),
+                                  (slice(0, None, 2), 1e-45, True)):
+        s = Setup(be, *shape, weights=weights, scale=scale, seed=sum(shape))
+        s.q.reshape(tokens * heads, dim)[zeros] = 0
+        s.k *= np.float32(keys)
+        d, c = s.old["k"]
+        s.old["k"] = ((d.astype(np.float32) * np.float32(keys)).astype(np.float16), c)
+        s.t["q"].copy_(torch.from_numpy(s.q.reshape(tokens, -1)))
+        s.t["k"].copy_(torch.from_numpy(s.k.reshape(tokens, -1)))
+        s.t["k_scales"][:, :filled] = torch.from_numpy(s.old["k"][0][:, :filled]).cuda()
+        s.before["k_scales"] = s.t["k_scales"].clone()
+        s.torch.cuda.synchronize()
+        s.run().check()

@@ -185,6 +185,14 @@ __host__ __device__ constexpr uint32_t q4_attend_smem(uint32_t row_warps) {
     return q4_warps(kColumns) * kQ4Stages * q4_stage_bytes<kBlocks>() + row_warps * (kColumns == kQ4Rows16 ? 4 : 2) * kBlocks * 512;
 }
 
+// What makes scores (in units of log 2) of the products of a row that is 2^(13 - e) as large.  Never zero, as it would be for a row of zeros or a very small scale: a masked score, minus
+// infinity, times zero is not a number.  The products' sums are below 2^45, so that with 2^-126 instead every score is zero to more than 32 bits of its exponential.
+constexpr float kQ4LeastFactor = 1.17549435e-38f;             // 2^-126
+__device__ __forceinline__ float q4_row_factor(float scale, int e) {
+    const int units = e - 13;                // in two steps, for it may be beyond what one power of two can be
+    return fmaxf(fabsf(scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2), kQ4LeastFactor);
+}
+
 // A warp turns one row of queries into the products' second operand.  A lane's words of a block are its dimensions 4t, 4t+2 | 16+4t, 16+4t+2 (low and high nibbles of
 // bytes 4t and 4t+2) and 4t+1, 4t+3 | 17+4t, 19+4t, of the lane's column; kDigits: columns 2r and 2r + 1 are row r's digits; else
 // a column is a row and the digits are two such sets.  The row, times a power of two, has its largest value in [2^13, 2^14).  Returns the row's factor, which makes scores
@@ -210,8 +218,7 @@ __device__ __forceinline__ float q4_lay_row(const float (&x)[kBlocks], uint4* to
             halves[(at * 4 + word) * 2 + half] = d ? other : first;
         }
     }
-    const int units = e - 13;                // in two steps, for it may be beyond what one power of two can be
-    return fabsf(scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2);
+    return q4_row_factor(scale, e);
 }
 
 // A lane's value of a block (0 .. kBlocks - 1 of the key, then of the value) of new token t, the key's rotated.

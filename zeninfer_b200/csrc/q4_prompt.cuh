@@ -240,10 +240,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
             const uint32_t at = (chunk / 8) * (kQPlane / kHalves) + r * 128 + (((chunk % 8) ^ (r & 7)) << 4);
             *reinterpret_cast<uint4*>(q_smem + at) = upper;
             *reinterpret_cast<uint4*>(q_smem + kQPlane + at) = lower;
-            if (chunk == 0) {
-                const int units = e - 13;
-                row_factor[r] = fabsf(p.scale) * 1.4426950408889634f * power_of_two(units / 2) * power_of_two(units - units / 2);
-            }
+            if (chunk == 0) row_factor[r] = q4_row_factor(p.scale, e);
             // the same for the launch that adds up what the slots received
             if (p.queries && blockIdx.x == 0) {
                 uint8_t* to = reinterpret_cast<uint8_t*>(p.queries) + (static_cast<size_t>(h) * gridDim.y + first_row / kQpRows) * 2 * kQPlane + at;
@@ -329,7 +326,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q4_prompt_kernel(const __grid_c
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[8 * c + i] = (__uint_as_float(part[0][i]) + __uint_as_float(part[1][i])) + __uint_as_float(part[2][i]);
                 }
-                by = factor * k_unit[j & 3];
+                by = fmaxf(factor * k_unit[j & 3], kQ4LeastFactor);      // the unit of a tile of tiny scales, 2^-23, may take the least factor to zero
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_empty);
