@@ -213,3 +213,28 @@ def test_the_samplers_kept_list_is_a_drafts_distribution(be):
     q = q4.distribution(drafted, 0.9, 100, 0.95)[None]
     out, accepted, probs = q4.verify(logits, [token], q, [0.4, 0.6], 0.9, 100, 0.95)
     assert int(c.t["accepted"][0]) == accepted and np.array_equal(c.t["out"].cpu().numpy(), out) and abs(float(c.t["probs"][0]) - probs[0]) <= 2.0 ** -40
+
+
+def test_a_goal_between_two_roundings_of_a_sum_is_reached_in_one_place(be):
+    """A row of 16 entries lies in four runs of four.  The sum up to the second run's end may be rounded once, as a multiply-add, or twice; the uniform number is chosen so that the first
+    of these has not reached the goal and the second has.  Either neighbour of that place is a right answer, and what the workspace held is none."""
+    from fractions import Fraction
+    rng = np.random.default_rng(8)
+    found = 0
+    while found < 48:
+        at = -rng.uniform(0.1, 3.0, 3).astype(np.float32)
+        shares = [3 * np.exp(float(x)) for x in at] + [3.0]
+        ahead, whole = shares[0], ((shares[0] + shares[1]) + shares[2]) + shares[3]
+        twice = ahead + shares[1]
+        exact = Fraction(ahead) + 3 * Fraction(float(np.exp(float(at[1]))))
+        once = float(exact)                                # a Fraction is rounded to the nearest
+        u = float(Fraction(twice) / Fraction(whole))
+        u = u if Fraction(u) * Fraction(whole) <= Fraction(twice) else float(np.nextafter(u, 0.0))
+        if not once < twice or Fraction(u) * Fraction(whole) <= Fraction(once):
+            continue
+        found += 1
+        row = np.full((1, 16), -np.inf, np.float32)
+        for r, x in enumerate([*at, np.float32(0.0)]):
+            row[0, 4 * r:4 * r + 3] = x
+        out, accepted, _ = Check(be, row, [], [u]).run()
+        assert accepted == 0 and out[0] in (6, 8), (found, out)

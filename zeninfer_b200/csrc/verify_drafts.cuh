@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     pdl_launch_dependents();
     if (tid < kVerifyPowers) powers[tid] = exp2(tid / 64.0);
     pdl_wait();
+    if (rank == 0 && tid == 0) p.draws[row] = -1;      // ahead of the barriers that the draw comes behind
     const float* logits = p.logits + row * p.logits_ld + base;
     const bool is_draft = row < p.drafts;
     long long token = is_draft ? __ldcg(p.tokens + row) : -1;
@@ -495,8 +496,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         if (const int at = place_of(static_cast<uint32_t>(id) - base); at >= 0) e[at] = fmax(e[at] - __ldcg(p.q_probs + list + j) * of_one, 0.0);
     }
     __syncthreads();
-    // The draw: the first entry with a share whose cumulative sum, in order of id, reaches u of the whole.  A thread's sums begin at what lies before its run; the sums at
-    // the runs' ends are formed by the same additions wherever they are compared, so that one thread at most finds the goal in its run.
+    // The draw: the first entry with a share whose cumulative sum, in order of id, reaches u of the whole.  A thread's sums begin at what lies before its run.  A CTA's end is the next
+    // one's beginning, formed by the same two rounded operations on both sides (no multiply-add, which rounds once), and it grows from CTA to CTA: one of them has the goal between its ends.
     double mine_left, before, cta_left;
     auto scan = [&]() {
         mine_left = 0.0;
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
         const double lanes = __shfl_up_sync(0xffffffffu, upto, 1);
         before = warps + (lane ? lanes : 0.0);
         mine_left = warps + upto;                   // where the run ends
-        cta_left = all * scale;
+        cta_left = __dmul_rn(all, scale);
     };
     scan();
     if (tid == 0) share.left = cta_left;
@@ -557,12 +558,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     // the product's rounding error decides where a sum equals it
     const double u = __ldcg(p.uniforms + p.drafts), goal = u * all, goal_rest = fma(u, all, -goal);
     auto at_goal = [&](double x) { return x > 0.0 && (x > goal || (x == goal && goal_rest <= 0.0)); };
-    auto reached = [&](double local) { return at_goal(ahead + local * scale); };
-    // the ends of runs by warps and lanes are monotone up to rounding; the first that has reached the goal is looked for, and the CTA's end is the others' beginning
+    auto reached = [&](double local) { return at_goal(__dadd_rn(ahead, __dmul_rn(local, scale))); };
+    // the ends of threads' runs grow up to rounding; the first that has reached the goal is looked for
     uint32_t first = reached(mine_left) ? tid : 0xffffffffu, none = 0, counted = 0;
     cta_range(none, first, counted);
-    const bool in_reach = !at_goal(ahead);                              // not before this CTA
-    if (in_reach && (first != 0xffffffffu || static_cast<int>(rank) == last_with_any)) {
+    // not before this CTA, and before the next one; where rounding left the row's last sum short, the last CTA with a share
+    if (!at_goal(ahead) && (at_goal(__dadd_rn(ahead, cta_left)) || static_cast<int>(rank) == last_with_any)) {
         if (first == 0xffffffffu) first = kVerifyThreads - 1;          // rounding left the last sum short: the last entry with a share
         // from the thread's run on backwards until there is an entry with a share (its own run has one but for rounding)
         if (tid == first) {
@@ -576,6 +577,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
             }
             for (int i = static_cast<int>(begin) - 1; found < 0 && i >= 0; --i) if (e[i] * scale > 0.0) found = i;
             for (uint32_t i = end; found < 0 && i < n; ++i) if (e[i] * scale > 0.0) found = static_cast<int>(i);
+            for (uint32_t i = 0; found < 0 && i < n; ++i) if (e[i] > 0.0) found = static_cast<int>(i);      // shares that only their sum keeps from vanishing
             if (found >= 0) p.draws[row] = static_cast<long long>(base) + (few ? static_cast<int>(places[found]) : found);
         }
     }
