@@ -213,3 +213,37 @@ def test_the_command(be, tmp_path, capsys):
         assert main(["generate", "--model", path, "--prompt-ids", ",".join(map(str, range(40))), "--max-new", "30"] + extra.split()) == 0
         ids[extra] = [int(t) for t in capsys.readouterr().out.strip().split("\n")[-1].split(",")]
         assert len(ids[extra]) == 30
+
+
+@pytest.mark.parametrize("kv", [{}, dict(kv="q4")], ids=str)
+@pytest.mark.parametrize("drafts", [3, 12])
+def test_drafts_are_checked_in_the_arithmetic_of_the_steps(be, monkeypatch, kv, drafts):
+    """A decoder as the registry loads it takes its prompt with 32-bit activations and its steps with int8 ones.  generate() draws from the steps' logits, so drafted tokens are
+    checked against blocks in the steps' mode; the prompt, and a caller's own forward_block, keep the prompt's."""
+    from zeninfer_b200.backend import ACT_INT8
+    cfg = config(64)
+    dec = LlamaDecoder(be, cfg, synthetic_tensors(cfg, SEED, STD), act_mode=ACT_INT8, prompt_act_mode=ACT_FP32, **kv)
+    product, modes = be.dev_gemm_q8_0, []
+
+    def recorded(*args, act_mode=ACT_INT8, **more):
+        modes.append(act_mode)
+        return product(*args, act_mode=act_mode, **more)
+
+    monkeypatch.setattr(be, "dev_gemm_q8_0", recorded)
+    try:
+        dec.capture()
+        prompt = np.random.default_rng(5).integers(0, cfg.vocab, 40).tolist()
+        assert len(dec.generate_drafted(prompt[:5], 20, drafts, lambda c, n: [1] * n)) == 20       # the first blocks of the decoder, in buffers that serve both modes
+        assert set(modes) == {ACT_INT8}
+        del modes[:]
+        greedy = dec.generate(prompt, 40)
+        assert set(modes) == {ACT_FP32}
+        of_prompt = len(modes)
+        del modes[:]
+        assert len(dec.generate_drafted(prompt, 40, drafts, lambda c, n: greedy[len(c) - 40:][:n])) == 40
+        assert set(modes[:of_prompt]) == {ACT_FP32} and set(modes[of_prompt:]) == {ACT_INT8}
+        del modes[:]
+        dec.forward_block(greedy[:9], 40, 9)
+        assert set(modes) == {ACT_FP32}
+    finally:
+        dec.close()

@@ -135,6 +135,7 @@ class LlamaDecoder(Decoder):
         import torch
         self.cfg, self.act_mode = cfg, act_mode
         self.prompt_act_mode = prompt_act_mode if prompt_act_mode not in (None, act_mode) else None
+        self.block_act_mode = None         # what generate_drafted's blocks run in, while they do
         self.fuse = "nsr" if fused is True else "" if fused is False else str(fused)
         if "p" in self.fuse and "s" in self.fuse:
             raise ValueError("SwiGLU is folded into the gate|up store ('p') or into the down prologue ('s'), not both")
@@ -381,8 +382,8 @@ class LlamaDecoder(Decoder):
         if getattr(self, "_pf", None) is None:
             torch, cfg, T, w = self.torch, self.cfg, self.PREFILL_CHUNK, self.world
             f32 = dict(dtype=torch.float32, device=self.dev)
-            mode = self._prefill_mode()
-            ws_bytes = max(self.be.gemm_workspace_bytes(T, n, mode) for n in (cfg.embedding, cfg.ffn // w, cfg.q_width // w))
+            modes = {self.act_mode} if self.prompt_act_mode is None else {self.act_mode, self.prompt_act_mode}
+            ws_bytes = max(self.be.gemm_workspace_bytes(T, n, mode) for n in (cfg.embedding, cfg.ffn // w, cfg.q_width // w) for mode in modes)
             # x, xn, tmp are whole on every rank; q, k, v, att, gate, up, hid hold this rank's heads / ffn rows
             self._pf = dict(x=torch.zeros((T, cfg.embedding), **f32), xn=torch.zeros((T, cfg.embedding), **f32), tmp=torch.zeros((T, cfg.embedding), **f32),
                             q=torch.zeros((T, cfg.q_width // w), **f32), k=torch.zeros((T, cfg.kv_width // w), **f32), v=torch.zeros((T, cfg.kv_width // w), **f32),
@@ -391,7 +392,9 @@ class LlamaDecoder(Decoder):
         return self._pf
 
     def _prefill_mode(self) -> int:
-        """Activation mode of the prompt block's products: prompt_act_mode when one was given, else the decode mode."""
+        """Activation mode of a block's products: the decode mode for a block of drafted tokens, else prompt_act_mode when one was given, else the decode mode."""
+        if self.block_act_mode is not None:
+            return self.block_act_mode
         return self.prompt_act_mode if self.prompt_act_mode is not None else self.act_mode
 
     def can_prefill_blocks(self) -> bool:
@@ -509,9 +512,11 @@ class LlamaDecoder(Decoder):
     def generate_drafted(self, prompt: list[int], max_new: int, drafts: int = 4, propose=None, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                          seed: int = 0) -> list[int]:
         """generate() with several tokens per pass of the model: `propose(context, drafts)` (default: look_up) drafts up to `drafts` tokens, forward_block
-        answers all of them, and zen_cuda_dev_verify_drafts keeps those that the model would have drawn, with one token more.  The tokens are distributed as
-        generate()'s are, greedy ones are its own up to the rounding of the block's products against the step's; what a seed draws differs, for a
-        block takes several random numbers at once.  A pass for which nothing is drafted is a step.  One GPU only."""
+        answers all of them, and zen_cuda_dev_verify_drafts keeps those that the model would have drawn, with one token more.  Blocks of drafts run in the
+        steps' activation mode, whatever the prompt's is, so the tokens are distributed as generate()'s are, and greedy ones are its own, up to the rounding of the block's products
+        against the step's (with int8 activations that moves a code of the next product here and there: logits within 2 to 3 % of their largest, 4 to 6 % over a cache in 4 bits, where
+        blocks in a 32-bit prompt mode were within 4 and 13 %); what a seed draws differs, for a block takes several random numbers at once.  A pass for which nothing is drafted is a
+        step.  One GPU only."""
         if self.world != 1:
             raise ValueError("generate_drafted: one GPU only")
         if not prompt or len(prompt) + max_new > self.max_positions:
@@ -553,7 +558,12 @@ class LlamaDecoder(Decoder):
             if len(proposed) > min(drafts, max_new - len(got) - 1) or any(not 0 <= t < self.vocab for t in proposed):
                 raise ValueError("generate_drafted: more tokens than asked for, or a token outside the vocabulary")
             if proposed:
-                new = draw(self.forward_block([got[-1]] + proposed, position, len(proposed) + 1), proposed)
+                self.block_act_mode = self.act_mode
+                try:
+                    rows = self.forward_block([got[-1]] + proposed, position, len(proposed) + 1)
+                finally:
+                    self.block_act_mode = None
+                new = draw(rows, proposed)
             else:
                 self._rewind(position)
                 with torch.cuda.stream(self.stream):
