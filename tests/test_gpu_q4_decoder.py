@@ -247,3 +247,40 @@ def test_drafts_are_checked_in_the_arithmetic_of_the_steps(be, monkeypatch, kv, 
         assert set(modes) == {ACT_FP32}
     finally:
         dec.close()
+
+
+@pytest.mark.parametrize("drafts", [2, 5, 16])
+def test_drafted_tokens_drop_slots_where_steps_do(be, drafts):
+    """Slots are dropped when a step finds none free, as in generate(), and never for a block whose tokens may be taken back."""
+    cfg = config(64)
+    dec = decoder(be, cfg, kv="q4", kv_slots=96, kv_keep=64)
+    try:
+        dec.capture()
+        prompt = np.random.default_rng(17).integers(0, cfg.vocab, 50).tolist()
+        drop, places = be.dev_q4_cache_evict, []
+
+        def dropped(*args, **more):
+            places.append((dec.place, dec.held))
+            return drop(*args, **more)
+
+        be.dev_q4_cache_evict = dropped
+        try:
+            greedy = dec.generate(prompt, 120, on_token=lambda t: None)
+            steps = places[:]
+            del places[:]
+            asked = []
+
+            def propose(context, n):
+                done = len(context) - len(prompt)
+                asked.append(n)
+                right = greedy[done:done + n]
+                wrong = done % 7                       # right ones, and wrong ones at every place
+                return [t if i != wrong else (t + 1) % cfg.vocab for i, t in enumerate(right)]
+
+            assert len(dec.generate_drafted(prompt, 120, drafts, propose)) == 120
+        finally:
+            del be.dev_q4_cache_evict
+        assert len(steps) == 3 * cfg.layers and set(places) == set(steps) and len(places) == len(steps)
+        assert all(held == dec.slots for _, held in places) and 1 <= min(asked) < max(asked) == drafts
+    finally:
+        dec.close()

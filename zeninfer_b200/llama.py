@@ -554,8 +554,11 @@ class LlamaDecoder(Decoder):
         if max_new > 0:
             got += draw(self.logits, [])
         while len(got) < max_new:
-            proposed = list(propose(prompt + got, min(drafts, max_new - len(got) - 1))) if max_new - len(got) > 1 else []
-            if len(proposed) > min(drafts, max_new - len(got) - 1) or any(not 0 <= t < self.vocab for t in proposed):
+            most = min(drafts, max_new - len(got) - 1)
+            if self.q4 and self.keep is not None:      # nothing is dropped for tokens that may be taken back: what the slots have no room for is not drafted, and a step drops
+                most = min(most, self.slots - (self.held - (self.place - position)) - 1)
+            proposed = list(propose(prompt + got, most)) if most > 0 else []
+            if len(proposed) > max(most, 0) or any(not 0 <= t < self.vocab for t in proposed):
                 raise ValueError("generate_drafted: more tokens than asked for, or a token outside the vocabulary")
             if proposed:
                 self.block_act_mode = self.act_mode
