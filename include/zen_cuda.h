@@ -657,7 +657,8 @@ typedef struct zen_cuda_q4_cache {
  *   - token t attends to slots 0 .. *filled + t, its own among them as the cache holds it; query head h reads kv head
  *     h / (heads / kv_heads); scale 0 means 1 / sqrt(head_dim);
  *   - weight_out (or NULL) [kv_heads][slots]: what a slot received, summed over the group's heads and the tokens, plus weight_in for
- *     slots below *filled; weight_in may be weight_out; slots behind the last token are left as they were;
+ *     slots below *filled; weight_in may be weight_out; slots behind the last token are left as they were.  Of a block whose last tokens are taken back
+ *     (*filled goes back), what they gave stays in weight_out: a caller that wants it out keeps weight_in apart and calls again with the tokens that stay;
  *   - k_held, v_held (or NULL) [tokens][kv_heads * head_dim]: the new keys and values as the cache holds them.
  * d_q [tokens][heads * head_dim] with rows q_ld apart, d_k and d_v [tokens][kv_heads * head_dim] with rows kv_ld apart (0: no gap);
  * d_out [tokens][heads * head_dim].  position and filled are read on the device, so a captured call serves every step; the caller

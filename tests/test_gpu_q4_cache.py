@@ -451,3 +451,24 @@ def test_rows_of_zeros_and_scales_that_leave_nothing_of_a_score(be, shape, keys)
         s.before["k_scales"] = s.t["k_scales"].clone()
         s.torch.cuda.synchronize()
         s.run().check()
+
+
+@pytest.mark.parametrize("tokens,stay,filled,heads,kv_heads,dim", [(2, 1, 30, 8, 2, 64), (5, 3, 700, 32, 8, 128), (9, 4, 70, 8, 2, 96), (40, 1, 300, 8, 2, 128), (64, 40, 2000, 16, 16, 64)])
+def test_the_weights_of_the_tokens_that_stay(be, tokens, stay, filled, heads, kv_heads, dim):
+    """A block writes its weights beside the old ones; called again with its first tokens it leaves what those alone give, and the same slots, whichever kernels take the two."""
+    import torch
+    s = Setup(be, tokens, filled, heads, kv_heads, dim, weights=True, seed=tokens).run()
+    s.check()
+    slots = {n: s.t[n].clone() for n in s.before}
+    rows = s.t["out"][:stay].clone()
+    s.tokens, s.q, s.k, s.v = stay, s.q[:stay], s.k[:stay], s.v[:stay]
+    s.t["weight_out"].fill_(-3.0)
+    room = torch.full((be.q4_attention_workspace_bytes(s.a, stay),), 0xAB, dtype=torch.uint8, device="cuda")
+    s.a.workspace, s.a.workspace_bytes = room.data_ptr(), room.numel()
+    torch.cuda.synchronize()
+    s.run()
+    assert all(torch.equal(x.view(torch.uint8), s.t[n].view(torch.uint8)) for n, x in slots.items())
+    out, received = s.expected()
+    w, n = s.t["weight_out"].cpu().numpy(), filled + stay
+    assert np.abs(w[:, :n] - received).max() <= (2 * s.away + 2.0 ** -19) * received.max() and (w[:, n:] == -3.0).all()
+    assert float((s.t["out"][:stay] - rows).abs().max()) <= 2 * s.tolerance

@@ -284,3 +284,31 @@ def test_drafted_tokens_drop_slots_where_steps_do(be, drafts):
         assert all(held == dec.slots for _, held in places) and 1 <= min(asked) < max(asked) == drafts
     finally:
         dec.close()
+
+
+def test_what_rejected_drafts_gave_stays_counted(be):
+    """Every token gives each query head's weight of 1 to the slots it sees.  With right drafts, or none, the slots have what the tokens of the sequence gave; rejected ones add to the slots that
+    were there before them."""
+    cfg = config(64)
+    dec = decoder(be, cfg, kv="q4", kv_slots=192, kv_keep=128)
+    try:
+        prompt = np.random.default_rng(19).integers(0, cfg.vocab, 40).tolist()
+        greedy = dec.generate(prompt, 60)
+
+        def given(propose):
+            assert len(dec.generate_drafted(prompt, 60, 4, propose)) == 60
+            dec.stream.synchronize()
+            sums = dec.weight[:, :, :dec.held].sum(-1).cpu().numpy() / (cfg.heads // cfg.kv_heads)
+            return sums, dec.held
+
+        right = lambda c, n: greedy[len(c) - 40:][:n]                                # noqa: E731
+        wrong = lambda c, n: [(t + 1) % cfg.vocab for t in greedy[len(c) - 40:][:n]]   # noqa: E731
+        for propose, more in ((lambda c, n: [], False), (right, False), (wrong, True)):
+            sums, held = given(propose)
+            assert held == 99
+            if more:
+                assert (sums > held + 1).all()
+            else:
+                assert (np.abs(sums - held) <= 1e-3 * held).all()
+    finally:
+        dec.close()

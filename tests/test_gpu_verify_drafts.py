@@ -238,3 +238,16 @@ def test_a_goal_between_two_roundings_of_a_sum_is_reached_in_one_place(be):
             row[0, 4 * r:4 * r + 3] = x
         out, accepted, _ = Check(be, row, [], [u]).run()
         assert accepted == 0 and out[0] in (6, 8), (found, out)
+
+
+def test_the_draw_is_not_limited_to_the_samplers_candidates(be):
+    """Of 4000 equal logits dev_sample considers the first 1024; a checked block's draw takes any, and the same ones where top_k says so."""
+    import torch
+    flat, pick, st = np.zeros((1, 4000), np.float32), torch.zeros(1, dtype=torch.int64, device="cuda"), torch.cuda.Stream()
+    for top_k in (0, 2000, 1024, 7):
+        c = Check(be, flat, [], [0.9999], top_k=top_k)
+        out, _, _ = c.run()
+        be.dev_sample(c.t["logits"].data_ptr(), 4000, 1.0, top_k, 1.0, 0.9999, pick.data_ptr(), st.cuda_stream)
+        be.dev_check(st.cuda_stream)
+        n = top_k or 4000
+        assert out[0] == int(np.ceil(0.9999 * n)) - 1 and int(pick) == int(np.ceil(0.9999 * min(n, CANDIDATES))) - 1

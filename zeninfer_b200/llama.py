@@ -463,7 +463,7 @@ class LlamaDecoder(Decoder):
         distribution after proposal i.  Afterwards the position is start_pos + len(tokens); a caller that rejects proposals
         passes the position after the last accepted token as the next start_pos (the cache rows past it are overwritten,
         as in the reference, whose caches are indexed by the position it is given; with a cache in 4 bits that drops slots, back to
-        where it last did).
+        where it last did, and what the tokens taken back gave to the slots before them stays in those slots' weights).
         The layers run through prefill() (tcgen05 GEMMs, causal block attention); the lm_head takes the tail rows through
         the decode kernel (up to eight, in the decode activation mode) or the GEMM (more, in the block's mode).  One GPU only."""
         if self.world != 1:
@@ -515,8 +515,10 @@ class LlamaDecoder(Decoder):
         answers all of them, and zen_cuda_dev_verify_drafts keeps those that the model would have drawn, with one token more.  Blocks of drafts run in the
         steps' activation mode, whatever the prompt's is, so the tokens are distributed as generate()'s are, and greedy ones are its own, up to the rounding of the block's products
         against the step's (with int8 activations that moves a code of the next product here and there: logits within 2 to 3 % of their largest, 4 to 6 % over a cache in 4 bits, where
-        blocks in a 32-bit prompt mode were within 4 and 13 %); what a seed draws differs, for a block takes several random numbers at once.  A pass for which nothing is drafted is a
-        step.  One GPU only."""
+        blocks in a 32-bit prompt mode were within 4 and 13 %); what a seed draws differs, for a block takes several random numbers at once.  Two things set the distributions apart:
+        generate() draws from the 1024 likeliest tokens at most (zen_cuda_dev_sample), this from all that the filters leave, which is the same with 1 <= top_k <= 1024; and where slots are
+        dropped (kv_slots), the attention that tokens gave before they were taken back stays counted, so that other slots may be the ones that received least.
+        A pass for which nothing is drafted is a step; slots are dropped by steps only.  One GPU only."""
         if self.world != 1:
             raise ValueError("generate_drafted: one GPU only")
         if not prompt or len(prompt) + max_new > self.max_positions:
