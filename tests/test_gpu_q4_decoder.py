@@ -312,3 +312,21 @@ def test_what_rejected_drafts_gave_stays_counted(be):
                 assert (np.abs(sums - held) <= 1e-3 * held).all()
     finally:
         dec.close()
+
+
+@pytest.mark.parametrize("options", [{}, dict(kv="q4")], ids=str)
+def test_drafts_by_look_up_are_those_of_look_up(be, options):
+    """Without a function of the caller's the context is looked up in an index that grows with it: the same drafts, and the same tokens."""
+    cfg = config(64)
+    dec = decoder(be, cfg, **options)
+    try:
+        prompt = (list(range(40)) * 2)[:70]
+        blocks = {}
+        block = dec.forward_block
+        for name, propose in (("index", None), ("scan", dec.look_up)):
+            asked = blocks[name] = []
+            dec.forward_block = lambda tokens, start, tail: (asked.append(tokens), block(tokens, start, tail))[1]
+            asked.append(dec.generate_drafted(prompt, 60, 4, propose, temperature=0.8, top_k=3, seed=4))
+        assert blocks["index"] == blocks["scan"] and len(blocks["index"]) > 2
+    finally:
+        dec.close()

@@ -177,3 +177,38 @@ def test_the_plain_model_with_a_cache_reads_blocks_as_it_reads_tokens():
     rows = [b.block([t], i)[0] for i, t in enumerate(tokens)]
     assert np.abs(whole - rows).max() <= 1e-9 * np.abs(whole).max()
     assert np.abs(b.block(tokens[5:], 5) - whole[5:]).max() <= 1e-9 * np.abs(whole).max()       # taken back and read again
+
+
+def test_an_index_of_the_context_drafts_what_looking_it_up_does():
+    from zeninfer_b200.llama import ContextIndex, LlamaDecoder
+    rng = np.random.default_rng(6)
+    for vocab, longest in ((2, 3), (4, 3), (30, 3), (5, 1)):
+        tokens, decoder = rng.integers(0, vocab, 300).tolist(), type("Decoder", (LlamaDecoder,), dict(LOOKUP=longest))
+        index, at = ContextIndex(tokens[:1], longest), 1
+        while at < len(tokens):
+            for drafts in (1, 4):
+                assert index.look_up(drafts) == LlamaDecoder.look_up(decoder, tokens[:at], drafts)
+            n = int(rng.integers(1, 6))
+            index.extend(tokens[at:at + n])
+            at += n
+
+
+def test_a_draft_from_the_index_reads_the_contexts_end_only():
+    from zeninfer_b200.llama import ContextIndex
+
+    class Counted(list):
+        read = 0
+
+        def __getitem__(self, at):
+            part = list.__getitem__(self, at)
+            Counted.read += len(part) if isinstance(at, slice) else 1
+            return part
+
+    index = ContextIndex([], 3)
+    index.tokens = Counted()
+    index.extend(range(20000))
+    Counted.read = 0
+    for t in range(50):
+        index.extend([t % 7])
+        index.look_up(4)
+    assert Counted.read <= 50 * (6 + 6 + 4)      # three runs to remember, three to look for, a draft

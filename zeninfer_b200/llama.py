@@ -103,6 +103,31 @@ def rope_tables(cfg: LlamaConfig, positions: int) -> tuple[np.ndarray, np.ndarra
     return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
 
 
+class ContextIndex:
+    """LlamaDecoder.look_up for a context that grows: where each run of up to `longest` tokens stood last with something behind it.  A draft costs what is new, not the
+    context's length (scanning 32000 tokens took 9 ms a pass, several steps of a model of 8 billion weights)."""
+
+    def __init__(self, tokens: list[int], longest: int) -> None:
+        self.tokens: list[int] = []
+        self.behind: list[dict] = [{} for _ in range(longest)]      # by length less one: the run -> the place behind it
+        self.extend(tokens)
+
+    def extend(self, tokens: list[int]) -> None:
+        for t in tokens:
+            end = len(self.tokens)
+            for n, places in enumerate(self.behind[:end], 1):
+                places[tuple(self.tokens[end - n:])] = end
+            self.tokens.append(t)
+
+    def look_up(self, drafts: int) -> list[int]:
+        end = len(self.tokens)
+        for n in range(min(len(self.behind), end - 1), 0, -1):
+            at = self.behind[n - 1].get(tuple(self.tokens[end - n:]))
+            if at is not None:
+                return self.tokens[at:at + drafts]
+        return []
+
+
 class LlamaDecoder(Decoder):
     """Holds the resident model and the step's device buffers.  `tensors` yields (name, array, is_matrix) as
     synthetic_tensors does; matrices must be Q8_0 raw blocks [rows, row_bytes]."""
@@ -526,7 +551,6 @@ class LlamaDecoder(Decoder):
         if not 1 <= drafts <= min(64, self.PREFILL_CHUNK - 1):
             raise ValueError("drafts: 1 .. 64, and less than a block")
         torch, be, st = self.torch, self.be, self.stream.cuda_stream
-        propose = propose or self.look_up
         rng = np.random.default_rng(seed)
         self.reset()
         i64 = dict(dtype=torch.int64, device=self.dev)
@@ -553,13 +577,16 @@ class LlamaDecoder(Decoder):
         with torch.cuda.stream(self.stream):
             self.feed_prompt(prompt)
         position = len(prompt)
+        index = None if propose else ContextIndex(prompt, self.LOOKUP)      # while the prompt runs
         if max_new > 0:
             got += draw(self.logits, [])
         while len(got) < max_new:
             most = min(drafts, max_new - len(got) - 1)
             if self.q4 and self.keep is not None:      # nothing is dropped for tokens that may be taken back: what the slots have no room for is not drafted, and a step drops
                 most = min(most, self.slots - (self.held - (self.place - position)) - 1)
-            proposed = list(propose(prompt + got, most)) if most > 0 else []
+            if index:
+                index.extend(got[len(index.tokens) - len(prompt):])
+            proposed = [] if most <= 0 else index.look_up(most) if index else list(propose(prompt + got, most))
             if len(proposed) > max(most, 0) or any(not 0 <= t < self.vocab for t in proposed):
                 raise ValueError("generate_drafted: more tokens than asked for, or a token outside the vocabulary")
             if proposed:
