@@ -330,3 +330,10 @@ def test_drafts_by_look_up_are_those_of_look_up(be, options):
         assert blocks["index"] == blocks["scan"] and len(blocks["index"]) > 2
     finally:
         dec.close()
+
+
+@pytest.mark.parametrize("slots", [0, -1, -64])
+def test_no_slots_are_refused(be, slots):
+    for keep in (None, 4):
+        with pytest.raises(ValueError, match="kv_slots"):
+            decoder(be, config(64), kv="q4", kv_slots=slots, kv_keep=keep)

@@ -213,6 +213,8 @@ class LlamaDecoder(Decoder):
         self.q4 = kv == "q4"
         if kv not in ("f32", "q4"):
             raise ValueError(f"kv = {kv!r}")
+        if kv_slots is not None and kv_slots < 1:
+            raise ValueError(f"kv_slots = {kv_slots}")
         if not self.q4:
             if kv_slots is not None or kv_keep is not None:
                 raise ValueError('kv_slots and kv_keep go with kv="q4"')
@@ -233,7 +235,7 @@ class LlamaDecoder(Decoder):
     def _init_q4(self, slots: int | None, keep: int | None, keep_first: int, keep_last: int | None) -> None:
         torch, be, cfg, w = self.torch, self.be, self.cfg, self.world
         up = lambda n: (n + 31) // 32 * 32
-        self.slots = up(slots or self.max_positions)
+        self.slots = up(self.max_positions if slots is None else slots)
         if self.slots >= self.max_positions:
             if keep is not None:
                 raise ValueError("kv_keep: the cache holds every position, nothing is dropped")
