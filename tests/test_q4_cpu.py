@@ -212,3 +212,14 @@ def test_a_draft_from_the_index_reads_the_contexts_end_only():
         index.extend([t % 7])
         index.look_up(4)
     assert Counted.read <= 50 * (6 + 6 + 4)      # three runs to remember, three to look for, a draft
+
+
+def test_tensors_that_the_device_cannot_read_make_no_cache():
+    import torch
+    tensors = lambda device: [torch.empty(shape(2, 64, 32), dtype=dtype, device=device)   # noqa: E731
+                              for shape, dtype in ((Q4Cache.codes_shape, torch.uint8), (Q4Cache.scales_shape, torch.float16)) * 2]
+    for device in ("cpu", "meta"):
+        with pytest.raises(ValueError, match=device):
+            Q4Cache.of(*tensors(device), kv_heads=2, head_dim=64, slots=32)
+    with pytest.raises(ValueError, match="v_codes does not hold"):
+        Q4Cache.of(*tensors("cpu")[:2], torch.empty(7, dtype=torch.uint8), torch.empty(7, dtype=torch.float16), kv_heads=2, head_dim=64, slots=32)

@@ -140,11 +140,14 @@ class Q4Cache(C.Structure):
 
     @classmethod
     def of(cls, k_codes, k_scales, v_codes, v_scales, *, kv_heads: int, head_dim: int, slots: int) -> "Q4Cache":
-        """The cache in these torch tensors: codes uint8, scales float16, contiguous, in the shapes above (or as many elements)."""
+        """The cache in these torch tensors: codes uint8, scales float16, contiguous, in the shapes above (or as many elements), of one GPU."""
         for t, size, what in ((k_codes, 1, "k_codes"), (v_codes, 1, "v_codes"), (k_scales, 2, "k_scales"), (v_scales, 2, "v_scales")):
             per_slot = head_dim // 2 if size == 1 else head_dim // 32
             if t.element_size() != size or not t.is_contiguous() or t.numel() != kv_heads * slots * per_slot:
                 raise ValueError(f"Q4Cache: {what} does not hold {kv_heads} heads of {slots} slots of {head_dim} values")
+        for t in (k_codes, v_codes, k_scales, v_scales):
+            if t.device.type != "cuda" or t.device != k_codes.device:
+                raise ValueError(f"Q4Cache: tensors on {t.device} and {k_codes.device}")
         return cls(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), kv_heads, head_dim, slots)
 
 
