@@ -683,7 +683,7 @@ typedef struct zen_cuda_q4_attention {
     void* workspace;
     size_t workspace_bytes;
 } zen_cuda_q4_attention;
-size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens); /* 0: not a valid call */
+size_t zen_cuda_q4_attention_workspace_bytes(const zen_cuda_q4_attention* a, size_t tokens); /* 0: not a valid call, or one beyond what a launch counts */
 int zen_cuda_dev_q4_attention(const zen_cuda_q4_attention* a, const float* d_q, const float* d_k, const float* d_v, size_t tokens, float* d_out,
                               void* stream);
 

@@ -223,3 +223,14 @@ def test_tensors_that_the_device_cannot_read_make_no_cache():
             Q4Cache.of(*tensors(device), kv_heads=2, head_dim=64, slots=32)
     with pytest.raises(ValueError, match="v_codes does not hold"):
         Q4Cache.of(*tensors("cpu")[:2], torch.empty(7, dtype=torch.uint8), torch.empty(7, dtype=torch.float16), kv_heads=2, head_dim=64, slots=32)
+
+
+def test_a_call_whose_last_launch_does_not_fit_a_grid_is_refused_before_the_first(lib):
+    """Many rows of heads of 96 with weights: 256 slots a CTA along a grid's second axis."""
+    bytes_of = lambda slots, tokens, **more: lib.zen_cuda_q4_attention_workspace_bytes(attention(cache(head_dim=96, slots=slots), pairs=48, **more), tokens)   # noqa: E731
+    weights = dict(weight_in=0x7000000, weight_out=0x7000000)
+    most = 65535 * 256
+    assert bytes_of(most, 40, **weights) > 0 and bytes_of(most + 32, 40, **weights) == 0
+    assert bytes_of(most + 32, 40) > 0 and bytes_of(most + 32, 16, **weights) > 0        # no weights, or few rows
+    big = attention(cache(head_dim=96, slots=most + 32), pairs=48, **weights)
+    assert "bad arguments" in refused(lib, lib.zen_cuda_dev_q4_attention(big, 16, 16, 16, 40, 16, None))

@@ -119,6 +119,7 @@ AttentionPlan attention_plan(const zen_cuda_q4_attention* a, size_t tokens) {
     while (row_warps < warps && row_warps * per_warp < rows) row_warps *= 2;
     const size_t cta_rows = row_warps * per_warp, row_ctas = (rows + cta_rows - 1) / cta_rows;
     if (row_ctas > 65535) return n;
+    if (a->weight_out && rows > zk::kQ4KeptRows && (a->cache.slots + zk::kReceivedSlots - 1) / zk::kReceivedSlots > 65535) return n;      // CTAs of the launch that adds them up, along y
     n.rows = u32(rows); n.padded = u32((rows + per_warp - 1) / per_warp * per_warp); n.row_warps = u32(row_warps); n.cta_rows = u32(cta_rows); n.row_ctas = u32(row_ctas);
     n.key_warps = u32(warps / row_warps);
     // runs of slots side by side until every SM has its CTAs, no run shorter than a tile a warp
