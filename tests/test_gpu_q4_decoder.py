@@ -337,3 +337,112 @@ def test_no_slots_are_refused(be, slots):
     for keep in (None, 4):
         with pytest.raises(ValueError, match="kv_slots"):
             decoder(be, config(64), kv="q4", kv_slots=slots, kv_keep=keep)
+
+
+@pytest.mark.parametrize("options", [{}, dict(kv="q4"), dict(kv="q4", kv_slots=96, kv_keep=64)], ids=str)
+@pytest.mark.parametrize("drafts", [1, 4, 13])
+@pytest.mark.parametrize("mode", ["int8", "fp32"])
+def test_a_drafted_token_is_the_pick_of_the_row_before_it(be, options, drafts, mode):
+    """Every token that comes back is the first of the largest logits of the row that the decoder formed for its place: a draft kept or dropped wrongly is another."""
+    from zeninfer_b200.backend import ACT_INT8
+    cfg = config(64)
+    dec = LlamaDecoder(be, cfg, synthetic_tensors(cfg, SEED, STD), act_mode=ACT_INT8 if mode == "int8" else ACT_FP32, prompt_act_mode=ACT_FP32, **options)
+    try:
+        dec.capture()
+        prompt = np.random.default_rng(drafts + 20).integers(0, cfg.vocab, 50).tolist()
+        greedy, rng, rows, lengths = dec.generate(prompt, 70), np.random.default_rng(1), {}, []
+        feed, block, step = dec.feed_prompt, dec.forward_block, dec.step
+
+        def feed_prompt(*args):
+            feed(*args)
+            rows[len(prompt) - 1] = dec.last_logits()
+
+        def forward_block(tokens, start, tail):
+            answer = block(tokens, start, tail)
+            dec.stream.synchronize()
+            rows.update(enumerate(answer.cpu().numpy(), start))
+            lengths.append(tail)
+            return answer
+
+        def one_step(want_token):
+            dec.stream.synchronize()
+            place = int(dec.pos.item())
+            step(want_token)
+            rows[place] = dec.last_logits()
+
+        def propose(context, n):
+            done = len(context) - len(prompt)
+            right = greedy[done:done + int(rng.integers(0, n + 1))]
+            return [t if rng.random() < 0.8 else int(rng.integers(cfg.vocab)) for t in right]
+
+        dec.feed_prompt, dec.forward_block, dec.step = feed_prompt, forward_block, one_step
+        got = dec.generate_drafted(prompt, 70, drafts, propose)
+        assert got == [int(rows[len(prompt) - 1 + i].argmax()) for i in range(70)]
+        assert max(lengths) > 1 and len(lengths) < 70
+    finally:
+        dec.close()
+
+
+def test_the_command_prints_what_the_decoder_gives(be, tmp_path, capsys, monkeypatch):
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(__file__), "golden"))
+    from make_llama_golden import write_gguf
+    from zeninfer_b200 import registry
+    from zeninfer_b200.__main__ import main
+    cfg = LlamaConfig(embedding=256, layers=2, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=700, rope_base=10000.0, context=256)
+    path, prompt = str(tmp_path / "m.gguf"), list(range(20)) * 2
+    write_gguf(path, cfg, synthetic_tensors(cfg, SEED, STD))
+    made = []
+    init = LlamaDecoder.__init__
+    monkeypatch.setattr(LlamaDecoder, "__init__", lambda self, *a, **k: (made.append(self), init(self, *a, **k))[1])
+    for extra, options, drafts in (("", {}, 0), ("--draft 3", {}, 3), ("--kv q4", dict(kv="q4"), 0), ("--kv q4 --draft 3", dict(kv="q4"), 3),
+                                   ("--kv q4 --kv-slots 64 --kv-keep 32 --draft 4", dict(kv="q4", kv_slots=64, kv_keep=32), 4),
+                                   ("--kv q4 --kv-slots 96 --temperature 0.8 --top-k 20 --top-p 0.9 --seed 3", dict(kv="q4", kv_slots=96), 0)):
+        assert main(["generate", "--model", path, "--prompt-ids", ",".join(map(str, prompt)), "--max-new", "50"] + extra.split()) == 0
+        ids = [int(t) for t in capsys.readouterr().out.strip().split("\n")[-1].split(",")]
+        dec = registry.load_model(be, path, **options)
+        try:
+            assert made[-2].q4 == dec.q4 == bool(options)
+            if options:
+                assert (made[-2].slots, made[-2].keep) == (dec.slots, dec.keep) == (options.get("kv_slots", 256), options.get("kv_keep", 72 if "kv_slots" in options else None))
+            sampling = dict(temperature=0.8, top_k=20, top_p=0.9, seed=3) if "temperature" in extra else {}
+            assert ids == (dec.generate_drafted(prompt, 50, drafts) if drafts else dec.generate(prompt, 50, **sampling))
+        finally:
+            dec.close()
+        made.clear()
+
+
+def test_a_rank_holds_its_own_heads(be):
+    """A sharded decoder's cache has this rank's heads: step by step the same attention, slots and weights as those heads of a decoder that has all.  (One rank after the other: nothing is exchanged
+    in this part.)"""
+    cfg = config(64)
+    options = dict(kv="q4", kv_slots=64, kv_keep=40)
+    whole = decoder(be, cfg, **options)
+    ranks = [decoder(be, cfg, rank=r, world=2, gather="nccl", **options) for r in range(2)]
+    try:
+        half = lambda t, r: t[r * (t.shape[0] // 2):(r + 1) * (t.shape[0] // 2)]   # noqa: E731
+        rng = np.random.default_rng(2)
+        for step in range(70):
+            import torch
+            for n in ("q", "k", "v"):
+                getattr(whole, n).copy_(torch.from_numpy(rng.standard_normal(getattr(whole, n).shape[0]).astype(np.float32)))
+                for r, dec in enumerate(ranks):
+                    getattr(dec, n).copy_(half(getattr(whole, n), r))
+            torch.cuda.synchronize()
+            for dec in (whole, *ranks):
+                dec._make_room(1)
+                st = dec.stream.cuda_stream
+                be.dev_q4_attention(dec.q4_calls[1], dec.q.data_ptr(), dec.k.data_ptr(), dec.v.data_ptr(), 1, dec.att_mine.data_ptr(), st)
+                be.dev_advance_position(dec.pos.data_ptr(), 1, st)
+                be.dev_advance_position(dec.filled.data_ptr(), 1, st)
+                be.dev_check(st)
+            for r, dec in enumerate(ranks):
+                assert torch.equal(dec.att_mine, half(whole.att, r)) and int(dec.filled) == int(whole.filled) == dec.held
+        for r, dec in enumerate(ranks):
+            assert dec.q4_calls[1].cache.kv_heads == 1 and dec.q4_calls[1].heads == cfg.heads // 2 and dec.floor == whole.floor == 40
+            for n in ("k_codes", "v_codes", "weight"):
+                assert torch.equal(dec.sequence.buffers[n][1], half(whole.sequence.buffers[n][1], r))
+    finally:
+        for dec in (whole, *ranks):
+            dec.close()
