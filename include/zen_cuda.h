@@ -704,7 +704,8 @@ int zen_cuda_dev_q4_cache_evict(const zen_cuda_q4_cache* from, const float* weig
  *   logits    [drafts + 1] rows of vocab floats, logits_ld apart: row i is the model's answer after draft i - 1
  *   p_i       the distribution zen_cuda_dev_sample draws from, of row i: finite logits only, the top_k highest (0: all; ties to the lowest ids),
  *             exp((v - max) / temperature) normalised in double, cut to the shortest run of the most likely that reaches top_p (outside (0, 1):
- *             no cut), without that call's limit on their number.  temperature 0: the greedy pick has all of it
+ *             no cut; masses count in 2^-51ths of the row's, rounded up), without that call's limit on their number.  temperature 0: the greedy pick
+ *             has all of it
  *   q_i       what the draft was drawn from, as zen_cuda_dev_sample leaves it: q_ids, q_probs [drafts][ZEN_CUDA_SAMPLE_MAX_CANDIDATES], q_count
  *             [drafts], ids distinct; all three NULL: the draft is certain (looked up, or a greedy pick)
  *   uniforms  [drafts + 1] doubles in [0, 1): draft i is accepted when uniforms[i] * q_i(x) < p_i(x); the last draws the token behind the

@@ -251,3 +251,16 @@ def test_the_draw_is_not_limited_to_the_samplers_candidates(be):
         be.dev_check(st.cuda_stream)
         n = top_k or 4000
         assert out[0] == int(np.ceil(0.9999 * n)) - 1 and int(pick) == int(np.ceil(0.9999 * min(n, CANDIDATES))) - 1
+
+
+@pytest.mark.parametrize("n,top_p,kept", [(6, 0.5, 3), (10, 0.5, 5), (12, 0.25, 3), (12, 0.75, 9), (20, 0.75, 15), (28, 0.25, 7), (1000, 0.5, 500), (1000, 0.125, 125), (3000, 0.75, 2250), (49, 0.5, 25)])
+def test_equal_entries_that_reach_the_share_exactly(be, n, top_p, kept):
+    """`kept` of n equal entries have top_p of the mass (the last case: reach it): the shortest run that reaches it has so many.  Alone, and with entries far below that have no mass."""
+    for vocab in (n, 3 * n, 9000):
+        row = np.full((2, vocab), -1e4, np.float32)
+        at = np.sort(np.random.default_rng(n).choice(vocab, n, replace=False))
+        row[:, at] = 1.25
+        for draft, u in ((kept - 1, 0.5), (kept, 0.5), (0, 0.999999)):      # the last that stays, the first that goes
+            out, accepted, probs = Check(be, row, [int(at[draft])], [0.0, u], top_p=top_p).run()
+            assert accepted == (draft < kept) and abs(probs[0] - (1.0 / kept if draft < kept else 0.0)) <= 2.0 ** -50
+            assert out[accepted] == at[int(np.ceil(u * kept)) - 1]

@@ -12,7 +12,7 @@
 // 1024 equal bins, which spreads logits far better than the bits of their keys do (eight bits of a key put most of a row into five bins, and
 // its threads queued up there: 290 us for 9 rows of 128256); the bin of the border is divided again while it holds more than a list
 // takes, and the entries of the list are compared with each other, equal values by id.  A mass is an integer, the exponential's 2^-51ths of the
-// row's sum, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
+// row's sum rounded up, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
 // added in a fixed order.
 // What bounds it: passes over the CTA's 16 entries a thread (load, exponentials, histogram, cut, two sums: 2 to 7 thousand cycles each) and a dozen cluster barriers of some 1500.
 // 9 rows of 128256, top-p: 31.0 us, 5 rows, top-k 40 and top-p: 31.6 us, 3 rows of 32000, no cut: 10.7 us; clusters of 16 CTAs take 63, 47 and 10.4, for eight of them fit the GPU at a time.
@@ -68,8 +68,9 @@ struct VerifyShare {
     uint32_t listed, bin_high, bin_low, any_each;
 };
 
-// The integer nearest to x, 0 <= x <= 2^51: what is left of 2^52 + x in its lower bits.
-__device__ __forceinline__ unsigned long long nearest(double x) { return static_cast<unsigned long long>(__double_as_longlong(x + 4503599627370496.0)) & 0xfffffffffffffull; }
+// The least integer that is not below e * unit, 0 <= e * unit <= 2^51: what is left of 2^52 + e * unit in its lower bits.  Upwards, so that masses which reach a share exactly (three
+// of six equal ones the half) reach it in integers too.
+__device__ __forceinline__ unsigned long long mass_of(double e, double unit) { return static_cast<unsigned long long>(__double_as_longlong(__fma_ru(e, unit, 4503599627370496.0))) & 0xfffffffffffffull; }
 
 // e^y for y <= 0, given 2^(j / 64) for j = 0 .. 63: y = n ln 2 / 64 + r with |r| < 0.0055, whose series up to r^5 / 120 leaves out less than 2^-54.  About half of the double-precision
 // instructions of exp.
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(const __gri
     double kept = whole;                           // the sum that makes probabilities of exponentials
     if (!greedy && p.top_p > 0.0f && p.top_p < 1.0f) {
         const double unit = kVerifyUnit * (scale / whole);
-        cut(max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit)), [&](uint32_t i) { return nearest(e[i] * unit); }, row_top, row_low);
+        cut(max(1ll, __double2ll_ru(static_cast<double>(p.top_p) * kVerifyUnit)), [&](uint32_t i) { return mass_of(e[i], unit); }, row_top, row_low);
         mine = 0.0;
 #pragma unroll 4
         for (uint32_t i = begin; i < end; ++i) mine += e[i];
