@@ -19,7 +19,9 @@
 // different rows, runs of slots (gridDim.x) and kv heads; what several warps have of one row is merged in shared memory, what several
 // CTAs have by a second launch.
 // What bounds it: instructions, not memory: unpacking and the matrix instructions of a tile, which no row of the block can do without.  12 rows of 8 kv heads of 128:
-// 20 us at 500 slots, 25.5 at 4003, 73 at 60000 (a byte read once would be 11 us there).
+// 20 us at 500 slots, 25.5 at 4003, 73 at 60000 (a byte read once would be 11 us there).  Steps of more than four rows come here too, as three launches: 28 / 4 and 64 / 8 heads of 128 take 14.8
+// and 15.9 us at 1000 slots, 18.6 and 21.3 at 8000.  So do prompts of other widths, whose tiles every warp fetches for itself: 512 tokens into an empty cache 58 us with 12 / 4 heads of 96,
+// 108 with 16 / 4 of 256.
 #pragma once
 #include <type_traits>
 

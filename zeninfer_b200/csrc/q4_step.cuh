@@ -7,8 +7,10 @@
 //   kCluster    the CTAs of a kv head are a cluster (up to eight): their sums meet through distributed shared memory, the scores stay in shared memory, and what the
 //               slots received is added before the launch ends
 //   else        runs of slots on all SMs; q4_finish_kernel puts them together
-// What bounds it: round trips and cluster barriers up to some thousand slots (5.7 us at 20 slots of 2 kv heads of 64, 8.6 at 1000 of 8 of 128 with weights, of which a launch is 3); the
-// instructions of a tile beyond (29.5 us at 65501 slots, 2.6 TB/s of codes and scales; the bytes alone would be 11.6).
+// What bounds it: round trips and two cluster barriers up to some thousand slots (5.7 us at 20 slots of 2 kv heads of 64, 8.6 at 1000 of 8 of 128 with weights, of which a launch is 3); beyond,
+// the instructions of the tiles' loop, where warps wait for the ALU pipe and for one another, and the ends of the launch around it (29.5 us at 65501 slots, 2.6 TB/s of codes and scales; the
+// bytes alone would be 11.6.  Over the whole launch 56 % of the issue slots and 53 % of the ALU pipe are used).  Which of the two is taken goes by the cache's size, for what is filled is
+// known on the device only: 1000 filled slots take 8.6 us in a cache of 8192 and 11.7 in one of 32768.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -14,8 +14,9 @@
 // takes, and the entries of the list are compared with each other, equal values by id.  A mass is an integer, the exponential's 2^-51ths of the
 // row's sum rounded up, added in three limbs of 17 bits by 32-bit atomics: its sums do not depend on the order in which threads add to a bin.  Sums of exponentials are
 // added in a fixed order.
-// What bounds it: passes over the CTA's 16 entries a thread (load, exponentials, histogram, cut, two sums: 2 to 7 thousand cycles each) and a dozen cluster barriers of some 1500.
-// 9 rows of 128256, top-p: 31.0 us, 5 rows, top-k 40 and top-p: 31.6 us, 3 rows of 32000, no cut: 10.7 us; clusters of 16 CTAs take 63, 47 and 10.4, for eight of them fit the GPU at a time.
+// What bounds it: passes over the CTA's 16 entries a thread (load, exponentials, histogram, cut, two sums: 2 to 7 thousand cycles each) and cluster barriers of some 1500: three without a cut,
+// six with top-p, ten with both, and two for each division behind a cut's first.
+// 9 rows of 128256, top-p: 31.3 us, 5 rows, top-k 40 and top-p: 32 to 33 us, 3 rows of 32000, no cut: 11.1 us; clusters of 16 CTAs took 63, 47 and 10.4, for eight of them fit the GPU at a time.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -545,7 +545,9 @@ class LlamaDecoder(Decoder):
         blocks in a 32-bit prompt mode were within 4 and 13 %); what a seed draws differs, for a block takes several random numbers at once.  Two things set the distributions apart:
         generate() draws from the 1024 likeliest tokens at most (zen_cuda_dev_sample), this from all that the filters leave, which is the same with 1 <= top_k <= 1024; and where slots are
         dropped (kv_slots), the attention that tokens gave before they were taken back stays counted, so that other slots may be the ones that received least.
-        A pass for which nothing is drafted is a step; slots are dropped by steps only.  One GPU only."""
+        A pass for which nothing is drafted is a step; slots are dropped by steps only.  A block costs several steps, whatever its length, so drafts pay where most of them are right: four layers of
+        the 8B shape, blocks of 2 to 16 tokens 1.1 to 1.2 ms behind 1000 tokens and 1.2 to 1.5 behind 32000 over a cache in 4 bits (a step 0.34 and 0.41), 1.3 to 1.5 and 10.6 over one in fp32
+        (0.34 and 1.13).  One GPU only."""
         if self.world != 1:
             raise ValueError("generate_drafted: one GPU only")
         if not prompt or len(prompt) + max_new > self.max_positions:
