@@ -446,3 +446,19 @@ def test_a_rank_holds_its_own_heads(be):
     finally:
         for dec in (whole, *ranks):
             dec.close()
+
+
+def test_a_look_up_of_a_subclass_is_asked(be):
+    cfg, asked = config(64), []
+
+    class Own(LlamaDecoder):
+        def look_up(self, context, drafts):
+            asked.append((len(context), drafts))
+            return context[:drafts]
+
+    dec = Own(be, cfg, synthetic_tensors(cfg, SEED, STD), act_mode=ACT_FP32)
+    try:
+        assert len(dec.generate_drafted(list(range(20)), 12, 3)) == 12
+        assert asked[0] == (21, 3) and all(1 <= n <= 3 for _, n in asked)
+    finally:
+        dec.close()

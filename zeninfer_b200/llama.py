@@ -545,7 +545,7 @@ class LlamaDecoder(Decoder):
         blocks in a 32-bit prompt mode were within 4 and 13 %); what a seed draws differs, for a block takes several random numbers at once.  Two things set the distributions apart:
         generate() draws from the 1024 likeliest tokens at most (zen_cuda_dev_sample), this from all that the filters leave, which is the same with 1 <= top_k <= 1024; and where slots are
         dropped (kv_slots), the attention that tokens gave before they were taken back stays counted, so that other slots may be the ones that received least.
-        A pass for which nothing is drafted is a step; slots are dropped by steps only.  A block costs several steps, whatever its length, so drafts pay where most of them are right: four layers of
+        A pass for which nothing is drafted is a step; behind the prompt, slots are dropped by steps only.  A block costs several steps, whatever its length, so drafts pay where most of them are right: four layers of
         the 8B shape, blocks of 2 to 16 tokens 1.1 to 1.2 ms behind 1000 tokens and 1.2 to 1.5 behind 32000 over a cache in 4 bits (a step 0.34 and 0.41), 1.3 to 1.5 and 10.6 over one in fp32
         (0.34 and 1.13).  One GPU only."""
         if self.world != 1:
@@ -555,6 +555,8 @@ class LlamaDecoder(Decoder):
         if not 1 <= drafts <= min(64, self.PREFILL_CHUNK - 1):
             raise ValueError("drafts: 1 .. 64, and less than a block")
         torch, be, st = self.torch, self.be, self.stream.cuda_stream
+        if propose is None and getattr(self.look_up, "__func__", None) is not LlamaDecoder.look_up:
+            propose = self.look_up                     # a subclass's own
         rng = np.random.default_rng(seed)
         self.reset()
         i64 = dict(dtype=torch.int64, device=self.dev)
